@@ -122,12 +122,12 @@ def _codes(gen, mats, rows, cols):
     return out
 
 
-def _weights(s, gen, mats, rows, cols, group):
+def _weights(s, gen, mats, rows, cols, group, gated):
     codes = _codes(gen, mats, rows, cols)
     scales = (0.009 * (0.8 + 0.4 * torch.rand(mats, rows, -(-cols // group), generator=gen, device="cuda"))).to(torch.bfloat16)
     if own:
         from constellation_amd.engine import Q4Matrix
-        s.held.append(Q4Matrix.pack(codes, scales, cols, group=group))
+        s.held.append(Q4Matrix.pack(codes, scales, cols, group=group, gated=gated))
         return s.held[-1]
     return codes, scales, cols, group
 
@@ -166,7 +166,7 @@ def prepare(case, seed):
             s.add = normal(t, h) if case.get("add") else None
             s.dout, s.dxs = (normal(t, h), normal(t * k, h)) if kind == "grad" else (None, None)
     elif kind == "product":
-        s.w = _weights(s, gen, 1, case["rows"], case["cols"], case["group"])
+        s.w = _weights(s, gen, 1, case["rows"], case["cols"], case["group"], case["gated"])
         s.x, s.x_scale = normal(t, case["cols"], dtype=torch.float32), None
         if dtype == torch.float8_e4m3fn:
             s.x, s.x_scale = _quantised(s.x)
@@ -175,8 +175,8 @@ def prepare(case, seed):
         s.grid = torch.tensor(E2M1 + [-v for v in E2M1], device="cuda")
     else:
         h, i, e, g = case["hidden"], case["inter"], case["experts"], case["group"]
-        s.gate_up = _weights(s, gen, e, 2 * i, h, g)
-        s.down = _weights(s, gen, e, h, i, g)
+        s.gate_up = _weights(s, gen, e, 2 * i, h, g, True)
+        s.down = _weights(s, gen, e, h, i, g, False)
         if own:
             from constellation_amd.engine import Q4Layer
             s.layer = Q4Layer(s.ctx, s.gate_up, s.down)
@@ -263,7 +263,7 @@ def run(s):
             dys, dw = ctx.combine_rows_grad(s.dout, s.ys, s.place, s.w)
             return {"dys": dys, "dw": dw, "dx": ctx.combine_rows(s.dxs, s.place)}
         if kind == "product":
-            return ctx.q4_matmul(s.w, s.x, x_scale=s.x_scale, gated=c["gated"])
+            return ctx.q4_matmul(s.w, s.x, x_scale=s.x_scale)
         return ctx.moe(s.layer, s.x, s.ids, s.w)
     if kind == "norm":
         total = (s.x.float() + s.residual.float()).to(s.x.dtype)
