@@ -21,7 +21,7 @@ CX_EDEVICE = -5
 
 CX_STATIC_SCRATCH_BYTES = 256 * 1024  # include/cx_moe.h
 
-FP16, BF16, F32 = 1, 2, 3
+FP16, BF16, F32, E4M3 = 1, 2, 3, 4
 
 
 class CxError(RuntimeError):
@@ -41,6 +41,15 @@ class ExpertDesc(C.Structure):
         ("gate_rb", C.c_int32), ("gate_cb", C.c_int32),
         ("down_rb", C.c_int32), ("down_cb", C.c_int32),
         ("gu_layout", C.c_int32), ("reserved", C.c_int32 * 3),
+    ]
+
+
+class Q4Desc(C.Structure):
+    """cx_q4_desc: a packed stack of 4-bit matrices in the arena."""
+    _fields_ = [
+        ("codes", C.c_void_p), ("scales", C.c_void_p),
+        ("n_mats", C.c_int32), ("rows", C.c_int32), ("cols", C.c_int32),
+        ("group", C.c_int32), ("gated", C.c_int32), ("reserved", C.c_int32 * 3),
     ]
 
 
@@ -99,6 +108,19 @@ _SIGS = {
     "cx_moe_layer_response_size": (C.c_size_t, [_I, _I]),
     "cx_moe_layer_request_run": (_I, [_P, _P, _P, C.c_size_t, _P, C.c_size_t,
                                       C.POINTER(C.c_size_t)]),
+    "cx_rms_norm": (_I, [_P, _P, _I, _P, _P, _I, _I, _I, C.c_float, _P, _P, _I, _P, _P, _P]),
+    "cx_sort_tokens": (_I, [_P, _P, _I, _I, _I, _P, _P, _P, _P]),
+    "cx_gather_rows": (_I, [_P, _P, C.c_size_t, _P, _I, _I, _P, _P]),
+    "cx_combine_rows": (_I, [_P, _P, _I, _P, _P, _P, _I, _I, _I, _P, _I, _P, _P]),
+    "cx_combine_rows_grad": (_I, [_P, _P, _I, _P, _I, _P, _P, _I, _I, _I, _P, _P, _P]),
+    "cx_q4_pack": (_I, [_I, _P, _P, _I, _I, _I, _I, _I, _P, C.POINTER(Q4Desc)]),
+    "cx_q4_free": (_I, [_I, C.POINTER(Q4Desc)]),
+    "cx_q4_scratch": (C.c_size_t, [C.POINTER(Q4Desc), _I]),
+    "cx_q4_matmul": (_I, [_P, C.POINTER(Q4Desc), _P, _I, _P, _I, _P, _I, _P, _I, _P, _I, _P,
+                          C.c_size_t, _P]),
+    "cx_q4_moe_scratch": (C.c_size_t, [C.POINTER(Q4Desc), C.POINTER(Q4Desc), _I, _I, _I]),
+    "cx_q4_moe": (_I, [_P, C.POINTER(Q4Desc), C.POINTER(Q4Desc), C.POINTER(Q4Desc),
+                       C.POINTER(Q4Desc), _P, _I, _I, _P, _P, _I, _P, _I, _P, _P, C.c_size_t, _P]),
     "cx_gen_fp8_matrix": (_I, [_P, C.c_uint64, C.c_uint64, _I, _I, _I, _I, C.c_float, _P, _P,
                                _P]),
     "cx_gen_normal": (_I, [_P, C.c_uint64, C.c_uint64, C.c_uint64, C.c_float, _I, _P, _P]),

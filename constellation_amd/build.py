@@ -33,7 +33,9 @@ SOURCES = {
     "cx_expert.hip": [],
     "cx_few.hip": [],
     "cx_pp.hip": [],
+    "cx_q4.hip": [],
     "cx_route.hip": [],
+    "cx_rows.hip": [],
     "cx_gen.hip": ["-ffp-contract=off"],
 }
 

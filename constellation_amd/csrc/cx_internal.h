@@ -111,6 +111,7 @@ enum : int {
     kErrNotResident = 2,
     kErrPlanOverflow = 4,
     kErrDuplicateRoute = 8,
+    kErrBadRow = 32,     // a place outside the sorted rows
     kErrBadWeight = 16,  // negative or non-finite route weight (validate_routes, moe_layer_runtime.py:96-97)
 };
 
@@ -301,5 +302,110 @@ hipError_t launch_gen_normal(uint64_t seed, uint64_t stream_id, uint64_t count,
                              float std_dev, int dtype, void* out, hipStream_t s);
 
 bool fast_path_ok(const cx_expert_desc& e);
+
+// ---------------------------------------------------------------------------
+// Rows around the experts (cx_rows.hip).  The sizes of a launch are checked by the
+// callers (rows_grid_ok).
+struct NormArgs {
+    const void* x;
+    const void* residual;  // nullable
+    const void* weight;    // nullable: ones
+    int x_dtype, w_dtype, y_dtype;
+    int n_tokens, hidden;
+    float eps;
+    void* sum;             // nullable, x_dtype
+    void* y;               // nullable
+    uint8_t* q;            // nullable
+    float* q_scale;        // [n_tokens, ceil(hidden / 128)], with q
+};
+hipError_t launch_rms_norm(const NormArgs& a, hipStream_t s);
+
+// A run of rows of one matrix: one work unit of the 4-bit products.  Entry 0 of an
+// item list is its head: {items, rows that have an expert, 0, 0}.
+struct Q4Item {
+    int expert, begin, rows, pad;
+};
+
+struct SortArgs {
+    const int32_t* ids;    // [n_tokens, top_k]
+    const float* weights;  // nullable: when given, a repeated expert or a bad weight is an error and its pair has no expert
+    int n_tokens, top_k, n_experts;
+    int shared;            // 1: every token also goes to a shared expert, as route top_k and expert n_experts
+    int32_t* order;        // [n_tokens * (top_k + shared)]
+    int32_t* offsets;      // nullable [n_experts + 1]
+    int32_t* place;        // [n_tokens, top_k + shared]
+    Q4Item* items;         // nullable: runs of up to item_rows rows of one expert
+    int item_rows;
+    int* err_flag;
+};
+hipError_t launch_sort_tokens(const SortArgs& a, hipStream_t s);
+
+struct GatherArgs {
+    const void* x;
+    void* xs;
+    const int32_t* place;
+    int n_tokens, top_k;
+    size_t row_bytes;
+    int* err_flag;
+};
+int64_t gather_workgroups(const GatherArgs& g);
+hipError_t launch_gather_rows(const GatherArgs& g, hipStream_t s);
+
+struct CombineArgs {
+    const void* ys;         // [n_rows, hidden]
+    const int32_t* place;   // [n_tokens, top_k]
+    const float* weights;   // nullable: ones; weights_step a token, and ones behind them
+    const void* add;        // nullable [n_tokens, hidden], out_dtype
+    int ys_dtype, out_dtype;
+    int n_tokens, top_k, weights_step, n_rows, hidden;
+    void* out;
+    float* out_f32;         // nullable
+    int* err_flag;
+};
+int64_t combine_workgroups(const CombineArgs& a);
+hipError_t launch_combine_rows(const CombineArgs& a, hipStream_t s);
+
+struct CombineGradArgs {
+    const void* dout;
+    const void* ys;
+    const int32_t* place;
+    const float* weights;  // nullable: ones
+    int dout_dtype, ys_dtype;
+    int n_tokens, top_k, n_rows, hidden;
+    void* dys;
+    float* dw;             // nullable
+    int* err_flag;
+};
+hipError_t launch_combine_grad(const CombineGradArgs& a, hipStream_t s);
+
+// ---------------------------------------------------------------------------
+// 4-bit products (cx_q4.hip).
+enum { kQ4Bf16 = 1, kQ4Fp16 = 2, kQ4E4m3 = 4, kQ4Planes = 5 };  // x and y; planes: bf16 hi + lo
+struct Q4Launch {
+    cx_q4_desc w;
+    cx_q4_desc shared;       // matrix of items with expert == w.n_mats (codes NULL: none)
+    const void* x;           // [*, cols]
+    const void* x_lo;        // planes
+    const float* x_scale;    // e4m3: [*, ceil(cols / 128)]
+    int x_type;
+    int n_x;                 // rows of x
+    int n_rows;              // rows of y
+    const int32_t* order;    // nullable: row p reads x row order[p] / top_k
+    int top_k;
+    const Q4Item* items;     // nullable: all rows belong to matrix 0
+    int item_rows;           // rows of an item, at most
+    int64_t max_items;       // of the list, its head included
+    void* y;                 // [n_rows, rows] ([n_rows, rows / 2] gated)
+    void* y_lo;
+    int y_type;              // CX_DTYPE_* or kQ4Planes
+};
+size_t q4_code_bytes(const cx_q4_desc& w);
+size_t q4_scale_bytes(const cx_q4_desc& w);
+hipError_t launch_q4_pack(const cx_q4_desc& w, const uint8_t* codes, const uint16_t* scales, hipStream_t s);
+hipError_t launch_q4_items(const int32_t* offsets, int n_mats, int n_rows, int item_rows, Q4Item* items, int* err_flag,
+                           hipStream_t s);
+int q4_item_rows(const cx_q4_desc& w, int n_rows, int n_mats);
+bool q4_grid_ok(const Q4Launch& L);
+hipError_t launch_q4(const Q4Launch& L, hipStream_t s);
 
 }  // namespace cx

@@ -783,6 +783,53 @@ int fill_route(cx_ctx* ctx, const void* x, int x_dtype, const void* w_router, in
 }  // namespace
 
 // ===========================================================================
+// Rows around the experts and 4-bit weights.
+namespace {
+
+bool act_any(int dtype) { return act16(dtype) || dtype == CX_DTYPE_F32; }
+
+int check_rows(cx_ctx* ctx, int n_tokens, int top_k, int64_t width) {
+    if (!ctx) return fail(CX_EINVAL, "NULL context");
+    if (n_tokens < 0 || top_k < 1 || top_k > 64) return fail(CX_EINVAL, "bad n_tokens/top_k");
+    if (width <= 0) return fail(CX_EINVAL, "rows must not be empty");
+    if ((int64_t)n_tokens * top_k > INT32_MAX) return fail(CX_EINVAL, "too many pairs: n_tokens * top_k must fit 31 bits");
+    return set_device(ctx->device);
+}
+
+int check_q4(const cx_q4_desc* w) {
+    if (!w || !w->codes || !w->scales) return fail(CX_EINVAL, "4-bit descriptor is NULL or empty");
+    if (w->n_mats <= 0 || w->rows <= 0 || w->cols <= 0 || (w->group != 32 && w->group != 64 && w->group != 128) ||
+        (w->gated && w->rows % 2 != 0))
+        return fail(CX_EINVAL, "bad 4-bit descriptor");
+    return CX_OK;
+}
+
+// Scratch of cx_q4_moe, in this order.
+struct Q4MoeScratch {
+    int64_t pairs, max_items;
+    int item_rows;
+    size_t items, order, place, h, h_lo, ys, bytes;
+};
+
+Q4MoeScratch q4_moe_scratch(const cx_q4_desc& gu, const cx_q4_desc& down, int shared, int n_tokens, int top_k) {
+    Q4MoeScratch z{};
+    auto up = [](size_t v) { return (v + 255) / 256 * 256; };
+    z.pairs = (int64_t)n_tokens * (top_k + shared);
+    z.item_rows = q4_item_rows(gu, (int)std::min<int64_t>(z.pairs, INT32_MAX), gu.n_mats + shared);
+    z.max_items = q4_max_items(z.pairs, gu.n_mats + shared, z.item_rows);
+    z.items = 0;
+    z.order = z.items + up(sizeof(Q4Item) * (size_t)z.max_items);
+    z.place = z.order + up(4 * (size_t)z.pairs);
+    z.h = z.place + up(4 * (size_t)z.pairs);
+    z.h_lo = z.h + up(2 * (size_t)z.pairs * down.cols);
+    z.ys = z.h_lo + up(2 * (size_t)z.pairs * down.cols);
+    z.bytes = z.ys + up(4 * (size_t)z.pairs * down.rows);
+    return z;
+}
+
+}  // namespace
+
+// ===========================================================================
 // Whole-layer wire message helpers (MoeLayerRequest / MoeLayerResponse, cx_moe.h).
 namespace {
 
@@ -1077,12 +1124,13 @@ int cx_ctx_sync(cx_ctx* ctx, void* stream) {
     if (flag != 0) {
         CX_HIP(hipMemsetAsync(ctx->err_flag, 0, sizeof(int), s));
         CX_HIP(hipStreamSynchronize(s));
-        return fail(CX_EDEVICE, "device check failed (flags 0x%x:%s%s%s%s%s)", flag,
+        return fail(CX_EDEVICE, "device check failed (flags 0x%x:%s%s%s%s%s%s)", flag,
                     (flag & kErrBadExpertId) ? " expert id out of range" : "",
                     (flag & kErrNotResident) ? " expert not resident" : "",
                     (flag & kErrPlanOverflow) ? " plan overflow" : "",
                     (flag & kErrDuplicateRoute) ? " expert routed twice for one token" : "",
-                    (flag & kErrBadWeight) ? " negative or non-finite route weight" : "");
+                    (flag & kErrBadWeight) ? " negative or non-finite route weight" : "",
+                    (flag & kErrBadRow) ? " row place or offset outside the rows" : "");
     }
     return CX_OK;
 }
@@ -1319,6 +1367,312 @@ int cx_moe_layer(cx_ctx* ctx, const cx_layer* layer, const void* x, int in_dtype
         return rc;
     return moe_run(ctx, layer, x, in_dtype, n_tokens, ids, w, top_k, y, out_dtype, y_f32, s,
                    n_tokens > kTileTok, &R);
+}
+
+// ---------------------------------------------------------------------------
+// Rows around the experts and 4-bit weights.
+
+int cx_rms_norm(cx_ctx* ctx, const void* x, int x_dtype, const void* residual, const void* weight, int w_dtype,
+                int n_tokens, int hidden, float eps, void* sum, void* y, int y_dtype, uint8_t* q, float* q_scale,
+                void* stream) {
+    DeviceRestore keep;
+    int rc = check_rows(ctx, n_tokens, 1, hidden);
+    if (rc) return rc;
+    if (hidden > kNormMaxHidden) return fail(CX_EINVAL, "hidden must be 1..%d", kNormMaxHidden);
+    if (!act_any(x_dtype) || (y && !act_any(y_dtype)) || (weight && !act_any(w_dtype)))
+        return fail(CX_EINVAL, "dtypes must be fp16, bf16 or fp32");
+    if (!(eps >= 0.0f)) return fail(CX_EINVAL, "eps must be >= 0");
+    if (n_tokens == 0) return CX_OK;
+    if (!x || (!y && !q) || (q && !q_scale)) return fail(CX_EINVAL, "NULL buffer");
+    if (!rows_grid_ok(n_tokens, 1024)) return fail(CX_EINVAL, "too many rows for one launch");
+    Span sp(ctx, "rms_norm", static_cast<hipStream_t>(stream));
+    CX_HIP(launch_rms_norm(NormArgs{x, residual, weight, x_dtype, w_dtype, y_dtype, n_tokens, hidden, eps, sum, y, q, q_scale},
+                           static_cast<hipStream_t>(stream)));
+    return CX_OK;
+}
+
+int cx_sort_tokens(cx_ctx* ctx, const int32_t* ids, int n_tokens, int top_k, int n_experts, int32_t* order,
+                   int32_t* offsets, int32_t* place, void* stream) {
+    DeviceRestore keep;
+    int rc = check_rows(ctx, n_tokens, top_k, 1);
+    if (rc) return rc;
+    if (n_experts < 1 || n_experts > kSortMaxExperts) return fail(CX_EINVAL, "n_experts must be 1..%d", kSortMaxExperts);
+    if (!offsets || (n_tokens > 0 && (!ids || !order || !place))) return fail(CX_EINVAL, "NULL buffer");
+    SortArgs a{};
+    a.ids = ids;
+    a.n_tokens = n_tokens;
+    a.top_k = top_k;
+    a.n_experts = n_experts;
+    a.order = order;
+    a.offsets = offsets;
+    a.place = place;
+    a.err_flag = ctx->err_flag;
+    Span sp(ctx, "sort", static_cast<hipStream_t>(stream));
+    CX_HIP(launch_sort_tokens(a, static_cast<hipStream_t>(stream)));
+    return CX_OK;
+}
+
+int cx_gather_rows(cx_ctx* ctx, const void* x, size_t row_bytes, const int32_t* place, int n_tokens, int top_k,
+                   void* xs, void* stream) {
+    DeviceRestore keep;
+    int rc = check_rows(ctx, n_tokens, top_k, row_bytes > 0 && row_bytes <= INT32_MAX ? (int64_t)row_bytes : 0);
+    if (rc) return rc;
+    if (n_tokens == 0) return CX_OK;
+    if (!x || !place || !xs) return fail(CX_EINVAL, "NULL buffer");
+    const GatherArgs g{x, xs, place, n_tokens, top_k, row_bytes, ctx->err_flag};
+    if (!rows_grid_ok(gather_workgroups(g), kRowThreads)) return fail(CX_EINVAL, "too many rows for one launch");
+    Span sp(ctx, "gather", static_cast<hipStream_t>(stream));
+    CX_HIP(launch_gather_rows(g, static_cast<hipStream_t>(stream)));
+    return CX_OK;
+}
+
+int cx_combine_rows(cx_ctx* ctx, const void* ys, int ys_dtype, const int32_t* place, const float* weights,
+                    const void* add, int n_tokens, int top_k, int hidden, void* out, int out_dtype, float* out_f32,
+                    void* stream) {
+    DeviceRestore keep;
+    int rc = check_rows(ctx, n_tokens, top_k, hidden);
+    if (rc) return rc;
+    if (!act_any(ys_dtype) || !act_any(out_dtype)) return fail(CX_EINVAL, "dtypes must be fp16, bf16 or fp32");
+    if (n_tokens == 0) return CX_OK;
+    if (!ys || !place || !out) return fail(CX_EINVAL, "NULL buffer");
+    CombineArgs a{};
+    a.ys = ys;
+    a.place = place;
+    a.weights = weights;
+    a.add = add;
+    a.ys_dtype = ys_dtype;
+    a.out_dtype = out_dtype;
+    a.n_tokens = n_tokens;
+    a.top_k = a.weights_step = top_k;
+    a.n_rows = n_tokens * top_k;
+    a.hidden = hidden;
+    a.out = out;
+    a.out_f32 = out_f32;
+    a.err_flag = ctx->err_flag;
+    if (!rows_grid_ok(combine_workgroups(a), kRowThreads)) return fail(CX_EINVAL, "too many rows for one launch");
+    Span sp(ctx, "combine", static_cast<hipStream_t>(stream));
+    CX_HIP(launch_combine_rows(a, static_cast<hipStream_t>(stream)));
+    return CX_OK;
+}
+
+int cx_combine_rows_grad(cx_ctx* ctx, const void* dout, int dout_dtype, const void* ys, int ys_dtype,
+                         const int32_t* place, const float* weights, int n_tokens, int top_k, int hidden, void* dys,
+                         float* dw, void* stream) {
+    DeviceRestore keep;
+    int rc = check_rows(ctx, n_tokens, top_k, hidden);
+    if (rc) return rc;
+    if (!act_any(ys_dtype) || !act_any(dout_dtype)) return fail(CX_EINVAL, "dtypes must be fp16, bf16 or fp32");
+    if (n_tokens == 0) return CX_OK;
+    if (!dout || !ys || !place || !dys) return fail(CX_EINVAL, "NULL buffer");
+    if (!rows_grid_ok((int64_t)n_tokens * top_k, kRowThreads)) return fail(CX_EINVAL, "too many rows for one launch");
+    Span sp(ctx, "combine_grad", static_cast<hipStream_t>(stream));
+    CX_HIP(launch_combine_grad(CombineGradArgs{dout, ys, place, weights, dout_dtype, ys_dtype, n_tokens, top_k,
+                                               n_tokens * top_k, hidden, dys, dw, ctx->err_flag},
+                               static_cast<hipStream_t>(stream)));
+    return CX_OK;
+}
+
+int cx_q4_pack(int device, const uint8_t* codes, const uint16_t* scales, int n_mats, int rows, int cols, int group,
+               int gated, void* stream, cx_q4_desc* out) {
+    DeviceRestore keep;
+    if (!out) return fail(CX_EINVAL, "NULL out");
+    std::memset(out, 0, sizeof(*out));
+    if (!codes || !scales) return fail(CX_EINVAL, "NULL buffer");
+    if (n_mats < 1 || n_mats > kSortMaxExperts || rows < 1 || cols < 1)
+        return fail(CX_EINVAL, "bad 4-bit shape (n_mats must be 1..%d)", kSortMaxExperts);
+    if (group != 32 && group != 64 && group != 128) return fail(CX_EINVAL, "group must be 32, 64 or 128");
+    if (gated && rows % 2 != 0) return fail(CX_EINVAL, "a gated matrix has an even number of rows");
+    int rc = set_device(device);
+    if (rc) return rc;
+    cx_q4_desc w{};
+    w.n_mats = n_mats;
+    w.rows = rows;
+    w.cols = cols;
+    w.group = group;
+    w.gated = gated != 0;
+    void *c = nullptr, *sc = nullptr;
+    if ((rc = arena_alloc(device, q4_code_bytes(w), &c))) return rc;
+    if ((rc = arena_alloc(device, q4_scale_bytes(w), &sc))) {
+        (void)arena_free(device, c, false);
+        return rc;
+    }
+    w.codes = static_cast<uint8_t*>(c);
+    w.scales = static_cast<uint16_t*>(sc);
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    hipError_t e = launch_q4_pack(w, codes, scales, s);
+    if (e == hipSuccess) e = hipStreamSynchronize(s);
+    if (e != hipSuccess) {
+        (void)arena_free(device, c, false);
+        (void)arena_free(device, sc, false);
+        return fail(CX_EHIP, "packing 4-bit weights failed: %s", hipGetErrorString(e));
+    }
+    *out = w;
+    return CX_OK;
+}
+
+int cx_q4_free(int device, cx_q4_desc* w) {
+    if (!w) return fail(CX_EINVAL, "4-bit descriptor is NULL or empty");
+    if (device < 0 || device >= 64) return fail(CX_EINVAL, "bad device");
+    int rc = CX_OK;
+    if (w->codes && (rc = arena_free(device, const_cast<uint8_t*>(w->codes)))) return rc;
+    if (w->scales && (rc = arena_free(device, const_cast<uint16_t*>(w->scales)))) return rc;
+    std::memset(w, 0, sizeof(*w));
+    return CX_OK;
+}
+
+size_t cx_q4_scratch(const cx_q4_desc* w, int n_rows) {
+    if (!w || w->n_mats < 1 || n_rows < 0) return 0;
+    return sizeof(Q4Item) * (size_t)q4_max_items(n_rows, w->n_mats, q4_item_rows(*w, n_rows, w->n_mats));
+}
+
+int cx_q4_matmul(cx_ctx* ctx, const cx_q4_desc* w, const void* x, int x_dtype, const float* x_scale, int n_x,
+                 const int32_t* order, int top_k, const int32_t* offsets, int n_rows, void* y, int y_dtype,
+                 void* scratch, size_t scratch_bytes, void* stream) {
+    DeviceRestore keep;
+    if (!ctx) return fail(CX_EINVAL, "NULL context");
+    int rc = check_q4(w);
+    if (rc) return rc;
+    if (!act16(x_dtype) && x_dtype != CX_DTYPE_E4M3) return fail(CX_EINVAL, "x must be fp16, bf16 or e4m3");
+    if (!act_any(y_dtype)) return fail(CX_EINVAL, "y must be fp16, bf16 or fp32");
+    if (n_rows < 0 || n_x < 0 || (order && top_k < 1)) return fail(CX_EINVAL, "bad n_rows, n_x or top_k");
+    if (!order && n_x != n_rows) return fail(CX_EINVAL, "without an order x and y have the same rows (%d and %d)", n_x, n_rows);
+    if (!offsets && w->n_mats != 1) return fail(CX_EINVAL, "a stack of %d matrices needs offsets", w->n_mats);
+    if (n_rows == 0) return CX_OK;
+    if (!y || (n_x > 0 && (!x || (x_dtype == CX_DTYPE_E4M3 && !x_scale)))) return fail(CX_EINVAL, "NULL buffer");
+    if (offsets && (!scratch || scratch_bytes < cx_q4_scratch(w, n_rows) || reinterpret_cast<uintptr_t>(scratch) % 16))
+        return fail(CX_EINVAL, "scratch must be %zu bytes, 16-byte aligned", cx_q4_scratch(w, n_rows));
+    if ((rc = set_device(ctx->device))) return rc;
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    Q4Launch L{};
+    L.w = *w;
+    L.x = x;
+    L.x_scale = x_scale;
+    L.x_type = x_dtype == CX_DTYPE_BF16 ? kQ4Bf16 : x_dtype == CX_DTYPE_FP16 ? kQ4Fp16 : kQ4E4m3;
+    L.n_x = n_x;
+    L.n_rows = n_rows;
+    L.order = order;
+    L.top_k = top_k;
+    L.y = y;
+    L.y_type = y_dtype;
+    L.item_rows = q4_item_rows(*w, n_rows, w->n_mats);
+    L.max_items = q4_max_items(n_rows, w->n_mats, L.item_rows);
+    if (!q4_grid_ok(L)) return fail(CX_EINVAL, "too many rows for one launch");
+    if (offsets) {
+        L.items = static_cast<const Q4Item*>(scratch);
+        Span sp(ctx, "plan", s);
+        CX_HIP(launch_q4_items(offsets, w->n_mats, n_rows, L.item_rows, static_cast<Q4Item*>(scratch), ctx->err_flag, s));
+    }
+    Span sp(ctx, "q4", s);
+    CX_HIP(launch_q4(L, s));
+    return CX_OK;
+}
+
+size_t cx_q4_moe_scratch(const cx_q4_desc* gate_up, const cx_q4_desc* down, int has_shared, int n_tokens, int top_k) {
+    if (!gate_up || !down || gate_up->n_mats < 1 || n_tokens < 0 || top_k < 0) return 0;
+    return q4_moe_scratch(*gate_up, *down, has_shared != 0, n_tokens, top_k).bytes;
+}
+
+int cx_q4_moe(cx_ctx* ctx, const cx_q4_desc* gate_up, const cx_q4_desc* down, const cx_q4_desc* shared_gate_up,
+              const cx_q4_desc* shared_down, const void* x, int in_dtype, int n_tokens, const int32_t* topk_ids,
+              const float* topk_w, int top_k, void* y, int out_dtype, float* y_f32, void* scratch,
+              size_t scratch_bytes, void* stream) {
+    DeviceRestore keep;
+    if (!ctx) return fail(CX_EINVAL, "NULL context");
+    int rc = check_q4(gate_up);
+    if (rc || (rc = check_q4(down))) return rc;
+    const int shared = shared_gate_up != nullptr;
+    if (shared != (shared_down != nullptr)) return fail(CX_EINVAL, "the shared expert needs both of its matrices");
+    if (!gate_up->gated || down->gated || gate_up->n_mats != down->n_mats || gate_up->rows != 2 * (int64_t)down->cols ||
+        gate_up->cols != down->rows)
+        return fail(CX_EINVAL, "a layer's matrices must be gated [2 * inter, hidden] and [hidden, inter], one of each per expert");
+    if (shared) {
+        if ((rc = check_q4(shared_gate_up)) || (rc = check_q4(shared_down))) return rc;
+        auto same = [](const cx_q4_desc& a, const cx_q4_desc& b) {
+            return a.n_mats == 1 && a.rows == b.rows && a.cols == b.cols && a.group == b.group && a.gated == b.gated;
+        };
+        if (!same(*shared_gate_up, *gate_up) || !same(*shared_down, *down))
+            return fail(CX_EINVAL, "the shared expert must have the layer's sizes and groups");
+    }
+    if (!act16(in_dtype) || !act16(out_dtype)) return fail(CX_EINVAL, "dtypes must be fp16/bf16");
+    if (n_tokens < 0 || top_k < 0 || top_k > 64 || top_k + shared < 1) return fail(CX_EINVAL, "bad n_tokens/top_k");
+    if ((int64_t)n_tokens * (top_k + shared) > INT32_MAX) return fail(CX_EINVAL, "too many pairs: n_tokens * top_k must fit 31 bits");
+    if (n_tokens == 0) return CX_OK;
+    if (!x || !y || (top_k > 0 && (!topk_ids || !topk_w))) return fail(CX_EINVAL, "NULL buffer");
+    const Q4MoeScratch z = q4_moe_scratch(*gate_up, *down, shared, n_tokens, top_k);
+    if (!scratch || scratch_bytes < z.bytes || reinterpret_cast<uintptr_t>(scratch) % 16)
+        return fail(CX_EINVAL, "scratch must be %zu bytes, 16-byte aligned", z.bytes);
+    if ((rc = set_device(ctx->device))) return rc;
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    char* m = static_cast<char*>(scratch);
+    SortArgs a{};
+    a.ids = topk_ids;
+    a.weights = topk_w;
+    a.n_tokens = n_tokens;
+    a.top_k = top_k;
+    a.n_experts = gate_up->n_mats;
+    a.shared = shared;
+    a.order = reinterpret_cast<int32_t*>(m + z.order);
+    a.place = reinterpret_cast<int32_t*>(m + z.place);
+    a.items = reinterpret_cast<Q4Item*>(m + z.items);
+    a.item_rows = z.item_rows;
+    a.err_flag = ctx->err_flag;
+    Q4Launch L{};
+    L.w = *gate_up;
+    if (shared) L.shared = *shared_gate_up;
+    L.x = x;
+    L.x_type = in_dtype == CX_DTYPE_BF16 ? kQ4Bf16 : kQ4Fp16;
+    L.n_x = n_tokens;
+    L.n_rows = (int)z.pairs;
+    L.order = a.order;
+    L.top_k = top_k + shared;
+    L.items = a.items;
+    L.item_rows = z.item_rows;
+    L.max_items = z.max_items;
+    L.y = m + z.h;
+    L.y_lo = m + z.h_lo;
+    L.y_type = kQ4Planes;
+    Q4Launch D = L;
+    D.w = *down;
+    if (shared) D.shared = *shared_down;
+    D.x = L.y;
+    D.x_lo = L.y_lo;
+    D.x_type = kQ4Planes;
+    D.n_x = (int)z.pairs;
+    D.order = nullptr;
+    D.y = m + z.ys;
+    D.y_lo = nullptr;
+    D.y_type = CX_DTYPE_F32;
+    CombineArgs c{};
+    c.ys = D.y;
+    c.ys_dtype = CX_DTYPE_F32;
+    c.place = a.place;
+    c.weights = topk_w;
+    c.weights_step = top_k;
+    c.out_dtype = out_dtype;
+    c.n_tokens = n_tokens;
+    c.top_k = top_k + shared;
+    c.n_rows = (int)z.pairs;
+    c.hidden = down->rows;
+    c.out = y;
+    c.out_f32 = y_f32;
+    c.err_flag = ctx->err_flag;
+    if (!q4_grid_ok(L) || !q4_grid_ok(D) || !rows_grid_ok(combine_workgroups(c), kRowThreads))
+        return fail(CX_EINVAL, "too many rows for one launch");
+    {
+        Span sp(ctx, "plan", s);
+        CX_HIP(launch_sort_tokens(a, s));
+    }
+    {
+        Span sp(ctx, "gate_up", s);
+        CX_HIP(launch_q4(L, s));
+    }
+    {
+        Span sp(ctx, "down", s);
+        CX_HIP(launch_q4(D, s));
+    }
+    Span sp(ctx, "combine", s);
+    CX_HIP(launch_combine_rows(c, s));
+    return CX_OK;
 }
 
 // ---------------------------------------------------------------------------

@@ -262,4 +262,20 @@ inline size_t plan_buffer_bytes(int n_tokens, int top_k, int n_experts, int has_
     return plan_bytes(z, n_tokens, top_k, true);
 }
 
+// ---------------------------------------------------------------------------
+// Rows around the experts and 4-bit products.
+constexpr int kSortMaxExperts = 1024;  // the counts of a workgroup's waves fit its LDS
+constexpr int kNormMaxHidden = 65536;  // a row in the registers of 1024 threads, 64 values each
+
+constexpr int kRowThreads = 256;       // workgroup of the gather and combine kernels
+
+// A launch's threads are counted in 32 bits.
+inline bool rows_grid_ok(int64_t workgroups, int threads) { return workgroups * threads < ((int64_t)1 << 32); }
+
+// Items of up to item_rows rows over n_mats matrices, entry 0 (the head) included: at
+// most one short item per matrix that has rows, and one of rows without a matrix.
+inline int64_t q4_max_items(int64_t n_rows, int n_mats, int item_rows) {
+    return 2 + (n_rows < n_mats ? n_rows : n_mats) + n_rows / item_rows;
+}
+
 }  // namespace cx

@@ -7,13 +7,13 @@ device.
 from __future__ import annotations
 
 import ctypes as C
-from typing import Optional, Sequence
+from typing import NamedTuple, Optional, Sequence, Union
 
 import numpy as np
 import torch
 
-from ._lib import (BF16, F32, FP16, CxError, DeviceInfo, ExpertDesc, MoeLayerRequestInfo, check,
-                   lib)
+from ._lib import (BF16, E4M3, F32, FP16, CxError, DeviceInfo, ExpertDesc, MoeLayerRequestInfo,
+                   Q4Desc, check, lib)
 
 _TORCH_TO_CX = {torch.float16: FP16, torch.bfloat16: BF16, torch.float32: F32}
 _CX_TO_TORCH = {FP16: torch.float16, BF16: torch.bfloat16, F32: torch.float32}
@@ -28,6 +28,25 @@ def cx_dtype(t: torch.dtype) -> int:
 
 def _ptr(t: Optional[torch.Tensor]) -> Optional[int]:
     return None if t is None else t.data_ptr()
+
+
+def _rows_2d(t: torch.Tensor) -> tuple[int, int]:
+    if t.dim() != 2:
+        raise ValueError(f"expected a 2D tensor, got shape {tuple(t.shape)}")
+    return t.shape[0], t.shape[1]
+
+
+def _places(place: torch.Tensor, n_tokens: int) -> int:
+    if place.dtype != torch.int32 or place.dim() != 2 or place.shape[0] != n_tokens or not place.is_contiguous():
+        raise ValueError(f"place must be contiguous int32 [{n_tokens}, top_k]")
+    return place.shape[1]
+
+
+def _check_pairs(rows: int, n_tokens: int, top_k: int, weights: Optional[torch.Tensor]) -> None:
+    if rows != n_tokens * top_k:
+        raise ValueError(f"{rows} sorted rows, {n_tokens} x {top_k} pairs")
+    if weights is not None and (weights.shape != (n_tokens, top_k) or weights.dtype != torch.float32):
+        raise ValueError(f"weights must be fp32 [{n_tokens}, {top_k}]")
 
 
 def _stream(device: int) -> int:
@@ -198,6 +217,83 @@ class Layer:
             self.handle = None
 
 
+class Norm(NamedTuple):
+    """What Context.rms_norm was asked for (None where it was not)."""
+    sum: Optional[torch.Tensor]    # x + residual, in x's type
+    y: Optional[torch.Tensor]
+    q: Optional[torch.Tensor]      # float8_e4m3fn
+    scale: Optional[torch.Tensor]  # fp32 [T, ceil(H / 128)]
+
+
+class Q4Matrix:
+    """A stack of matrices with 4-bit weights, packed in the library's HBM arena
+    (cx_q4_desc): e2m1 codes and a bf16 scale per row and `group` columns."""
+
+    def __init__(self, device: int, desc: Q4Desc):
+        self.device = device
+        self.desc = desc
+        self._live = True
+
+    @classmethod
+    def pack(cls, codes: torch.Tensor, scales: torch.Tensor, cols: int, *, group: int = 128,
+             gated: bool = False) -> "Q4Matrix":
+        """codes: uint8 [n_mats, rows, ceil(cols / 2)] (or [rows, ...] for one), two
+        columns a byte, the even one in the lower nibble; scales: bf16 [n_mats,
+        rows, ceil(cols / group)].  gated: the rows are a gate matrix and then
+        an up matrix of the same size, whose product is silu(gate) * up."""
+        if codes.dim() == 2:
+            codes, scales = codes.unsqueeze(0), scales.unsqueeze(0)
+        if codes.dtype != torch.uint8 or scales.dtype != torch.bfloat16:
+            raise TypeError("codes must be uint8 and scales bfloat16")
+        if group not in (32, 64, 128):
+            raise ValueError("group must be 32, 64 or 128")
+        E, N = codes.shape[:2]
+        if codes.dim() != 3 or cols < 1 or codes.shape[2] != (cols + 1) // 2 or \
+                scales.shape != (E, N, -(-cols // group)):
+            raise ValueError(f"codes {tuple(codes.shape)} and scales {tuple(scales.shape)} do not hold "
+                             f"matrices of {cols} columns in groups of {group}")
+        if codes.device.type != "cuda" or scales.device != codes.device:
+            raise ValueError("codes and scales must be on one HIP device")
+        codes, scales = codes.contiguous(), scales.contiguous()
+        dev, d = codes.device.index, Q4Desc()
+        check(lib().cx_q4_pack(dev, codes.data_ptr(), scales.data_ptr(), E, N, cols, group, int(gated),
+                               _stream(dev), C.byref(d)))
+        return cls(dev, d)
+
+    @property
+    def out_cols(self) -> int:
+        """Columns of a product with this matrix."""
+        return self.desc.rows // 2 if self.desc.gated else self.desc.rows
+
+    def free(self) -> None:
+        if self._live:
+            check(lib().cx_q4_free(self.device, C.byref(self.desc)))
+            self._live = False
+
+
+class Q4Layer:
+    """A layer of 4-bit experts: `gate_up` a gated stack [E, 2 * inter, hidden],
+    `down` a stack [E, hidden, inter], `shared` the shared expert's two (stacks of
+    one), if the layer has one.  Context.moe and Context.moe_layer take it in
+    place of a Layer, and so does moe_dispatch.LocalNode."""
+
+    def __init__(self, ctx: "Context", gate_up: Q4Matrix, down: Q4Matrix,
+                 shared: Optional[tuple[Q4Matrix, Q4Matrix]] = None):
+        g, d = gate_up.desc, down.desc
+        if not g.gated or d.gated or g.n_mats != d.n_mats or g.rows != 2 * d.cols or g.cols != d.rows:
+            raise ValueError("a layer's matrices must be gated [E, 2 * inter, hidden] and [E, hidden, inter]")
+        for own, of in zip(shared or (), (g, d)):
+            s = own.desc
+            if (s.n_mats, s.rows, s.cols, s.group, s.gated) != (1, of.rows, of.cols, of.group, of.gated):
+                raise ValueError("the shared expert must have the layer's sizes and groups")
+        if any(m.device != ctx.device for m in (gate_up, down, *(shared or ()))):
+            raise ValueError("a layer's matrices must be on its context's device")
+        self.ctx = ctx
+        self.gate_up, self.down, self.shared = gate_up, down, shared
+        self.n_experts, self.hidden, self.inter = g.n_mats, d.rows, d.cols
+        self.experts = [self] * self.n_experts  # every expert of the stack is resident
+
+
 class Context:
     """One per device and worker thread (cx_ctx)."""
 
@@ -279,8 +375,164 @@ class Context:
                                     self.stream()))
         return out
 
+    # -- rows around the experts -------------------------------------------------
+    def _here(self, *tensors: Optional[torch.Tensor]) -> None:
+        for t in tensors:
+            if t is not None and (t.device.type != "cuda" or t.device.index != self.device):
+                raise ValueError(f"tensor on {t.device}, context on cuda:{self.device}")
+
+    def rms_norm(self, x: torch.Tensor, weight: Optional[torch.Tensor] = None, *, eps: float = 1e-6,
+                 residual: Optional[torch.Tensor] = None, out_dtype: Optional[torch.dtype] = None,
+                 want_y: bool = True, quantize: bool = False) -> Norm:
+        """RMS norm of x (+ residual) [T, H]: `sum` the residual stream where a
+        residual is given, `y` in out_dtype (x's), and with quantize `q` in e4m3
+        with `scale` per token and 128 columns."""
+        self._here(x, weight, residual)
+        T, H = _rows_2d(x)
+        if residual is not None and (residual.shape != x.shape or residual.dtype != x.dtype):
+            raise ValueError("residual must have x's shape and type")
+        if weight is not None and weight.shape != (H,):
+            raise ValueError(f"weight must be [{H}]")
+        if not (want_y or quantize):
+            raise ValueError("nothing to compute: want_y or quantize")
+        x = x.contiguous()
+        residual = None if residual is None else residual.contiguous()
+        weight = None if weight is None else weight.contiguous()
+        dt = cx_dtype(x.dtype)
+        out_dtype = out_dtype or x.dtype
+        s = None if residual is None else torch.empty_like(x)
+        y = torch.empty((T, H), dtype=out_dtype, device=x.device) if want_y else None
+        q = scale = None
+        if quantize:
+            q = torch.empty((T, H), dtype=torch.float8_e4m3fn, device=x.device)
+            scale = torch.empty((T, (H + 127) // 128), dtype=torch.float32, device=x.device)
+        check(lib().cx_rms_norm(self.handle, x.data_ptr(), dt, _ptr(residual), _ptr(weight),
+                                dt if weight is None else cx_dtype(weight.dtype), T, H, eps, _ptr(s), _ptr(y),
+                                cx_dtype(out_dtype), _ptr(q), _ptr(scale), self.stream()))
+        return Norm(s, y, q, scale)
+
+    def sort_tokens(self, ids: torch.Tensor, n_experts: int):
+        """(order [T * K], offsets [n_experts + 1], place [T, K]), all int32: the
+        pairs t * K + k sorted by expert (cx_sort_tokens)."""
+        self._here(ids)
+        T, K = _rows_2d(ids)
+        ids = ids.to(torch.int32).contiguous()
+        order = torch.empty(T * K, dtype=torch.int32, device=ids.device)
+        offsets = torch.empty(n_experts + 1, dtype=torch.int32, device=ids.device)
+        place = torch.empty((T, K), dtype=torch.int32, device=ids.device)
+        check(lib().cx_sort_tokens(self.handle, ids.data_ptr(), T, K, n_experts, order.data_ptr(),
+                                   offsets.data_ptr(), place.data_ptr(), self.stream()))
+        return order, offsets, place
+
+    def gather_rows(self, x: torch.Tensor, place: torch.Tensor) -> torch.Tensor:
+        """Rows of x [T, H] (any type) in sorted order [T * K, H]; zeros where a
+        pair has no expert.  Its gradient: combine_rows(dxs, place)."""
+        self._here(x, place)
+        T, H = _rows_2d(x)
+        K = _places(place, T)
+        x = x.contiguous()
+        xs = torch.empty((T * K, H), dtype=x.dtype, device=x.device)
+        check(lib().cx_gather_rows(self.handle, x.data_ptr(), H * x.element_size(), place.data_ptr(), T, K,
+                                   xs.data_ptr(), self.stream()))
+        return xs
+
+    def combine_rows(self, ys: torch.Tensor, place: torch.Tensor, weights: Optional[torch.Tensor] = None, *,
+                     add: Optional[torch.Tensor] = None,
+                     out_dtype: Optional[torch.dtype] = None) -> torch.Tensor:
+        """Sorted rows ys [T * K, H] back to tokens: [T, H] in out_dtype (ys's),
+        the sum over k of weights[t, k] * ys[place[t, k]] (+ add[t])."""
+        self._here(ys, place, weights, add)
+        P, H = _rows_2d(ys)
+        T = place.shape[0]
+        K = _places(place, T)
+        out_dtype = out_dtype or ys.dtype
+        _check_pairs(P, T, K, weights)
+        if add is not None and (add.shape != (T, H) or add.dtype != out_dtype):
+            raise ValueError(f"add must be [{T}, {H}] in the output's type")
+        ys = ys.contiguous()
+        weights = None if weights is None else weights.contiguous()
+        add = None if add is None else add.contiguous()
+        out = torch.empty((T, H), dtype=out_dtype, device=ys.device)
+        check(lib().cx_combine_rows(self.handle, ys.data_ptr(), cx_dtype(ys.dtype), place.data_ptr(),
+                                    _ptr(weights), _ptr(add), T, K, H, out.data_ptr(), cx_dtype(out_dtype),
+                                    None, self.stream()))
+        return out
+
+    def combine_rows_grad(self, dout: torch.Tensor, ys: torch.Tensor, place: torch.Tensor,
+                          weights: Optional[torch.Tensor] = None):
+        """(dys [T * K, H] in ys's type, dw fp32 [T, K]) of combine_rows."""
+        self._here(dout, ys, place, weights)
+        P, H = _rows_2d(ys)
+        T = place.shape[0]
+        K = _places(place, T)
+        _check_pairs(P, T, K, weights)
+        if dout.shape != (T, H):
+            raise ValueError(f"dout must be [{T}, {H}]")
+        dout, ys = dout.contiguous(), ys.contiguous()
+        weights = None if weights is None else weights.contiguous()
+        dys = torch.empty_like(ys)
+        dw = torch.empty((T, K), dtype=torch.float32, device=ys.device)
+        check(lib().cx_combine_rows_grad(self.handle, dout.data_ptr(), cx_dtype(dout.dtype), ys.data_ptr(),
+                                         cx_dtype(ys.dtype), place.data_ptr(), _ptr(weights), T, K, H,
+                                         dys.data_ptr(), dw.data_ptr(), self.stream()))
+        return dys, dw
+
+    # -- 4-bit weights -------------------------------------------------------------
+    def q4_matmul(self, w: Q4Matrix, x: torch.Tensor, *, x_scale: Optional[torch.Tensor] = None,
+                  offsets: Optional[torch.Tensor] = None, order: Optional[torch.Tensor] = None,
+                  top_k: int = 1, out_dtype: Optional[torch.dtype] = None) -> torch.Tensor:
+        """x W^T (silu(x G^T) * (x U^T) for a gated matrix) in out_dtype (x's; bf16
+        for e4m3 x, which comes with rms_norm's scale).  A stack of matrices takes
+        the rows offsets[e] .. offsets[e + 1] - 1 through matrix e; with `order`,
+        row p is row order[p] // top_k of x (sort_tokens' offsets and order)."""
+        self._here(x, x_scale, offsets, order)
+        T, K = _rows_2d(x)
+        d = w.desc
+        if w.device != self.device:
+            raise ValueError(f"matrix on cuda:{w.device}, context on cuda:{self.device}")
+        if K != d.cols:
+            raise ValueError(f"x has {K} columns, the matrix {d.cols}")
+        f8 = x.dtype == torch.float8_e4m3fn
+        if f8 != (x_scale is not None):
+            raise ValueError("x_scale comes with e4m3 x, and only with it")
+        if f8 and (x_scale.shape != (T, (K + 127) // 128) or x_scale.dtype != torch.float32):
+            raise ValueError(f"x_scale must be fp32 [{T}, {(K + 127) // 128}]")
+        for name, t, n in (("offsets", offsets, d.n_mats + 1), ("order", order, None)):
+            if t is not None and (t.dtype != torch.int32 or t.dim() != 1 or not t.is_contiguous()
+                                  or (n is not None and t.shape[0] != n)):
+                raise ValueError(f"{name} must be a contiguous int32 vector" + (f" of {n}" if n else ""))
+        P = T if order is None else order.shape[0]
+        x = x.contiguous()
+        x_scale = None if x_scale is None else x_scale.contiguous()
+        out_dtype = out_dtype or (torch.bfloat16 if f8 else x.dtype)
+        y = torch.empty((P, w.out_cols), dtype=out_dtype, device=x.device)
+        scratch, size = None, 0
+        if offsets is not None:
+            size = lib().cx_q4_scratch(C.byref(d), P)
+            scratch = torch.empty(size, dtype=torch.uint8, device=x.device)
+        check(lib().cx_q4_matmul(self.handle, C.byref(d), x.data_ptr(), E4M3 if f8 else cx_dtype(x.dtype),
+                                 _ptr(x_scale), T, _ptr(order), top_k, _ptr(offsets), P, y.data_ptr(),
+                                 cx_dtype(out_dtype), _ptr(scratch), size, self.stream()))
+        return y
+
+    def _q4_moe(self, layer: Q4Layer, x, topk_ids, topk_w, y, yf):
+        T = x.shape[0]
+        K = topk_ids.shape[1] if topk_ids.dim() == 2 else 0
+        self._here(x, topk_ids, topk_w)
+        if x.shape[1] != layer.hidden:
+            raise ValueError(f"x has {x.shape[1]} columns, the layer {layer.hidden}")
+        if K and (topk_ids.shape != (T, K) or topk_w.shape != (T, K)):
+            raise ValueError(f"routes must be [{T}, top_k]")
+        gu, dn = C.byref(layer.gate_up.desc), C.byref(layer.down.desc)
+        sg, sd = (C.byref(m.desc) for m in layer.shared) if layer.shared else (None, None)
+        size = lib().cx_q4_moe_scratch(gu, dn, int(layer.shared is not None), T, K)
+        scratch = torch.empty(size, dtype=torch.uint8, device=x.device)
+        check(lib().cx_q4_moe(self.handle, gu, dn, sg, sd, x.data_ptr(), cx_dtype(x.dtype), T,
+                              topk_ids.data_ptr(), topk_w.data_ptr(), K, y.data_ptr(), cx_dtype(y.dtype),
+                              _ptr(yf), scratch.data_ptr(), size, self.stream()))
+
     # -- grouped MoE -----------------------------------------------------------
-    def moe(self, layer: Layer, x: torch.Tensor, topk_ids: torch.Tensor, topk_w: torch.Tensor, *,
+    def moe(self, layer: Union[Layer, Q4Layer], x: torch.Tensor, topk_ids: torch.Tensor, topk_w: torch.Tensor, *,
             out_dtype: Optional[torch.dtype] = None, want_f32: bool = False,
             prefill: Optional[bool] = None):
         x = x.contiguous()
@@ -294,6 +546,9 @@ class Context:
         fn = lib().cx_moe_prefill if prefill else lib().cx_moe_decode
         ids = topk_ids.to(torch.int32).contiguous()
         w = topk_w.to(torch.float32).contiguous()
+        if isinstance(layer, Q4Layer):
+            self._q4_moe(layer, x, ids, w, y, yf)
+            return (y, yf) if want_f32 else y
         check(fn(self.handle, layer.handle, x.data_ptr(), cx_dtype(x.dtype), T, ids.data_ptr(),
                  w.data_ptr(), K, y.data_ptr(), cx_dtype(out_dtype), _ptr(yf), self.stream()))
         return (y, yf) if want_f32 else y
@@ -312,7 +567,7 @@ class Context:
                                              out.ctypes.data, out.size, C.byref(n)))
         return out[:n.value].tobytes()
 
-    def moe_layer(self, layer: Layer, x: torch.Tensor, w_router: torch.Tensor, bias: torch.Tensor, *,
+    def moe_layer(self, layer: Union[Layer, Q4Layer], x: torch.Tensor, w_router: torch.Tensor, bias: torch.Tensor, *,
                   resident: Optional[torch.Tensor] = None, n_group: int = 8, topk_group: int = 4,
                   top_k: int = 8, norm_topk_prob: bool = True, routed_scaling_factor: float = 2.5,
                   out_dtype: Optional[torch.dtype] = None, want_f32: bool = False, out=None):
@@ -326,6 +581,13 @@ class Context:
             w = torch.empty((T, top_k), dtype=torch.float32, device=x.device)
         else:
             y, yf, ids, w = out
+        if isinstance(layer, Q4Layer):
+            check(lib().cx_route(self.handle, x.data_ptr(), cx_dtype(x.dtype), w_router.data_ptr(),
+                                 cx_dtype(w_router.dtype), bias.data_ptr(), _ptr(resident), T, layer.hidden,
+                                 layer.n_experts, n_group, topk_group, top_k, int(norm_topk_prob),
+                                 routed_scaling_factor, ids.data_ptr(), w.data_ptr(), self.stream()))
+            self._q4_moe(layer, x, ids, w, y, yf)
+            return y, yf, ids, w
         check(lib().cx_moe_layer(self.handle, layer.handle, x.data_ptr(), cx_dtype(x.dtype), T,
                                  w_router.data_ptr(), cx_dtype(w_router.dtype), bias.data_ptr(),
                                  _ptr(resident), n_group, topk_group, top_k, int(norm_topk_prob),

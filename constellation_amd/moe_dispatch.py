@@ -15,7 +15,8 @@ each node once:
   * LocalNode — experts resident on this process's GPU (engine.Layer per
     layer id): cx_moe_decode / cx_moe_prefill on the device tensors, with no
     host copy.  When one local node holds every expert of the layer,
-    run_moe_layer_batched routes and computes in one cx_moe_layer call.
+    run_moe_layer_batched routes and computes in one cx_moe_layer call.  A
+    layer may be an engine.Q4Layer (4-bit experts): cx_q4_moe.
   * RemoteNode — an expert node reached through a caller-supplied transport
     (a function from one framed request to one framed reply, or a socket to
     a worker port): one MoeLayerRequest (msg 42, v1 framing
@@ -293,3 +294,22 @@ def run_moe_layer_batched(nodes: Sequence[Node], hidden: torch.Tensor, layer_id:
     y = run_topk_moe_layer(nodes, x, layer_id, ids, w, n_experts=E, shared=shared,
                            out_dtype=out_dtype)
     return (y.view(-1) if was_1d else y), ids, w
+
+
+def run_moe_block(nodes: Sequence[Node], hidden: torch.Tensor, residual: Optional[torch.Tensor],
+                  layer_id: int, norm_weight: torch.Tensor, gate_weight: torch.Tensor,
+                  e_score_correction_bias: torch.Tensor, *, eps: float = 1e-6, **router):
+    """The sparse half of a decoder layer for a whole token batch: the residual's
+    addition and the RMS norm before the experts (cx_rms_norm), then
+    run_moe_layer_batched on the normed rows.  hidden: the attention's output
+    [T, H] (or [H]) on the HIP device; residual: the stream it is added to, or
+    None for a first layer.  Returns (y, stream, topk_ids, topk_w): the next
+    layer adds y to `stream`.  `router`: run_moe_layer_batched's options."""
+    x, was_1d = _as_2d(hidden)
+    dev = _hip_device(x)
+    ctx = _context(dev)
+    with torch.cuda.device(dev):
+        n = ctx.rms_norm(x, norm_weight, eps=eps, residual=None if residual is None else residual.reshape(x.shape))
+    stream = x if n.sum is None else n.sum
+    y, ids, w = run_moe_layer_batched(nodes, n.y, layer_id, gate_weight, e_score_correction_bias, **router)
+    return (y.view(-1), stream.view(-1), ids, w) if was_1d else (y, stream, ids, w)

@@ -44,8 +44,10 @@ enum {
 };
 
 /* Activation dtypes.  1 and 2 are the wire values of common::ActivationDType
- * (common/protocol.h:48-52); 3 is fp32, used by the router and parity outputs. */
-enum { CX_DTYPE_FP16 = 1, CX_DTYPE_BF16 = 2, CX_DTYPE_F32 = 3 };
+ * (common/protocol.h:48-52); 3 is fp32, used by the router and parity outputs;
+ * 4 is e4m3 with a fp32 scale per row and 128 columns, the 8-bit output of
+ * cx_rms_norm and an input of the 4-bit products. */
+enum { CX_DTYPE_FP16 = 1, CX_DTYPE_BF16 = 2, CX_DTYPE_F32 = 3, CX_DTYPE_E4M3 = 4 };
 
 CX_API const char* cx_last_error(void);
 CX_API const char* cx_version(void);
@@ -274,6 +276,125 @@ CX_API int cx_moe_layer(cx_ctx* ctx, const cx_layer* layer,
                  int top_k, int norm_topk_prob, float routed_scaling_factor,
                  void* y, int out_dtype, float* y_f32,
                  int32_t* topk_ids, float* topk_w, void* stream);
+
+/* ---- rows around the experts -----------------------------------------------
+ * What a decoder layer does between its attention and its experts, and what a
+ * program with experts of its own does around them.  No counterpart in the
+ * reference's expert path (its server runs norm and residual in torch).  None of
+ * these calls allocates, copies or waits, so all of them can be captured into a
+ * graph; they use no scratch, so calls on different streams may overlap.  Rows
+ * are contiguous and may start at any address of their type's alignment; rows
+ * and widths whose bytes are multiples of 16 take the wide accesses.  A call of
+ * no tokens does nothing. */
+
+/* s = x + residual, rounded to x's type (the residual stream); then the RMS norm
+ * of s as it was rounded:
+ *   y = s / sqrt(mean(s^2) + eps) * weight
+ * in 16 or 32 bits, and / or in e4m3 (OCP, saturating, nearest even) with a scale
+ * per token and 128 columns, from the fp32 y:
+ *   q_scale[t][b] = max(max |y[t][128 b ..]| / 448, 1e-12),  q = e4m3(y / q_scale)
+ * (a quotient within a few 2^-24 of two neighbours' middle may take either).
+ * residual, weight (ones), sum, y and q are nullable, but one of y and q is
+ * needed; q comes with q_scale [n_tokens, ceil(hidden / 128)].  sum may be x or
+ * residual itself; the other buffers must not overlap.  A NaN or an infinity in s
+ * makes its row what the formula gives; a NaN in a block makes its q_scale NaN.
+ * Sums are in fp32.  hidden is at most 65536. */
+CX_API int cx_rms_norm(cx_ctx* ctx, const void* x, int x_dtype, const void* residual,
+                const void* weight, int w_dtype, int n_tokens, int hidden, float eps,
+                void* sum, void* y, int y_dtype, uint8_t* q, float* q_scale, void* stream);
+
+/* Token-expert pairs in the experts' order.  Pair i = t * top_k + k names expert
+ * ids[t][k]; rows are the pairs sorted by expert, stable, those whose id is
+ * negative (or out of range: also reported by cx_ctx_sync) behind all others.
+ *   order[row]     the row's pair, or its complement ~pair behind the last expert
+ *   offsets[e]     first row of expert e; offsets[n_experts] = rows with an expert
+ *   place[t][k]    the pair's row, or ~row (negative) where it has no expert
+ * The same expert twice for one token is two pairs.  n_experts is at most 1024.
+ * Nothing depends on the order in which workgroups run. */
+CX_API int cx_sort_tokens(cx_ctx* ctx, const int32_t* ids, int n_tokens, int top_k, int n_experts,
+                   int32_t* order, int32_t* offsets, int32_t* place, void* stream);
+
+/* xs[place[t][k]] = x[t] for rows of row_bytes bytes (of any type: 8-bit rows and
+ * their scales are two calls); rows without an expert are zeros.  With the places
+ * of cx_sort_tokens all n_tokens * top_k rows of xs are written.  A place outside
+ * them is skipped and reported by cx_ctx_sync.  Its gradient is cx_combine_rows
+ * without weights. */
+CX_API int cx_gather_rows(cx_ctx* ctx, const void* x, size_t row_bytes, const int32_t* place,
+                   int n_tokens, int top_k, void* xs, void* stream);
+
+/* out[t] = sum over k of weights[t][k] * ys[place[t][k]] + add[t], summed in fp32
+ * in that order and rounded once; pairs without an expert are left out, whatever
+ * their weight and row hold.  weights (ones) and add (of out's type) are nullable;
+ * out_f32 (nullable) receives the sum before its rounding.  out may be add itself.
+ * ys: [n_tokens * top_k, hidden] in 16 or 32 bits; top_k is at most 64. */
+CX_API int cx_combine_rows(cx_ctx* ctx, const void* ys, int ys_dtype, const int32_t* place,
+                    const float* weights, const void* add, int n_tokens, int top_k, int hidden,
+                    void* out, int out_dtype, float* out_f32, void* stream);
+
+/* The gradients of cx_combine_rows at ys and at weights:
+ *   dys[place[t][k]] = weights[t][k] * dout[t],  dw[t][k] = <dout[t], ys[place[t][k]]>
+ * zeros for pairs without an expert (the gradient at add is dout).  dys has ys's
+ * type; dw (nullable) is fp32, summed in fp32 in a fixed order. */
+CX_API int cx_combine_rows_grad(cx_ctx* ctx, const void* dout, int dout_dtype, const void* ys, int ys_dtype,
+                         const int32_t* place, const float* weights, int n_tokens, int top_k,
+                         int hidden, void* dys, float* dw, void* stream);
+
+/* ---- 4-bit weights ----------------------------------------------------------
+ * A stack of n_mats matrices [rows, cols] of e2m1 codes (0, 0.5, 1, 1.5, 2, 3, 4, 6
+ * and their negatives, sign in the top bit) with a bf16 scale per row and `group`
+ * columns (32, 64 or 128), packed into 16 x 128 tiles in the HBM arena.  An 8-bit
+ * power-of-two scale is a bf16 too.  gated: rows is even and the two halves are
+ * the gate and the up matrix of one product, silu(gate . x) * (up . x). */
+typedef struct cx_q4_desc {
+    const uint8_t* codes;
+    const uint16_t* scales;
+    int32_t n_mats, rows, cols, group, gated;
+    int32_t reserved[3]; /* zero */
+} cx_q4_desc;
+
+/* Packs device-resident row-major codes [n_mats, rows, ceil(cols / 2)] (the lower
+ * nibble is the even column; cols may be odd) and scales [n_mats, rows,
+ * ceil(cols / group)] into arena memory.  Runs on `stream` and waits for it. */
+CX_API int cx_q4_pack(int device, const uint8_t* codes, const uint16_t* scales, int n_mats, int rows,
+               int cols, int group, int gated, void* stream, cx_q4_desc* out);
+/* Frees a packed stack (after the device's work, as cx_free_device) and zeroes
+ * the descriptor. */
+CX_API int cx_q4_free(int device, cx_q4_desc* w);
+
+/* y = x W^T (gated: silu(x G^T) * (x U^T)), fp32 accumulation of exact products,
+ * rounded once.
+ * x: [*, cols] fp16, bf16, or e4m3 with x_scale [*, ceil(cols / 128)].
+ * y: [n_rows, rows] (gated: rows / 2) in fp16, bf16 or fp32.
+ * offsets NULL: one matrix (n_mats 1) for all rows.  Otherwise rows
+ * offsets[e] .. offsets[e + 1] - 1 go through matrix e (cx_sort_tokens' offsets,
+ * [n_mats + 1]) and the rows behind the last matrix's are zeros; offsets that
+ * decrease or leave the rows are cut and reported by cx_ctx_sync.
+ * order NULL: row p of y is row p of x.  Otherwise it is row order[p] / top_k
+ * (cx_sort_tokens' order: the gather needs no launch of its own); a row whose
+ * entry is negative or past n_x reads as zeros.
+ * scratch: cx_q4_scratch bytes of device memory, 16-byte aligned, of the caller's
+ * (only with offsets; NULL otherwise), in use until the call's work is done. */
+CX_API size_t cx_q4_scratch(const cx_q4_desc* w, int n_rows);
+CX_API int cx_q4_matmul(cx_ctx* ctx, const cx_q4_desc* w, const void* x, int x_dtype, const float* x_scale,
+                 int n_x, const int32_t* order, int top_k, const int32_t* offsets, int n_rows,
+                 void* y, int y_dtype, void* scratch, size_t scratch_bytes, void* stream);
+
+/* A layer of 4-bit experts on given routes, as cx_moe_decode / cx_moe_prefill do
+ * it for fp8 ones: same outputs, order of sums (route order, shared expert last)
+ * and route checks (a negative id is skipped; an id out of range, an expert listed
+ * twice for one token and a bad weight are skipped and reported by cx_ctx_sync).
+ * gate_up: gated [2 * inter, hidden] per expert; down: [hidden, inter] per expert;
+ * shared_gate_up / shared_down (nullable, together): the shared expert, stacks of
+ * one with the same sizes and groups.  Any n_tokens, 0 included.
+ * scratch: cx_q4_moe_scratch bytes of the caller's, as above; a captured graph
+ * keeps using the scratch it was captured with. */
+CX_API size_t cx_q4_moe_scratch(const cx_q4_desc* gate_up, const cx_q4_desc* down, int has_shared,
+                         int n_tokens, int top_k);
+CX_API int cx_q4_moe(cx_ctx* ctx, const cx_q4_desc* gate_up, const cx_q4_desc* down,
+              const cx_q4_desc* shared_gate_up, const cx_q4_desc* shared_down,
+              const void* x, int in_dtype, int n_tokens, const int32_t* topk_ids,
+              const float* topk_w, int top_k, void* y, int out_dtype, float* y_f32,
+              void* scratch, size_t scratch_bytes, void* stream);
 
 /* ---- whole-layer wire message ---------------------------------------------
  * MoeLayerRequest (msg_type 42) / MoeLayerResponse (43): one request per
