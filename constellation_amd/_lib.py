@@ -115,7 +115,7 @@ _SIGS = {
     "cx_combine_rows_grad": (_I, [_P, _P, _I, _P, _I, _P, _P, _I, _I, _I, _P, _P, _P]),
     "cx_q4_pack": (_I, [_I, _P, _P, _I, _I, _I, _I, _I, _P, C.POINTER(Q4Desc)]),
     "cx_q4_free": (_I, [_I, C.POINTER(Q4Desc)]),
-    "cx_q4_scratch": (C.c_size_t, [C.POINTER(Q4Desc), _I]),
+    "cx_q4_scratch": (C.c_size_t, [C.POINTER(Q4Desc), _I, _I, _I, _I]),
     "cx_q4_matmul": (_I, [_P, C.POINTER(Q4Desc), _P, _I, _P, _I, _P, _I, _P, _I, _P, _I, _P,
                           C.c_size_t, _P]),
     "cx_q4_moe_scratch": (C.c_size_t, [C.POINTER(Q4Desc), C.POINTER(Q4Desc), _I, _I, _I]),

@@ -4,8 +4,9 @@
 // 16 rows one after another.  Lane l of a wave holds the codes that an MFMA 16x16x32
 // takes from it in one 16-byte piece: row l % 16; dword j the columns 32 j + 8 (l / 16)
 // .. + 7, so that MFMA j covers the columns 32 j .. 32 j + 31, within one group of any
-// size, and a wave's load of a tile is one contiguous 1 KB.  The tile's scales, 16 rows x
-// 128 / group, are in the order of the accumulators: [l / 16][group][4 rows].
+// size, and a wave's load of a tile is one contiguous 1 KB.  The tile's scales are
+// fp16 [16 rows][128 / group], divided by a power of two per row that lies behind
+// them all as fp32 [n_mats][row tiles][16].
 // A `gated` matrix has 8 rows of its first half and the same 8 of its second half in
 // a tile, so that both factors of an output meet in one accumulator tile.
 #pragma once
@@ -19,6 +20,10 @@ constexpr int kQ4FewWaves = 8;
 
 __host__ __device__ inline int q4_row_tiles(const cx_q4_desc& w) { return w.gated ? (w.rows / 2 + 7) / 8 : (w.rows + 15) / 16; }
 __host__ __device__ inline int q4_col_tiles(const cx_q4_desc& w) { return (w.cols + 127) / 128; }
+
+__host__ __device__ inline const float* q4_row_scales(const cx_q4_desc& w) {
+    return reinterpret_cast<const float*>(w.scales + (size_t)w.n_mats * q4_row_tiles(w) * q4_col_tiles(w) * (128 / w.group) * 16);
+}
 
 // Eight codes -> eight bf16 / fp16, exact.
 __device__ __forceinline__ bf16x8 q4_bf16(uint32_t w) {
@@ -64,7 +69,9 @@ __device__ __forceinline__ u32x4 q4_x8(const void* row, int col, int cols, bool 
     }
 }
 
-__device__ __forceinline__ float q4_scale(uint32_t pair, int i) { return __uint_as_float(i & 1 ? pair & 0xFFFF0000u : pair << 16); }
+__device__ __forceinline__ float q4_scale(const uint32_t* sc, int i) {
+    return static_cast<float>(__builtin_bit_cast(f16x2, sc[i >> 1])[i & 1]);
+}
 
 __device__ __forceinline__ void q4_store(const Q4Launch& L, size_t at, float v) {
     if (L.y_type == CX_DTYPE_F32) {
@@ -127,7 +134,7 @@ __global__ __launch_bounds__(64 * kQ4FewWaves) void k_q4_few(Q4Launch L, int RT,
             if ((j + 1) % (4 / NG) == 0) {
                 const int g = j / (4 / NG);
 #pragma unroll
-                for (int i = 0; i < 4; ++i) acc[i] += q4_scale(sc[2 * g + (i >> 1)], i) * (XT == kQ4E4m3 ? xs * part[i] : part[i]);
+                for (int i = 0; i < 4; ++i) acc[i] += q4_scale(sc, i * NG + g) * (XT == kQ4E4m3 ? xs * part[i] : part[i]);
                 part = f32x4{};
             }
         }
@@ -139,6 +146,7 @@ __global__ __launch_bounds__(64 * kQ4FewWaves) void k_q4_few(Q4Launch L, int RT,
 #pragma unroll
     for (int i = 0; i < kQ4FewWaves; ++i) v += red[i][threadIdx.x];
     const int tt = threadIdx.x >> 4, r = threadIdx.x & 15;
+    v *= q4_row_scales(w)[tile0 / KT * 16 + (threadIdx.x & 15)];
     if (L.w.gated) {
         const float up = __shfl_down(v, 8);
         v = v / (1.0f + __expf(-v)) * up;

@@ -15,7 +15,8 @@ __device__ __forceinline__ int q4_src_row(const cx_q4_desc& w, int rt, int r) {
 }
 
 __global__ __launch_bounds__(256) void k_q4_pack(cx_q4_desc w, const uint8_t* codes, const uint16_t* scales,
-                                                 uint32_t* dst, uint16_t* dst_scale, int64_t tiles) {
+                                                 const float* row_scale, uint32_t* dst, uint16_t* dst_scale,
+                                                 int64_t tiles) {
     const int RT = q4_row_tiles(w), KT = q4_col_tiles(w), lane = threadIdx.x & 63;
     const int groups = (w.cols + w.group - 1) / w.group, NG = 128 / w.group;
     const int stride = (w.cols + 1) / 2, r = lane & 15, q = lane >> 4;
@@ -38,12 +39,67 @@ __global__ __launch_bounds__(256) void k_q4_pack(cx_q4_desc w, const uint8_t* co
             }
         }
         *reinterpret_cast<u32x4*>(dst + tile * 256 + lane * 4) = u32x4{d[0], d[1], d[2], d[3]};
-        if (lane < 16 * NG) {  // [quarter][group][4 rows]
-            const int i = lane & 3, g = (lane >> 2) % NG, n2 = q4_src_row(w, rt, (lane >> 2) / NG * 4 + i);
-            const int at = kt * NG + g;
-            dst_scale[tile * 16 * NG + lane] = n2 >= 0 && at < groups ? scales[(mat * w.rows + n2) * (int64_t)groups + at] : 0;
+        if (lane < 16 * NG) {  // [16 rows][group]
+            const int g = lane % NG, r2 = lane / NG, n2 = q4_src_row(w, rt, r2), at = kt * NG + g;
+            const float up = n2 >= 0 ? 1.0f / row_scale[(mat * RT + rt) * 16 + r2] : 1.0f;
+            const float s = n2 >= 0 && at < groups ? __uint_as_float((uint32_t)scales[(mat * w.rows + n2) * (int64_t)groups + at] << 16) : 0.0f;
+            dst_scale[tile * 16 * NG + lane] = (uint16_t)f16_rne(s * up);
         }
     }
+}
+
+// Per row the power of two that brings its largest scale to 2^11 .. 2^12: below it, a
+// code times a scale (2 and 8 significant bits) is exact in fp16 over 27 binades of
+// scales, and smaller ones are off by less than 2^-36 of the row's largest weight.
+// The powers run from 2^-126 to 2^116, whose reciprocals are normal numbers, too.
+__global__ __launch_bounds__(256) void k_q4_row_scales(cx_q4_desc w, const uint16_t* scales, float* row_scale, int64_t rows) {
+    const int RT = q4_row_tiles(w), lane = threadIdx.x & 63, groups = (w.cols + w.group - 1) / w.group;
+    for (int64_t i = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); i < rows; i += (int64_t)gridDim.x * 4) {
+        const int r = (int)(i & 15), rt = (int)(i / 16 % RT), n = q4_src_row(w, rt, r);
+        const uint16_t* src = scales + (i / 16 / RT * w.rows + n) * (int64_t)groups;
+        uint32_t most = 0;
+        for (int g = lane; n >= 0 && g < groups; g += 64) {
+            const uint32_t v = src[g] & 0x7FFFu;
+            if (v < 0x7F80u) most = max(most, v);  // infinities and NaN stay themselves
+        }
+#pragma unroll
+        for (int m = 32; m >= 1; m >>= 1) most = max(most, (uint32_t)__shfl_xor((int)most, m));
+        const int e = min(max((int)(most >> 7) - 11, 1), 243);
+        if (lane == 0) row_scale[i] = most == 0 ? 1.0f : __uint_as_float((uint32_t)e << 23);
+    }
+}
+
+// Rows of x as fp16 times a power of two per row, in rows of whole 128-column tiles,
+// zeros behind the row.  The row's largest value comes to 2^14 .. 2^15, so bf16
+// values (8 significant bits) are exact down to 2^-31 of it and the others off by less than
+// 2^-39 of it: nothing next to the sums' own 2^-24.  fp32 values are rounded to 11 bits.
+template <int DT>
+__global__ __launch_bounds__(256) void k_q4_rows(const void* x, int cols, int padded, uint16_t* dst, float* scale) {
+    __shared__ uint32_t part[4];
+    const int tid = threadIdx.x;
+    const size_t row = (size_t)blockIdx.x * cols;
+    auto value = [&](int c) {
+        if constexpr (DT == CX_DTYPE_F32)
+            return static_cast<const float*>(x)[row + c];
+        else if constexpr (DT == CX_DTYPE_BF16)
+            return __uint_as_float((uint32_t)static_cast<const uint16_t*>(x)[row + c] << 16);
+        else
+            return static_cast<float>(static_cast<const _Float16*>(x)[row + c]);
+    };
+    uint32_t most = 0;
+    for (int c = tid; c < cols; c += 256) {
+        const uint32_t b = __float_as_uint(value(c)) & 0x7FFFFFFFu;
+        if (b < 0x7F800000u) most = max(most, b);
+    }
+#pragma unroll
+    for (int m = 32; m >= 1; m >>= 1) most = max(most, (uint32_t)__shfl_xor((int)most, m));
+    if ((tid & 63) == 0) part[tid >> 6] = most;
+    __syncthreads();
+    most = max(max(part[0], part[1]), max(part[2], part[3]));
+    const int e = most == 0 ? 127 : min(max((int)(most >> 23) - 14, 1), 253);
+    const float up = __uint_as_float((uint32_t)(254 - e) << 23);
+    if (tid == 0) scale[blockIdx.x] = __uint_as_float((uint32_t)e << 23);
+    for (int c = tid; c < padded; c += 256) dst[(size_t)blockIdx.x * padded + c] = c < cols ? (uint16_t)f16_rne(value(c) * up) : 0;
 }
 
 // The runs of rows that `offsets` give each matrix, cut to item_rows.  Offsets that
@@ -84,14 +140,16 @@ __global__ __launch_bounds__(1024) void k_q4_items(const int32_t* offsets, int n
 
 size_t q4_code_bytes(const cx_q4_desc& w) { return (size_t)w.n_mats * q4_row_tiles(w) * q4_col_tiles(w) * kQ4Tile; }
 size_t q4_scale_bytes(const cx_q4_desc& w) {
-    return (size_t)w.n_mats * q4_row_tiles(w) * q4_col_tiles(w) * (128 / w.group) * 32;
+    return (size_t)w.n_mats * q4_row_tiles(w) * ((size_t)q4_col_tiles(w) * (128 / w.group) * 32 + 64);
 }
 
 hipError_t launch_q4_pack(const cx_q4_desc& w, const uint8_t* codes, const uint16_t* scales, hipStream_t s) {
-    const int64_t tiles = (int64_t)w.n_mats * q4_row_tiles(w) * q4_col_tiles(w);
-    const unsigned wgs = (unsigned)std::min<int64_t>((tiles + 3) / 4, 16384);
-    cx_launch(k_q4_pack, dim3(wgs), dim3(256), 0, s, w, codes, scales, reinterpret_cast<uint32_t*>(const_cast<uint8_t*>(w.codes)),
-              const_cast<uint16_t*>(w.scales), tiles);
+    const int64_t rows = (int64_t)w.n_mats * q4_row_tiles(w) * 16, tiles = rows / 16 * q4_col_tiles(w);
+    float* row_scale = const_cast<float*>(q4_row_scales(w));
+    auto wgs = [](int64_t units) { return dim3((unsigned)std::min<int64_t>((units + 3) / 4, 16384)); };
+    cx_launch(k_q4_row_scales, wgs(rows), dim3(256), 0, s, w, scales, row_scale, rows);
+    cx_launch(k_q4_pack, wgs(tiles), dim3(256), 0, s, w, codes, scales, row_scale,
+              reinterpret_cast<uint32_t*>(const_cast<uint8_t*>(w.codes)), const_cast<uint16_t*>(w.scales), tiles);
     return hipGetLastError();
 }
 
@@ -101,15 +159,12 @@ hipError_t launch_q4_items(const int32_t* offsets, int n_mats, int n_rows, int i
     return hipGetLastError();
 }
 
-int q4_item_rows(const cx_q4_desc& w, int n_rows, int n_mats) {
-    (void)w, (void)n_rows, (void)n_mats;
-    return kTileTok;
-}
-
 namespace {
 int64_t few_workgroups(const Q4Launch& L) {
     return (L.items != nullptr ? L.max_items : (L.n_rows + kTileTok - 1) / kTileTok) * q4_row_tiles(L.w);
 }
+
+size_t up256(size_t v) { return (v + 255) / 256 * 256; }
 
 template <int XT>
 hipError_t few_groups(const Q4Launch& L, hipStream_t s) {
@@ -120,9 +175,27 @@ hipError_t few_groups(const Q4Launch& L, hipStream_t s) {
 }
 }  // namespace
 
-bool q4_grid_ok(const Q4Launch& L) { return rows_grid_ok(few_workgroups(L), 64 * kQ4FewWaves); }
+bool q4_grid_ok(const Q4Launch& L) {
+    return rows_grid_ok(few_workgroups(L), 64 * kQ4FewWaves) && rows_grid_ok(L.n_x, 256) &&
+           (int64_t)L.n_x * q4_col_tiles(L.w) * 16 < ((int64_t)1 << 32);  // the GEMM's places in x, in 16 bytes
+}
+
+size_t q4_x_scratch(const cx_q4_desc& w, int n_x) { return up256((size_t)n_x * q4_col_tiles(w) * 256) + up256((size_t)n_x * 4); }
 
 hipError_t launch_q4(const Q4Launch& L, hipStream_t s) {
+    if (L.item_rows > kTileTok && L.x_type != kQ4E4m3) {
+        const int padded = q4_col_tiles(L.w) * 128;
+        Q4Launch G = L;
+        if (L.x_type != kQ4Fp16 || padded != L.w.cols || !dma_aligned(L.x)) {
+            uint16_t* x = static_cast<uint16_t*>(L.x_scratch);
+            float* scale = reinterpret_cast<float*>(static_cast<char*>(L.x_scratch) + up256((size_t)L.n_x * padded * 2));
+            auto k = L.x_type == kQ4Bf16 ? k_q4_rows<CX_DTYPE_BF16> : L.x_type == kQ4Fp16 ? k_q4_rows<CX_DTYPE_FP16> : k_q4_rows<CX_DTYPE_F32>;
+            if (L.n_x > 0) cx_launch(k, dim3((unsigned)L.n_x), dim3(256), 0, s, L.x, L.w.cols, padded, x, scale);
+            G.x = x;
+            G.x_scale = scale;
+        }
+        return launch_q4_gemm(G, s);
+    }
     switch (L.x_type) {
         case kQ4Bf16: return few_groups<kQ4Bf16>(L, s);
         case kQ4Fp16: return few_groups<kQ4Fp16>(L, s);

@@ -804,26 +804,46 @@ int check_q4(const cx_q4_desc* w) {
     return CX_OK;
 }
 
-// Scratch of cx_q4_moe, in this order.
+size_t align_up(size_t v) { return (v + 255) / 256 * 256; }
+
+// Scratch of cx_q4_matmul: the items, then x as the GEMM reads it.
+struct Q4Scratch {
+    int item_rows;
+    int64_t max_items;
+    size_t x, bytes;
+};
+
+Q4Scratch q4_scratch(const cx_q4_desc& w, int x_dtype, int n_x, int n_rows, bool with_offsets) {
+    Q4Scratch z{};
+    z.item_rows = x_dtype == CX_DTYPE_E4M3 ? kTileTok : q4_item_rows(n_rows, w.n_mats);
+    z.max_items = q4_max_items(n_rows, w.n_mats, z.item_rows);
+    z.x = with_offsets ? align_up(sizeof(Q4Item) * (size_t)z.max_items) : 0;
+    z.bytes = z.x + (z.item_rows > kTileTok ? q4_x_scratch(w, n_x) : 0);
+    return z;
+}
+
+// Scratch of cx_q4_moe.  h: two bf16 planes for the kernel of few rows, fp32 for the
+// GEMM.
 struct Q4MoeScratch {
     int64_t pairs, max_items;
     int item_rows;
-    size_t items, order, place, h, h_lo, ys, bytes;
+    size_t items, order, place, x, h, hx, ys, bytes;
 };
 
 Q4MoeScratch q4_moe_scratch(const cx_q4_desc& gu, const cx_q4_desc& down, int shared, int n_tokens, int top_k) {
     Q4MoeScratch z{};
-    auto up = [](size_t v) { return (v + 255) / 256 * 256; };
     z.pairs = (int64_t)n_tokens * (top_k + shared);
-    z.item_rows = q4_item_rows(gu, (int)std::min<int64_t>(z.pairs, INT32_MAX), gu.n_mats + shared);
+    z.item_rows = q4_item_rows(z.pairs, gu.n_mats + shared);
     z.max_items = q4_max_items(z.pairs, gu.n_mats + shared, z.item_rows);
+    const bool gemm = z.item_rows > kTileTok;
     z.items = 0;
-    z.order = z.items + up(sizeof(Q4Item) * (size_t)z.max_items);
-    z.place = z.order + up(4 * (size_t)z.pairs);
-    z.h = z.place + up(4 * (size_t)z.pairs);
-    z.h_lo = z.h + up(2 * (size_t)z.pairs * down.cols);
-    z.ys = z.h_lo + up(2 * (size_t)z.pairs * down.cols);
-    z.bytes = z.ys + up(4 * (size_t)z.pairs * down.rows);
+    z.order = z.items + align_up(sizeof(Q4Item) * (size_t)z.max_items);
+    z.place = z.order + align_up(4 * (size_t)z.pairs);
+    z.x = z.place + align_up(4 * (size_t)z.pairs);
+    z.h = z.x + (gemm ? q4_x_scratch(gu, n_tokens) : 0);
+    z.hx = z.h + align_up(4 * (size_t)z.pairs * down.cols);
+    z.ys = z.hx + (gemm ? q4_x_scratch(down, (int)z.pairs) : 0);
+    z.bytes = z.ys + align_up(4 * (size_t)z.pairs * down.rows);
     return z;
 }
 
@@ -1520,9 +1540,9 @@ int cx_q4_free(int device, cx_q4_desc* w) {
     return CX_OK;
 }
 
-size_t cx_q4_scratch(const cx_q4_desc* w, int n_rows) {
-    if (!w || w->n_mats < 1 || n_rows < 0) return 0;
-    return sizeof(Q4Item) * (size_t)q4_max_items(n_rows, w->n_mats, q4_item_rows(*w, n_rows, w->n_mats));
+size_t cx_q4_scratch(const cx_q4_desc* w, int x_dtype, int n_x, int n_rows, int with_offsets) {
+    if (!w || w->n_mats < 1 || n_x < 0 || n_rows < 0) return 0;
+    return q4_scratch(*w, x_dtype, n_x, n_rows, with_offsets != 0).bytes;
 }
 
 int cx_q4_matmul(cx_ctx* ctx, const cx_q4_desc* w, const void* x, int x_dtype, const float* x_scale, int n_x,
@@ -1539,8 +1559,9 @@ int cx_q4_matmul(cx_ctx* ctx, const cx_q4_desc* w, const void* x, int x_dtype, c
     if (!offsets && w->n_mats != 1) return fail(CX_EINVAL, "a stack of %d matrices needs offsets", w->n_mats);
     if (n_rows == 0) return CX_OK;
     if (!y || (n_x > 0 && (!x || (x_dtype == CX_DTYPE_E4M3 && !x_scale)))) return fail(CX_EINVAL, "NULL buffer");
-    if (offsets && (!scratch || scratch_bytes < cx_q4_scratch(w, n_rows) || reinterpret_cast<uintptr_t>(scratch) % 16))
-        return fail(CX_EINVAL, "scratch must be %zu bytes, 16-byte aligned", cx_q4_scratch(w, n_rows));
+    const Q4Scratch z = q4_scratch(*w, x_dtype, n_x, n_rows, offsets != nullptr);
+    if (z.bytes && (!scratch || scratch_bytes < z.bytes || reinterpret_cast<uintptr_t>(scratch) % 16))
+        return fail(CX_EINVAL, "scratch must be %zu bytes, 16-byte aligned", z.bytes);
     if ((rc = set_device(ctx->device))) return rc;
     hipStream_t s = static_cast<hipStream_t>(stream);
     Q4Launch L{};
@@ -1554,8 +1575,9 @@ int cx_q4_matmul(cx_ctx* ctx, const cx_q4_desc* w, const void* x, int x_dtype, c
     L.top_k = top_k;
     L.y = y;
     L.y_type = y_dtype;
-    L.item_rows = q4_item_rows(*w, n_rows, w->n_mats);
-    L.max_items = q4_max_items(n_rows, w->n_mats, L.item_rows);
+    L.item_rows = z.item_rows;
+    L.max_items = z.max_items;
+    L.x_scratch = static_cast<char*>(scratch) + z.x;
     if (!q4_grid_ok(L)) return fail(CX_EINVAL, "too many rows for one launch");
     if (offsets) {
         L.items = static_cast<const Q4Item*>(scratch);
@@ -1628,15 +1650,18 @@ int cx_q4_moe(cx_ctx* ctx, const cx_q4_desc* gate_up, const cx_q4_desc* down, co
     L.items = a.items;
     L.item_rows = z.item_rows;
     L.max_items = z.max_items;
+    const bool gemm = z.item_rows > kTileTok;
+    L.x_scratch = m + z.x;
     L.y = m + z.h;
-    L.y_lo = m + z.h_lo;
-    L.y_type = kQ4Planes;
+    L.y_lo = m + z.h + 2 * (size_t)z.pairs * down->cols;
+    L.y_type = gemm ? CX_DTYPE_F32 : kQ4Planes;
     Q4Launch D = L;
     D.w = *down;
     if (shared) D.shared = *shared_down;
     D.x = L.y;
     D.x_lo = L.y_lo;
-    D.x_type = kQ4Planes;
+    D.x_type = gemm ? kQ4F32 : kQ4Planes;
+    D.x_scratch = m + z.hx;
     D.n_x = (int)z.pairs;
     D.order = nullptr;
     D.y = m + z.ys;

@@ -506,11 +506,10 @@ class Context:
         x_scale = None if x_scale is None else x_scale.contiguous()
         out_dtype = out_dtype or (torch.bfloat16 if f8 else x.dtype)
         y = torch.empty((P, w.out_cols), dtype=out_dtype, device=x.device)
-        scratch, size = None, 0
-        if offsets is not None:
-            size = lib().cx_q4_scratch(C.byref(d), P)
-            scratch = torch.empty(size, dtype=torch.uint8, device=x.device)
-        check(lib().cx_q4_matmul(self.handle, C.byref(d), x.data_ptr(), E4M3 if f8 else cx_dtype(x.dtype),
+        dt = E4M3 if f8 else cx_dtype(x.dtype)
+        size = lib().cx_q4_scratch(C.byref(d), dt, T, P, int(offsets is not None))
+        scratch = torch.empty(size, dtype=torch.uint8, device=x.device) if size else None
+        check(lib().cx_q4_matmul(self.handle, C.byref(d), x.data_ptr(), dt,
                                  _ptr(x_scale), T, _ptr(order), top_k, _ptr(offsets), P, y.data_ptr(),
                                  cx_dtype(out_dtype), _ptr(scratch), size, self.stream()))
         return y

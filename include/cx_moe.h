@@ -373,8 +373,8 @@ CX_API int cx_q4_free(int device, cx_q4_desc* w);
  * (cx_sort_tokens' order: the gather needs no launch of its own); a row whose
  * entry is negative or past n_x reads as zeros.
  * scratch: cx_q4_scratch bytes of device memory, 16-byte aligned, of the caller's
- * (only with offsets; NULL otherwise), in use until the call's work is done. */
-CX_API size_t cx_q4_scratch(const cx_q4_desc* w, int n_rows);
+ * (NULL where that is 0), in use until the call's work is done. */
+CX_API size_t cx_q4_scratch(const cx_q4_desc* w, int x_dtype, int n_x, int n_rows, int with_offsets);
 CX_API int cx_q4_matmul(cx_ctx* ctx, const cx_q4_desc* w, const void* x, int x_dtype, const float* x_scale,
                  int n_x, const int32_t* order, int top_k, const int32_t* offsets, int n_rows,
                  void* y, int y_dtype, void* scratch, size_t scratch_bytes, void* stream);

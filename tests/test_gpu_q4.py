@@ -435,7 +435,7 @@ def test_refusals(gpu):
         refused(pack(E=1025), "bad 4-bit shape")
         refused(pack(N=31, gated=1), "even number of rows")
         refused(pack(c=None), "NULL buffer")
-        need = L.cx_q4_scratch(C.byref(w.desc), 4)
+        need = L.cx_q4_scratch(C.byref(w.desc), BF16, 4, 4, 1)
 
         def mm(desc=w.desc, dt=BF16, xs=None, n_x=4, off=i32.data_ptr(), order=None, P=4, odt=BF16, scr=buf.data_ptr(), sz=need, K=1):
             return L.cx_q4_matmul(gpu.handle, C.byref(desc) if desc is not None else None, x.data_ptr(), dt, xs, n_x, order, K, off, P,
