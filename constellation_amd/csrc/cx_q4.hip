@@ -102,6 +102,14 @@ __global__ __launch_bounds__(256) void k_q4_rows(const void* x, int cols, int pa
     for (int c = tid; c < padded; c += 256) dst[(size_t)blockIdx.x * padded + c] = c < cols ? (uint16_t)f16_rne(value(c) * up) : 0;
 }
 
+// Rows of e4m3 as fp16 (exact) in rows of whole 128-column tiles, zeros behind the row.
+__global__ __launch_bounds__(256) void k_q4_rows8(const uint8_t* x, int cols, int padded, uint16_t* dst) {
+    for (int c = threadIdx.x; c < padded; c += 256) {
+        const uint32_t v = c < cols ? x[(size_t)blockIdx.x * cols + c] : 0;
+        dst[(size_t)blockIdx.x * padded + c] = __builtin_bit_cast(uint16_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(v, 1.0f, false)[0]);
+    }
+}
+
 // The runs of rows that `offsets` give each matrix, cut to item_rows.  Offsets that
 // go back or past the rows are cut to what is there, so that no item leaves it.
 __global__ __launch_bounds__(1024) void k_q4_items(const int32_t* offsets, int n_mats, int n_rows, int item_rows,
@@ -183,10 +191,15 @@ bool q4_grid_ok(const Q4Launch& L) {
 size_t q4_x_scratch(const cx_q4_desc& w, int n_x) { return up256((size_t)n_x * q4_col_tiles(w) * 256) + up256((size_t)n_x * 4); }
 
 hipError_t launch_q4(const Q4Launch& L, hipStream_t s) {
-    if (L.item_rows > kTileTok && L.x_type != kQ4E4m3) {
+    if (L.item_rows > kTileTok) {
         const int padded = q4_col_tiles(L.w) * 128;
         Q4Launch G = L;
-        if (L.x_type != kQ4Fp16 || padded != L.w.cols || !dma_aligned(L.x)) {
+        if (L.x_type == kQ4E4m3) {
+            if (L.n_x > 0)
+                cx_launch(k_q4_rows8, dim3((unsigned)L.n_x), dim3(256), 0, s, static_cast<const uint8_t*>(L.x), L.w.cols, padded,
+                          static_cast<uint16_t*>(L.x_scratch));
+            G.x = L.x_scratch;
+        } else if (L.x_type != kQ4Fp16 || padded != L.w.cols || !dma_aligned(L.x)) {
             uint16_t* x = static_cast<uint16_t*>(L.x_scratch);
             float* scale = reinterpret_cast<float*>(static_cast<char*>(L.x_scratch) + up256((size_t)L.n_x * padded * 2));
             auto k = L.x_type == kQ4Bf16 ? k_q4_rows<CX_DTYPE_BF16> : L.x_type == kQ4Fp16 ? k_q4_rows<CX_DTYPE_FP16> : k_q4_rows<CX_DTYPE_F32>;

@@ -13,12 +13,14 @@ struct Q4GemmArgs {
     cx_q4_desc w, shared;
     const uint16_t* x;        // [n_x, padded]
     const float* x_row_scale; // nullable [n_x]
+    const float* x_scale;     // XS: [n_x, KT]
     int padded;               // columns of a row of x: KT * 128
     int n_x, n_rows, top_k;
     const int32_t* order;
     const Q4Item* items;
     void* y;
     int y_type;
+    int item_rows;
     int RT, KT, RB;           // row tiles, column tiles, row blocks
 };
 
@@ -39,7 +41,92 @@ __device__ __forceinline__ void q4_gemm_turn() {
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
 }
 
-template <int NG, int RTW, int NT>
+// The accumulators, times the rows' powers of two, to y.  A wave turns 16 rows of x at a
+// time in its own part of the LDS, so that it stores whole lines of y (as they lie in
+// the accumulators, a lane has 4 neighbours of one row: 8 bytes in 16 bits).
+template <int RTW, int NT>
+__device__ __forceinline__ void q4_gemm_store(const Q4GemmArgs& L, const f32x4 (&acc)[NT][RTW], unsigned char* lds, const cx_q4_desc& w,
+                                              size_t mat, int rb, int begin, int rows) {
+    constexpr int kPitch = RTW * 16 + 4;  // floats; 16 rows' pieces then lie in different banks
+    static_assert(16 * kPitch * 4 * kQ4GemmWaves <= kQ4GemmBuf, "turned tiles");
+    const int wave = wave_id(), lane = threadIdx.x & 63, t = lane & 15, q = lane >> 4;
+    float* turn = reinterpret_cast<float*>(lds) + wave * 16 * kPitch;
+    const int rt0 = (rb * kQ4GemmWaves + wave) * RTW;
+    const int width = w.gated ? w.rows / 2 : w.rows;
+    const int c0 = rt0 * (w.gated ? 8 : 16), cols = RTW * (w.gated ? 8 : 16);  // of this wave
+    const bool wide = L.y_type == CX_DTYPE_F32;
+    const bool vec = width % (wide ? 4 : 8) == 0 && (reinterpret_cast<uintptr_t>(L.y) & 15) == 0;
+    const int per = wide ? 4 : 8, lanes = cols / per;  // columns of a lane's store, lanes of a row
+    f32x4 rs[RTW];
+#pragma unroll
+    for (int m = 0; m < RTW; ++m)
+        rs[m] = *reinterpret_cast<const f32x4*>(q4_row_scales(w) + (mat * L.RT + min(rt0 + m, L.RT - 1)) * 16 + 4 * q);
+    // rows n * 16 + t: whether they exist in x (rows of the order without a pair are zeros) and their power of two
+    float xs[NT];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+        const int r = n * 16 + t, p = begin + r;
+        xs[n] = 1.0f;
+        if (r < rows && (L.order != nullptr || L.x_row_scale != nullptr)) {
+            const int pair = L.order != nullptr ? L.order[p] : p * L.top_k, xr = pair / L.top_k;
+            if (pair < 0 || xr >= L.n_x)
+                xs[n] = 0.0f;
+            else if (L.x_row_scale != nullptr)
+                xs[n] = L.x_row_scale[xr];
+        }
+    }
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+        if (n * 16 >= rows) continue;
+#pragma unroll
+        for (int m = 0; m < RTW; ++m) {
+            f32x4 v = acc[n][m] * rs[m];
+            v = xs[n] == 0.0f ? f32x4{} : v * f32x4{xs[n], xs[n], xs[n], xs[n]};
+            int c = m * 16 + 4 * q;
+            if (w.gated) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const float up = __shfl_xor(v[i], 32);
+                    v[i] = v[i] / (1.0f + __expf(-v[i])) * up;
+                }
+                c = m * 8 + 4 * (q & 1);
+            }
+            if (!w.gated || q < 2) *reinterpret_cast<f32x4*>(turn + t * kPitch + c) = v;
+        }
+        __builtin_amdgcn_wave_barrier();
+        for (int i = lane; i < 16 * lanes; i += 64) {
+            const int r = i / lanes, c = (i - r * lanes) * per, left = width - c0 - c;
+            if (n * 16 + r >= rows || left <= 0) continue;
+            const float* src = turn + r * kPitch + c;
+            const size_t at = (size_t)(begin + n * 16 + r) * width + c0 + c;
+            if (wide) {
+                const f32x4 v = *reinterpret_cast<const f32x4*>(src);
+                float* y = static_cast<float*>(L.y) + at;
+                if (vec) {
+                    *reinterpret_cast<f32x4*>(y) = v;
+                } else {
+                    for (int k = 0; k < min(left, 4); ++k) y[k] = src[k];
+                }
+            } else {
+                uint16_t* y = static_cast<uint16_t*>(L.y) + at;
+                if (vec) {
+                    const f32x4 a = *reinterpret_cast<const f32x4*>(src), b = *reinterpret_cast<const f32x4*>(src + 4);
+                    *reinterpret_cast<u32x4*>(y) = u32x4{cast_out(a[0], L.y_type) | (cast_out(a[1], L.y_type) << 16), cast_out(a[2], L.y_type) | (cast_out(a[3], L.y_type) << 16),
+                                                         cast_out(b[0], L.y_type) | (cast_out(b[1], L.y_type) << 16), cast_out(b[2], L.y_type) | (cast_out(b[3], L.y_type) << 16)};
+                } else {
+                    for (int k = 0; k < min(left, 8); ++k) y[k] = (uint16_t)cast_out(src[k], L.y_type);
+                }
+            }
+        }
+        __builtin_amdgcn_wave_barrier();
+    }
+}
+
+// XS (e4m3 rows of x, as fp16): each column tile's sums are scaled by the row's x_scale in
+// fp32 before they are added up, with items of up to 64 rows for the second set of sums.
+// The matrix cores' own 8-bit products would be twice as fast, but drop what lies 2^13
+// below the largest product of an instruction, and sums here are kept to fp32.
+template <int NG, int RTW, int NT, bool XS>
 __device__ __forceinline__ void q4_gemm_tile(const Q4GemmArgs& L, unsigned char* lds0, unsigned char* lds1, const cx_q4_desc& w,
                                              size_t mat, int rb, int begin, int rows) {
     const int wave = wave_id(), lane = threadIdx.x & 63, t = lane & 15, q = lane >> 4;
@@ -62,15 +149,25 @@ __device__ __forceinline__ void q4_gemm_tile(const Q4GemmArgs& L, unsigned char*
     for (int m = 0; m < RTW; ++m) {
         const int rt = min((rb * kQ4GemmWaves + wave) * RTW + m, L.RT - 1);
         const size_t tile = (mat * L.RT + rt) * (size_t)KT;
-        wp[m] = w.codes + tile * kQ4Tile + lane * 16;
-        sp[m] = w.scales + tile * 16 * NG + t * NG;
+        wp[m] = w.codes + tile * kQ4Tile;
+        sp[m] = w.scales + tile * 16 * NG;
     }
     struct Sc {  // the lane's row's scales of a tile
         uint32_t d[(NG + 1) / 2];
     };
-    f32x4 acc[NT][RTW] = {};
+    f32x4 acc[NT][RTW] = {}, sum[XS ? NT : 1][RTW] = {};
     u32x4 a[2][RTW];
     Sc s[2][RTW];
+    const float* xsp[XS ? NT : 1];
+    float xs[2][XS ? NT : 1];
+    if constexpr (XS) {
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+            int xr = begin + (n * 16 + t < rows ? n * 16 + t : 0);
+            if (L.order != nullptr) xr = max(L.order[xr], 0) / L.top_k;
+            xsp[n] = L.x_scale + (size_t)(xr < L.n_x ? xr : 0) * KT;
+        }
+    }
     auto fetch = [&](int kt, auto to, unsigned char* buf) {
 #pragma unroll
         for (int i = 0; i < NT; ++i)
@@ -78,12 +175,15 @@ __device__ __forceinline__ void q4_gemm_tile(const Q4GemmArgs& L, unsigned char*
                                              (__attribute__((address_space(3))) void*)(buf + i * 4096 + wave * 1024), 16, 0, 0);
 #pragma unroll
         for (int m = 0; m < RTW; ++m) {
-            a[to][m] = ld16(wp[m] + (size_t)kt * kQ4Tile);
+            a[to][m] = ld16(wp[m] + (size_t)kt * kQ4Tile + (uint32_t)lane * 16);
             if constexpr (NG == 1)
-                s[to][m].d[0] = sp[m][kt * 16];
+                s[to][m].d[0] = (sp[m] + (size_t)kt * 16)[(uint32_t)t];
             else
-                s[to][m] = *reinterpret_cast<const Sc*>(sp[m] + kt * 16 * NG);
+                s[to][m] = *reinterpret_cast<const Sc*>(sp[m] + (size_t)kt * 16 * NG + (uint32_t)t * NG);
         }
+        if constexpr (XS)
+#pragma unroll
+            for (int n = 0; n < NT; ++n) xs[to][n] = xsp[n][kt];
     };
     auto multiply = [&](auto from, const unsigned char* buf) {
         // Steps of RTW MFMAs on one fragment of x, in this order: the fragment after the
@@ -111,9 +211,24 @@ __device__ __forceinline__ void q4_gemm_tile(const Q4GemmArgs& L, unsigned char*
 #pragma unroll
                 for (int m = n * RTW / NT; m < (n + 1) * RTW / NT; ++m) convert(j + 1, m);
 #pragma unroll
-            for (int m = 0; m < RTW; ++m) acc[n][m] = Mma<true>::mma(fa[j & 1][m], Mma<true>::bits(b[i % 3]), acc[n][m]);
+            for (int m = 0; m < RTW; ++m)
+                acc[n][m] = Mma<true>::mma(fa[j & 1][m], Mma<true>::bits(b[i % 3]), XS && j == 0 ? f32x4{} : acc[n][m]);
         }
         __builtin_amdgcn_sched_barrier(0);
+        if constexpr (!XS)
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int m = 0; m < RTW; ++m) asm volatile("" : "+v"(acc[n][m]));  // keeps the sums where they are: no copies of them at the loop's end
+        if constexpr (XS)
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int m = 0; m < RTW; ++m) {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) sum[n][m][i] = __builtin_fmaf(xs[from][n], acc[n][m][i], sum[n][m][i]);
+                    asm volatile("" : "+v"(sum[n][m]));  // keeps the sums where they are: no copies of them at the loop's end
+                }
     };
     constexpr std::integral_constant<int, 0> even{};
     constexpr std::integral_constant<int, 1> odd{};
@@ -128,53 +243,17 @@ __device__ __forceinline__ void q4_gemm_tile(const Q4GemmArgs& L, unsigned char*
         multiply(odd, lds1);
         q4_gemm_turn();
     }
-    const int width = w.gated ? w.rows / 2 : w.rows;
-    const float* rs = q4_row_scales(w) + mat * L.RT * 16;
-#pragma unroll
-    for (int n = 0; n < NT; ++n) {
-        const int r = n * 16 + t, p = begin + r;
-        float xs = 1.0f;
-        bool none = false;  // a row of the order without a pair: zeros
-        if (r < rows && (L.order != nullptr || L.x_row_scale != nullptr)) {
-            const int pair = L.order != nullptr ? L.order[p] : p * L.top_k, xr = pair / L.top_k;
-            none = pair < 0 || xr >= L.n_x;
-            if (!none && L.x_row_scale != nullptr) xs = L.x_row_scale[xr];
-        }
-#pragma unroll
-        for (int m = 0; m < RTW; ++m) {
-            const int rt = (rb * kQ4GemmWaves + wave) * RTW + m;
-            f32x4 v = acc[n][m];
-            if (rt < L.RT) v *= *reinterpret_cast<const f32x4*>(rs + rt * 16 + 4 * q);
-            v = none ? f32x4{} : v * f32x4{xs, xs, xs, xs};
-            int c = rt * 16 + 4 * q;
-            bool mine = rt < L.RT && r < rows;
-            if (w.gated) {
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const float up = __shfl_xor(v[i], 32);
-                    v[i] = v[i] / (1.0f + __expf(-v[i])) * up;
-                }
-                c = rt * 8 + 4 * q;
-                mine = mine && q < 2;
-            }
-            const size_t at = (size_t)p * width + c;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                if (!mine || c + i >= width) continue;
-                if (L.y_type == CX_DTYPE_F32)
-                    static_cast<float*>(L.y)[at + i] = v[i];
-                else
-                    static_cast<uint16_t*>(L.y)[at + i] = (uint16_t)cast_out(v[i], L.y_type);
-            }
-        }
-    }
+    if constexpr (XS)
+        q4_gemm_store<RTW, NT>(L, sum, lds0, w, mat, rb, begin, rows);
+    else
+        q4_gemm_store<RTW, NT>(L, acc, lds0, w, mat, rb, begin, rows);
 }
 
-template <int NG, int RTW>
+template <int NG, int RTW, bool XS>
 __global__ __launch_bounds__(64 * kQ4GemmWaves, 2) void k_q4_gemm(Q4GemmArgs L) {
     __shared__ __attribute__((aligned(16))) unsigned char lds0[kQ4GemmBuf], lds1[kQ4GemmBuf];
     const int idx = blockIdx.x / L.RB, rb = blockIdx.x - idx * L.RB;
-    int expert = 0, begin = idx * kQ4GemmRows, rows = min(kQ4GemmRows, L.n_rows - begin);
+    int expert = 0, begin = idx * L.item_rows, rows = min(L.item_rows, L.n_rows - begin);
     if (L.items != nullptr) {
         if (idx >= L.items[0].expert) return;
         const Q4Item it = ld_uniform(L.items + 1 + idx);
@@ -193,14 +272,21 @@ __global__ __launch_bounds__(64 * kQ4GemmWaves, 2) void k_q4_gemm(Q4GemmArgs L) 
     const bool other = expert == L.w.n_mats;
     const cx_q4_desc& w = other ? L.shared : L.w;
     const size_t mat = other ? 0 : (size_t)expert;
-    if (rows > 96)
-        q4_gemm_tile<NG, RTW, 8>(L, lds0, lds1, w, mat, rb, begin, rows);
-    else if (rows > 64)
-        q4_gemm_tile<NG, RTW, 6>(L, lds0, lds1, w, mat, rb, begin, rows);
+    auto tile = [&](auto nt) {
+        q4_gemm_tile<NG, RTW, nt, XS>(L, lds0, lds1, w, mat, rb, begin, rows);
+    };
+    if constexpr (!XS) {
+        if (rows > 112) return tile(std::integral_constant<int, 8>{});
+        if (rows > 96) return tile(std::integral_constant<int, 7>{});
+        if (rows > 80) return tile(std::integral_constant<int, 6>{});
+        if (rows > 64) return tile(std::integral_constant<int, 5>{});
+    }
+    if (rows > 48)
+        tile(std::integral_constant<int, 4>{});
     else if (rows > 32)
-        q4_gemm_tile<NG, RTW, 4>(L, lds0, lds1, w, mat, rb, begin, rows);
+        tile(std::integral_constant<int, 3>{});
     else
-        q4_gemm_tile<NG, RTW, 2>(L, lds0, lds1, w, mat, rb, begin, rows);
+        tile(std::integral_constant<int, 2>{});
 }
 
 }  // namespace cx

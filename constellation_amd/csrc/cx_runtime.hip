@@ -815,7 +815,7 @@ struct Q4Scratch {
 
 Q4Scratch q4_scratch(const cx_q4_desc& w, int x_dtype, int n_x, int n_rows, bool with_offsets) {
     Q4Scratch z{};
-    z.item_rows = x_dtype == CX_DTYPE_E4M3 ? kTileTok : q4_item_rows(n_rows, w.n_mats);
+    z.item_rows = q4_item_rows(n_rows, w.n_mats, x_dtype == CX_DTYPE_E4M3);
     z.max_items = q4_max_items(n_rows, w.n_mats, z.item_rows);
     z.x = with_offsets ? align_up(sizeof(Q4Item) * (size_t)z.max_items) : 0;
     z.bytes = z.x + (z.item_rows > kTileTok ? q4_x_scratch(w, n_x) : 0);
@@ -833,7 +833,7 @@ struct Q4MoeScratch {
 Q4MoeScratch q4_moe_scratch(const cx_q4_desc& gu, const cx_q4_desc& down, int shared, int n_tokens, int top_k) {
     Q4MoeScratch z{};
     z.pairs = (int64_t)n_tokens * (top_k + shared);
-    z.item_rows = q4_item_rows(z.pairs, gu.n_mats + shared);
+    z.item_rows = q4_item_rows(z.pairs, gu.n_mats + shared, false);
     z.max_items = q4_max_items(z.pairs, gu.n_mats + shared, z.item_rows);
     const bool gemm = z.item_rows > kTileTok;
     z.items = 0;

@@ -273,9 +273,11 @@ constexpr int kRowThreads = 256;       // workgroup of the gather and combine ke
 inline bool rows_grid_ok(int64_t workgroups, int threads) { return workgroups * threads < ((int64_t)1 << 32); }
 
 // Rows of x per work item: 16 for the kernel of few rows, which streams a matrix's weights
-// once per item, else up to 128 for the GEMM.
+// once per item, else up to 128 for the GEMM (64 where it keeps a second set of sums).
 constexpr int kQ4GemmRows = 128;
-inline int q4_item_rows(int64_t n_rows, int n_mats) { return n_rows > (int64_t)kTileTok * n_mats ? kQ4GemmRows : kTileTok; }
+inline int q4_item_rows(int64_t n_rows, int n_mats, bool two_sums) {
+    return n_rows <= (int64_t)kTileTok * n_mats ? kTileTok : two_sums ? kQ4GemmRows / 2 : kQ4GemmRows;
+}
 
 // Items of up to item_rows rows over n_mats matrices, entry 0 (the head) included: at
 // most one short item per matrix that has rows, and one of rows without a matrix.
