@@ -34,6 +34,7 @@ SOURCES = {
     "cx_few.hip": [],
     "cx_pp.hip": [],
     "cx_q4.hip": [],
+    "cx_q4_dec.hip": [],
     "cx_q4_gemm.hip": [],
     "cx_route.hip": [],
     "cx_rows.hip": [],

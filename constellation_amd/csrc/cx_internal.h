@@ -380,12 +380,11 @@ hipError_t launch_combine_grad(const CombineGradArgs& a, hipStream_t s);
 
 // ---------------------------------------------------------------------------
 // 4-bit products (cx_q4.hip).
-enum { kQ4Bf16 = 1, kQ4Fp16 = 2, kQ4F32 = 3, kQ4E4m3 = 4, kQ4Planes = 5 };  // x and y; planes: bf16 hi + lo
+enum { kQ4Bf16 = 1, kQ4Fp16 = 2, kQ4F32 = 3, kQ4E4m3 = 4 };  // types of x
 struct Q4Launch {
     cx_q4_desc w;
     cx_q4_desc shared;       // matrix of items with expert == w.n_mats (codes NULL: none)
     const void* x;           // [*, cols]
-    const void* x_lo;        // planes
     const float* x_scale;    // e4m3: [*, ceil(cols / 128)]
     int x_type;
     int n_x;                 // rows of x
@@ -396,8 +395,7 @@ struct Q4Launch {
     int item_rows;           // rows of an item, at most
     int64_t max_items;       // of the list, its head included
     void* y;                 // [n_rows, rows] ([n_rows, rows / 2] gated)
-    void* y_lo;
-    int y_type;              // CX_DTYPE_* or kQ4Planes
+    int y_type;              // CX_DTYPE_*
     void* x_scratch;         // q4_x_scratch bytes
 };
 size_t q4_code_bytes(const cx_q4_desc& w);
@@ -406,6 +404,7 @@ hipError_t launch_q4_pack(const cx_q4_desc& w, const uint8_t* codes, const uint1
 hipError_t launch_q4_items(const int32_t* offsets, int n_mats, int n_rows, int item_rows, Q4Item* items, int* err_flag,
                            hipStream_t s);
 size_t q4_x_scratch(const cx_q4_desc& w, int n_x);  // of products with items of more than 16 rows
+hipError_t launch_q4_dec(const Q4Launch& L, int splits, int64_t items, hipStream_t s);
 hipError_t launch_q4_gemm(const Q4Launch& L, hipStream_t s);
 bool q4_grid_ok(const Q4Launch& L);
 hipError_t launch_q4(const Q4Launch& L, hipStream_t s);

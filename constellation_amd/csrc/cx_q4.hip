@@ -168,29 +168,48 @@ hipError_t launch_q4_items(const int32_t* offsets, int n_mats, int n_rows, int i
 }
 
 namespace {
-int64_t few_workgroups(const Q4Launch& L) {
-    return (L.items != nullptr ? L.max_items : (L.n_rows + kTileTok - 1) / kTileTok) * q4_row_tiles(L.w);
-}
 
 size_t up256(size_t v) { return (v + 255) / 256 * 256; }
 
-template <int XT>
-hipError_t few_groups(const Q4Launch& L, hipStream_t s) {
-    const int RT = q4_row_tiles(L.w);
-    auto k = L.w.group == 128 ? k_q4_few<XT, 1> : L.w.group == 64 ? k_q4_few<XT, 2> : k_q4_few<XT, 4>;
-    cx_launch(k, dim3((unsigned)few_workgroups(L)), dim3(64 * kQ4FewWaves), 0, s, L, RT, q4_col_tiles(L.w));
+// Ranges of the columns per row tile: enough waves for 16 a CU, of at least 4 column tiles.
+int column_splits(int64_t waves, int KT, int most) {
+    int n = 1;
+    while (n < most && waves * n < 4096 && KT / n >= 4) n *= 2;
+    return n;
+}
+
+// The matrices that have rows, at most.
+int64_t busy_mats(const Q4Launch& L) { return L.items != nullptr ? std::min(L.n_rows, L.w.n_mats) : (L.n_rows + L.item_rows - 1) / L.item_rows; }
+int64_t item_bound(const Q4Launch& L) { return L.items != nullptr ? L.max_items : (L.n_rows + L.item_rows - 1) / L.item_rows; }
+
+template <int XT, int NG>
+hipError_t few_launch(const Q4Launch& L, hipStream_t s) {
+    const int RT = q4_row_tiles(L.w), KT = q4_col_tiles(L.w), el = L.x_type == kQ4E4m3 ? 1 : 2;
+    const int64_t busy = busy_mats(L);
+    const bool vec = L.w.cols % 8 == 0 && (reinterpret_cast<uintptr_t>(L.x) & (8 * el - 1)) == 0 && (int64_t)L.n_x * L.w.cols * el < (int64_t)kOob;
+    const int rw = L.n_rows > 4 * busy ? 2 : 1, splits = column_splits(busy * ((RT + rw - 1) / rw), KT, kQ4FewWaves);
+    const int per = kQ4FewWaves / splits * rw, row_blocks = (RT + per - 1) / per;
+    auto k = vec ? (rw == 2 ? k_q4_few<XT, NG, 2, true> : k_q4_few<XT, NG, 1, true>) : (rw == 2 ? k_q4_few<XT, NG, 2, false> : k_q4_few<XT, NG, 1, false>);
+    cx_launch(k, dim3((unsigned)(item_bound(L) * row_blocks)), dim3(64 * kQ4FewWaves), 0, s, L, RT, KT, splits, row_blocks);
     return hipGetLastError();
 }
+
+template <int XT>
+hipError_t few_groups(const Q4Launch& L, hipStream_t s) {
+    return L.w.group == 128 ? few_launch<XT, 1>(L, s) : L.w.group == 64 ? few_launch<XT, 2>(L, s) : few_launch<XT, 4>(L, s);
+}
+
 }  // namespace
 
 bool q4_grid_ok(const Q4Launch& L) {
-    return rows_grid_ok(few_workgroups(L), 64 * kQ4FewWaves) && rows_grid_ok(L.n_x, 256) &&
+    return rows_grid_ok(item_bound(L) * q4_row_tiles(L.w), 64 * kQ4FewWaves) && rows_grid_ok(L.n_x, 256) &&
            (int64_t)L.n_x * q4_col_tiles(L.w) * 16 < ((int64_t)1 << 32);  // the GEMM's places in x, in 16 bytes
 }
 
 size_t q4_x_scratch(const cx_q4_desc& w, int n_x) { return up256((size_t)n_x * q4_col_tiles(w) * 256) + up256((size_t)n_x * 4); }
 
 hipError_t launch_q4(const Q4Launch& L, hipStream_t s) {
+    if (L.item_rows < kTileTok) return launch_q4_dec(L, column_splits(busy_mats(L) * q4_row_tiles(L.w), q4_col_tiles(L.w), kQ4DecWaves), item_bound(L), s);
     if (L.item_rows > kTileTok) {
         const int padded = q4_col_tiles(L.w) * 128;
         Q4Launch G = L;
@@ -212,8 +231,7 @@ hipError_t launch_q4(const Q4Launch& L, hipStream_t s) {
     switch (L.x_type) {
         case kQ4Bf16: return few_groups<kQ4Bf16>(L, s);
         case kQ4Fp16: return few_groups<kQ4Fp16>(L, s);
-        case kQ4E4m3: return few_groups<kQ4E4m3>(L, s);
-        default: return few_groups<kQ4Planes>(L, s);
+        default: return few_groups<kQ4E4m3>(L, s);
     }
 }
 

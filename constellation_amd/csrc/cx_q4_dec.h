@@ -1,0 +1,218 @@
+// cx_q4_dec.h — products with 4-bit weights for up to four rows of x per item: decode.
+#pragma once
+
+#include "cx_q4.h"
+
+namespace cx {
+
+struct Q4DecArgs {
+    Q4Launch L;
+    int RT, KT;
+    int splits;      // ranges of the columns per row tile
+    int row_blocks;  // workgroups per item
+    int lds_rows;    // rows of x staged, at most 4
+};
+
+// A wave takes one row tile and one range of the column tiles; the partial sums of the ranges
+// are added in order.  HBM bounds it as long as enough bytes are in flight: a wave's ring holds U
+// tiles of codes (1 KB each) and refills a place as soon as it has multiplied it.
+//
+// x is staged once per workgroup as fp16 in LDS: fp16 and e4m3 values as they are, others
+// times the power of two that brings the row's largest value to 2^14 .. 2^15 (bf16 is then
+// exact down to 2^-31 of it; fp32, the h of an expert, is rounded to 11 bits).  The codes
+// times their scales are exact in fp16 (k_q4_row_scales), so the MFMAs sum exact products.
+template <int XT, int NG, int U>
+__global__ __launch_bounds__(64 * kQ4DecWaves) void k_q4_dec(Q4DecArgs A) {
+    constexpr bool kScaled = XT == kQ4E4m3;  // a scale per row and column tile
+    const Q4Launch& L = A.L;
+    __shared__ float row_up[4];
+    __shared__ uint32_t tops[4][kQ4DecWaves];
+    extern __shared__ __attribute__((aligned(16))) unsigned char staged[];
+    const int RT = A.RT, KT = A.KT, idx = blockIdx.x / A.row_blocks, block = blockIdx.x - idx * A.row_blocks;
+    const int wave = wave_id(), lane = threadIdx.x & 63, t = lane & 15, q = lane >> 4, tid = threadIdx.x;
+    const int groups = kQ4DecWaves / A.splits, rg = wave / A.splits, ks = wave - rg * A.splits;
+    int expert = 0, begin = idx * L.item_rows, np = min(L.item_rows, L.n_rows - begin);
+    if (L.items != nullptr) {
+        if (idx >= L.items[0].expert) return;
+        const Q4Item it = ld_uniform(L.items + 1 + idx);
+        expert = it.expert;
+        begin = it.begin;
+        np = it.rows;
+    }
+    const bool other = expert == L.w.n_mats;
+    const cx_q4_desc& w = other ? L.shared : L.w;
+    const size_t mat = other ? 0 : (size_t)max(expert, 0);
+    const int cols = L.w.cols, pitch = KT * 256 + kQ4LdsPad, rt = block * groups + rg;
+    float* xs_lds = reinterpret_cast<float*>(staged + A.lds_rows * pitch);  // kScaled: [lds_rows][KT]
+
+    // ---- the ring: bounded loads, so that places past the range read as zeros and cost nothing
+    const size_t tile0 = (mat * RT + min(rt, RT - 1)) * (size_t)KT;
+    const int per = (KT + A.splits - 1) / A.splits, k0 = ks * per, k1 = expert < 0 || rt >= RT ? k0 : min(KT, k0 + per);
+    const __amdgpu_buffer_rsrc_t rw = make_rsrc(w.codes + tile0 * kQ4Tile, (uint32_t)max(k1, 0) * kQ4Tile);
+    const __amdgpu_buffer_rsrc_t rs = make_rsrc(w.scales + tile0 * 16 * NG, (uint32_t)max(k1, 0) * 32 * NG);
+    u32x4 a[U];
+    uint32_t s[U][(NG + 1) / 2];
+    auto fetch = [&](int kt, int u) {
+        a[u] = bld16(rw, (uint32_t)kt * kQ4Tile + (uint32_t)lane * 16);
+        const uint32_t at = (uint32_t)kt * 32 * NG + (uint32_t)t * 2 * NG;
+        if constexpr (NG == 1) {
+            s[u][0] = __builtin_amdgcn_raw_buffer_load_b16(rs, at, 0, 0);
+        } else if constexpr (NG == 2) {
+            s[u][0] = __builtin_amdgcn_raw_buffer_load_b32(rs, at, 0, 0);
+        } else {
+            typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+            const u32x2 v = __builtin_bit_cast(u32x2, __builtin_amdgcn_raw_buffer_load_b64(rs, at, 0, 0));
+            s[u][0] = v[0], s[u][1] = v[1];
+        }
+    };
+
+    // ---- x: loads first, so that waiting for them does not wait for the weights
+    constexpr int kWords = XT == kQ4F32 ? 8 : XT == kQ4E4m3 ? 2 : 4;  // of a piece of 8 values
+    const bool vec = cols % 8 == 0 && (reinterpret_cast<uintptr_t>(L.x) & (XT == kQ4E4m3 ? 7 : 15)) == 0;
+    for (int r = 0; r < A.lds_rows; ++r) {
+        int xr = r < np && expert >= 0 ? begin + r : -1;
+        if (xr >= 0 && L.order != nullptr) {
+            const int pair = L.order[xr];
+            xr = pair < 0 ? -1 : pair / L.top_k;
+        }
+        if (xr >= L.n_x) xr = -1;
+        const size_t row = (size_t)max(xr, 0) * cols;
+        uint32_t v[kQ4DecPieces][kWords];
+#pragma unroll
+        for (int i = 0; i < kQ4DecPieces; ++i) {
+            const int c = (i * 64 * kQ4DecWaves + tid) * 8;
+#pragma unroll
+            for (int k = 0; k < kWords; ++k) v[i][k] = 0;
+            if (xr < 0 || c >= cols) continue;
+            const char* src = static_cast<const char*>(L.x) + (row + c) * (kWords / 2);
+            if (vec) {
+                if constexpr (kWords == 2) {
+                    const uint2 d = *reinterpret_cast<const uint2*>(src);
+                    v[i][0] = d.x, v[i][1] = d.y;
+                } else {
+#pragma unroll
+                    for (int k = 0; k < kWords; k += 4) {
+                        const u32x4 d = ld16(src + 4 * k);
+#pragma unroll
+                        for (int n = 0; n < 4; ++n) v[i][k + n] = d[n];
+                    }
+                }
+            } else {
+#pragma unroll
+                for (int k = 0; k < 8; ++k) {
+                    if (c + k >= cols) continue;
+                    if constexpr (kWords == 8)
+                        v[i][k] = reinterpret_cast<const uint32_t*>(src)[k];
+                    else if constexpr (kWords == 4)
+                        v[i][k / 2] |= (uint32_t)reinterpret_cast<const uint16_t*>(src)[k] << (16 * (k & 1));
+                    else
+                        v[i][k / 4] |= (uint32_t)reinterpret_cast<const uint8_t*>(src)[k] << (8 * (k & 3));
+                }
+            }
+        }
+        if (r == 0) {
+#pragma unroll
+            for (int u = 0; u < U; ++u) fetch(k0 + u, u);
+        }
+        auto bits = [&](int i, int k) -> uint32_t {  // value k of piece i as fp32
+            if constexpr (XT == kQ4F32)
+                return v[i][k];
+            else
+                return k & 1 ? v[i][k / 2] & 0xFFFF0000u : v[i][k / 2] << 16;
+        };
+        float up = 1.0f;
+        if constexpr (XT == kQ4Bf16 || XT == kQ4F32) {
+            uint32_t most = 0;
+#pragma unroll
+            for (int i = 0; i < kQ4DecPieces; ++i)
+#pragma unroll
+                for (int k = 0; k < 8; ++k) {
+                    const uint32_t b = bits(i, k) & 0x7FFFFFFFu;
+                    if (b < 0x7F800000u) most = max(most, b);  // infinities and NaN stay themselves
+                }
+#pragma unroll
+            for (int m = 32; m >= 1; m >>= 1) most = max(most, (uint32_t)__shfl_xor((int)most, m));
+            if (lane == 0) tops[r][wave] = most;
+            __syncthreads();
+#pragma unroll
+            for (int i = 0; i < kQ4DecWaves; ++i) most = max(most, tops[r][i]);
+            const int e = most == 0 ? 127 : min(max((int)(most >> 23) - 14, 1), 253);
+            up = __uint_as_float((uint32_t)(254 - e) << 23);
+            if (tid == 0) row_up[r] = __uint_as_float((uint32_t)e << 23);
+        } else if (tid == 0) {
+            row_up[r] = 1.0f;
+        }
+#pragma unroll
+        for (int i = 0; i < kQ4DecPieces; ++i) {
+            const int p = i * 64 * kQ4DecWaves + tid;
+            if (p >= KT * 16) continue;
+            u32x4 o;
+            if constexpr (XT == kQ4Fp16) {
+                o = u32x4{v[i][0], v[i][1], v[i][2], v[i][3]};
+            } else if constexpr (XT == kQ4E4m3) {
+                o = __builtin_bit_cast(u32x4, cvt8_f16(v[i][0], v[i][1]));
+            } else {
+#pragma unroll
+                for (int k = 0; k < 4; ++k)
+                    o[k] = f16_rne(__uint_as_float(bits(i, 2 * k)) * up) | (f16_rne(__uint_as_float(bits(i, 2 * k + 1)) * up) << 16);
+            }
+            *reinterpret_cast<u32x4*>(staged + r * pitch + p * 16) = o;
+        }
+        if constexpr (kScaled)
+            for (int k = tid; k < KT; k += 64 * kQ4DecWaves) xs_lds[r * KT + k] = xr >= 0 ? L.x_scale[(size_t)xr * KT + k] : 0.0f;
+    }
+    __syncthreads();
+
+    // ---- the products; lanes of rows that are not there read another row, whose sums are dropped
+    const int lr = min(t, A.lds_rows - 1);
+    const unsigned char* in = staged + lr * pitch + q * 16;
+    f32x4 acc[2] = {};
+    auto multiply = [&](int kt, int u) {
+        u32x4 b[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) b[j] = *reinterpret_cast<const u32x4*>(in + kt * 256 + j * 64);
+        f32x4 part[2] = {};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const int g = j * NG / 4;
+            const _Float16 sc = __builtin_bit_cast(f16x2, s[u][g / 2])[g % 2];
+            const f16x8 f = q4_f16(a[u][j]) * f16x8{sc, sc, sc, sc, sc, sc, sc, sc};
+            f32x4& sum = kScaled ? part[j & 1] : acc[j & 1];
+            sum = Mma<true>::mma(f, Mma<true>::bits(b[j]), sum);
+        }
+        if constexpr (kScaled) {
+            const float x = xs_lds[lr * KT + kt];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) acc[0][i] += x * (part[0][i] + part[1][i]);
+        }
+    };
+    for (int kt = k0; kt < k1; kt += U) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            if (kt + u >= k1) break;
+            __builtin_amdgcn_sched_barrier(0);
+            multiply(kt + u, u);
+            fetch(kt + U + u, u);
+        }
+    }
+    acc[0] += acc[1];
+    __syncthreads();  // x has been read: the sums take its place
+    float(*red)[256] = reinterpret_cast<float(*)[256]>(staged);
+    *reinterpret_cast<f32x4*>(&red[wave][t * 16 + q * 4]) = acc[0];
+    __syncthreads();
+    const int width = L.w.gated ? L.w.rows / 2 : L.w.rows;
+    for (int i = tid; i < groups * 64; i += 64 * kQ4DecWaves) {  // 4 rows x 16 of each row tile
+        const int g = i >> 6, o = block * groups + g, tt = (i & 63) >> 4, r = i & 15;
+        float v = 0.0f;
+        for (int k = 0; k < A.splits; ++k) v += red[g * A.splits + k][i & 63];
+        v *= q4_row_scales(w)[(mat * RT + min(o, RT - 1)) * 16 + r] * row_up[min(tt, A.lds_rows - 1)];
+        if (L.w.gated) {
+            const float other_half = __shfl_down(v, 8);
+            v = v / (1.0f + __expf(-v)) * other_half;
+        }
+        const int n = L.w.gated ? o * 8 + r : o * 16 + r;
+        if (tt < np && o < RT && n < width && (!L.w.gated || r < 8)) q4_store(L, (size_t)(begin + tt) * width + n, v);
+    }
+}
+
+}  // namespace cx

@@ -815,15 +815,14 @@ struct Q4Scratch {
 
 Q4Scratch q4_scratch(const cx_q4_desc& w, int x_dtype, int n_x, int n_rows, bool with_offsets) {
     Q4Scratch z{};
-    z.item_rows = q4_item_rows(n_rows, w.n_mats, x_dtype == CX_DTYPE_E4M3);
+    z.item_rows = q4_item_rows(n_rows, w.n_mats, w.cols, x_dtype == CX_DTYPE_E4M3);
     z.max_items = q4_max_items(n_rows, w.n_mats, z.item_rows);
     z.x = with_offsets ? align_up(sizeof(Q4Item) * (size_t)z.max_items) : 0;
     z.bytes = z.x + (z.item_rows > kTileTok ? q4_x_scratch(w, n_x) : 0);
     return z;
 }
 
-// Scratch of cx_q4_moe.  h: two bf16 planes for the kernel of few rows, fp32 for the
-// GEMM.
+// Scratch of cx_q4_moe.
 struct Q4MoeScratch {
     int64_t pairs, max_items;
     int item_rows;
@@ -833,7 +832,9 @@ struct Q4MoeScratch {
 Q4MoeScratch q4_moe_scratch(const cx_q4_desc& gu, const cx_q4_desc& down, int shared, int n_tokens, int top_k) {
     Q4MoeScratch z{};
     z.pairs = (int64_t)n_tokens * (top_k + shared);
-    z.item_rows = q4_item_rows(z.pairs, gu.n_mats + shared, false);
+    // both products take the same items; in between h is fp32, which the decode kernel and the GEMM read
+    z.item_rows = q4_item_rows(z.pairs, gu.n_mats + shared, std::max(gu.cols, down.cols), false);
+    if (z.item_rows == kTileTok) z.item_rows = kQ4GemmRows;
     z.max_items = q4_max_items(z.pairs, gu.n_mats + shared, z.item_rows);
     const bool gemm = z.item_rows > kTileTok;
     z.items = 0;
@@ -1650,22 +1651,18 @@ int cx_q4_moe(cx_ctx* ctx, const cx_q4_desc* gate_up, const cx_q4_desc* down, co
     L.items = a.items;
     L.item_rows = z.item_rows;
     L.max_items = z.max_items;
-    const bool gemm = z.item_rows > kTileTok;
     L.x_scratch = m + z.x;
     L.y = m + z.h;
-    L.y_lo = m + z.h + 2 * (size_t)z.pairs * down->cols;
-    L.y_type = gemm ? CX_DTYPE_F32 : kQ4Planes;
+    L.y_type = CX_DTYPE_F32;
     Q4Launch D = L;
     D.w = *down;
     if (shared) D.shared = *shared_down;
     D.x = L.y;
-    D.x_lo = L.y_lo;
-    D.x_type = gemm ? kQ4F32 : kQ4Planes;
+    D.x_type = kQ4F32;
     D.x_scratch = m + z.hx;
     D.n_x = (int)z.pairs;
     D.order = nullptr;
     D.y = m + z.ys;
-    D.y_lo = nullptr;
     D.y_type = CX_DTYPE_F32;
     CombineArgs c{};
     c.ys = D.y;

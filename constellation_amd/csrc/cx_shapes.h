@@ -272,10 +272,22 @@ constexpr int kRowThreads = 256;       // workgroup of the gather and combine ke
 // A launch's threads are counted in 32 bits.
 inline bool rows_grid_ok(int64_t workgroups, int threads) { return workgroups * threads < ((int64_t)1 << 32); }
 
-// Rows of x per work item: 16 for the kernel of few rows, which streams a matrix's weights
-// once per item, else up to 128 for the GEMM (64 where it keeps a second set of sums).
+// Rows of x per work item: up to 4 for the decode kernel, which stages them in LDS; up to 16
+// for the kernel of few rows, which reads them from L2; up to 128 for the GEMM (64 where
+// it keeps a second set of sums).  The first two stream a matrix's weights once per item.
 constexpr int kQ4GemmRows = 128;
-inline int q4_item_rows(int64_t n_rows, int n_mats, bool two_sums) {
+constexpr int kQ4DecWaves = 8, kQ4DecPieces = 2;  // waves and, of a staged row, 8-value pieces a thread
+constexpr int kQ4DecCols = kQ4DecPieces * 64 * kQ4DecWaves * 8;
+constexpr int kQ4LdsPad = 64;  // bytes behind a staged row, so that four rows lie in different banks
+inline size_t q4_dec_lds(int cols, int rows) { return (size_t)rows * ((size_t)((cols + 127) / 128) * (256 + 4) + kQ4LdsPad); }
+inline int q4_dec_rows(int cols) {
+    int rows = cols <= kQ4DecCols ? 4 : 0;
+    while (rows > 0 && q4_dec_lds(cols, rows) > 63 * 1024) --rows;
+    return rows;
+}
+inline int q4_item_rows(int64_t n_rows, int n_mats, int cols, bool two_sums) {
+    const int dec = q4_dec_rows(cols);
+    if (dec > 0 && (n_rows <= dec || (n_mats > 1 && n_rows <= n_mats))) return dec;
     return n_rows <= (int64_t)kTileTok * n_mats ? kTileTok : two_sums ? kQ4GemmRows / 2 : kQ4GemmRows;
 }
 
