@@ -328,7 +328,7 @@ struct Q4Item {
 
 struct SortArgs {
     const int32_t* ids;    // [n_tokens, top_k]
-    const float* weights;  // nullable: when given, a repeated expert or a bad weight is an error and its pair has no expert
+    const float* weights;  // nullable: when given, a repeated expert or a bad weight is an error and its pair's place negative
     int n_tokens, top_k, n_experts;
     int shared;            // 1: every token also goes to a shared expert, as route top_k and expert n_experts
     int32_t* order;        // [n_tokens * (top_k + shared)]

@@ -171,10 +171,11 @@ namespace {
 
 size_t up256(size_t v) { return (v + 255) / 256 * 256; }
 
-// Ranges of the columns per row tile: enough waves for 16 a CU, of at least 4 column tiles.
+// Ranges of the columns per row tile: as many waves as 16 a CU take at once, of at least 2
+// column tiles.
 int column_splits(int64_t waves, int KT, int most) {
     int n = 1;
-    while (n < most && waves * n < 4096 && KT / n >= 4) n *= 2;
+    while (n < most && waves * n * 2 <= 4096 && KT / n >= 4) n *= 2;
     return n;
 }
 

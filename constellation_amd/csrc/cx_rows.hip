@@ -205,26 +205,27 @@ hipError_t norm_vpt(const NormArgs& a, hipStream_t s) {
 }
 
 // ---------------------------------------------------------------------------
-// Pairs sorted by expert: a stable counting sort.  Pair i = t * K' + k, K' = top_k,
-// or top_k + 1 where a shared expert takes every token as its last route; key =
-// the expert, the shared one after all others, pairs without an expert last.
+// Pairs sorted by expert: a stable counting sort of the ids, i = t * top_k + k; ids that
+// name no expert have the last key.  Where a shared expert takes every token as one more
+// route, its rows follow those of all experts, in token order.
 //
-// Up to 64 workgroups each place a share of consecutive pairs.  Each counts the
-// keys of all pairs and of those before its share, so none waits for another; within
-// its share, 512 pairs at a time, a pair's rank is its rank in the wave (the lanes
-// of the same key, one ballot per bit of the key) after the counts of the waves and
-// pairs before.  Counts are integers: the order of the atomics changes nothing.
-constexpr int kSortThreads = 512, kSortWaves = kSortThreads / 64;
+// Up to 64 workgroups each place a share of consecutive ids.  Each counts the keys of
+// all ids, those before its share apart, so none waits for another; within its share, 512
+// ids at a time, an id's rank is its rank in the wave (the lanes of the same key, one
+// ballot per bit of the key) after the counts of the waves and ids before.  Counts are
+// integers: the order of the atomics changes nothing.  Reading the ids bounds it, so eight
+// loads a thread are in flight: 32,768 ids in XXX us, 8 in XXX.
+constexpr int kSortThreads = 512, kSortWaves = kSortThreads / 64, kSortLoads = 8;
 constexpr int kSortKeys = kSortMaxExperts + 2;  // experts, the shared one, none
 
 // First index of each key from its count, in place; entry n gets the total.
+template <int PER>
 __device__ __forceinline__ void scan_counts(int* v, int n, int* wave_tot) {
-    constexpr int kPer = (kSortKeys + kSortThreads) / kSortThreads;
     const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
-    int own[kPer], sum = 0;
+    int own[PER], sum = 0;
 #pragma unroll
-    for (int i = 0; i < kPer; ++i) {
-        own[i] = tid * kPer + i < n ? v[tid * kPer + i] : 0;
+    for (int i = 0; i < PER; ++i) {
+        own[i] = tid * PER + i < n ? v[tid * PER + i] : 0;
         sum += own[i];
     }
     int inc = sum;
@@ -236,99 +237,159 @@ __device__ __forceinline__ void scan_counts(int* v, int n, int* wave_tot) {
     if (lane == 63) wave_tot[w] = inc;
     __syncthreads();
     int base = inc - sum;
-    for (int i = 0; i < w; ++i) base += wave_tot[i];
 #pragma unroll
-    for (int i = 0; i < kPer; ++i) {
-        if (tid * kPer + i <= n) v[tid * kPer + i] = base;
+    for (int i = 0; i < kSortWaves; ++i)
+        if (i < w) base += wave_tot[i];
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+        if (tid * PER + i <= n) v[tid * PER + i] = base;
         base += own[i];
     }
     __syncthreads();
 }
 
+// SMALL: up to 512 ids and 510 keys: one workgroup, whose ranks give the counts.
+template <bool SMALL>
 __global__ __launch_bounds__(kSortThreads) void k_sort_tokens(SortArgs a) {
-    __shared__ int first[kSortKeys + 1], next[kSortKeys + 1], items[kSortKeys + 1];
-    __shared__ int hist[kSortWaves][kSortKeys];
+    constexpr int kKeys = SMALL ? kSortThreads : kSortKeys, kPer = SMALL ? 1 : (kSortKeys + kSortThreads) / kSortThreads;
+    __shared__ int first[kKeys + 1], next[kKeys + 1], items[kKeys + 1];
+    __shared__ int hist[kSortWaves][kKeys];
     __shared__ int wave_tot[kSortWaves];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const int K = a.top_k, E = a.n_experts, KE = K + a.shared, NK = E + a.shared, P = a.n_tokens * KE;
+    const int K = a.top_k, KE = K + a.shared, NK = a.n_experts, N = a.n_tokens * K;  // key NK: none
     const int bits = 32 - __builtin_clz(NK);
-    const int chunks = (P + kSortThreads - 1) / kSortThreads;
+    const int chunks = (N + kSortThreads - 1) / kSortThreads;
     const int per = (chunks + (int)gridDim.x - 1) / (int)gridDim.x * kSortThreads;
-    const int begin = min(P, (int)blockIdx.x * per), end = min(P, begin + per);
+    const int begin = min(N, (int)blockIdx.x * per), end = min(N, begin + per);
+    auto key = [&](int id) { return id >= 0 && id < NK ? id : NK; };
     int err = 0;
-    auto key = [&](int i) {
-        const int t = i / KE, k = i - t * KE;
-        if (k == K) return E;  // the shared expert
-        const int32_t* row = a.ids + (size_t)t * K;
-        const int e = row[k];
-        if (e < 0) return NK;
-        int bad = e >= E ? kErrBadExpertId : 0;
-        if (a.weights != nullptr) {
-            for (int j = 0; j < k; ++j)
-                if (row[j] == e) bad |= kErrDuplicateRoute;
-            if (!route_weight_ok(a.weights[(size_t)t * K + k])) bad |= kErrBadWeight;
+    auto place = [&](int i, int e, int row) {
+        const int t = i / K, k = i - t * K;
+        bool held = e < NK;
+        if (held && a.weights != nullptr) {
+            // a repeated expert or a bad weight: the row stays, no token takes it
+            int bad = route_weight_ok(a.weights[i]) ? 0 : kErrBadWeight;
+            for (int j = 1; j <= k; ++j)
+                if (a.ids[i - j] == e) bad |= kErrDuplicateRoute;
+            err |= bad;
+            held = bad == 0;
         }
-        err |= bad;
-        return bad ? NK : e;
+        const int pair = t * KE + k;
+        a.place[pair] = held ? row : ~row;
+        a.order[row] = e < NK ? pair : ~pair;
     };
-    for (int e = tid; e <= NK + 1; e += kSortThreads) first[e] = next[e] = 0;
-    __syncthreads();
-    for (int i = tid; i < P; i += kSortThreads) {
-        const int e = key(i);
-        atomicAdd(&first[e], 1);
-        if (i < begin) atomicAdd(&next[e], 1);
-    }
-    __syncthreads();
-    if (blockIdx.x == 0 && a.items != nullptr) {
-        for (int e = tid; e < NK; e += kSortThreads) items[e] = (first[e] + a.item_rows - 1) / a.item_rows;
-        __syncthreads();
-        scan_counts(items, NK, wave_tot);
-    }
-    scan_counts(first, NK + 1, wave_tot);
-    if (blockIdx.x == 0) {
-        if (a.offsets != nullptr)
-            for (int e = tid; e <= E; e += kSortThreads) a.offsets[e] = first[e];
-        if (a.items != nullptr) {
-            for (int e = tid; e < NK; e += kSortThreads)
-                for (int i = items[e], p = first[e]; p < first[e + 1]; ++i, p += a.item_rows)
-                    a.items[1 + i] = Q4Item{e, p, min(a.item_rows, first[e + 1] - p), 0};
-            if (tid == 0) a.items[0] = Q4Item{items[NK], first[NK], 0, 0};
-        }
-        if (err && a.err_flag != nullptr) atomicOr(a.err_flag, err);
-    }
-    for (int e = tid; e <= NK; e += kSortThreads) next[e] += first[e];
-    for (int c = begin; c < end; c += kSortThreads) {
-        for (int e = tid; e < kSortWaves * kSortKeys; e += kSortThreads) (&hist[0][0])[e] = 0;
-        __syncthreads();
-        const int i = c + tid;
-        const bool live = i < end;
-        const int e = live ? key(i) : NK;
+    auto rank_in_wave = [&](int e, bool live, int& count) {
         uint64_t same = __ballot(live);
         for (int b = 0; b < bits; ++b) {
             const uint64_t set = __ballot((e >> b) & 1);
             same &= ((e >> b) & 1) ? set : ~set;
         }
-        const int rank = __popcll(same & ((1ull << lane) - 1));
-        if (live && rank == 0) hist[wave][e] = __popcll(same);
-        __syncthreads();
-        for (int b = tid; b <= NK; b += kSortThreads) {
-            int at = next[b];
-            for (int w = 0; w < kSortWaves; ++w) {
-                const int n = hist[w][b];
-                hist[w][b] = at;
-                at += n;
-            }
-            next[b] = at;
-        }
-        __syncthreads();
-        if (live) {
-            const int row = hist[wave][e] + rank;
-            const bool held = e < NK;
-            a.place[i] = held ? row : ~row;
-            a.order[row] = held ? i : ~i;
-        }
-        __syncthreads();
+        count = __popcll(same);
+        return __popcll(same & ((1ull << lane) - 1));
+    };
+    const int own = SMALL && tid < N ? a.ids[tid] : 0;
+    for (int e = tid; e <= NK + 1; e += kSortThreads) first[e] = next[e] = 0;
+    if constexpr (SMALL) {
+        for (int w = 0; w < kSortWaves; ++w)
+            if (tid <= NK) hist[w][tid] = 0;
     }
+    __syncthreads();
+    int own_rank = 0;
+    if constexpr (SMALL) {
+        int n;
+        own_rank = rank_in_wave(key(own), tid < N, n);
+        if (tid < N && own_rank == 0) hist[wave][key(own)] = n;
+        if (tid < N && own >= NK) err |= kErrBadExpertId;
+        __syncthreads();
+        if (tid <= NK) {
+            int at = 0;
+#pragma unroll
+            for (int w = 0; w < kSortWaves; ++w) {
+                const int c = hist[w][tid];
+                hist[w][tid] = at;
+                at += c;
+            }
+            first[tid] = at;
+        }
+    } else {
+        for (int i0 = 0; i0 < N; i0 += kSortLoads * kSortThreads) {
+            int id[kSortLoads];
+#pragma unroll
+            for (int u = 0; u < kSortLoads; ++u) id[u] = a.ids[min(i0 + u * kSortThreads + tid, N - 1)];
+#pragma unroll
+            for (int u = 0; u < kSortLoads; ++u) {
+                const int i = i0 + u * kSortThreads + tid;
+                if (i >= N) continue;
+                if (id[u] >= NK) err |= kErrBadExpertId;
+                atomicAdd(i < begin ? &next[key(id[u])] : &first[key(id[u])], 1);
+            }
+        }
+        __syncthreads();
+        for (int e = tid; e <= NK; e += kSortThreads) first[e] += next[e];
+    }
+    __syncthreads();
+    if (blockIdx.x == 0 && a.items != nullptr) {
+        for (int e = tid; e < NK; e += kSortThreads) items[e] = (first[e] + a.item_rows - 1) / a.item_rows;
+        __syncthreads();
+        scan_counts<kPer>(items, NK, wave_tot);
+    }
+    scan_counts<kPer>(first, NK + 1, wave_tot);
+    const int shared_row = first[NK];  // the shared expert's rows, then those without an expert
+    const int none = a.shared ? a.n_tokens : 0;
+    if (blockIdx.x == 0) {
+        if (a.offsets != nullptr)
+            for (int e = tid; e <= NK; e += kSortThreads) a.offsets[e] = first[e];
+        if (a.items != nullptr) {
+            for (int e = tid; e < NK; e += kSortThreads)
+                for (int i = items[e], p = first[e]; p < first[e + 1]; ++i, p += a.item_rows)
+                    a.items[1 + i] = Q4Item{e, p, min(a.item_rows, first[e + 1] - p), 0};
+            const int more = (none + a.item_rows - 1) / a.item_rows;
+            for (int i = tid; i < more; i += kSortThreads)
+                a.items[1 + items[NK] + i] = Q4Item{NK, shared_row + i * a.item_rows, min(a.item_rows, none - i * a.item_rows), 0};
+            if (tid == 0) a.items[0] = Q4Item{items[NK] + more, shared_row + none, 0, 0};
+        }
+    }
+    if (a.shared)
+        for (int t = blockIdx.x * kSortThreads + tid; t < a.n_tokens; t += gridDim.x * kSortThreads) {
+            a.place[t * KE + K] = shared_row + t;
+            a.order[shared_row + t] = t * KE + K;
+        }
+    auto row_of = [&](int e, int at) { return e < NK ? at : at + none; };
+    if constexpr (SMALL) {
+        if (tid < N) {
+            const int e = key(own);
+            place(tid, e, row_of(e, first[e] + hist[wave][e] + own_rank));
+        }
+    } else {
+        for (int e = tid; e <= NK; e += kSortThreads) next[e] += first[e];
+        for (int c = begin; c < end; c += kSortThreads) {
+            const int i = c + tid;
+            const bool live = i < end;
+            const int e = live ? key(a.ids[i]) : NK;
+            for (int b = tid; b <= NK; b += kSortThreads)
+#pragma unroll
+                for (int w = 0; w < kSortWaves; ++w) hist[w][b] = 0;
+            int n;
+            const int rank = rank_in_wave(e, live, n);
+            __syncthreads();
+            if (live && rank == 0) hist[wave][e] = n;
+            __syncthreads();
+            for (int b = tid; b <= NK; b += kSortThreads) {
+                int at = next[b];
+#pragma unroll
+                for (int w = 0; w < kSortWaves; ++w) {
+                    const int h = hist[w][b];
+                    hist[w][b] = at;
+                    at += h;
+                }
+                next[b] = at;
+            }
+            __syncthreads();
+            if (live) place(i, e, row_of(e, hist[wave][e] + rank));
+            __syncthreads();
+        }
+    }
+    if (err && a.err_flag != nullptr) atomicOr(a.err_flag, err);
 }
 
 // ---------------------------------------------------------------------------
@@ -366,43 +427,119 @@ hipError_t gather_as(const GatherArgs& g, hipStream_t s) {
 }
 
 // ---------------------------------------------------------------------------
+// Eight columns of a thread for the sums below: with VEC the eight from 8 * lane on, as
+// 16-byte accesses; otherwise every kRowThreads-th, so that neighbouring threads still touch
+// neighbouring values of rows that start anywhere.  A load is kept as it arrives, so
+// that the loads of several rows are in flight together.
+template <int DT, bool VEC>
+struct Cols {
+    static constexpr int kStep = VEC ? 1 : kRowThreads;
+    uint32_t d[VEC ? (DT == CX_DTYPE_F32 ? 8 : 4) : 8];
+
+    // columns at, at + kStep, ...; `left` of the row's columns are left from `at` on (those past them repeat the last)
+    __device__ __forceinline__ void load(const void* base, size_t at, int left) {
+        if constexpr (VEC) {
+#pragma unroll
+            for (int i = 0; i < (int)(sizeof(d) / 16); ++i) {
+                const u32x4 v = ld16(static_cast<const char*>(base) + at * (DT == CX_DTYPE_F32 ? 4 : 2) + 16 * i);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) d[4 * i + j] = v[j];
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const size_t p = at + min(i * kStep, (left - 1) / kStep * kStep);
+                if constexpr (DT == CX_DTYPE_F32)
+                    d[i] = static_cast<const uint32_t*>(base)[p];
+                else
+                    d[i] = static_cast<const uint16_t*>(base)[p];
+            }
+        }
+    }
+    __device__ __forceinline__ float get(int i) const {
+        if constexpr (DT == CX_DTYPE_F32) return __uint_as_float(d[i]);
+        const uint32_t h = !VEC ? d[i] : i & 1 ? d[i >> 1] >> 16 : d[i >> 1] & 0xFFFFu;
+        if constexpr (DT == CX_DTYPE_BF16) return __uint_as_float(h << 16);
+        return static_cast<float>(__builtin_bit_cast(_Float16, static_cast<uint16_t>(h)));
+    }
+};
+
+// The same with the type known at run time.
+template <bool VEC>
+__device__ __forceinline__ void load_cols(const void* base, int dtype, size_t at, int left, float (&v)[8]) {
+    auto as = [&](auto c) {
+        c.load(base, at, left);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = c.get(i);
+    };
+    if (dtype == CX_DTYPE_BF16)
+        as(Cols<CX_DTYPE_BF16, VEC>{});
+    else if (dtype == CX_DTYPE_FP16)
+        as(Cols<CX_DTYPE_FP16, VEC>{});
+    else
+        as(Cols<CX_DTYPE_F32, VEC>{});
+}
+
+template <bool VEC>
+__device__ __forceinline__ void store_cols(void* base, int dtype, size_t at, int left, const float (&v)[8]) {
+    if constexpr (VEC) {
+        store8<true>(base, dtype, at, left, v);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            if (i * kRowThreads >= left) continue;
+            if (dtype == CX_DTYPE_F32)
+                static_cast<float*>(base)[at + i * kRowThreads] = v[i];
+            else
+                static_cast<uint16_t*>(base)[at + i * kRowThreads] = (uint16_t)cast_out(v[i], dtype);
+        }
+    }
+}
+
+// A thread's first column of the c-th 8 * kRowThreads columns of a row.
+template <bool VEC>
+__device__ __forceinline__ int first_col(int c) {
+    return c * 8 * kRowThreads + (VEC ? 8 : 1) * (int)threadIdx.x;
+}
+
 // out[t] = sum over k, in this order and in fp32, of w[t, k] * ys[place[t, k]], then
 // + add[t], rounded once.  Eight columns of one token per thread; the loads of eight
 // routes are in flight together.
 template <int DT, bool VEC>
 __global__ __launch_bounds__(kRowThreads) void k_combine_rows(CombineArgs a, int chunks) {
-    const int t = blockIdx.x / chunks, c = ((blockIdx.x - t * chunks) * kRowThreads + threadIdx.x) * 8;
-    const int H = a.hidden, K = a.top_k, left = H - c;
+    const int t = blockIdx.x / chunks, H = a.hidden, K = a.top_k, c = first_col<VEC>(blockIdx.x - t * chunks), left = H - c;
     if (left <= 0) return;
     float acc[8] = {};
     for (int k0 = 0; k0 < K; k0 += 8) {
-        float v[8][8], w[8];
+        Cols<DT, VEC> v[8];
+        int p[8];
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
-            const size_t i = (size_t)t * K + k0 + k;
-            int p = k0 + k < K ? a.place[i] : -1;
-            if (p >= a.n_rows) {
+            p[k] = k0 + k < K ? a.place[(size_t)t * K + k0 + k] : -1;
+            if (p[k] >= a.n_rows) {
                 atomicOr(a.err_flag, kErrBadRow);
-                p = -1;
+                p[k] = -1;
             }
-            w[k] = p < 0 ? 0.0f : a.weights != nullptr && k0 + k < a.weights_step ? a.weights[(size_t)t * a.weights_step + k0 + k] : 1.0f;
-#pragma unroll
-            for (int j = 0; j < 8; ++j) v[k][j] = 0.0f;
-            if (p >= 0) load8<DT, VEC>(a.ys, (size_t)p * H + c, left, v[k]);
         }
 #pragma unroll
-        for (int k = 0; k < 8; ++k)
+        for (int k = 0; k < 8; ++k)  // of a pair without an expert: row 0, which is there, and left out below
+            v[k].load(a.ys, (size_t)max(p[k], 0) * H + c, left);
 #pragma unroll
-            for (int j = 0; j < 8; ++j) acc[j] += w[k] * v[k][j];
+        for (int k = 0; k < 8; ++k) {
+            if (p[k] < 0) continue;
+            const float w = a.weights != nullptr && k0 + k < a.weights_step ? a.weights[(size_t)t * a.weights_step + k0 + k] : 1.0f;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) acc[j] += w * v[k].get(j);
+        }
     }
     if (a.add != nullptr) {
         float v[8];
-        load8<VEC>(a.add, a.out_dtype, (size_t)t * H + c, left, v);
+        load_cols<VEC>(a.add, a.out_dtype, (size_t)t * H + c, left, v);
 #pragma unroll
         for (int j = 0; j < 8; ++j) acc[j] += v[j];
     }
-    store8<VEC>(a.out, a.out_dtype, (size_t)t * H + c, left, acc);
-    if (a.out_f32 != nullptr) store8<CX_DTYPE_F32, VEC>(a.out_f32, (size_t)t * H + c, left, acc);
+    store_cols<VEC>(a.out, a.out_dtype, (size_t)t * H + c, left, acc);
+    if (a.out_f32 != nullptr) store_cols<VEC>(a.out_f32, CX_DTYPE_F32, (size_t)t * H + c, left, acc);
 }
 
 // Its gradient: dys[place[t, k]] = w[t, k] * dout[t] and dw[t, k] = <dout[t],
@@ -412,6 +549,7 @@ __global__ __launch_bounds__(kRowThreads) void k_combine_rows(CombineArgs a, int
 // the lanes and waves in a fixed order.
 template <int DT, bool VEC>
 __global__ __launch_bounds__(kRowThreads) void k_combine_grad(CombineGradArgs a, int routes, int splits) {
+    constexpr int kNone = -1, kZeros = INT32_MIN;  // no such route; a row of zeros (kZeros | row)
     __shared__ float part[4][8];
     const int t = blockIdx.x / splits, k0 = (blockIdx.x - t * splits) * routes;
     const int H = a.hidden, n = min(routes, a.top_k - k0), tid = threadIdx.x;
@@ -420,38 +558,36 @@ __global__ __launch_bounds__(kRowThreads) void k_combine_grad(CombineGradArgs a,
     float w[8], dot[8] = {};
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
-        const int p = k < n ? a.place[first + k] : 0;
-        row[k] = p < 0 ? ~p : p;
-        w[k] = k < n && p >= 0 ? (a.weights != nullptr ? a.weights[first + k] : 1.0f) : 0.0f;
-        if (k >= n) row[k] = -1;
-        if (row[k] >= a.n_rows) {
-            atomicOr(a.err_flag, kErrBadRow);
-            row[k] = -1;
-        }
-        if (k < n && p < 0 && row[k] >= 0) row[k] |= INT32_MIN;  // zeros, no product
+        const int p = k < n ? a.place[first + k] : 0, at = p < 0 ? ~p : p;
+        w[k] = k < n && a.weights != nullptr ? a.weights[first + k] : 1.0f;
+        row[k] = k >= n || at >= a.n_rows ? kNone : p < 0 ? at | kZeros : at;
+        if (k < n && at >= a.n_rows) atomicOr(a.err_flag, kErrBadRow);
     }
-    for (int c = tid * 8; c < H; c += kRowThreads * 8) {
+    for (int b = 0, c = first_col<VEC>(0); c < H; c = first_col<VEC>(++b)) {
         const int left = H - c;
-        float d[8], v[8][8];
-        load8<VEC>(a.dout, a.dout_dtype, (size_t)t * H + c, left, d);
+        float d[8];
+        Cols<DT, VEC> v[8];
 #pragma unroll
         for (int k = 0; k < 8; ++k)
-            if (row[k] >= 0) load8<DT, VEC>(a.ys, (size_t)row[k] * H + c, left, v[k]);
+            if (k < routes) v[k].load(a.ys, (size_t)max(row[k], 0) * H + c, left);
+        load_cols<VEC>(a.dout, a.dout_dtype, (size_t)t * H + c, left, d);
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
-            if (row[k] == -1) continue;
+            if (row[k] == kNone) continue;
             float o[8];
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-                if (row[k] >= 0) dot[k] += d[j] * v[k][j];
+                const bool in = VEC || j * kRowThreads < left;
+                if (row[k] >= 0 && in) dot[k] += d[j] * v[k].get(j);
                 o[j] = row[k] >= 0 ? w[k] * d[j] : 0.0f;
             }
-            store8<DT, VEC>(a.dys, (size_t)(row[k] & INT32_MAX) * H + c, left, o);
+            store_cols<VEC>(a.dys, DT, (size_t)(row[k] & INT32_MAX) * H + c, left, o);
         }
     }
     if (a.dw == nullptr) return;
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
+        if (k >= routes) break;
         const float v = wave_sum(dot[k]);
         if ((tid & 63) == 0) part[tid >> 6][k] = v;
     }
@@ -472,9 +608,13 @@ hipError_t launch_rms_norm(const NormArgs& a, hipStream_t s) {
 }
 
 hipError_t launch_sort_tokens(const SortArgs& a, hipStream_t s) {
-    const int64_t pairs = (int64_t)a.n_tokens * (a.top_k + a.shared);
-    const int64_t wgs = std::max<int64_t>(1, std::min<int64_t>(64, (pairs + kSortThreads - 1) / kSortThreads));
-    cx_launch(k_sort_tokens, dim3((unsigned)wgs), dim3(kSortThreads), 0, s, a);
+    const int64_t ids = (int64_t)a.n_tokens * a.top_k;
+    if (ids <= kSortThreads && a.n_experts + 2 <= kSortThreads) {
+        cx_launch(k_sort_tokens<true>, dim3(1), dim3(kSortThreads), 0, s, a);
+    } else {
+        const int64_t wgs = std::min<int64_t>(64, (ids + kSortThreads - 1) / kSortThreads);
+        cx_launch(k_sort_tokens<false>, dim3((unsigned)wgs), dim3(kSortThreads), 0, s, a);
+    }
     return hipGetLastError();
 }
 

@@ -49,8 +49,8 @@ def _check_pairs(rows: int, n_tokens: int, top_k: int, weights: Optional[torch.T
         raise ValueError(f"weights must be fp32 [{n_tokens}, {top_k}]")
 
 
-def _stream(device: int) -> int:
-    return torch.cuda.current_stream(device).cuda_stream
+# the current stream's handle without a Stream object around it: a microsecond less a call
+_stream = torch._C._cuda_getCurrentRawStream
 
 
 def device_count() -> int:
@@ -378,7 +378,7 @@ class Context:
     # -- rows around the experts -------------------------------------------------
     def _here(self, *tensors: Optional[torch.Tensor]) -> None:
         for t in tensors:
-            if t is not None and (t.device.type != "cuda" or t.device.index != self.device):
+            if t is not None and t.get_device() != self.device:  # -1 on the CPU
                 raise ValueError(f"tensor on {t.device}, context on cuda:{self.device}")
 
     def rms_norm(self, x: torch.Tensor, weight: Optional[torch.Tensor] = None, *, eps: float = 1e-6,
@@ -401,11 +401,11 @@ class Context:
         dt = cx_dtype(x.dtype)
         out_dtype = out_dtype or x.dtype
         s = None if residual is None else torch.empty_like(x)
-        y = torch.empty((T, H), dtype=out_dtype, device=x.device) if want_y else None
+        y = torch.empty_like(x, dtype=out_dtype) if want_y else None
         q = scale = None
         if quantize:
-            q = torch.empty((T, H), dtype=torch.float8_e4m3fn, device=x.device)
-            scale = torch.empty((T, (H + 127) // 128), dtype=torch.float32, device=x.device)
+            q = torch.empty_like(x, dtype=torch.float8_e4m3fn)
+            scale = x.new_empty((T, (H + 127) // 128), dtype=torch.float32)
         check(lib().cx_rms_norm(self.handle, x.data_ptr(), dt, _ptr(residual), _ptr(weight),
                                 dt if weight is None else cx_dtype(weight.dtype), T, H, eps, _ptr(s), _ptr(y),
                                 cx_dtype(out_dtype), _ptr(q), _ptr(scale), self.stream()))
