@@ -404,7 +404,48 @@ hipError_t launch_q4_pack(const cx_q4_desc& w, const uint8_t* codes, const uint1
 hipError_t launch_q4_items(const int32_t* offsets, int n_mats, int n_rows, int item_rows, Q4Item* items, int* err_flag,
                            hipStream_t s);
 size_t q4_x_scratch(const cx_q4_desc& w, int n_x);  // of products with items of more than 16 rows
-hipError_t launch_q4_dec(const Q4Launch& L, int splits, int64_t items, hipStream_t s);
+// Given routes, one item per pair: what a layer over a few tokens has instead of a plan.
+struct Q4Routes {
+    const int32_t* ids;    // [n_tokens, top_k]; nullable: no routes, L.items or one matrix
+    const float* weights;
+    int top_k, shared;     // shared: one more route of every token, to L.shared
+    int* err_flag;
+
+    // The expert that route k of token t names (n_mats: the shared one), -1: none.
+    __device__ __forceinline__ int expert(int t, int k, int n_mats) const {
+        if (k == top_k) return n_mats;
+        const int e = ids[(size_t)t * top_k + k];
+        return e >= 0 && e < n_mats ? e : -1;
+    }
+    // Why the route is to be left out all the same (0: it is not): one look at the ids before it, a lane each.
+    __device__ __forceinline__ int fault(int t, int k, int n_mats, int lane) const {
+        if (k == top_k) return 0;
+        const int32_t* row = ids + (size_t)t * top_k;
+        const int e = row[k], before = lane < k ? row[lane] : -1;  // top_k is at most 64
+        if (e < 0) return 0;
+        int bad = e >= n_mats ? kErrBadExpertId : 0;
+        if (__ballot(before == e) != 0) bad |= kErrDuplicateRoute;
+        if (!route_weight_ok(weights[(size_t)t * top_k + k])) bad |= kErrBadWeight;
+        return bad;
+    }
+};
+
+// The down projections of given routes and their sum.
+struct Q4DecSumArgs {
+    cx_q4_desc w, shared;
+    Q4Routes routes;
+    const float* h;  // [n_tokens * (top_k + shared), cols]
+    void* y;         // [n_tokens, rows]
+    float* y_f32;    // nullable
+    int out_dtype, RT, KT;
+};
+
+hipError_t launch_q4_dec(const Q4Launch& L, const Q4Routes* routes, int splits, int64_t items, hipStream_t s);
+hipError_t launch_q4_dec_sum(const Q4DecSumArgs& A, int n_tokens, hipStream_t s);
+// A layer on a few tokens in two launches: gate/up of every pair (L: x and h, one row per
+// pair), then down and sum (D: h).
+hipError_t launch_q4_routes(const Q4Launch& L, const Q4Launch& D, const Q4Routes& routes, int n_tokens, void* y, int out_dtype,
+                            float* y_f32, hipStream_t s);
 hipError_t launch_q4_gemm(const Q4Launch& L, hipStream_t s);
 bool q4_grid_ok(const Q4Launch& L);
 hipError_t launch_q4(const Q4Launch& L, hipStream_t s);

@@ -209,8 +209,18 @@ bool q4_grid_ok(const Q4Launch& L) {
 
 size_t q4_x_scratch(const cx_q4_desc& w, int n_x) { return up256((size_t)n_x * q4_col_tiles(w) * 256) + up256((size_t)n_x * 4); }
 
+hipError_t launch_q4_routes(const Q4Launch& L, const Q4Launch& D, const Q4Routes& routes, int n_tokens, void* y, int out_dtype,
+                            float* y_f32, hipStream_t s) {
+    const int ke = routes.top_k + routes.shared;
+    const int64_t pairs = (int64_t)n_tokens * ke;
+    const hipError_t e = launch_q4_dec(L, &routes, column_splits(pairs * q4_row_tiles(L.w), q4_col_tiles(L.w), kQ4DecWaves), pairs, s);
+    if (e != hipSuccess) return e;
+    return launch_q4_dec_sum(Q4DecSumArgs{D.w, D.shared, routes, static_cast<const float*>(D.x), y, y_f32, out_dtype,
+                                          q4_row_tiles(D.w), q4_col_tiles(D.w)}, n_tokens, s);
+}
+
 hipError_t launch_q4(const Q4Launch& L, hipStream_t s) {
-    if (L.item_rows < kTileTok) return launch_q4_dec(L, column_splits(busy_mats(L) * q4_row_tiles(L.w), q4_col_tiles(L.w), kQ4DecWaves), item_bound(L), s);
+    if (L.item_rows < kTileTok) return launch_q4_dec(L, nullptr, column_splits(busy_mats(L) * q4_row_tiles(L.w), q4_col_tiles(L.w), kQ4DecWaves), item_bound(L), s);
     if (L.item_rows > kTileTok) {
         const int padded = q4_col_tiles(L.w) * 128;
         Q4Launch G = L;

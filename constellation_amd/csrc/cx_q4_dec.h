@@ -7,10 +7,39 @@ namespace cx {
 
 struct Q4DecArgs {
     Q4Launch L;
+    Q4Routes routes;
     int RT, KT;
     int splits;      // ranges of the columns per row tile
     int row_blocks;  // workgroups per item
     int lds_rows;    // rows of x staged, at most 4
+};
+
+// A wave's ring of column tiles of one row tile: codes, and the scales of the lane's row.  The
+// loads are bounded, so that tiles past the range read as zeros and cost nothing.
+template <int NG, int U>
+struct Q4Ring {
+    u32x4 a[U];
+    uint32_t s[U][(NG + 1) / 2];
+
+    __device__ __forceinline__ void fetch(__amdgpu_buffer_rsrc_t codes, __amdgpu_buffer_rsrc_t scales, int kt, int u, int lane) {
+        a[u] = bld16(codes, (uint32_t)kt * kQ4Tile + (uint32_t)lane * 16);
+        const uint32_t at = (uint32_t)kt * 32 * NG + (uint32_t)(lane & 15) * 2 * NG;
+        if constexpr (NG == 1) {
+            s[u][0] = __builtin_amdgcn_raw_buffer_load_b16(scales, at, 0, 0);
+        } else if constexpr (NG == 2) {
+            s[u][0] = __builtin_amdgcn_raw_buffer_load_b32(scales, at, 0, 0);
+        } else {
+            typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+            const u32x2 v = __builtin_bit_cast(u32x2, __builtin_amdgcn_raw_buffer_load_b64(scales, at, 0, 0));
+            s[u][0] = v[0], s[u][1] = v[1];
+        }
+    }
+    // The lane's eight weights of MFMA j of the tile in place u.
+    __device__ __forceinline__ f16x8 weights(int u, int j) const {
+        const int g = j * NG / 4;
+        const _Float16 sc = __builtin_bit_cast(f16x2, s[u][g / 2])[g % 2];
+        return q4_f16(a[u][j]) * f16x8{sc, sc, sc, sc, sc, sc, sc, sc};
+    }
 };
 
 // A wave takes one row tile and one range of the column tiles; the partial sums of the ranges
@@ -39,32 +68,28 @@ __global__ __launch_bounds__(64 * kQ4DecWaves) void k_q4_dec(Q4DecArgs A) {
         begin = it.begin;
         np = it.rows;
     }
+    int x_row = -1;  // with routes: the token
+    if (A.routes.ids != nullptr || A.routes.shared) {
+        const int ke = A.routes.top_k + A.routes.shared;
+        x_row = idx / ke;
+        expert = A.routes.expert(x_row, idx - x_row * ke, L.w.n_mats);
+        if (block == 0 && wave == 0) {
+            const int err = A.routes.fault(x_row, idx - x_row * ke, L.w.n_mats, lane);
+            if (err && lane == 0) atomicOr(A.routes.err_flag, err);
+        }
+        if (expert < 0) return;  // its row is not read
+    }
     const bool other = expert == L.w.n_mats;
     const cx_q4_desc& w = other ? L.shared : L.w;
     const size_t mat = other ? 0 : (size_t)max(expert, 0);
     const int cols = L.w.cols, pitch = KT * 256 + kQ4LdsPad, rt = block * groups + rg;
     float* xs_lds = reinterpret_cast<float*>(staged + A.lds_rows * pitch);  // kScaled: [lds_rows][KT]
 
-    // ---- the ring: bounded loads, so that places past the range read as zeros and cost nothing
     const size_t tile0 = (mat * RT + min(rt, RT - 1)) * (size_t)KT;
     const int per = (KT + A.splits - 1) / A.splits, k0 = ks * per, k1 = expert < 0 || rt >= RT ? k0 : min(KT, k0 + per);
     const __amdgpu_buffer_rsrc_t rw = make_rsrc(w.codes + tile0 * kQ4Tile, (uint32_t)max(k1, 0) * kQ4Tile);
     const __amdgpu_buffer_rsrc_t rs = make_rsrc(w.scales + tile0 * 16 * NG, (uint32_t)max(k1, 0) * 32 * NG);
-    u32x4 a[U];
-    uint32_t s[U][(NG + 1) / 2];
-    auto fetch = [&](int kt, int u) {
-        a[u] = bld16(rw, (uint32_t)kt * kQ4Tile + (uint32_t)lane * 16);
-        const uint32_t at = (uint32_t)kt * 32 * NG + (uint32_t)t * 2 * NG;
-        if constexpr (NG == 1) {
-            s[u][0] = __builtin_amdgcn_raw_buffer_load_b16(rs, at, 0, 0);
-        } else if constexpr (NG == 2) {
-            s[u][0] = __builtin_amdgcn_raw_buffer_load_b32(rs, at, 0, 0);
-        } else {
-            typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
-            const u32x2 v = __builtin_bit_cast(u32x2, __builtin_amdgcn_raw_buffer_load_b64(rs, at, 0, 0));
-            s[u][0] = v[0], s[u][1] = v[1];
-        }
-    };
+    Q4Ring<NG, U> ring;
 
     // ---- x: loads first, so that waiting for them does not wait for the weights
     constexpr int kWords = XT == kQ4F32 ? 8 : XT == kQ4E4m3 ? 2 : 4;  // of a piece of 8 values
@@ -75,6 +100,7 @@ __global__ __launch_bounds__(64 * kQ4DecWaves) void k_q4_dec(Q4DecArgs A) {
             const int pair = L.order[xr];
             xr = pair < 0 ? -1 : pair / L.top_k;
         }
+        if (x_row >= 0) xr = x_row;
         if (xr >= L.n_x) xr = -1;
         const size_t row = (size_t)max(xr, 0) * cols;
         uint32_t v[kQ4DecPieces][kWords];
@@ -112,7 +138,7 @@ __global__ __launch_bounds__(64 * kQ4DecWaves) void k_q4_dec(Q4DecArgs A) {
         }
         if (r == 0) {
 #pragma unroll
-            for (int u = 0; u < U; ++u) fetch(k0 + u, u);
+            for (int u = 0; u < U; ++u) ring.fetch(rw, rs, k0 + u, u, lane);
         }
         auto bits = [&](int i, int k) -> uint32_t {  // value k of piece i as fp32
             if constexpr (XT == kQ4F32)
@@ -174,11 +200,8 @@ __global__ __launch_bounds__(64 * kQ4DecWaves) void k_q4_dec(Q4DecArgs A) {
         f32x4 part[2] = {};
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-            const int g = j * NG / 4;
-            const _Float16 sc = __builtin_bit_cast(f16x2, s[u][g / 2])[g % 2];
-            const f16x8 f = q4_f16(a[u][j]) * f16x8{sc, sc, sc, sc, sc, sc, sc, sc};
             f32x4& sum = kScaled ? part[j & 1] : acc[j & 1];
-            sum = Mma<true>::mma(f, Mma<true>::bits(b[j]), sum);
+            sum = Mma<true>::mma(ring.weights(u, j), Mma<true>::bits(b[j]), sum);
         }
         if constexpr (kScaled) {
             const float x = xs_lds[lr * KT + kt];
@@ -192,7 +215,7 @@ __global__ __launch_bounds__(64 * kQ4DecWaves) void k_q4_dec(Q4DecArgs A) {
             if (kt + u >= k1) break;
             __builtin_amdgcn_sched_barrier(0);
             multiply(kt + u, u);
-            fetch(kt + U + u, u);
+            ring.fetch(rw, rs, kt + U + u, u, lane);
         }
     }
     acc[0] += acc[1];
@@ -213,6 +236,118 @@ __global__ __launch_bounds__(64 * kQ4DecWaves) void k_q4_dec(Q4DecArgs A) {
         const int n = L.w.gated ? o * 8 + r : o * 16 + r;
         if (tt < np && o < RT && n < width && (!L.w.gated || r < 8)) q4_store(L, (size_t)(begin + tt) * width + n, v);
     }
+}
+
+// The down projections of a token's routes and their weighted sum, for a few tokens: a wave per
+// route, all on the same row tile, whose results are summed in route order (the shared
+// expert last) and rounded once.  Each wave stages its own row of h as k_q4_dec does, so
+// the only barrier is the one before the sum.
+template <int NG, int U>
+__global__ __launch_bounds__(1024) void k_q4_dec_sum(Q4DecSumArgs A) {
+    extern __shared__ __attribute__((aligned(16))) unsigned char staged[];
+    const int RT = A.RT, KT = A.KT, tok = blockIdx.x / RT, rt = blockIdx.x - tok * RT;
+    const int wave = wave_id(), waves = blockDim.x >> 6, lane = threadIdx.x & 63, t = lane & 15, q = lane >> 4;
+    const int ke = A.routes.top_k + A.routes.shared, cols = A.w.cols, pitch = KT * 256 + kQ4LdsPad;
+    float* red = reinterpret_cast<float*>(staged + waves * pitch);  // [ke][16]
+    float* weight = red + ke * 16;
+    unsigned char* mine = staged + wave * pitch;
+    for (int k = wave; k < ke; k += waves) {
+        const int expert = A.routes.expert(tok, k, A.w.n_mats);
+        const bool other = expert == A.w.n_mats;
+        const cx_q4_desc& w = other ? A.shared : A.w;
+        const size_t tile0 = ((size_t)(other ? 0 : max(expert, 0)) * RT + rt) * (size_t)KT;
+        const uint32_t tiles = expert < 0 ? 0 : (uint32_t)KT;  // none: zeros
+        const __amdgpu_buffer_rsrc_t rw = make_rsrc(w.codes + tile0 * kQ4Tile, tiles * kQ4Tile);
+        const __amdgpu_buffer_rsrc_t rs = make_rsrc(w.scales + tile0 * 16 * NG, tiles * 32 * NG);
+        Q4Ring<NG, U> ring;
+        // h: the row's largest value first, then its fp16 image
+        const float* h = A.h + ((size_t)tok * ke + k) * cols;
+        uint32_t most = 0;
+        f32x4 held[kQ4SumHeld][2];
+        auto piece = [&](int c, f32x4 (&v)[2]) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i >> 2][i & 3] = c + i < cols ? h[c + i] : 0.0f;
+        };
+        const bool vec = cols % 8 == 0;
+#pragma unroll
+        for (int i = 0; i < kQ4SumHeld; ++i) {
+            const int c = (i * 64 + lane) * 8;
+            held[i][0] = held[i][1] = f32x4{};
+            if (c >= cols) continue;
+            if (vec) {
+                held[i][0] = *reinterpret_cast<const f32x4*>(h + c);
+                held[i][1] = *reinterpret_cast<const f32x4*>(h + c + 4);
+            } else {
+                piece(c, held[i]);
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) ring.fetch(rw, rs, u, u, lane);
+        // a route that is left out: no weight, whatever its row holds (the gate/up launch has reported it)
+        const bool used = expert >= 0 && A.routes.fault(tok, k, A.w.n_mats, lane) == 0;
+        if (lane == 0) weight[k] = !used ? 0.0f : k < A.routes.top_k ? A.routes.weights[(size_t)tok * A.routes.top_k + k] : 1.0f;
+        auto take = [&](const f32x4 (&v)[2]) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const uint32_t b = __float_as_uint(v[i >> 2][i & 3]) & 0x7FFFFFFFu;
+                if (b < 0x7F800000u) most = max(most, b);
+            }
+        };
+#pragma unroll
+        for (int i = 0; i < kQ4SumHeld; ++i) take(held[i]);
+        for (int c = (kQ4SumHeld * 64 + lane) * 8; c < cols; c += 512) {
+            f32x4 v[2];
+            piece(c, v);
+            take(v);
+        }
+#pragma unroll
+        for (int m = 32; m >= 1; m >>= 1) most = max(most, (uint32_t)__shfl_xor((int)most, m));
+        const int e = most == 0 ? 127 : min(max((int)(most >> 23) - 14, 1), 253);
+        const float up = __uint_as_float((uint32_t)(254 - e) << 23), down = __uint_as_float((uint32_t)e << 23);
+        auto put = [&](int c, const f32x4 (&v)[2]) {
+            uint32_t o[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) o[i] = f16_rne(v[i >> 1][2 * (i & 1)] * up) | (f16_rne(v[i >> 1][2 * (i & 1) + 1] * up) << 16);
+            *reinterpret_cast<u32x4*>(mine + c * 2) = u32x4{o[0], o[1], o[2], o[3]};
+        };
+#pragma unroll
+        for (int i = 0; i < kQ4SumHeld; ++i)
+            if ((i * 64 + lane) * 8 < KT * 128) put((i * 64 + lane) * 8, held[i]);
+        for (int c = (kQ4SumHeld * 64 + lane) * 8; c < KT * 128; c += 512) {
+            f32x4 v[2] = {};
+            if (c < cols) piece(c, v);
+            put(c, v);
+        }
+        __builtin_amdgcn_wave_barrier();
+        f32x4 acc[2] = {};
+        for (int kt = 0; kt < KT; kt += U) {
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                if (kt + u >= KT) break;
+                __builtin_amdgcn_sched_barrier(0);
+                u32x4 b[4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) b[j] = *reinterpret_cast<const u32x4*>(mine + (kt + u) * 256 + j * 64 + q * 16);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) acc[j & 1] = Mma<true>::mma(ring.weights(u, j), Mma<true>::bits(b[j]), acc[j & 1]);
+                ring.fetch(rw, rs, kt + U + u, u, lane);
+            }
+        }
+        if (t == 0) {
+            const f32x4 scale = *reinterpret_cast<const f32x4*>(q4_row_scales(w) + tile0 / KT * 16 + 4 * q);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) red[k * 16 + 4 * q + i] = used ? (acc[0][i] + acc[1][i]) * scale[i] * down : 0.0f;
+        }
+        __builtin_amdgcn_wave_barrier();
+    }
+    __syncthreads();
+    const int n = rt * 16 + threadIdx.x;
+    if (threadIdx.x >= 16 || n >= A.w.rows) return;
+    float v = 0.0f;
+    for (int k = 0; k < ke; ++k) v += weight[k] * red[k * 16 + threadIdx.x];
+    const size_t at = (size_t)tok * A.w.rows + n;
+    static_cast<uint16_t*>(A.y)[at] = (uint16_t)cast_out(v, A.out_dtype);
+    if (A.y_f32 != nullptr) A.y_f32[at] = v;
 }
 
 }  // namespace cx

@@ -23,20 +23,28 @@ hipError_t dec_groups(const Q4DecArgs& A, int64_t items, hipStream_t s) {
 
 }  // namespace
 
-hipError_t launch_q4_dec(const Q4Launch& L, int splits, int64_t items, hipStream_t s) {
+hipError_t launch_q4_dec(const Q4Launch& L, const Q4Routes* routes, int splits, int64_t items, hipStream_t s) {
     Q4DecArgs A{};
     A.L = L;
+    if (routes) A.routes = *routes;
     A.RT = q4_row_tiles(L.w);
     A.KT = q4_col_tiles(L.w);
     A.splits = splits;
     A.row_blocks = (A.RT + kQ4DecWaves / splits - 1) / (kQ4DecWaves / splits);
-    A.lds_rows = std::min(L.item_rows, L.n_rows);
+    A.lds_rows = routes ? 1 : std::min(L.item_rows, L.n_rows);
     switch (L.x_type) {
         case kQ4Bf16: return dec_groups<kQ4Bf16>(A, items, s);
         case kQ4Fp16: return dec_groups<kQ4Fp16>(A, items, s);
         case kQ4F32: return dec_groups<kQ4F32>(A, items, s);
         default: return dec_groups<kQ4E4m3>(A, items, s);
     }
+}
+
+hipError_t launch_q4_dec_sum(const Q4DecSumArgs& A, int n_tokens, hipStream_t s) {
+    const int ke = A.routes.top_k + A.routes.shared, waves = std::min(ke, 16);
+    auto k = A.w.group == 128 ? k_q4_dec_sum<1, 12> : A.w.group == 64 ? k_q4_dec_sum<2, 12> : k_q4_dec_sum<4, 10>;
+    cx_launch(k, dim3((unsigned)(n_tokens * A.RT)), dim3(64 * waves), (uint32_t)q4_sum_lds(A.w.cols, ke), s, A);
+    return hipGetLastError();
 }
 
 }  // namespace cx

@@ -1678,6 +1678,14 @@ int cx_q4_moe(cx_ctx* ctx, const cx_q4_desc* gate_up, const cx_q4_desc* down, co
     c.out = y;
     c.out_f32 = y_f32;
     c.err_flag = ctx->err_flag;
+    if (q4_routes_ok(n_tokens, top_k, down->rows, down->cols, shared)) {
+        L.order = nullptr;
+        L.items = nullptr;
+        L.item_rows = 1;
+        Span sp(ctx, "experts", s);
+        CX_HIP(launch_q4_routes(L, D, Q4Routes{topk_ids, topk_w, top_k, shared, ctx->err_flag}, n_tokens, y, out_dtype, y_f32, s));
+        return CX_OK;
+    }
     if (!q4_grid_ok(L) || !q4_grid_ok(D) || !rows_grid_ok(combine_workgroups(c), kRowThreads))
         return fail(CX_EINVAL, "too many rows for one launch");
     {
