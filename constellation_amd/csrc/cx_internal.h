@@ -417,11 +417,14 @@ struct Q4Routes {
         const int e = ids[(size_t)t * top_k + k];
         return e >= 0 && e < n_mats ? e : -1;
     }
-    // Why the route is to be left out all the same (0: it is not): one look at the ids before it, a lane each.
-    __device__ __forceinline__ int fault(int t, int k, int n_mats, int lane) const {
+    // Why the route is to be left out all the same (0: it is not), with what `before` loaded: the
+    // token's earlier ids, a lane each.
+    __device__ __forceinline__ int before(int t, int k, int lane) const {
+        return k < top_k && lane < k ? ids[(size_t)t * top_k + lane] : -1;  // top_k is at most 64
+    }
+    __device__ __forceinline__ int fault(int t, int k, int n_mats, int before) const {
         if (k == top_k) return 0;
-        const int32_t* row = ids + (size_t)t * top_k;
-        const int e = row[k], before = lane < k ? row[lane] : -1;  // top_k is at most 64
+        const int e = ids[(size_t)t * top_k + k];
         if (e < 0) return 0;
         int bad = e >= n_mats ? kErrBadExpertId : 0;
         if (__ballot(before == e) != 0) bad |= kErrDuplicateRoute;

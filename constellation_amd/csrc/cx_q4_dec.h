@@ -74,7 +74,7 @@ __global__ __launch_bounds__(64 * kQ4DecWaves) void k_q4_dec(Q4DecArgs A) {
         x_row = idx / ke;
         expert = A.routes.expert(x_row, idx - x_row * ke, L.w.n_mats);
         if (block == 0 && wave == 0) {
-            const int err = A.routes.fault(x_row, idx - x_row * ke, L.w.n_mats, lane);
+            const int k = idx - x_row * ke, err = A.routes.fault(x_row, k, L.w.n_mats, A.routes.before(x_row, k, lane));
             if (err && lane == 0) atomicOr(A.routes.err_flag, err);
         }
         if (expert < 0) return;  // its row is not read
@@ -246,105 +246,86 @@ template <int NG, int U>
 __global__ __launch_bounds__(1024) void k_q4_dec_sum(Q4DecSumArgs A) {
     extern __shared__ __attribute__((aligned(16))) unsigned char staged[];
     const int RT = A.RT, KT = A.KT, tok = blockIdx.x / RT, rt = blockIdx.x - tok * RT;
-    const int wave = wave_id(), waves = blockDim.x >> 6, lane = threadIdx.x & 63, t = lane & 15, q = lane >> 4;
-    const int ke = A.routes.top_k + A.routes.shared, cols = A.w.cols, pitch = KT * 256 + kQ4LdsPad;
-    float* red = reinterpret_cast<float*>(staged + waves * pitch);  // [ke][16]
+    const int wave = wave_id(), lane = threadIdx.x & 63, t = lane & 15, q = lane >> 4;
+    const int ke = A.routes.top_k + A.routes.shared, cols = A.w.cols, pitch = KT * 256 + kQ4LdsPad, k = wave;
+    float* red = reinterpret_cast<float*>(staged + ke * pitch);  // [ke][16]
     float* weight = red + ke * 16;
     unsigned char* mine = staged + wave * pitch;
-    for (int k = wave; k < ke; k += waves) {
-        const int expert = A.routes.expert(tok, k, A.w.n_mats);
-        const bool other = expert == A.w.n_mats;
-        const cx_q4_desc& w = other ? A.shared : A.w;
-        const size_t tile0 = ((size_t)(other ? 0 : max(expert, 0)) * RT + rt) * (size_t)KT;
-        const uint32_t tiles = expert < 0 ? 0 : (uint32_t)KT;  // none: zeros
-        const __amdgpu_buffer_rsrc_t rw = make_rsrc(w.codes + tile0 * kQ4Tile, tiles * kQ4Tile);
-        const __amdgpu_buffer_rsrc_t rs = make_rsrc(w.scales + tile0 * 16 * NG, tiles * 32 * NG);
-        Q4Ring<NG, U> ring;
-        // h: the row's largest value first, then its fp16 image
-        const float* h = A.h + ((size_t)tok * ke + k) * cols;
-        uint32_t most = 0;
-        f32x4 held[kQ4SumHeld][2];
-        auto piece = [&](int c, f32x4 (&v)[2]) {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) v[i >> 2][i & 3] = c + i < cols ? h[c + i] : 0.0f;
-        };
-        const bool vec = cols % 8 == 0;
-#pragma unroll
-        for (int i = 0; i < kQ4SumHeld; ++i) {
-            const int c = (i * 64 + lane) * 8;
-            held[i][0] = held[i][1] = f32x4{};
-            if (c >= cols) continue;
-            if (vec) {
-                held[i][0] = *reinterpret_cast<const f32x4*>(h + c);
-                held[i][1] = *reinterpret_cast<const f32x4*>(h + c + 4);
-            } else {
-                piece(c, held[i]);
-            }
-        }
-#pragma unroll
-        for (int u = 0; u < U; ++u) ring.fetch(rw, rs, u, u, lane);
-        // a route that is left out: no weight, whatever its row holds (the gate/up launch has reported it)
-        const bool used = expert >= 0 && A.routes.fault(tok, k, A.w.n_mats, lane) == 0;
-        if (lane == 0) weight[k] = !used ? 0.0f : k < A.routes.top_k ? A.routes.weights[(size_t)tok * A.routes.top_k + k] : 1.0f;
-        auto take = [&](const f32x4 (&v)[2]) {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const uint32_t b = __float_as_uint(v[i >> 2][i & 3]) & 0x7FFFFFFFu;
-                if (b < 0x7F800000u) most = max(most, b);
-            }
-        };
-#pragma unroll
-        for (int i = 0; i < kQ4SumHeld; ++i) take(held[i]);
-        for (int c = (kQ4SumHeld * 64 + lane) * 8; c < cols; c += 512) {
-            f32x4 v[2];
-            piece(c, v);
-            take(v);
-        }
-#pragma unroll
-        for (int m = 32; m >= 1; m >>= 1) most = max(most, (uint32_t)__shfl_xor((int)most, m));
-        const int e = most == 0 ? 127 : min(max((int)(most >> 23) - 14, 1), 253);
-        const float up = __uint_as_float((uint32_t)(254 - e) << 23), down = __uint_as_float((uint32_t)e << 23);
-        auto put = [&](int c, const f32x4 (&v)[2]) {
-            uint32_t o[4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) o[i] = f16_rne(v[i >> 1][2 * (i & 1)] * up) | (f16_rne(v[i >> 1][2 * (i & 1) + 1] * up) << 16);
-            *reinterpret_cast<u32x4*>(mine + c * 2) = u32x4{o[0], o[1], o[2], o[3]};
-        };
+    // in the order of their waits: h's row and the token's other ids, then the weights
+    const __amdgpu_buffer_rsrc_t rh = make_rsrc(A.h + ((size_t)tok * ke + k) * cols, (uint32_t)cols * 4);
+    u32x4 held[kQ4SumHeld][2];
+    if (cols % 8 == 0) {
 #pragma unroll
         for (int i = 0; i < kQ4SumHeld; ++i)
-            if ((i * 64 + lane) * 8 < KT * 128) put((i * 64 + lane) * 8, held[i]);
-        for (int c = (kQ4SumHeld * 64 + lane) * 8; c < KT * 128; c += 512) {
-            f32x4 v[2] = {};
-            if (c < cols) piece(c, v);
-            put(c, v);
+#pragma unroll
+            for (int d = 0; d < 2; ++d) held[i][d] = bld16(rh, (uint32_t)(i * 64 + lane) * 32 + 16 * d);
+    } else {
+#pragma unroll
+        for (int i = 0; i < kQ4SumHeld; ++i)
+#pragma unroll
+            for (int d = 0; d < 8; ++d) held[i][d >> 2][d & 3] = __builtin_amdgcn_raw_buffer_load_b32(rh, (uint32_t)(i * 64 + lane) * 32 + 4 * d, 0, 0);
+    }
+    const int before = A.routes.before(tok, k, lane), expert = A.routes.expert(tok, k, A.w.n_mats);
+    const bool other = expert == A.w.n_mats;
+    const cx_q4_desc& w = other ? A.shared : A.w;
+    const size_t tile0 = ((size_t)(other ? 0 : max(expert, 0)) * RT + rt) * (size_t)KT;
+    const uint32_t tiles = expert < 0 ? 0 : (uint32_t)KT;  // none: zeros
+    const __amdgpu_buffer_rsrc_t rw = make_rsrc(w.codes + tile0 * kQ4Tile, tiles * kQ4Tile);
+    const __amdgpu_buffer_rsrc_t rs = make_rsrc(w.scales + tile0 * 16 * NG, tiles * 32 * NG);
+    Q4Ring<NG, U> ring;
+#pragma unroll
+    for (int u = 0; u < U; ++u) ring.fetch(rw, rs, u, u, lane);
+    __builtin_amdgcn_sched_barrier(0);
+    // a route that is left out: no weight, whatever its row holds (the gate/up launch has reported it)
+    const bool used = expert >= 0 && A.routes.fault(tok, k, A.w.n_mats, before) == 0;
+    if (lane == 0) weight[k] = !used ? 0.0f : k < A.routes.top_k ? A.routes.weights[(size_t)tok * A.routes.top_k + k] : 1.0f;
+    uint32_t most = 0;
+#pragma unroll
+    for (int i = 0; i < kQ4SumHeld; ++i)
+#pragma unroll
+        for (int d = 0; d < 8; ++d) {
+            const uint32_t b = held[i][d >> 2][d & 3] & 0x7FFFFFFFu;
+            if (b < 0x7F800000u) most = max(most, b);
         }
-        __builtin_amdgcn_wave_barrier();
-        f32x4 acc[2] = {};
-        for (int kt = 0; kt < KT; kt += U) {
 #pragma unroll
-            for (int u = 0; u < U; ++u) {
-                if (kt + u >= KT) break;
-                __builtin_amdgcn_sched_barrier(0);
-                u32x4 b[4];
+    for (int m = 32; m >= 1; m >>= 1) most = max(most, (uint32_t)__shfl_xor((int)most, m));
+    const int e = most == 0 ? 127 : min(max((int)(most >> 23) - 14, 1), 253);
+    const float up = __uint_as_float((uint32_t)(254 - e) << 23), down = __uint_as_float((uint32_t)e << 23);
 #pragma unroll
-                for (int j = 0; j < 4; ++j) b[j] = *reinterpret_cast<const u32x4*>(mine + (kt + u) * 256 + j * 64 + q * 16);
+    for (int i = 0; i < kQ4SumHeld; ++i) {
+        const int c = (i * 64 + lane) * 8;
+        if (c >= KT * 128) continue;
+        u32x4 o;
 #pragma unroll
-                for (int j = 0; j < 4; ++j) acc[j & 1] = Mma<true>::mma(ring.weights(u, j), Mma<true>::bits(b[j]), acc[j & 1]);
-                ring.fetch(rw, rs, kt + U + u, u, lane);
-            }
+        for (int d = 0; d < 4; ++d)
+            o[d] = f16_rne(__uint_as_float(held[i][d >> 1][2 * (d & 1)]) * up) | (f16_rne(__uint_as_float(held[i][d >> 1][2 * (d & 1) + 1]) * up) << 16);
+        *reinterpret_cast<u32x4*>(mine + c * 2) = o;
+    }
+    __builtin_amdgcn_wave_barrier();
+    f32x4 acc[2] = {};
+    for (int kt = 0; kt < KT; kt += U) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            if (kt + u >= KT) break;
+            __builtin_amdgcn_sched_barrier(0);
+            u32x4 b[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) b[j] = *reinterpret_cast<const u32x4*>(mine + (kt + u) * 256 + j * 64 + q * 16);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) acc[j & 1] = Mma<true>::mma(ring.weights(u, j), Mma<true>::bits(b[j]), acc[j & 1]);
+            ring.fetch(rw, rs, kt + U + u, u, lane);
         }
-        if (t == 0) {
-            const f32x4 scale = *reinterpret_cast<const f32x4*>(q4_row_scales(w) + tile0 / KT * 16 + 4 * q);
+    }
+    if (t == 0) {
+        const f32x4 scale = *reinterpret_cast<const f32x4*>(q4_row_scales(w) + tile0 / KT * 16 + 4 * q);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) red[k * 16 + 4 * q + i] = used ? (acc[0][i] + acc[1][i]) * scale[i] * down : 0.0f;
-        }
-        __builtin_amdgcn_wave_barrier();
+        for (int i = 0; i < 4; ++i) red[k * 16 + 4 * q + i] = used ? (acc[0][i] + acc[1][i]) * scale[i] * down : 0.0f;
     }
     __syncthreads();
     const int n = rt * 16 + threadIdx.x;
     if (threadIdx.x >= 16 || n >= A.w.rows) return;
     float v = 0.0f;
-    for (int k = 0; k < ke; ++k) v += weight[k] * red[k * 16 + threadIdx.x];
+    for (int r = 0; r < ke; ++r) v += weight[r] * red[r * 16 + threadIdx.x];
     const size_t at = (size_t)tok * A.w.rows + n;
     static_cast<uint16_t*>(A.y)[at] = (uint16_t)cast_out(v, A.out_dtype);
     if (A.y_f32 != nullptr) A.y_f32[at] = v;

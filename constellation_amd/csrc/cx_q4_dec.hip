@@ -41,9 +41,9 @@ hipError_t launch_q4_dec(const Q4Launch& L, const Q4Routes* routes, int splits, 
 }
 
 hipError_t launch_q4_dec_sum(const Q4DecSumArgs& A, int n_tokens, hipStream_t s) {
-    const int ke = A.routes.top_k + A.routes.shared, waves = std::min(ke, 16);
-    auto k = A.w.group == 128 ? k_q4_dec_sum<1, 12> : A.w.group == 64 ? k_q4_dec_sum<2, 12> : k_q4_dec_sum<4, 10>;
-    cx_launch(k, dim3((unsigned)(n_tokens * A.RT)), dim3(64 * waves), (uint32_t)q4_sum_lds(A.w.cols, ke), s, A);
+    const int ke = A.routes.top_k + A.routes.shared;
+    auto k = A.w.group == 128 ? k_q4_dec_sum<1, 12> : A.w.group == 64 ? k_q4_dec_sum<2, 12> : k_q4_dec_sum<4, 12>;
+    cx_launch(k, dim3((unsigned)(n_tokens * A.RT)), dim3(64 * ke), (uint32_t)q4_sum_lds(A.w.cols, ke), s, A);
     return hipGetLastError();
 }
 

@@ -285,14 +285,14 @@ inline int q4_dec_rows(int cols) {
     while (rows > 0 && q4_dec_lds(cols, rows) > 63 * 1024) --rows;
     return rows;
 }
-// LDS of the down projections and sum of one token's routes: a staged row per wave, 16 sums and a weight per route.
+// LDS of the down projections and sum of one token's routes: a staged row, 16 sums and a weight per route, a
+// wave each.
 constexpr int kQ4SumHeld = 4;  // 8-value pieces of a row per lane
-inline size_t q4_sum_lds(int cols, int routes) {
-    return (size_t)std::min(routes, 16) * ((size_t)((cols + 127) / 128) * 256 + kQ4LdsPad) + (size_t)routes * 68;
-}
+inline size_t q4_sum_lds(int cols, int routes) { return (size_t)routes * ((size_t)((cols + 127) / 128) * 256 + kQ4LdsPad + 68); }
 // A layer on one token's routes, without a plan.
 inline bool q4_routes_ok(int n_tokens, int top_k, int hidden, int inter, int shared) {
-    return n_tokens == 1 && hidden <= kQ4DecCols && q4_sum_lds(inter, top_k + shared) <= 60 * 1024;
+    return n_tokens == 1 && hidden <= kQ4DecCols && inter <= kQ4SumHeld * 512 && top_k + shared <= 16 &&
+           q4_sum_lds(inter, top_k + shared) <= 63 * 1024;
 }
 inline int q4_item_rows(int64_t n_rows, int n_mats, int cols, bool two_sums) {
     const int dec = q4_dec_rows(cols);
