@@ -326,6 +326,13 @@ struct Q4Item {
     int expert, begin, rows, pad;
 };
 
+// Items from, from + step, ... of the n that rows begin .. begin + rows - 1 of a matrix are cut
+// to: equal ones of whole 16-row tiles, so that the last is not a short one.
+__device__ inline void q4_put_items(Q4Item* items, int n, int expert, int begin, int rows, int from, int step) {
+    const int per = n == 0 ? 0 : n == 1 || rows < 16 * n ? (rows + n - 1) / n : (rows + 16 * n - 1) / (16 * n) * 16;
+    for (int i = from; i < n; i += step) items[i] = Q4Item{expert, begin + i * per, max(0, min(per, rows - i * per)), 0};
+}
+
 struct SortArgs {
     const int32_t* ids;    // [n_tokens, top_k]
     const float* weights;  // nullable: when given, a repeated expert or a bad weight is an error and its pair's place negative

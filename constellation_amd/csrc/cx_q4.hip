@@ -73,40 +73,111 @@ __global__ __launch_bounds__(256) void k_q4_row_scales(cx_q4_desc w, const uint1
 // zeros behind the row.  The row's largest value comes to 2^14 .. 2^15, so bf16
 // values (8 significant bits) are exact down to 2^-31 of it and the others off by less than
 // 2^-39 of it: nothing next to the sums' own 2^-24.  fp32 values are rounded to 11 bits.
+//
+// A row is read once, kPieces pieces of 8 values a thread in registers (wider rows are read
+// again for what lies behind), 16 bytes at a time where it starts on them.
+constexpr int kRowPieces = 4;
+
+template <int DT>
+__device__ __forceinline__ void q4_row_piece(const void* x, size_t row, int c, int cols, bool vec, float (&v)[8]) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = 0.0f;
+    if (c >= cols) return;
+    if constexpr (DT == CX_DTYPE_F32) {
+        const float* p = static_cast<const float*>(x) + row + c;
+        if (vec) {
+            const f32x4 a = *reinterpret_cast<const f32x4*>(p), b = *reinterpret_cast<const f32x4*>(p + 4);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) v[i] = a[i], v[4 + i] = b[i];
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                if (c + i < cols) v[i] = p[i];
+        }
+    } else if constexpr (DT == CX_DTYPE_E4M3) {
+        const uint8_t* p = static_cast<const uint8_t*>(x) + row + c;
+        uint32_t a = 0, b = 0;
+        if (vec) {
+            const uint2 d = *reinterpret_cast<const uint2*>(p);
+            a = d.x, b = d.y;
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                if (c + i < cols) (i < 4 ? a : b) |= (uint32_t)p[i] << (8 * (i & 3));
+        }
+        const f16x8 f = cvt8_f16(a, b);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = (float)f[i];
+    } else {
+        const uint16_t* p = static_cast<const uint16_t*>(x) + row + c;
+        uint32_t h[8] = {};
+        if (vec) {
+            const u32x4 d = ld16(p);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) h[i] = i & 1 ? d[i >> 1] >> 16 : d[i >> 1] & 0xFFFFu;
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                if (c + i < cols) h[i] = p[i];
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            v[i] = DT == CX_DTYPE_BF16 ? __uint_as_float(h[i] << 16) : (float)__builtin_bit_cast(_Float16, (uint16_t)h[i]);
+    }
+}
+
+// e4m3 rows (exact in fp16) and fp16 rows are copied as they are, with a scale of 1.
 template <int DT>
 __global__ __launch_bounds__(256) void k_q4_rows(const void* x, int cols, int padded, uint16_t* dst, float* scale) {
     __shared__ uint32_t part[4];
     const int tid = threadIdx.x;
-    const size_t row = (size_t)blockIdx.x * cols;
-    auto value = [&](int c) {
-        if constexpr (DT == CX_DTYPE_F32)
-            return static_cast<const float*>(x)[row + c];
-        else if constexpr (DT == CX_DTYPE_BF16)
-            return __uint_as_float((uint32_t)static_cast<const uint16_t*>(x)[row + c] << 16);
-        else
-            return static_cast<float>(static_cast<const _Float16*>(x)[row + c]);
-    };
-    uint32_t most = 0;
-    for (int c = tid; c < cols; c += 256) {
-        const uint32_t b = __float_as_uint(value(c)) & 0x7FFFFFFFu;
-        if (b < 0x7F800000u) most = max(most, b);
-    }
+    const size_t row = (size_t)blockIdx.x * cols, out = (size_t)blockIdx.x * padded;
+    constexpr int kEl = DT == CX_DTYPE_F32 ? 4 : DT == CX_DTYPE_E4M3 ? 1 : 2, kSpan = kRowPieces * 256 * 8;
+    const bool vec = cols % 8 == 0 && (reinterpret_cast<uintptr_t>(x) & (kEl == 1 ? 7 : 15)) == 0;
+    float v[kRowPieces][8];
 #pragma unroll
-    for (int m = 32; m >= 1; m >>= 1) most = max(most, (uint32_t)__shfl_xor((int)most, m));
-    if ((tid & 63) == 0) part[tid >> 6] = most;
-    __syncthreads();
-    most = max(max(part[0], part[1]), max(part[2], part[3]));
-    const int e = most == 0 ? 127 : min(max((int)(most >> 23) - 14, 1), 253);
-    const float up = __uint_as_float((uint32_t)(254 - e) << 23);
-    if (tid == 0) scale[blockIdx.x] = __uint_as_float((uint32_t)e << 23);
-    for (int c = tid; c < padded; c += 256) dst[(size_t)blockIdx.x * padded + c] = c < cols ? (uint16_t)f16_rne(value(c) * up) : 0;
-}
-
-// Rows of e4m3 as fp16 (exact) in rows of whole 128-column tiles, zeros behind the row.
-__global__ __launch_bounds__(256) void k_q4_rows8(const uint8_t* x, int cols, int padded, uint16_t* dst) {
-    for (int c = threadIdx.x; c < padded; c += 256) {
-        const uint32_t v = c < cols ? x[(size_t)blockIdx.x * cols + c] : 0;
-        dst[(size_t)blockIdx.x * padded + c] = __builtin_bit_cast(uint16_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(v, 1.0f, false)[0]);
+    for (int i = 0; i < kRowPieces; ++i) q4_row_piece<DT>(x, row, (i * 256 + tid) * 8, cols, vec, v[i]);
+    float up = 1.0f;
+    if constexpr (DT == CX_DTYPE_BF16 || DT == CX_DTYPE_F32) {
+        uint32_t most = 0;
+        auto take = [&](const float (&f)[8]) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const uint32_t b = __float_as_uint(f[i]) & 0x7FFFFFFFu;
+                if (b < 0x7F800000u) most = max(most, b);
+            }
+        };
+#pragma unroll
+        for (int i = 0; i < kRowPieces; ++i) take(v[i]);
+        for (int c = kSpan + tid * 8; c < cols; c += 2048) {
+            float f[8];
+            q4_row_piece<DT>(x, row, c, cols, vec, f);
+            take(f);
+        }
+#pragma unroll
+        for (int m = 32; m >= 1; m >>= 1) most = max(most, (uint32_t)__shfl_xor((int)most, m));
+        if ((tid & 63) == 0) part[tid >> 6] = most;
+        __syncthreads();
+        most = max(max(part[0], part[1]), max(part[2], part[3]));
+        const int e = most == 0 ? 127 : min(max((int)(most >> 23) - 14, 1), 253);
+        up = __uint_as_float((uint32_t)(254 - e) << 23);
+        if (tid == 0) scale[blockIdx.x] = __uint_as_float((uint32_t)e << 23);
+    } else if (tid == 0) {
+        scale[blockIdx.x] = 1.0f;
+    }
+    auto put = [&](int c, const float (&f)[8]) {
+        u32x4 o;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) o[i] = f16_rne(f[2 * i] * up) | (f16_rne(f[2 * i + 1] * up) << 16);
+        *reinterpret_cast<u32x4*>(dst + out + c) = o;
+    };
+#pragma unroll
+    for (int i = 0; i < kRowPieces; ++i)
+        if ((i * 256 + tid) * 8 < padded) put((i * 256 + tid) * 8, v[i]);
+    for (int c = kSpan + tid * 8; c < padded; c += 2048) {
+        float f[8];
+        q4_row_piece<DT>(x, row, c, cols, vec, f);
+        put(c, f);
     }
 }
 
@@ -136,11 +207,9 @@ __global__ __launch_bounds__(1024) void k_q4_items(const int32_t* offsets, int n
         cnt[e] = v;
         __syncthreads();
     }
-    Q4Item* at = items + 1 + cnt[e] - n;
-    for (int i = 0; i < n; ++i) at[i] = Q4Item{e, begin + i * item_rows, min(item_rows, rows - i * item_rows), 0};
+    q4_put_items(items + 1 + cnt[e] - n, n, e, begin, rows, 0, 1);
     const int held = top[1023], all = cnt[1023], rest = (n_rows - held + item_rows - 1) / item_rows;
-    for (int i = e; i < rest; i += 1024)  // rows behind the last matrix's: zeros
-        items[1 + all + i] = Q4Item{-1, held + i * item_rows, min(item_rows, n_rows - held - i * item_rows), 0};
+    q4_put_items(items + 1 + all, rest, -1, held, n_rows - held, e, 1024);  // rows behind the last matrix's: zeros
     if (e == 0) items[0] = Q4Item{all + rest, held, 0, 0};
 }
 
@@ -224,18 +293,16 @@ hipError_t launch_q4(const Q4Launch& L, hipStream_t s) {
     if (L.item_rows > kTileTok) {
         const int padded = q4_col_tiles(L.w) * 128;
         Q4Launch G = L;
-        if (L.x_type == kQ4E4m3) {
-            if (L.n_x > 0)
-                cx_launch(k_q4_rows8, dim3((unsigned)L.n_x), dim3(256), 0, s, static_cast<const uint8_t*>(L.x), L.w.cols, padded,
-                          static_cast<uint16_t*>(L.x_scratch));
-            G.x = L.x_scratch;
-        } else if (L.x_type != kQ4Fp16 || padded != L.w.cols || !dma_aligned(L.x)) {
+        if (L.x_type != kQ4Fp16 || padded != L.w.cols || !dma_aligned(L.x)) {
             uint16_t* x = static_cast<uint16_t*>(L.x_scratch);
             float* scale = reinterpret_cast<float*>(static_cast<char*>(L.x_scratch) + up256((size_t)L.n_x * padded * 2));
-            auto k = L.x_type == kQ4Bf16 ? k_q4_rows<CX_DTYPE_BF16> : L.x_type == kQ4Fp16 ? k_q4_rows<CX_DTYPE_FP16> : k_q4_rows<CX_DTYPE_F32>;
+            auto k = L.x_type == kQ4Bf16   ? k_q4_rows<CX_DTYPE_BF16>
+                     : L.x_type == kQ4Fp16 ? k_q4_rows<CX_DTYPE_FP16>
+                     : L.x_type == kQ4F32  ? k_q4_rows<CX_DTYPE_F32>
+                                           : k_q4_rows<CX_DTYPE_E4M3>;
             if (L.n_x > 0) cx_launch(k, dim3((unsigned)L.n_x), dim3(256), 0, s, L.x, L.w.cols, padded, x, scale);
             G.x = x;
-            G.x_scale = scale;
+            if (L.x_type != kQ4E4m3) G.x_scale = scale;
         }
         return launch_q4_gemm(G, s);
     }

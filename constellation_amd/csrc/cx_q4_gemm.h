@@ -185,6 +185,16 @@ __device__ __forceinline__ void q4_gemm_tile(const Q4GemmArgs& L, unsigned char*
 #pragma unroll
             for (int n = 0; n < NT; ++n) xs[to][n] = xsp[n][kt];
     };
+    auto scaled_add = [&](auto from, int n) {
+        if constexpr (XS) {
+#pragma unroll
+            for (int m = 0; m < RTW; ++m) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) sum[n][m][i] = __builtin_fmaf(xs[from][n], acc[n][m][i], sum[n][m][i]);
+                asm volatile("" : "+v"(sum[n][m]));
+            }
+        }
+    };
     auto multiply = [&](auto from, const unsigned char* buf) {
         // Steps of RTW MFMAs on one fragment of x, in this order: the fragment after the
         // next is read and the next columns' weights are converted while they run.
@@ -213,22 +223,17 @@ __device__ __forceinline__ void q4_gemm_tile(const Q4GemmArgs& L, unsigned char*
 #pragma unroll
             for (int m = 0; m < RTW; ++m)
                 acc[n][m] = Mma<true>::mma(fa[j & 1][m], Mma<true>::bits(b[i % 3]), XS && j == 0 ? f32x4{} : acc[n][m]);
+            if (XS && j == 3 && n > 0) scaled_add(from, n - 1);  // while this step's products are on their way
         }
         __builtin_amdgcn_sched_barrier(0);
-        if constexpr (!XS)
+        if constexpr (XS) {
+            scaled_add(from, NT - 1);
+        } else {
 #pragma unroll
             for (int n = 0; n < NT; ++n)
 #pragma unroll
                 for (int m = 0; m < RTW; ++m) asm volatile("" : "+v"(acc[n][m]));  // keeps the sums where they are: no copies of them at the loop's end
-        if constexpr (XS)
-#pragma unroll
-            for (int n = 0; n < NT; ++n)
-#pragma unroll
-                for (int m = 0; m < RTW; ++m) {
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) sum[n][m][i] = __builtin_fmaf(xs[from][n], acc[n][m][i], sum[n][m][i]);
-                    asm volatile("" : "+v"(sum[n][m]));  // keeps the sums where they are: no copies of them at the loop's end
-                }
+        }
     };
     constexpr std::integral_constant<int, 0> even{};
     constexpr std::integral_constant<int, 1> odd{};

@@ -341,11 +341,9 @@ __global__ __launch_bounds__(kSortThreads) void k_sort_tokens(SortArgs a) {
             for (int e = tid; e <= NK; e += kSortThreads) a.offsets[e] = first[e];
         if (a.items != nullptr) {
             for (int e = tid; e < NK; e += kSortThreads)
-                for (int i = items[e], p = first[e]; p < first[e + 1]; ++i, p += a.item_rows)
-                    a.items[1 + i] = Q4Item{e, p, min(a.item_rows, first[e + 1] - p), 0};
+                q4_put_items(a.items + 1 + items[e], items[e + 1] - items[e], e, first[e], first[e + 1] - first[e], 0, 1);
             const int more = (none + a.item_rows - 1) / a.item_rows;
-            for (int i = tid; i < more; i += kSortThreads)
-                a.items[1 + items[NK] + i] = Q4Item{NK, shared_row + i * a.item_rows, min(a.item_rows, none - i * a.item_rows), 0};
+            q4_put_items(a.items + 1 + items[NK], more, NK, shared_row, none, tid, kSortThreads);
             if (tid == 0) a.items[0] = Q4Item{items[NK] + more, shared_row + none, 0, 0};
         }
     }

@@ -233,6 +233,7 @@ class Q4Matrix:
         self.device = device
         self.desc = desc
         self._live = True
+        self._scratch: dict = {}  # sizes by call shape
 
     @classmethod
     def pack(cls, codes: torch.Tensor, scales: torch.Tensor, cols: int, *, group: int = 128,
@@ -497,7 +498,8 @@ class Context:
             raise ValueError("x_scale comes with e4m3 x, and only with it")
         if f8 and (x_scale.shape != (T, (K + 127) // 128) or x_scale.dtype != torch.float32):
             raise ValueError(f"x_scale must be fp32 [{T}, {(K + 127) // 128}]")
-        for name, t, n in (("offsets", offsets, d.n_mats + 1), ("order", order, None)):
+        for name, t, n in (("offsets", offsets, d.n_mats + 1), ("order", order, None)) if offsets is not None or \
+                order is not None else ():
             if t is not None and (t.dtype != torch.int32 or t.dim() != 1 or not t.is_contiguous()
                                   or (n is not None and t.shape[0] != n)):
                 raise ValueError(f"{name} must be a contiguous int32 vector" + (f" of {n}" if n else ""))
@@ -507,7 +509,10 @@ class Context:
         out_dtype = out_dtype or (torch.bfloat16 if f8 else x.dtype)
         y = torch.empty((P, w.out_cols), dtype=out_dtype, device=x.device)
         dt = E4M3 if f8 else cx_dtype(x.dtype)
-        size = lib().cx_q4_scratch(C.byref(d), dt, T, P, int(offsets is not None))
+        key = (dt, T, P, offsets is None)
+        size = w._scratch.get(key)
+        if size is None:
+            size = w._scratch[key] = lib().cx_q4_scratch(C.byref(d), dt, T, P, int(offsets is not None))
         scratch = torch.empty(size, dtype=torch.uint8, device=x.device) if size else None
         check(lib().cx_q4_matmul(self.handle, C.byref(d), x.data_ptr(), dt,
                                  _ptr(x_scale), T, _ptr(order), top_k, _ptr(offsets), P, y.data_ptr(),
