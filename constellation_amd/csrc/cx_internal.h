@@ -396,6 +396,7 @@ struct Q4Launch {
     int x_type;
     int n_x;                 // rows of x
     int n_rows;              // rows of y
+    int n_mats;              // matrices that rows are dealt to
     const int32_t* order;    // nullable: row p reads x row order[p] / top_k
     int top_k;
     const Q4Item* items;     // nullable: all rows belong to matrix 0
@@ -404,12 +405,14 @@ struct Q4Launch {
     void* y;                 // [n_rows, rows] ([n_rows, rows / 2] gated)
     int y_type;              // CX_DTYPE_*
     void* x_scratch;         // q4_x_scratch bytes
+    float* part;             // q4_part_bytes
 };
 size_t q4_code_bytes(const cx_q4_desc& w);
 size_t q4_scale_bytes(const cx_q4_desc& w);
 hipError_t launch_q4_pack(const cx_q4_desc& w, const uint8_t* codes, const uint16_t* scales, hipStream_t s);
 hipError_t launch_q4_items(const int32_t* offsets, int n_mats, int n_rows, int item_rows, Q4Item* items, int* err_flag,
                            hipStream_t s);
+size_t q4_part_bytes(const cx_q4_desc& w, int64_t n_rows, int n_mats, int item_rows);  // the GEMM's partial sums
 size_t q4_x_scratch(const cx_q4_desc& w, int n_x);  // of products with items of more than 16 rows
 // Given routes, one item per pair: what a layer over a few tokens has instead of a plan.
 struct Q4Routes {

@@ -272,7 +272,8 @@ hipError_t few_groups(const Q4Launch& L, hipStream_t s) {
 }  // namespace
 
 bool q4_grid_ok(const Q4Launch& L) {
-    return rows_grid_ok(item_bound(L) * q4_row_tiles(L.w), 64 * kQ4FewWaves) && rows_grid_ok(L.n_x, 256) &&
+    const int RT = q4_row_tiles(L.w);
+    return rows_grid_ok(item_bound(L) * (RT + 16), 1024) && rows_grid_ok(L.n_x, 256) && rows_grid_ok((int64_t)L.n_rows * RT * 4 / 256 + 1, 256) &&
            (int64_t)L.n_x * q4_col_tiles(L.w) * 16 < ((int64_t)1 << 32);  // the GEMM's places in x, in 16 bytes
 }
 

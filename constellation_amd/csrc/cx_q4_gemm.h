@@ -20,7 +20,8 @@ struct Q4GemmArgs {
     const Q4Item* items;
     void* y;
     int y_type;
-    int item_rows;
+    float* part;              // [splits, n_rows, RT * 16]
+    int item_rows, splits;
     int RT, KT, RB;           // row tiles, column tiles, row blocks
 };
 
@@ -46,16 +47,18 @@ __device__ __forceinline__ void q4_gemm_turn() {
 // the accumulators, a lane has 4 neighbours of one row: 8 bytes in 16 bits).
 template <int RTW, int NT>
 __device__ __forceinline__ void q4_gemm_store(const Q4GemmArgs& L, const f32x4 (&acc)[NT][RTW], unsigned char* lds, const cx_q4_desc& w,
-                                              size_t mat, int rb, int begin, int rows) {
+                                              size_t mat, int rb, int ks, int begin, int rows) {
     constexpr int kPitch = RTW * 16 + 4;  // floats; 16 rows' pieces then lie in different banks
     static_assert(16 * kPitch * 4 * kQ4GemmWaves <= kQ4GemmBuf, "turned tiles");
     const int wave = wave_id(), lane = threadIdx.x & 63, t = lane & 15, q = lane >> 4;
     float* turn = reinterpret_cast<float*>(lds) + wave * 16 * kPitch;
     const int rt0 = (rb * kQ4GemmWaves + wave) * RTW;
-    const int width = w.gated ? w.rows / 2 : w.rows;
-    const int c0 = rt0 * (w.gated ? 8 : 16), cols = RTW * (w.gated ? 8 : 16);  // of this wave
-    const bool wide = L.y_type == CX_DTYPE_F32;
-    const bool vec = width % (wide ? 4 : 8) == 0 && (reinterpret_cast<uintptr_t>(L.y) & 15) == 0;
+    const bool parts = L.splits > 1, gated = w.gated && !parts;  // partial sums: tiles as they are
+    const int width = parts ? L.RT * 16 : gated ? w.rows / 2 : w.rows;
+    const int c0 = rt0 * (gated ? 8 : 16), cols = RTW * (gated ? 8 : 16);  // of this wave
+    void* out = parts ? L.part + (size_t)ks * L.n_rows * width : L.y;
+    const bool wide = parts || L.y_type == CX_DTYPE_F32;
+    const bool vec = width % (wide ? 4 : 8) == 0 && (reinterpret_cast<uintptr_t>(out) & 15) == 0;
     const int per = wide ? 4 : 8, lanes = cols / per;  // columns of a lane's store, lanes of a row
     f32x4 rs[RTW];
 #pragma unroll
@@ -83,7 +86,7 @@ __device__ __forceinline__ void q4_gemm_store(const Q4GemmArgs& L, const f32x4 (
             f32x4 v = acc[n][m] * rs[m];
             v = xs[n] == 0.0f ? f32x4{} : v * f32x4{xs[n], xs[n], xs[n], xs[n]};
             int c = m * 16 + 4 * q;
-            if (w.gated) {
+            if (gated) {
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     const float up = __shfl_xor(v[i], 32);
@@ -91,7 +94,7 @@ __device__ __forceinline__ void q4_gemm_store(const Q4GemmArgs& L, const f32x4 (
                 }
                 c = m * 8 + 4 * (q & 1);
             }
-            if (!w.gated || q < 2) *reinterpret_cast<f32x4*>(turn + t * kPitch + c) = v;
+            if (!gated || q < 2) *reinterpret_cast<f32x4*>(turn + t * kPitch + c) = v;
         }
         __builtin_amdgcn_wave_barrier();
         for (int i = lane; i < 16 * lanes; i += 64) {
@@ -101,14 +104,14 @@ __device__ __forceinline__ void q4_gemm_store(const Q4GemmArgs& L, const f32x4 (
             const size_t at = (size_t)(begin + n * 16 + r) * width + c0 + c;
             if (wide) {
                 const f32x4 v = *reinterpret_cast<const f32x4*>(src);
-                float* y = static_cast<float*>(L.y) + at;
+                float* y = static_cast<float*>(out) + at;
                 if (vec) {
                     *reinterpret_cast<f32x4*>(y) = v;
                 } else {
                     for (int k = 0; k < min(left, 4); ++k) y[k] = src[k];
                 }
             } else {
-                uint16_t* y = static_cast<uint16_t*>(L.y) + at;
+                uint16_t* y = static_cast<uint16_t*>(out) + at;
                 if (vec) {
                     const f32x4 a = *reinterpret_cast<const f32x4*>(src), b = *reinterpret_cast<const f32x4*>(src + 4);
                     *reinterpret_cast<u32x4*>(y) = u32x4{cast_out(a[0], L.y_type) | (cast_out(a[1], L.y_type) << 16), cast_out(a[2], L.y_type) | (cast_out(a[3], L.y_type) << 16),
@@ -128,7 +131,7 @@ __device__ __forceinline__ void q4_gemm_store(const Q4GemmArgs& L, const f32x4 (
 // below the largest product of an instruction, and sums here are kept to fp32.
 template <int NG, int RTW, int NT, bool XS>
 __device__ __forceinline__ void q4_gemm_tile(const Q4GemmArgs& L, unsigned char* lds0, unsigned char* lds1, const cx_q4_desc& w,
-                                             size_t mat, int rb, int begin, int rows) {
+                                             size_t mat, int rb, int ks, int begin, int rows) {
     const int wave = wave_id(), lane = threadIdx.x & 63, t = lane & 15, q = lane >> 4;
     const int KT = L.KT;
     // x: load i brings rows 16 i + 4 wave .. + 3 of the item, each lane 16 bytes; slot s of
@@ -237,27 +240,28 @@ __device__ __forceinline__ void q4_gemm_tile(const Q4GemmArgs& L, unsigned char*
     };
     constexpr std::integral_constant<int, 0> even{};
     constexpr std::integral_constant<int, 1> odd{};
-    fetch(0, even, lds0);
+    const int per = (KT + L.splits - 1) / L.splits, k0 = ks * per, k1 = min(KT, k0 + per);
+    if (k0 < k1) fetch(k0, even, lds0);
     q4_gemm_turn();
-    for (int kt = 0; kt < KT; kt += 2) {
-        if (kt + 1 < KT) fetch(kt + 1, odd, lds1);
+    for (int kt = k0; kt < k1; kt += 2) {
+        if (kt + 1 < k1) fetch(kt + 1, odd, lds1);
         multiply(even, lds0);
         q4_gemm_turn();
-        if (kt + 1 >= KT) break;
-        if (kt + 2 < KT) fetch(kt + 2, even, lds0);
+        if (kt + 1 >= k1) break;
+        if (kt + 2 < k1) fetch(kt + 2, even, lds0);
         multiply(odd, lds1);
         q4_gemm_turn();
     }
     if constexpr (XS)
-        q4_gemm_store<RTW, NT>(L, sum, lds0, w, mat, rb, begin, rows);
+        q4_gemm_store<RTW, NT>(L, sum, lds0, w, mat, rb, ks, begin, rows);
     else
-        q4_gemm_store<RTW, NT>(L, acc, lds0, w, mat, rb, begin, rows);
+        q4_gemm_store<RTW, NT>(L, acc, lds0, w, mat, rb, ks, begin, rows);
 }
 
 template <int NG, int RTW, bool XS>
 __global__ __launch_bounds__(64 * kQ4GemmWaves, 2) void k_q4_gemm(Q4GemmArgs L) {
     __shared__ __attribute__((aligned(16))) unsigned char lds0[kQ4GemmBuf], lds1[kQ4GemmBuf];
-    const int idx = blockIdx.x / L.RB, rb = blockIdx.x - idx * L.RB;
+    const int per = L.RB * L.splits, idx = blockIdx.x / per, unit = blockIdx.x - idx * per, ks = unit / L.RB, rb = unit - ks * L.RB;
     int expert = 0, begin = idx * L.item_rows, rows = min(L.item_rows, L.n_rows - begin);
     if (L.items != nullptr) {
         if (idx >= L.items[0].expert) return;
@@ -267,18 +271,21 @@ __global__ __launch_bounds__(64 * kQ4GemmWaves, 2) void k_q4_gemm(Q4GemmArgs L) 
         rows = it.rows;
     }
     if (expert < 0) {  // rows behind the last matrix's
-        const int width = L.w.gated ? L.w.rows / 2 : L.w.rows, per = kQ4GemmWaves * RTW * (L.w.gated ? 8 : 16);
-        const int size = L.y_type == CX_DTYPE_F32 ? 2 : 1;  // in 16-bit units
+        const bool parts = L.splits > 1, wide = parts || L.y_type == CX_DTYPE_F32;
+        const int width = parts ? L.RT * 16 : L.w.gated ? L.w.rows / 2 : L.w.rows;
+        const int n = kQ4GemmWaves * RTW * (L.w.gated && !parts ? 8 : 16), left = width - rb * n;
+        char* out = parts ? reinterpret_cast<char*>(L.part + (size_t)ks * L.n_rows * width) : static_cast<char*>(L.y);
+        const size_t el = wide ? 4 : 2;
         for (int r = 0; r < rows; ++r)
-            for (int c = threadIdx.x; c < per * size; c += 64 * kQ4GemmWaves)
-                if (rb * per * size + c < width * size) static_cast<uint16_t*>(L.y)[((size_t)(begin + r) * width) * size + rb * per * size + c] = 0;
+            for (int c = threadIdx.x * 2; c < min(n, left) * (int)el; c += 128 * kQ4GemmWaves)
+                *reinterpret_cast<uint16_t*>(out + ((size_t)(begin + r) * width + rb * n) * el + c) = 0;
         return;
     }
     const bool other = expert == L.w.n_mats;
     const cx_q4_desc& w = other ? L.shared : L.w;
     const size_t mat = other ? 0 : (size_t)expert;
     auto tile = [&](auto nt) {
-        q4_gemm_tile<NG, RTW, nt, XS>(L, lds0, lds1, w, mat, rb, begin, rows);
+        q4_gemm_tile<NG, RTW, nt, XS>(L, lds0, lds1, w, mat, rb, ks, begin, rows);
     };
     if constexpr (!XS) {
         if (rows > 112) return tile(std::integral_constant<int, 8>{});
@@ -292,6 +299,30 @@ __global__ __launch_bounds__(64 * kQ4GemmWaves, 2) void k_q4_gemm(Q4GemmArgs L) 
         tile(std::integral_constant<int, 3>{});
     else
         tile(std::integral_constant<int, 2>{});
+}
+
+// The partial sums of the ranges, added in order, and what follows the sums.
+__global__ __launch_bounds__(256) void k_q4_sum(const float* part, int splits, int n_rows, int pitch, int gated, int width, void* y,
+                                                int y_type, int units) {
+    const size_t at = (size_t)blockIdx.x * 256 + threadIdx.x;
+    const size_t p = at / units;
+    const int n = (int)(at - p * units) * 4;
+    if (p >= (size_t)n_rows) return;
+    const float* src = part + p * pitch + (gated ? n / 8 * 16 + n % 8 : n);
+    f32x4 a = {}, b = {};
+    for (int s = 0; s < splits; ++s) {
+        a += *reinterpret_cast<const f32x4*>(src + (size_t)s * n_rows * pitch);
+        if (gated) b += *reinterpret_cast<const f32x4*>(src + (size_t)s * n_rows * pitch + 8);
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float v = gated ? a[i] / (1.0f + __expf(-a[i])) * b[i] : a[i];
+        if (n + i >= width) continue;
+        if (y_type == CX_DTYPE_F32)
+            static_cast<float*>(y)[p * width + n + i] = v;
+        else
+            static_cast<uint16_t*>(y)[p * width + n + i] = (uint16_t)cast_out(v, y_type);
+    }
 }
 
 }  // namespace cx

@@ -3,6 +3,17 @@
 
 namespace cx {
 
+namespace {
+int splits_of(const cx_q4_desc& w, int64_t n_rows, int n_mats, int item_rows) {
+    return item_rows > kTileTok ? q4_gemm_splits(q4_row_tiles(w), q4_col_tiles(w), n_rows, n_mats, item_rows) : 1;
+}
+}  // namespace
+
+size_t q4_part_bytes(const cx_q4_desc& w, int64_t n_rows, int n_mats, int item_rows) {
+    const int s = splits_of(w, n_rows, n_mats, item_rows);
+    return s > 1 ? (size_t)s * n_rows * q4_row_tiles(w) * 64 : 0;
+}
+
 hipError_t launch_q4_gemm(const Q4Launch& L, hipStream_t s) {
     Q4GemmArgs a{};
     a.w = L.w;
@@ -21,14 +32,21 @@ hipError_t launch_q4_gemm(const Q4Launch& L, hipStream_t s) {
     a.items = L.items;
     a.y = L.y;
     a.y_type = L.y_type;
-    constexpr int kRtw = 4;
+    constexpr int kRtw = kQ4GemmBlock / kQ4GemmWaves;
+    a.part = L.part;
+    a.splits = splits_of(L.w, L.n_rows, L.n_mats, L.item_rows);
     a.RB = (a.RT + kQ4GemmWaves * kRtw - 1) / (kQ4GemmWaves * kRtw);
     const int64_t items = L.items != nullptr ? L.max_items : (L.n_rows + L.item_rows - 1) / L.item_rows;
     const bool xs = L.x_type == kQ4E4m3;
     auto k = L.w.group == 128  ? (xs ? k_q4_gemm<1, kRtw, true> : k_q4_gemm<1, kRtw, false>)
              : L.w.group == 64 ? (xs ? k_q4_gemm<2, kRtw, true> : k_q4_gemm<2, kRtw, false>)
                                : (xs ? k_q4_gemm<4, kRtw, true> : k_q4_gemm<4, kRtw, false>);
-    cx_launch(k, dim3((unsigned)(items * a.RB)), dim3(64 * kQ4GemmWaves), 0, s, a);
+    cx_launch(k, dim3((unsigned)(items * a.RB * a.splits)), dim3(64 * kQ4GemmWaves), 0, s, a);
+    if (a.splits > 1) {
+        const int width = L.w.gated ? L.w.rows / 2 : L.w.rows, units = (width + 3) / 4;
+        cx_launch(k_q4_sum, dim3((unsigned)(((int64_t)L.n_rows * units + 255) / 256)), dim3(256), 0, s, static_cast<const float*>(L.part),
+                  a.splits, L.n_rows, a.RT * 16, L.w.gated, width, L.y, L.y_type, units);
+    }
     return hipGetLastError();
 }
 

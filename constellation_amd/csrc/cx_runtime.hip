@@ -806,11 +806,11 @@ int check_q4(const cx_q4_desc* w) {
 
 size_t align_up(size_t v) { return (v + 255) / 256 * 256; }
 
-// Scratch of cx_q4_matmul: the items, then x as the GEMM reads it.
+// Scratch of cx_q4_matmul: the items, x as the GEMM reads it, its partial sums.
 struct Q4Scratch {
     int item_rows;
     int64_t max_items;
-    size_t x, bytes;
+    size_t x, part, bytes;
 };
 
 Q4Scratch q4_scratch(const cx_q4_desc& w, int x_dtype, int n_x, int n_rows, bool with_offsets) {
@@ -818,7 +818,8 @@ Q4Scratch q4_scratch(const cx_q4_desc& w, int x_dtype, int n_x, int n_rows, bool
     z.item_rows = q4_item_rows(n_rows, w.n_mats, w.cols, x_dtype == CX_DTYPE_E4M3);
     z.max_items = q4_max_items(n_rows, w.n_mats, z.item_rows);
     z.x = with_offsets ? align_up(sizeof(Q4Item) * (size_t)z.max_items) : 0;
-    z.bytes = z.x + (z.item_rows > kTileTok ? q4_x_scratch(w, n_x) : 0);
+    z.part = z.x + (z.item_rows > kTileTok ? q4_x_scratch(w, n_x) : 0);
+    z.bytes = z.part + q4_part_bytes(w, n_rows, w.n_mats, z.item_rows);
     return z;
 }
 
@@ -826,7 +827,7 @@ Q4Scratch q4_scratch(const cx_q4_desc& w, int x_dtype, int n_x, int n_rows, bool
 struct Q4MoeScratch {
     int64_t pairs, max_items;
     int item_rows;
-    size_t items, order, place, x, h, hx, ys, bytes;
+    size_t items, order, place, x, h, hx, ys, part, bytes;
 };
 
 Q4MoeScratch q4_moe_scratch(const cx_q4_desc& gu, const cx_q4_desc& down, int shared, int n_tokens, int top_k) {
@@ -844,7 +845,9 @@ Q4MoeScratch q4_moe_scratch(const cx_q4_desc& gu, const cx_q4_desc& down, int sh
     z.h = z.x + (gemm ? q4_x_scratch(gu, n_tokens) : 0);
     z.hx = z.h + align_up(4 * (size_t)z.pairs * down.cols);
     z.ys = z.hx + (gemm ? q4_x_scratch(down, (int)z.pairs) : 0);
-    z.bytes = z.ys + align_up(4 * (size_t)z.pairs * down.rows);
+    z.part = z.ys + align_up(4 * (size_t)z.pairs * down.rows);
+    auto parts = [&](const cx_q4_desc& w) { return q4_part_bytes(w, z.pairs, w.n_mats + shared, z.item_rows); };
+    z.bytes = z.part + std::max(parts(gu), parts(down));
     return z;
 }
 
@@ -1578,7 +1581,9 @@ int cx_q4_matmul(cx_ctx* ctx, const cx_q4_desc* w, const void* x, int x_dtype, c
     L.y_type = y_dtype;
     L.item_rows = z.item_rows;
     L.max_items = z.max_items;
+    L.n_mats = w->n_mats;
     L.x_scratch = static_cast<char*>(scratch) + z.x;
+    L.part = reinterpret_cast<float*>(static_cast<char*>(scratch) + z.part);
     if (!q4_grid_ok(L)) return fail(CX_EINVAL, "too many rows for one launch");
     if (offsets) {
         L.items = static_cast<const Q4Item*>(scratch);
@@ -1651,7 +1656,9 @@ int cx_q4_moe(cx_ctx* ctx, const cx_q4_desc* gate_up, const cx_q4_desc* down, co
     L.items = a.items;
     L.item_rows = z.item_rows;
     L.max_items = z.max_items;
+    L.n_mats = gate_up->n_mats + shared;
     L.x_scratch = m + z.x;
+    L.part = reinterpret_cast<float*>(m + z.part);
     L.y = m + z.h;
     L.y_type = CX_DTYPE_F32;
     Q4Launch D = L;

@@ -300,6 +300,28 @@ inline int q4_item_rows(int64_t n_rows, int n_mats, int cols, bool two_sums) {
     return n_rows <= (int64_t)kTileTok * n_mats ? kTileTok : two_sums ? kQ4GemmRows / 2 : kQ4GemmRows;
 }
 
+// Ranges of the columns that the GEMM deals to workgroups of their own, whose partial sums a
+// second launch adds: as many as cost least by this estimate, in us.  A workgroup (256
+// weight rows, an item of nt 16-row tiles) takes 0.6 + 0.17 nt a column tile on a CU of its own
+// (measured: 0.94, 1.2 and 1.96 with 2, 4 and 8), 1 + nt / 10 times that beside a second one; the
+// partial sums are written and read at 4.5 MB a us, and the launch is 3.
+constexpr int kQ4GemmBlock = 16;  // row tiles of a workgroup
+inline int q4_gemm_splits(int row_tiles, int col_tiles, int64_t n_rows, int n_mats, int item_rows) {
+    if (n_rows <= 0) return 1;
+    const int64_t items = std::max<int64_t>(n_mats > 1 ? std::min<int64_t>(n_mats, n_rows) : 1, (n_rows + item_rows - 1) / item_rows);
+    const double nt = std::min<double>(item_rows / 16, std::max(2.0, (double)((n_rows + 16 * items - 1) / (16 * items))));
+    const int64_t wgs = items * ((row_tiles + kQ4GemmBlock - 1) / kQ4GemmBlock);
+    int best = 1;
+    double least = 0;
+    for (int s = 1; s <= 16 && (s == 1 || col_tiles / s >= 2); s *= 2) {
+        const double rounds = (double)((wgs * s + 511) / 512), beside = wgs * s > 256 ? 1 + nt / 10 : 1;
+        const double cost = rounds * ((col_tiles + s - 1) / s) * (0.6 + 0.17 * nt) * beside +
+                            (s > 1 ? 3 + 2.0 * s * (double)n_rows * row_tiles * 64 / 4.5e6 : 0);
+        if (s == 1 || cost < least) least = cost, best = s;
+    }
+    return best;
+}
+
 // Items of up to item_rows rows over n_mats matrices, entry 0 (the head) included: at
 // most one short item per matrix that has rows, and one of rows without a matrix.
 inline int64_t q4_max_items(int64_t n_rows, int n_mats, int item_rows) {
