@@ -138,13 +138,13 @@ __device__ __forceinline__ void q4_gemm_tile(const Q4GemmArgs& L, unsigned char*
     // row r gets the row's piece s ^ (r % 16), so that the 16 rows of a fragment lie in
     // 16 different places of the banks.
     const int tr = threadIdx.x >> 4, piece = (threadIdx.x & 15) ^ tr;
-    uint32_t xoff[NT];  // in 16-byte pieces; rows that do not exist read another and are never stored
+    uint32_t xoff[NT];  // in bytes; rows that do not exist read another and are never stored
 #pragma unroll
     for (int i = 0; i < NT; ++i) {
         const int r = i * 16 + tr;
         int xr = begin + (r < rows ? r : 0);
         if (L.order != nullptr) xr = max(L.order[xr], 0) / L.top_k;
-        xoff[i] = (uint32_t)(xr < L.n_x ? xr : 0) * (uint32_t)(L.padded / 8) + piece;
+        xoff[i] = (uint32_t)(xr < L.n_x ? xr : 0) * (uint32_t)(L.padded * 2) + piece * 16;
     }
     const uint8_t* wp[RTW];
     const uint16_t* sp[RTW];
@@ -161,20 +161,17 @@ __device__ __forceinline__ void q4_gemm_tile(const Q4GemmArgs& L, unsigned char*
     f32x4 acc[NT][RTW] = {}, sum[XS ? NT : 1][RTW] = {};
     u32x4 a[2][RTW];
     Sc s[2][RTW];
-    const float* xsp[XS ? NT : 1];
-    float xs[2][XS ? NT : 1];
+    uint32_t xso = 0;  // XS: wave 0 brings the rows' scales, a lane each, behind their 64 rows
     if constexpr (XS) {
-#pragma unroll
-        for (int n = 0; n < NT; ++n) {
-            int xr = begin + (n * 16 + t < rows ? n * 16 + t : 0);
-            if (L.order != nullptr) xr = max(L.order[xr], 0) / L.top_k;
-            xsp[n] = L.x_scale + (size_t)(xr < L.n_x ? xr : 0) * KT;
-        }
+        static_assert(NT <= 4, "64 rows");
+        int xr = begin + (lane < rows ? lane : 0);
+        if (L.order != nullptr) xr = max(L.order[xr], 0) / L.top_k;
+        xso = (uint32_t)(xr < L.n_x ? xr : 0) * (uint32_t)KT;
     }
     auto fetch = [&](int kt, auto to, unsigned char* buf) {
 #pragma unroll
         for (int i = 0; i < NT; ++i)
-            __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(L.x + ((size_t)xoff[i] + kt * 16) * 8),
+            __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(reinterpret_cast<const char*>(L.x) + (size_t)kt * 256 + xoff[i]),
                                              (__attribute__((address_space(3))) void*)(buf + i * 4096 + wave * 1024), 16, 0, 0);
 #pragma unroll
         for (int m = 0; m < RTW; ++m) {
@@ -185,15 +182,17 @@ __device__ __forceinline__ void q4_gemm_tile(const Q4GemmArgs& L, unsigned char*
                 s[to][m] = *reinterpret_cast<const Sc*>(sp[m] + (size_t)kt * 16 * NG + (uint32_t)t * NG);
         }
         if constexpr (XS)
-#pragma unroll
-            for (int n = 0; n < NT; ++n) xs[to][n] = xsp[n][kt];
+            if (wave == 0)
+                __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(L.x_scale + kt + xso),
+                                                 (__attribute__((address_space(3))) void*)(buf + 16384), 4, 0, 0);
     };
-    auto scaled_add = [&](auto from, int n) {
+    auto scaled_add = [&](const unsigned char* buf, int n) {
         if constexpr (XS) {
+            const float x = *reinterpret_cast<const float*>(buf + 16384 + (n * 16 + t) * 4);
 #pragma unroll
             for (int m = 0; m < RTW; ++m) {
 #pragma unroll
-                for (int i = 0; i < 4; ++i) sum[n][m][i] = __builtin_fmaf(xs[from][n], acc[n][m][i], sum[n][m][i]);
+                for (int i = 0; i < 4; ++i) sum[n][m][i] = __builtin_fmaf(x, acc[n][m][i], sum[n][m][i]);
                 asm volatile("" : "+v"(sum[n][m]));
             }
         }
@@ -226,11 +225,11 @@ __device__ __forceinline__ void q4_gemm_tile(const Q4GemmArgs& L, unsigned char*
 #pragma unroll
             for (int m = 0; m < RTW; ++m)
                 acc[n][m] = Mma<true>::mma(fa[j & 1][m], Mma<true>::bits(b[i % 3]), XS && j == 0 ? f32x4{} : acc[n][m]);
-            if (XS && j == 3 && n > 0) scaled_add(from, n - 1);  // while this step's products are on their way
+            if (XS && j == 3 && n > 0) scaled_add(buf, n - 1);  // while this step's products are on their way
         }
         __builtin_amdgcn_sched_barrier(0);
         if constexpr (XS) {
-            scaled_add(from, NT - 1);
+            scaled_add(buf, NT - 1);
         } else {
 #pragma unroll
             for (int n = 0; n < NT; ++n)
