@@ -53,6 +53,15 @@ __device__ __forceinline__ void load8(const void* base, int dtype, size_t at, in
         load8<CX_DTYPE_F32, VEC>(base, at, left, v);
 }
 
+// Two values rounded to a 16-bit type (nearest even), the first in the lower half.
+template <int DT>
+__device__ __forceinline__ uint32_t round2(float a, float b) {
+    if constexpr (DT == CX_DTYPE_BF16)
+        return __builtin_bit_cast(uint32_t, bf16x2{static_cast<__bf16>(a), static_cast<__bf16>(b)});  // one v_cvt_pk_bf16_f32
+    else
+        return __builtin_bit_cast(uint32_t, f16x2{static_cast<_Float16>(a), static_cast<_Float16>(b)});
+}
+
 template <int DT, bool VEC>
 __device__ __forceinline__ void store8(void* base, size_t at, int left, const float (&v)[8]) {
     if constexpr (DT == CX_DTYPE_F32) {
@@ -67,15 +76,13 @@ __device__ __forceinline__ void store8(void* base, size_t at, int left, const fl
         }
     } else {
         uint16_t* p = static_cast<uint16_t*>(base) + at;
-        uint32_t h[8];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) h[i] = cast_out(v[i], DT);
+        const u32x4 h = {round2<DT>(v[0], v[1]), round2<DT>(v[2], v[3]), round2<DT>(v[4], v[5]), round2<DT>(v[6], v[7])};
         if constexpr (VEC) {
-            *reinterpret_cast<u32x4*>(p) = u32x4{h[0] | (h[1] << 16), h[2] | (h[3] << 16), h[4] | (h[5] << 16), h[6] | (h[7] << 16)};
+            *reinterpret_cast<u32x4*>(p) = h;
         } else {
 #pragma unroll
             for (int i = 0; i < 8; ++i)
-                if (i < left) p[i] = static_cast<uint16_t>(h[i]);
+                if (i < left) p[i] = static_cast<uint16_t>(h[i >> 1] >> (16 * (i & 1)));
         }
     }
 }
@@ -88,16 +95,6 @@ __device__ __forceinline__ void store8(void* base, int dtype, size_t at, int lef
         store8<CX_DTYPE_FP16, VEC>(base, at, left, v);
     else
         store8<CX_DTYPE_F32, VEC>(base, at, left, v);
-}
-
-template <int DT>
-__device__ __forceinline__ float rounded(float f) {
-    if constexpr (DT == CX_DTYPE_BF16)
-        return __uint_as_float(bf16_rne(f) << 16);
-    else if constexpr (DT == CX_DTYPE_FP16)
-        return static_cast<float>(static_cast<_Float16>(f));
-    else
-        return f;
 }
 
 __device__ __forceinline__ float wave_sum(float v) {
@@ -141,7 +138,15 @@ __global__ __launch_bounds__(1024) void k_rms_norm(NormArgs a) {
             float r[8];
             load8<DT, VEC>(a.residual, row + c, left, r);
 #pragma unroll
-            for (int j = 0; j < 8; ++j) s[i][j] = rounded<DT>(s[i][j] + r[j]);
+            for (int j = 0; j < 8; ++j) s[i][j] += r[j];
+            if constexpr (DT != CX_DTYPE_F32) {
+#pragma unroll
+                for (int j = 0; j < 8; j += 2) {
+                    const uint32_t h = round2<DT>(s[i][j], s[i][j + 1]);
+                    s[i][j] = DT == CX_DTYPE_BF16 ? __uint_as_float(h << 16) : (float)__builtin_bit_cast(f16x2, h)[0];
+                    s[i][j + 1] = DT == CX_DTYPE_BF16 ? __uint_as_float(h & 0xFFFF0000u) : (float)__builtin_bit_cast(f16x2, h)[1];
+                }
+            }
         }
     }
 #pragma unroll
@@ -164,24 +169,48 @@ __global__ __launch_bounds__(1024) void k_rms_norm(NormArgs a) {
 #pragma unroll
         for (int j = 0; j < 8; ++j) w[j] = 1.0f;
         if (left > 0 && a.weight != nullptr) load8<VEC>(a.weight, a.w_dtype, c, left, w);
+        // n: y before the row's factor, exact for 16-bit rows and weights
+        float n[8];
         uint32_t most = 0;
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-            s[i][j] = s[i][j] * inv * w[j];
-            if (j < left) most = max(most, __float_as_uint(s[i][j]) & 0x7FFFFFFFu);
+            n[j] = s[i][j] * w[j];
+            most = max(most, __float_as_uint(n[j]) & 0x7FFFFFFFu);  // columns past the row are zeros
         }
-        if (a.y != nullptr && left > 0) store8<VEC>(a.y, a.y_dtype, row + c, left, s[i]);
+        if (a.y != nullptr && left > 0) {
+            float y[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) y[j] = s[i][j] * inv * w[j];
+            store8<VEC>(a.y, a.y_dtype, row + c, left, y);
+        }
         if (a.q == nullptr) continue;
-        float scale = __uint_as_float(row16_max(most)) / 448.0f;
-        scale = scale < 1e-12f ? 1e-12f : scale;
+        const float top = __uint_as_float(row16_max(most));
+        float scale = top * inv / 448.0f;
+        const bool plain = scale >= 1e-12f && top > 1e-30f && top < 1e30f;  // neither zeros nor infinities nor NaN
+        if (!plain) {  // a whole block's lanes: from y itself
+            most = 0;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                n[j] = s[i][j] * inv * w[j];
+                most = max(most, __float_as_uint(n[j]) & 0x7FFFFFFFu);
+            }
+            scale = __uint_as_float(row16_max(most)) / 448.0f;
+            scale = scale < 1e-12f ? 1e-12f : scale;
+        }
         if (left <= 0) continue;
         if ((v & 15) == 0) a.q_scale[(size_t)blockIdx.x * (size_t)((H + 127) >> 7) + (v >> 4)] = scale;
-        const float up = 1.0f / scale;
+        // y / scale = 448 n / top: the row's factor, and with it its rounding, falls out.  The division is
+        // refined to a correctly rounded one, since a code flips where the quotient crosses a border.
+        const float by = plain ? top : scale, inv_by = 1.0f / by, gain = plain ? 448.0f : 1.0f;
+        auto quotient = [&](int j) {
+            const float num = n[j] * gain, r = num * inv_by, better = __builtin_fmaf(__builtin_fmaf(-r, by, num), inv_by, r);
+            return plain ? better : r;
+        };
         uint32_t b[2];
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
-            int d = __builtin_amdgcn_cvt_pk_fp8_f32(s[i][4 * j] * up, s[i][4 * j + 1] * up, 0, false);
-            b[j] = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(s[i][4 * j + 2] * up, s[i][4 * j + 3] * up, d, true);
+            int d = __builtin_amdgcn_cvt_pk_fp8_f32(quotient(4 * j), quotient(4 * j + 1), 0, false);
+            b[j] = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(quotient(4 * j + 2), quotient(4 * j + 3), d, true);
         }
         uint8_t* q = a.q + row + c;
         if constexpr (VEC) {
