@@ -326,11 +326,10 @@ struct Q4Item {
     int expert, begin, rows, pad;
 };
 
-// Items from, from + step, ... of the n that rows begin .. begin + rows - 1 of a matrix are cut
-// to: equal ones of whole 16-row tiles, so that the last is not a short one.
+// Items from, from + step, ... of the n (q4_item_share) that rows begin .. begin + rows - 1 of a matrix are cut to.
 __device__ inline void q4_put_items(Q4Item* items, int n, int expert, int begin, int rows, int from, int step) {
-    const int per = n == 0 ? 0 : n == 1 || rows < 16 * n ? (rows + n - 1) / n : (rows + 16 * n - 1) / (16 * n) * 16;
-    for (int i = from; i < n; i += step) items[i] = Q4Item{expert, begin + i * per, max(0, min(per, rows - i * per)), 0};
+    const int share = q4_item_share(n, rows);
+    for (int i = from; i < n; i += step) items[i] = Q4Item{expert, begin + i * share, min(share, rows - i * share), 0};
 }
 
 struct SortArgs {

@@ -273,8 +273,9 @@ hipError_t few_groups(const Q4Launch& L, hipStream_t s) {
 
 bool q4_grid_ok(const Q4Launch& L) {
     const int RT = q4_row_tiles(L.w);
-    return rows_grid_ok(item_bound(L) * (RT + 16), 1024) && rows_grid_ok(L.n_x, 256) && rows_grid_ok((int64_t)L.n_rows * RT * 4 / 256 + 1, 256) &&
-           (int64_t)L.n_x * q4_col_tiles(L.w) * 256 < ((int64_t)1 << 32);  // the GEMM's places in x, in bytes
+    if (!rows_grid_ok(item_bound(L) * (RT + 16), 1024)) return false;
+    return L.item_rows <= kTileTok || (rows_grid_ok(L.n_x, 256) && rows_grid_ok((int64_t)L.n_rows * RT * 4 / 256 + 1, 256) &&
+                                       (int64_t)L.n_x * q4_col_tiles(L.w) * 256 < ((int64_t)1 << 32));  // the GEMM's places in x, in bytes
 }
 
 size_t q4_x_scratch(const cx_q4_desc& w, int n_x) { return up256((size_t)n_x * q4_col_tiles(w) * 256) + up256((size_t)n_x * 4); }

@@ -786,13 +786,15 @@ int fill_route(cx_ctx* ctx, const void* x, int x_dtype, const void* w_router, in
 // Rows around the experts and 4-bit weights.
 namespace {
 
+constexpr int64_t kMaxPairs = 1 << 30;  // indexes of pairs, and of the ids a workgroup looks ahead to, fit an int
+
 bool act_any(int dtype) { return act16(dtype) || dtype == CX_DTYPE_F32; }
 
 int check_rows(cx_ctx* ctx, int n_tokens, int top_k, int64_t width) {
     if (!ctx) return fail(CX_EINVAL, "NULL context");
     if (n_tokens < 0 || top_k < 1 || top_k > 64) return fail(CX_EINVAL, "bad n_tokens/top_k");
     if (width <= 0) return fail(CX_EINVAL, "rows must not be empty");
-    if ((int64_t)n_tokens * top_k > INT32_MAX) return fail(CX_EINVAL, "too many pairs: n_tokens * top_k must fit 31 bits");
+    if ((int64_t)n_tokens * top_k > kMaxPairs) return fail(CX_EINVAL, "too many pairs: n_tokens * top_k must be at most 2^30");
     return set_device(ctx->device);
 }
 
@@ -1502,8 +1504,8 @@ int cx_q4_pack(int device, const uint8_t* codes, const uint16_t* scales, int n_m
     if (!out) return fail(CX_EINVAL, "NULL out");
     std::memset(out, 0, sizeof(*out));
     if (!codes || !scales) return fail(CX_EINVAL, "NULL buffer");
-    if (n_mats < 1 || n_mats > kSortMaxExperts || rows < 1 || cols < 1)
-        return fail(CX_EINVAL, "bad 4-bit shape (n_mats must be 1..%d)", kSortMaxExperts);
+    if (n_mats < 1 || n_mats > kSortMaxExperts || rows < 1 || cols < 1 || rows > (1 << 24) || cols > (1 << 24))
+        return fail(CX_EINVAL, "bad 4-bit shape (n_mats must be 1..%d, rows and cols 1..2^24)", kSortMaxExperts);
     if (group != 32 && group != 64 && group != 128) return fail(CX_EINVAL, "group must be 32, 64 or 128");
     if (gated && rows % 2 != 0) return fail(CX_EINVAL, "a gated matrix has an even number of rows");
     int rc = set_device(device);
@@ -1562,7 +1564,8 @@ int cx_q4_matmul(cx_ctx* ctx, const cx_q4_desc* w, const void* x, int x_dtype, c
     if (!order && n_x != n_rows) return fail(CX_EINVAL, "without an order x and y have the same rows (%d and %d)", n_x, n_rows);
     if (!offsets && w->n_mats != 1) return fail(CX_EINVAL, "a stack of %d matrices needs offsets", w->n_mats);
     if (n_rows == 0) return CX_OK;
-    if (!y || (n_x > 0 && (!x || (x_dtype == CX_DTYPE_E4M3 && !x_scale)))) return fail(CX_EINVAL, "NULL buffer");
+    if (n_x == 0) return fail(CX_EINVAL, "x has no rows");
+    if (!y || !x || (x_dtype == CX_DTYPE_E4M3 && !x_scale)) return fail(CX_EINVAL, "NULL buffer");
     const Q4Scratch z = q4_scratch(*w, x_dtype, n_x, n_rows, offsets != nullptr);
     if (z.bytes && (!scratch || scratch_bytes < z.bytes || reinterpret_cast<uintptr_t>(scratch) % 16))
         return fail(CX_EINVAL, "scratch must be %zu bytes, 16-byte aligned", z.bytes);
@@ -1623,7 +1626,7 @@ int cx_q4_moe(cx_ctx* ctx, const cx_q4_desc* gate_up, const cx_q4_desc* down, co
     }
     if (!act16(in_dtype) || !act16(out_dtype)) return fail(CX_EINVAL, "dtypes must be fp16/bf16");
     if (n_tokens < 0 || top_k < 0 || top_k > 64 || top_k + shared < 1) return fail(CX_EINVAL, "bad n_tokens/top_k");
-    if ((int64_t)n_tokens * (top_k + shared) > INT32_MAX) return fail(CX_EINVAL, "too many pairs: n_tokens * top_k must fit 31 bits");
+    if ((int64_t)n_tokens * (top_k + shared) > kMaxPairs) return fail(CX_EINVAL, "too many pairs: n_tokens * top_k must be at most 2^30");
     if (n_tokens == 0) return CX_OK;
     if (!x || !y || (top_k > 0 && (!topk_ids || !topk_w))) return fail(CX_EINVAL, "NULL buffer");
     const Q4MoeScratch z = q4_moe_scratch(*gate_up, *down, shared, n_tokens, top_k);

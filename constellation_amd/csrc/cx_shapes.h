@@ -322,6 +322,13 @@ inline int q4_gemm_splits(int row_tiles, int col_tiles, int64_t n_rows, int n_ma
     return best;
 }
 
+// Rows of each of the n items that `rows` rows are cut to (the last has what is left): equal
+// ones of whole 16-row tiles, so that the last is not a short one.  n is the least that holds
+// them, so no item is empty: (n - 1) shares are at most (n - 1) * item_rows, fewer than the rows.
+constexpr int q4_item_share(int n, int rows) {
+    return n == 0 ? 0 : n == 1 || rows < 16 * n ? (rows + n - 1) / n : (rows + 16 * n - 1) / (16 * n) * 16;
+}
+
 // Items of up to item_rows rows over n_mats matrices, entry 0 (the head) included: at
 // most one short item per matrix that has rows, and one of rows without a matrix.
 inline int64_t q4_max_items(int64_t n_rows, int n_mats, int item_rows) {

@@ -561,6 +561,8 @@ class Context:
     def moe_layer_request(self, layer: Layer, body: bytes) -> bytes:
         """Runs one MoeLayerRequest body (host bytes, moe_layer_protocol) on
         `layer` and returns the MoeLayerResponse body (host bytes)."""
+        if not isinstance(layer, Layer):
+            raise TypeError("a whole-layer message runs on a Layer (fp8 experts)")
         info = MoeLayerRequestInfo()
         b = np.frombuffer(body, np.uint8)
         check(lib().cx_moe_layer_request_peek(b.ctypes.data, b.size, C.byref(info)))

@@ -149,7 +149,9 @@ CX_API int cx_ctx_sync(cx_ctx* ctx, void* stream);
 
 /* Per-kernel timing with HIP events recorded on the launch stream around
  * every kernel the context launches (kernels: "route", "plan", "gate_up",
- * "down", "combine").  cx_ctx_profile(ctx, 1) starts collecting (and clears
+ * "down", "combine"; of the calls around the experts "rms_norm", "sort",
+ * "gather", "combine", "combine_grad", "q4", and "experts" for a 4-bit layer's
+ * launches on one token).  cx_ctx_profile(ctx, 1) starts collecting (and clears
  * totals), 0 stops.  cx_ctx_profile_read synchronises on the recorded events
  * and returns the launch count and summed milliseconds of one kernel. */
 CX_API int cx_ctx_profile(cx_ctx* ctx, int enable);
@@ -364,7 +366,10 @@ CX_API int cx_q4_free(int device, cx_q4_desc* w);
 /* y = x W^T (gated: silu(x G^T) * (x U^T)), fp32 accumulation of exact products,
  * rounded once.
  * x: [*, cols] fp16, bf16, or e4m3 with x_scale [*, ceil(cols / 128)].
- * y: [n_rows, rows] (gated: rows / 2) in fp16, bf16 or fp32.
+ * y: [n_rows, rows] (gated: rows / 2) in fp16, bf16 or fp32.  With more than
+ * 16 rows per matrix, bf16 rows of x take part as fp16 times a power of two per
+ * row: exact but for values below 2^-31 of the row's largest, which are off by
+ * less than 2^-39 of that.
  * offsets NULL: one matrix (n_mats 1) for all rows.  Otherwise rows
  * offsets[e] .. offsets[e + 1] - 1 go through matrix e (cx_sort_tokens' offsets,
  * [n_mats + 1]) and the rows behind the last matrix's are zeros; offsets that

@@ -433,6 +433,7 @@ def test_refusals(gpu):
         refused(pack(g=16), "group must be")
         refused(pack(E=0), "bad 4-bit shape")
         refused(pack(E=1025), "bad 4-bit shape")
+        refused(pack(N=1 << 25), "bad 4-bit shape")
         refused(pack(N=31, gated=1), "even number of rows")
         refused(pack(c=None), "NULL buffer")
         need = L.cx_q4_scratch(C.byref(w.desc), BF16, 4, 4, 1)
@@ -448,6 +449,7 @@ def test_refusals(gpu):
         refused(mm(odt=E4M3), "y must be")
         refused(mm(P=-1), "bad n_rows")
         refused(mm(n_x=3), "same rows")
+        refused(mm(n_x=0, order=i32.data_ptr()), "x has no rows")
         refused(mm(off=None), "needs offsets")
         refused(mm(sz=need - 1), "scratch must be")
         refused(mm(scr=buf.data_ptr() + 4), "scratch must be")
@@ -475,6 +477,8 @@ def test_refusals(gpu):
             gpu.rms_norm(x.cpu())
         with pytest.raises(ValueError, match="residual"):
             gpu.rms_norm(x, residual=x[:2])
+        with pytest.raises(TypeError, match="fp8"):
+            gpu.moe_layer_request(w, b"")
         with pytest.raises(ValueError, match="nothing to compute"):
             gpu.rms_norm(x, want_y=False)
         with pytest.raises(ValueError, match="place"):
@@ -485,3 +489,57 @@ def test_refusals(gpu):
         torch.cuda.synchronize()
     finally:
         w.free()
+
+
+def test_q4_two_streams_and_ragged_stacks(gpu):
+    """Two products of one context on two streams at once, each with its own scratch; and a
+    stack through each kernel with row counts about its item sizes."""
+    from constellation_amd.engine import Q4Matrix
+    print("[q4] two streams", flush=True)
+    K, N, E = 320, 80, 3
+    codes, scales = make(5, E, N, K, 64)
+    w = Q4Matrix.pack(codes.cuda(), scales.cuda(), K, group=64)
+    W = dense(codes, scales, K, 64)
+    try:
+        for cuts in ((0, 1, 1, 2), (0, 16, 33, 34), (0, 17, 20, 48), (0, 129, 129, 130), (0, 256, 400, 401), (0, 113, 210, 467)):
+            off = torch.tensor(cuts, dtype=torch.int32)
+            P = cuts[-1]
+            x = rand(P, P, K, dtype=BF)
+            want = torch.cat([x[a:b].double() @ W[e].T for e, (a, b) in enumerate(zip(cuts, cuts[1:]))])
+            tol = torch.cat([x[a:b].double().abs() @ W[e].abs().T for e, (a, b) in enumerate(zip(cuts, cuts[1:]))]) * (K + 8) * U
+            xs = [x.cuda(), (2 * x).cuda()]  # exact: a power of two
+            offs, out = off.cuda(), [None, None]
+            torch.cuda.synchronize()
+            streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+            for _ in range(3):
+                for i, s in enumerate(streams):
+                    with torch.cuda.stream(s):
+                        out[i] = gpu.q4_matmul(w, xs[i], offsets=offs)
+            torch.cuda.synchronize()
+            for i in (0, 1):
+                near(out[i], (i + 1) * want, rounded((i + 1) * want, (i + 1) * tol, BF), cuts)
+    finally:
+        w.free()
+
+
+def test_q4_layer_against_single_expert_calls(gpu):
+    """A layer of 70 tokens with every token on the same experts equals the products called one after another
+    in fp32, and one token alone (its own kernels) equals its row up to the roundings of h."""
+    from constellation_amd.engine import Q4Layer, Q4Matrix
+    print("[q4] layer against products", flush=True)
+    E, H, I, T = 4, 384, 256, 70
+    gu, dn = make(1, E, 2 * I, H, 32), make(2, E, H, I, 128)
+    mats = [Q4Matrix.pack(gu[0].cuda(), gu[1].cuda(), H, group=32, gated=True), Q4Matrix.pack(dn[0].cuda(), dn[1].cuda(), I)]
+    try:
+        layer = Q4Layer(gpu, *mats)
+        x, w = rand(3, T, H, dtype=BF), torch.rand(T, 2, generator=torch.Generator().manual_seed(4))
+        ids = torch.tensor([[2, 0]] * T, dtype=torch.int32)
+        _, yf = gpu.moe(layer, x.cuda(), ids.cuda(), w.cuda(), want_f32=True)
+        want, tol = layer_ref(x.double(), ids, w, dense(gu[0], gu[1], H, 32), dense(dn[0], dn[1], I, 128), 2.0 ** -12)
+        near(yf, want, tol, "layer")
+        for t in (0, 33):
+            _, one = gpu.moe(layer, x[t:t + 1].cuda(), ids[t:t + 1].cuda(), w[t:t + 1].cuda(), want_f32=True)
+            near(one, want[t:t + 1], tol[t:t + 1], t)
+    finally:
+        for m in mats:
+            m.free()
