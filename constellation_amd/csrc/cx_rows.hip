@@ -639,7 +639,7 @@ hipError_t launch_sort_tokens(const SortArgs& a, hipStream_t s) {
     if (ids <= kSortThreads && a.n_experts + 2 <= kSortThreads) {
         cx_launch(k_sort_tokens<true>, dim3(1), dim3(kSortThreads), 0, s, a);
     } else {
-        const int64_t wgs = std::min<int64_t>(64, (ids + kSortThreads - 1) / kSortThreads);
+        const int64_t wgs = std::clamp<int64_t>((ids + kSortThreads - 1) / kSortThreads, 1, 64);
         cx_launch(k_sort_tokens<false>, dim3((unsigned)wgs), dim3(kSortThreads), 0, s, a);
     }
     return hipGetLastError();

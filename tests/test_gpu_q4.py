@@ -16,6 +16,9 @@ U = 2.0 ** -24
 BF, HF, SF, F8 = torch.bfloat16, torch.float16, torch.float32, torch.float8_e4m3fn
 HALF = {BF: 2.0 ** -8, HF: 2.0 ** -11, SF: 2.0 ** -24}
 TINY = {BF: 2.0 ** -134, HF: 2.0 ** -25, SF: 2.0 ** -150}
+# h takes part in the down product as fp16 times a power of two per row: 11 significant bits, whose
+# half step is at most 2^-11 of the value (1 + 2^-11 lies between 1 and its neighbour 1 + 2^-10)
+H_HALF = 2.0 ** -11
 E2M1 = torch.tensor([0, .5, 1, 1.5, 2, 3, 4, 6, 0, -.5, -1, -1.5, -2, -3, -4, -6], dtype=torch.float64)
 
 
@@ -236,8 +239,7 @@ def test_q4_layer(gpu, T, K, E, H, I, group, dtype, shared):
         torch.cuda.synchronize()
         gpu.sync()
         D = [dense(c, s, k, group) for (c, s), k in ((gu, H), (dn, I), (sg, H), (sd, I))]
-        # h is kept to 16 significant bits or more
-        want, tol = layer_ref(x.double(), ids, w, D[0], D[1], 2.0 ** -12, (D[2], D[3]) if shared else None)
+        want, tol = layer_ref(x.double(), ids, w, D[0], D[1], H_HALF, (D[2], D[3]) if shared else None)
         near(yf, want, tol, "fp32")
         near(y, want, rounded(want, tol, dtype), "rounded")
         if not shared:
@@ -535,11 +537,32 @@ def test_q4_layer_against_single_expert_calls(gpu):
         x, w = rand(3, T, H, dtype=BF), torch.rand(T, 2, generator=torch.Generator().manual_seed(4))
         ids = torch.tensor([[2, 0]] * T, dtype=torch.int32)
         _, yf = gpu.moe(layer, x.cuda(), ids.cuda(), w.cuda(), want_f32=True)
-        want, tol = layer_ref(x.double(), ids, w, dense(gu[0], gu[1], H, 32), dense(dn[0], dn[1], I, 128), 2.0 ** -12)
+        want, tol = layer_ref(x.double(), ids, w, dense(gu[0], gu[1], H, 32), dense(dn[0], dn[1], I, 128), H_HALF)
         near(yf, want, tol, "layer")
         for t in (0, 33):
             _, one = gpu.moe(layer, x[t:t + 1].cuda(), ids[t:t + 1].cuda(), w[t:t + 1].cuda(), want_f32=True)
             near(one, want[t:t + 1], tol[t:t + 1], t)
+    finally:
+        for m in mats:
+            m.free()
+
+
+def test_q4_layer_of_the_shared_expert_alone(gpu):
+    """Tokens without routes (top_k 0) through a layer of 600 experts: the shared one takes them all."""
+    from constellation_amd.engine import Q4Layer, Q4Matrix
+    print("[q4] shared expert alone", flush=True)
+    E, H, I = 600, 40, 24
+    stacks = [make(i, n, *s, 32) for i, (n, s) in enumerate(((E, (2 * I, H)), (E, (H, I)), (1, (2 * I, H)), (1, (H, I))))]
+    mats = [Q4Matrix.pack(c.cuda(), s.cuda(), k, group=32, gated=gt) for (c, s), k, gt in zip(stacks, (H, I, H, I), (True, False) * 2)]
+    try:
+        layer = Q4Layer(gpu, mats[0], mats[1], (mats[2], mats[3]))
+        D = [dense(c, s, k, 32) for (c, s), k in zip(stacks, (H, I, H, I))]
+        for T in (1, 2, 150):
+            x, ids, w = rand(T, T, H, dtype=BF), torch.empty(T, 0, dtype=torch.int32), torch.empty(T, 0)
+            _, yf = gpu.moe(layer, x.cuda(), ids.cuda(), w.cuda(), want_f32=True)
+            gpu.sync()
+            want, tol = layer_ref(x.double(), ids, w, D[0], D[1], H_HALF, (D[2], D[3]))
+            near(yf, want, tol, T)
     finally:
         for m in mats:
             m.free()

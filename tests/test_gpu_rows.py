@@ -359,3 +359,13 @@ def test_rows_in_graphs_and_streams(gpu):
         for k, (a, b) in enumerate(zip(got, want)):
             assert torch.equal(a, b), (i, k)
     del g
+
+
+@pytest.mark.parametrize("E", [1, 510, 511, 600, 1024])
+def test_sort_no_tokens(gpu, E):
+    """No pairs at all, on both sides of the sort's limits for one workgroup."""
+    print(f"[rows] sort nothing over {E}", flush=True)
+    for K in (1, 8):
+        order, offsets, place = gpu.sort_tokens(torch.empty((0, K), dtype=torch.int32, device="cuda"), E)
+        assert order.numel() == 0 and place.shape == (0, K) and offsets.cpu().tolist() == [0] * (E + 1)
+    gpu.sync()
