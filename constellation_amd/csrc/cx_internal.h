@@ -332,6 +332,37 @@ __device__ inline void q4_put_items(Q4Item* items, int n, int expert, int begin,
     for (int i = from; i < n; i += step) items[i] = Q4Item{expert, begin + i * share, min(share, rows - i * share), 0};
 }
 
+// Where a matrix's items start in a list whose long items come first, by the rows of its
+// items (shares) in 16s: the workgroups that end a launch are then the short ones.
+// Among equals the order is that of the atomics, and nothing that is computed depends on it.
+// `totals` in LDS: zeros before the first barrier; count() before the second, all() and place() after it.
+struct Q4LongFirst {
+    static constexpr int kClasses = kQ4GemmRows / 16;
+    int* totals;  // [2][kClasses]
+
+    __device__ __forceinline__ static int items(int rows, int item_rows) { return (rows + item_rows - 1) / item_rows; }
+    __device__ __forceinline__ static int cls(int n, int rows) {
+        return kClasses - min(kClasses, max(1, (q4_item_share(n, rows) + 15) / 16));
+    }
+    __device__ __forceinline__ void count(int n, int rows) const {
+        if (n > 0) atomicAdd(&totals[cls(n, rows)], n);
+    }
+    __device__ __forceinline__ int all() const {
+        int v = 0;
+#pragma unroll
+        for (int b = 0; b < kClasses; ++b) v += totals[b];
+        return v;
+    }
+    __device__ __forceinline__ int place(int n, int rows) const {
+        if (n == 0) return 0;
+        const int c = cls(n, rows);
+        int at = atomicAdd(&totals[kClasses + c], n);
+#pragma unroll
+        for (int b = 0; b < kClasses; ++b) at += b < c ? totals[b] : 0;
+        return at;
+    }
+};
+
 struct SortArgs {
     const int32_t* ids;    // [n_tokens, top_k]
     const float* weights;  // nullable: when given, a repeated expert or a bad weight is an error and its pair's place negative

@@ -185,8 +185,9 @@ __global__ __launch_bounds__(256) void k_q4_rows(const void* x, int cols, int pa
 // go back or past the rows are cut to what is there, so that no item leaves it.
 __global__ __launch_bounds__(1024) void k_q4_items(const int32_t* offsets, int n_mats, int n_rows, int item_rows,
                                                    Q4Item* items, int* err_flag) {
-    __shared__ int top[1024], cnt[1024];
+    __shared__ int top[1024], totals[2 * Q4LongFirst::kClasses];
     const int e = threadIdx.x;
+    if (e < 2 * Q4LongFirst::kClasses) totals[e] = 0;
     const int raw0 = offsets[min(e, n_mats)], raw1 = offsets[min(e + 1, n_mats)];
     if (e < n_mats && (raw0 > raw1 || raw0 < 0 || raw1 > n_rows || (e == 0 && raw0 != 0))) atomicOr(err_flag, kErrBadRow);
     top[e] = min(max(raw1, 0), n_rows);
@@ -198,17 +199,13 @@ __global__ __launch_bounds__(1024) void k_q4_items(const int32_t* offsets, int n
         __syncthreads();
     }
     const int begin = e == 0 ? 0 : top[e - 1], rows = e < n_mats ? top[e] - begin : 0;
-    const int n = (rows + item_rows - 1) / item_rows;
-    cnt[e] = n;
+    const Q4LongFirst list{totals};
+    const int n = list.items(rows, item_rows);
+    list.count(n, rows);
     __syncthreads();
-    for (int d = 1; d < 1024; d <<= 1) {
-        const int v = e >= d ? cnt[e] + cnt[e - d] : cnt[e];
-        __syncthreads();
-        cnt[e] = v;
-        __syncthreads();
-    }
-    q4_put_items(items + 1 + cnt[e] - n, n, e, begin, rows, 0, 1);
-    const int held = top[1023], all = cnt[1023], rest = (n_rows - held + item_rows - 1) / item_rows;
+    q4_put_items(items + 1 + list.place(n, rows), n, e, begin, rows, 0, 1);
+    const int all = list.all();
+    const int held = top[1023], rest = (n_rows - held + item_rows - 1) / item_rows;
     q4_put_items(items + 1 + all, rest, -1, held, n_rows - held, e, 1024);  // rows behind the last matrix's: zeros
     if (e == 0) items[0] = Q4Item{all + rest, held, 0, 0};
 }

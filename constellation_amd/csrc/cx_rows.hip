@@ -281,7 +281,7 @@ __device__ __forceinline__ void scan_counts(int* v, int n, int* wave_tot) {
 template <bool SMALL>
 __global__ __launch_bounds__(kSortThreads) void k_sort_tokens(SortArgs a) {
     constexpr int kKeys = SMALL ? kSortThreads : kSortKeys, kPer = SMALL ? 1 : (kSortKeys + kSortThreads) / kSortThreads;
-    __shared__ int first[kKeys + 1], next[kKeys + 1], items[kKeys + 1];
+    __shared__ int first[kKeys + 1], next[kKeys + 1], totals[2 * Q4LongFirst::kClasses];
     __shared__ int hist[kSortWaves][kKeys];
     __shared__ int wave_tot[kSortWaves];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
@@ -318,6 +318,7 @@ __global__ __launch_bounds__(kSortThreads) void k_sort_tokens(SortArgs a) {
     };
     const int own = SMALL && tid < N ? a.ids[tid] : 0;
     for (int e = tid; e <= NK + 1; e += kSortThreads) first[e] = next[e] = 0;
+    if (tid < 2 * Q4LongFirst::kClasses) totals[tid] = 0;
     if constexpr (SMALL) {
         for (int w = 0; w < kSortWaves; ++w)
             if (tid <= NK) hist[w][tid] = 0;
@@ -357,11 +358,6 @@ __global__ __launch_bounds__(kSortThreads) void k_sort_tokens(SortArgs a) {
         for (int e = tid; e <= NK; e += kSortThreads) first[e] += next[e];
     }
     __syncthreads();
-    if (blockIdx.x == 0 && a.items != nullptr) {
-        for (int e = tid; e < NK; e += kSortThreads) items[e] = (first[e] + a.item_rows - 1) / a.item_rows;
-        __syncthreads();
-        scan_counts<kPer>(items, NK, wave_tot);
-    }
     scan_counts<kPer>(first, NK + 1, wave_tot);
     const int shared_row = first[NK];  // the shared expert's rows, then those without an expert
     const int none = a.shared ? a.n_tokens : 0;
@@ -369,11 +365,20 @@ __global__ __launch_bounds__(kSortThreads) void k_sort_tokens(SortArgs a) {
         if (a.offsets != nullptr)
             for (int e = tid; e <= NK; e += kSortThreads) a.offsets[e] = first[e];
         if (a.items != nullptr) {
-            for (int e = tid; e < NK; e += kSortThreads)
-                q4_put_items(a.items + 1 + items[e], items[e + 1] - items[e], e, first[e], first[e + 1] - first[e], 0, 1);
-            const int more = (none + a.item_rows - 1) / a.item_rows;
-            q4_put_items(a.items + 1 + items[NK], more, NK, shared_row, none, tid, kSortThreads);
-            if (tid == 0) a.items[0] = Q4Item{items[NK] + more, shared_row + none, 0, 0};
+            const int more = (none + a.item_rows - 1) / a.item_rows;  // of the shared expert, whose items are the longest
+            q4_put_items(a.items + 1, more, NK, shared_row, none, tid, kSortThreads);
+            const Q4LongFirst list{totals};
+            for (int e = tid; e < NK; e += kSortThreads) {
+                const int rows = first[e + 1] - first[e];
+                list.count(list.items(rows, a.item_rows), rows);
+            }
+            __syncthreads();
+            for (int e = tid; e < NK; e += kSortThreads) {
+                const int rows = first[e + 1] - first[e], n = list.items(rows, a.item_rows);
+                q4_put_items(a.items + 1 + more + list.place(n, rows), n, e, first[e], rows, 0, 1);
+            }
+            const int all = more + list.all();
+            if (tid == 0) a.items[0] = Q4Item{all, shared_row + none, 0, 0};
         }
     }
     if (a.shared)

@@ -566,3 +566,39 @@ def test_q4_layer_of_the_shared_expert_alone(gpu):
     finally:
         for m in mats:
             m.free()
+
+
+@pytest.mark.parametrize("E,shared", [(5, True), (200, False), (1024, True)])
+def test_q4_layer_skewed_routes(gpu, E, shared):
+    """Experts of no, one and hundreds of rows in one call: items of every length, from one and from
+    several workgroups of the sort, and of two experts a thread."""
+    from constellation_amd.engine import Q4Layer, Q4Matrix
+    print(f"[q4] skewed over {E} shared {shared}", flush=True)
+    H, I, T, K = 72, 32, 700, 3
+    stacks = [make(i + E, n, *s, 32) for i, (n, s) in enumerate(((E, (2 * I, H)), (E, (H, I)), (1, (2 * I, H)), (1, (H, I))))]
+    mats = [Q4Matrix.pack(c.cuda(), s.cuda(), k, group=32, gated=gt) for (c, s), k, gt in zip(stacks, (H, I, H, I), (True, False) * 2)]
+    try:
+        layer = Q4Layer(gpu, mats[0], mats[1], (mats[2], mats[3]) if shared else None)
+        g = torch.Generator().manual_seed(E)
+        lean = torch.randn(E, generator=g) * 2
+        ids = (torch.randn(T, E, generator=g) + lean).topk(K, dim=1).indices.to(torch.int32)
+        x, w = rand(1, T, H, dtype=BF), torch.rand(T, K, generator=g)
+        _, yf = gpu.moe(layer, x.cuda(), ids.cuda(), w.cuda(), want_f32=True)
+        gpu.sync()
+        D = [dense(c, s, k, 32) for (c, s), k in zip(stacks, (H, I, H, I))]
+        want, tol = layer_ref(x.double(), ids, w, D[0], D[1], H_HALF, (D[2], D[3]) if shared else None)
+        near(yf, want, tol, E)
+        # the same rows as a stack's: some matrices without rows, rows behind the last one
+        order, offsets, _ = gpu.sort_tokens(ids.cuda(), E)
+        for gap in (0, 37):
+            off = offsets.cpu().clamp(max=T * K - gap)
+            got = gpu.q4_matmul(mats[1], x.cuda()[:, :I].contiguous(), offsets=off.cuda(), order=order, top_k=K, out_dtype=SF).cpu().double()
+            gpu.sync()
+            e_of = torch.searchsorted(off[1:].long(), torch.arange(T * K), right=True)
+            src = x.double()[(order.cpu() // K).long(), :I]
+            rows = torch.stack([D[1][min(int(e), E - 1)] @ v if e < E else torch.zeros(H, dtype=torch.float64) for e, v in zip(e_of, src)])
+            size = torch.stack([D[1][min(int(e), E - 1)].abs() @ v.abs() for e, v in zip(e_of, src)])
+            near(got, rows, size * (I + 8) * U + TINY[SF], (E, gap))
+    finally:
+        for m in mats:
+            m.free()
