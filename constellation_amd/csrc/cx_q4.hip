@@ -237,11 +237,12 @@ namespace {
 
 size_t up256(size_t v) { return (v + 255) / 256 * 256; }
 
-// Ranges of the columns per row tile: as many waves as 16 a CU take at once, of at least 2
-// column tiles.
-int column_splits(int64_t waves, int KT, int most) {
+// Ranges of the columns per row tile: up to `all` waves in the launch (16 a CU are 4096), of at least 2
+// column tiles each.  The kernel of few rows, whose waves wait for x now and then, takes twice as many
+// (18432 x 7168, 1 and 16 rows: 22.8 and 32 us, with 4096 waves 26.8 and 39.8); the decode kernel does not gain.
+int column_splits(int64_t waves, int KT, int most, int64_t all) {
     int n = 1;
-    while (n < most && waves * n * 2 <= 4096 && KT / n >= 4) n *= 2;
+    while (n < most && waves * n * 2 <= all && KT / n >= 4) n *= 2;
     return n;
 }
 
@@ -254,7 +255,9 @@ hipError_t few_launch(const Q4Launch& L, hipStream_t s) {
     const int RT = q4_row_tiles(L.w), KT = q4_col_tiles(L.w), el = L.x_type == kQ4E4m3 ? 1 : 2;
     const int64_t busy = busy_mats(L);
     const bool vec = L.w.cols % 8 == 0 && (reinterpret_cast<uintptr_t>(L.x) & (8 * el - 1)) == 0 && (int64_t)L.n_x * L.w.cols * el < (int64_t)kOob;
-    const int rw = L.n_rows > 4 * busy ? 2 : 1, splits = column_splits(busy * ((RT + rw - 1) / rw), KT, kQ4FewWaves);
+    // two row tiles a wave, on one read of x, where that leaves enough waves (7168 x 2048, 1 row: 5.5 and 8.2 us;
+    // 4096 x 7168: 8.0 and 7.2, 512 x 512: 5.1 and 4.4)
+    const int rw = RT > 256 ? 2 : 1, splits = column_splits(busy * ((RT + rw - 1) / rw), KT, kQ4FewWaves, 8192);
     const int per = kQ4FewWaves / splits * rw, row_blocks = (RT + per - 1) / per;
     auto k = vec ? (rw == 2 ? k_q4_few<XT, NG, 2, true> : k_q4_few<XT, NG, 1, true>) : (rw == 2 ? k_q4_few<XT, NG, 2, false> : k_q4_few<XT, NG, 1, false>);
     cx_launch(k, dim3((unsigned)(item_bound(L) * row_blocks)), dim3(64 * kQ4FewWaves), 0, s, L, RT, KT, splits, row_blocks);
@@ -281,14 +284,14 @@ hipError_t launch_q4_routes(const Q4Launch& L, const Q4Launch& D, const Q4Routes
                             float* y_f32, hipStream_t s) {
     const int ke = routes.top_k + routes.shared;
     const int64_t pairs = (int64_t)n_tokens * ke;
-    const hipError_t e = launch_q4_dec(L, &routes, column_splits(pairs * q4_row_tiles(L.w), q4_col_tiles(L.w), kQ4DecWaves), pairs, s);
+    const hipError_t e = launch_q4_dec(L, &routes, column_splits(pairs * q4_row_tiles(L.w), q4_col_tiles(L.w), kQ4DecWaves, 4096), pairs, s);
     if (e != hipSuccess) return e;
     return launch_q4_dec_sum(Q4DecSumArgs{D.w, D.shared, routes, static_cast<const float*>(D.x), y, y_f32, out_dtype,
                                           q4_row_tiles(D.w), q4_col_tiles(D.w)}, n_tokens, s);
 }
 
 hipError_t launch_q4(const Q4Launch& L, hipStream_t s) {
-    if (L.item_rows < kTileTok) return launch_q4_dec(L, nullptr, column_splits(busy_mats(L) * q4_row_tiles(L.w), q4_col_tiles(L.w), kQ4DecWaves), item_bound(L), s);
+    if (L.item_rows < kTileTok) return launch_q4_dec(L, nullptr, column_splits(busy_mats(L) * q4_row_tiles(L.w), q4_col_tiles(L.w), kQ4DecWaves, 4096), item_bound(L), s);
     if (L.item_rows > kTileTok) {
         const int padded = q4_col_tiles(L.w) * 128;
         Q4Launch G = L;

@@ -817,7 +817,7 @@ struct Q4Scratch {
 
 Q4Scratch q4_scratch(const cx_q4_desc& w, int x_dtype, int n_x, int n_rows, bool with_offsets) {
     Q4Scratch z{};
-    z.item_rows = q4_item_rows(n_rows, w.n_mats, w.cols, x_dtype == CX_DTYPE_E4M3);
+    z.item_rows = q4_item_rows(n_rows, w.n_mats, w.rows, w.cols, x_dtype == CX_DTYPE_E4M3);
     z.max_items = q4_max_items(n_rows, w.n_mats, z.item_rows);
     z.x = with_offsets ? align_up(sizeof(Q4Item) * (size_t)z.max_items) : 0;
     z.part = z.x + (z.item_rows > kTileTok ? q4_x_scratch(w, n_x) : 0);
@@ -836,8 +836,7 @@ Q4MoeScratch q4_moe_scratch(const cx_q4_desc& gu, const cx_q4_desc& down, int sh
     Q4MoeScratch z{};
     z.pairs = (int64_t)n_tokens * (top_k + shared);
     // both products take the same items; in between h is fp32, which the decode kernel and the GEMM read
-    z.item_rows = q4_item_rows(z.pairs, gu.n_mats + shared, std::max(gu.cols, down.cols), false);
-    if (z.item_rows == kTileTok) z.item_rows = kQ4GemmRows;
+    z.item_rows = q4_layer_rows(z.pairs, gu.n_mats + shared, std::max(gu.cols, down.cols));
     z.max_items = q4_max_items(z.pairs, gu.n_mats + shared, z.item_rows);
     const bool gemm = z.item_rows > kTileTok;
     z.items = 0;

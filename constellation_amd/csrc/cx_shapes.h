@@ -274,7 +274,7 @@ inline bool rows_grid_ok(int64_t workgroups, int threads) { return workgroups * 
 
 // Rows of x per work item: up to 4 for the decode kernel, which stages them in LDS; up to 16
 // for the kernel of few rows, which reads them from L2; up to 128 for the GEMM (64 where
-// it keeps a second set of sums).  The first two stream a matrix's weights once per item.
+// it keeps a second set of sums).
 constexpr int kQ4GemmRows = 128;
 constexpr int kQ4DecWaves = 8, kQ4DecPieces = 2;  // waves and, of a staged row, 8-value pieces a thread
 constexpr int kQ4DecCols = kQ4DecPieces * 64 * kQ4DecWaves * 8;
@@ -294,10 +294,25 @@ inline bool q4_routes_ok(int n_tokens, int top_k, int hidden, int inter, int sha
     return n_tokens == 1 && hidden <= kQ4DecCols && inter <= kQ4SumHeld * 512 && top_k + shared <= 16 &&
            q4_sum_lds(inter, top_k + shared) <= 63 * 1024;
 }
-inline int q4_item_rows(int64_t n_rows, int n_mats, int cols, bool two_sums) {
+// The kernel of a product by its items' rows.  One matrix and up to 16 rows: few rows (bf16 4096 x 7168,
+// 1 and 4 rows: 7.2 and 8.2 us, decode kernel 8.1 and 11.5; 16 rows 11.7, GEMM at 17 22.7), whose reads of x
+// need whole pieces of 8 columns: otherwise the decode kernel as far as it goes, then, unless columns are
+// few, the GEMM (4096 x 7161, 4 to 16 rows: 22 us, few rows 26 to 42; 1000 x 1411: 13, 12 to 17).  A stack: the decode
+// kernel while matrices have one row on average (64 of 4096 x 7168, 64 rows: 122 us, GEMM 162; 96 rows
+// 173 and 177), then the GEMM (256 rows: 190 us, few rows 310; 1024: 208 and 357), but few rows up to
+// 16 a matrix while all codes are so few that launches decide (8 of 512 x 1024: 9 to 10 us, GEMM
+// 15 to 17; 16 of 1024 x 2048: 15 to 28 and 19 to 22).
+constexpr int64_t kQ4SmallStack = 8 << 20;  // bytes of codes
+inline int q4_item_rows(int64_t n_rows, int n_mats, int rows, int cols, bool two_sums) {
     const int dec = q4_dec_rows(cols);
-    if (dec > 0 && (n_rows <= dec || (n_mats > 1 && n_rows <= n_mats))) return dec;
-    return n_rows <= (int64_t)kTileTok * n_mats ? kTileTok : two_sums ? kQ4GemmRows / 2 : kQ4GemmRows;
+    if (dec > 0 && n_rows <= (n_mats > 1 ? n_mats : cols % 8 != 0 ? dec : 0)) return dec;
+    const bool small = n_mats == 1 || (int64_t)n_mats * rows * cols / 2 <= kQ4SmallStack, pieces = cols % 8 == 0 || cols <= 1024;
+    return small && pieces && n_rows <= (int64_t)kTileTok * n_mats ? kTileTok : two_sums ? kQ4GemmRows / 2 : kQ4GemmRows;
+}
+// Of a layer, whose second product reads the first one's fp32 rows: the decode kernel or the GEMM.
+inline int q4_layer_rows(int64_t n_rows, int n_mats, int cols) {
+    const int dec = q4_dec_rows(cols);
+    return dec > 0 && n_rows <= std::max(n_mats, dec) ? dec : kQ4GemmRows;
 }
 
 // Ranges of the columns that the GEMM deals to workgroups of their own, whose partial sums a

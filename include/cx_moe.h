@@ -366,10 +366,10 @@ CX_API int cx_q4_free(int device, cx_q4_desc* w);
 /* y = x W^T (gated: silu(x G^T) * (x U^T)), fp32 accumulation of exact products,
  * rounded once.
  * x: [*, cols] fp16, bf16, or e4m3 with x_scale [*, ceil(cols / 128)].
- * y: [n_rows, rows] (gated: rows / 2) in fp16, bf16 or fp32.  With more than
- * 16 rows per matrix, bf16 rows of x take part as fp16 times a power of two per
- * row: exact but for values below 2^-31 of the row's largest, which are off by
- * less than 2^-39 of that.
+ * y: [n_rows, rows] (gated: rows / 2) in fp16, bf16 or fp32.  bf16 rows of x
+ * may take part as fp16 times a power of two per row: exact but for values below
+ * 2^-31 of the row's largest, which are off by less than 2^-39 of that.  All
+ * sums stay finite for scales below 2^80 and rows of x below 2^88.
  * offsets NULL: one matrix (n_mats 1) for all rows.  Otherwise rows
  * offsets[e] .. offsets[e + 1] - 1 go through matrix e (cx_sort_tokens' offsets,
  * [n_mats + 1]) and the rows behind the last matrix's are zeros; offsets that
@@ -390,7 +390,10 @@ CX_API int cx_q4_matmul(cx_ctx* ctx, const cx_q4_desc* w, const void* x, int x_d
  * twice for one token and a bad weight are skipped and reported by cx_ctx_sync).
  * gate_up: gated [2 * inter, hidden] per expert; down: [hidden, inter] per expert;
  * shared_gate_up / shared_down (nullable, together): the shared expert, stacks of
- * one with the same sizes and groups.  Any n_tokens, 0 included.
+ * one with the same sizes and groups.  h = silu(gate) * up is kept in fp32 and
+ * takes part in the down product as fp16 times a power of two per row (11 bits).
+ * n_tokens may be 0; a call whose padded rows of x or h would pass 4 GB in fp16
+ * (about 299,000 tokens of 7168, or a million pairs of 2048) is refused.
  * scratch: cx_q4_moe_scratch bytes of the caller's, as above; a captured graph
  * keeps using the scratch it was captured with. */
 CX_API size_t cx_q4_moe_scratch(const cx_q4_desc* gate_up, const cx_q4_desc* down, int has_shared,

@@ -16,7 +16,8 @@ using namespace cx;
 extern "C" {
 int share(int n, int rows) { return q4_item_share(n, rows); }
 int64_t most(int64_t rows, int mats, int item) { return q4_max_items(rows, mats, item); }
-int item(int64_t rows, int mats, int cols, int two) { return q4_item_rows(rows, mats, cols, two); }
+int item(int64_t rows, int mats, int n, int cols, int two) { return q4_item_rows(rows, mats, n, cols, two); }
+int layer(int64_t rows, int mats, int cols) { return q4_layer_rows(rows, mats, cols); }
 int dec_rows(int cols) { return q4_dec_rows(cols); }
 size_t dec_lds(int cols, int rows) { return q4_dec_lds(cols, rows); }
 int routes(int t, int k, int h, int i, int sh) { return q4_routes_ok(t, k, h, i, sh); }
@@ -36,7 +37,8 @@ def rules(tmp_path_factory):
     L.most.restype = C.c_int64
     L.dec_lds.restype = L.sum_lds.restype = C.c_size_t
     L.most.argtypes = [C.c_int64, C.c_int, C.c_int]
-    L.item.argtypes = [C.c_int64, C.c_int, C.c_int, C.c_int]
+    L.item.argtypes = [C.c_int64, C.c_int, C.c_int, C.c_int, C.c_int]
+    L.layer.argtypes = [C.c_int64, C.c_int, C.c_int]
     L.splits.argtypes = [C.c_int, C.c_int, C.c_int64, C.c_int, C.c_int]
     return L
 
@@ -70,14 +72,23 @@ def test_staged_rows_fit_the_lds(rules):
         assert 0 <= rows <= 4 and (rows == 0) == (cols > 8192)
         if rows:
             assert rules.dec_lds(cols, rows) <= 64 * 1024 - 256
-            assert rules.item(1, 1, cols, 0) == rows
-        assert rules.item(10 ** 6, 1, cols, 0) == 128 and rules.item(10 ** 6, 1, cols, 1) == 64
+            assert rules.item(1, 1, 64, cols, 0) == (rows if cols % 8 else 16) and rules.item(8, 8, 64, cols, 0) == rows
+            assert rules.layer(1, 1, cols) == rules.layer(rows, 1, cols) == rules.layer(64, 64, cols) == rows
+        assert rules.layer(65, 64, cols) == 128 and rules.item(16, 1, 64, cols, 0) == (16 if cols % 8 == 0 or cols <= 1024 else 128)
+        assert rules.item(10 ** 6, 1, 64, cols, 0) == 128 and rules.item(10 ** 6, 1, 64, cols, 1) == 64
     for inter in range(1, 2100, 17):
         for k in (1, 2, 8, 9, 15, 16, 17, 64):
             if rules.routes(1, k, 7168, inter, 0):
                 assert k <= 16 and inter <= 2048 and rules.sum_lds(inter, k) <= 64 * 1024
             assert not rules.routes(2, k, 7168, inter, 0)
     assert rules.routes(1, 8, 7168, 2048, 1)
+
+
+def test_stacks_by_their_size(rules):
+    """Few rows per matrix: by launches where the codes are few, and without overflow where they are many."""
+    assert rules.item(64, 8, 512, 1024, 0) == 16 and rules.item(129, 8, 512, 1024, 0) == 128
+    assert rules.item(600, 64, 4096, 7168, 0) == 128 and rules.item(600, 64, 4096, 7168, 1) == 64
+    assert rules.item(5000, 1024, 1 << 24, 1 << 24, 0) == 128
 
 
 def test_ranges_of_the_columns(rules):
