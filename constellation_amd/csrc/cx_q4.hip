@@ -74,8 +74,9 @@ __global__ __launch_bounds__(256) void k_q4_row_scales(cx_q4_desc w, const uint1
 // values (8 significant bits) are exact down to 2^-31 of it and the others off by less than
 // 2^-39 of it: nothing next to the sums' own 2^-24.  fp32 values are rounded to 11 bits.
 //
-// A row is read once, kPieces pieces of 8 values a thread in registers (wider rows are read
-// again for what lies behind), 16 bytes at a time where it starts on them.
+// A row is read once, kRowPieces pieces of 8 values a thread in registers (wider rows are read
+// again for what lies behind), 16 bytes at a time where it starts on them.  1024 bf16 rows of 7168 take 9
+// us, 8192 fp32 rows of 2048 22 (100 MB, 4.6 TB/s), 3001 e4m3 rows of 2048 7.
 constexpr int kRowPieces = 4;
 
 template <int DT>

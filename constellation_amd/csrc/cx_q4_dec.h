@@ -44,7 +44,9 @@ struct Q4Ring {
 
 // A wave takes one row tile and one range of the column tiles; the partial sums of the ranges
 // are added in order.  HBM bounds it as long as enough bytes are in flight: a wave's ring holds U
-// tiles of codes (1 KB each) and refills a place as soon as it has multiplied it.
+// tiles of codes (1 KB each) and refills a place as soon as it has multiplied it.  Gate and up
+// of 8 experts of 7168 x 2048 for one token, 121 MB: 24 us, 5 TB/s; 64 rows over 40 of 64 matrices of 4096 x 7168,
+// 605 MB: 122 us.  (x from L2, as the kernel of few rows has it: 161 us.)
 //
 // x is staged once per workgroup as fp16 in LDS: fp16 and e4m3 values as they are, others
 // times the power of two that brings the row's largest value to 2^14 .. 2^15 (bf16 is then
@@ -241,7 +243,7 @@ __global__ __launch_bounds__(64 * kQ4DecWaves) void k_q4_dec(Q4DecArgs A) {
 // The down projections of a token's routes and their weighted sum, for a few tokens: a wave per
 // route, all on the same row tile, whose results are summed in route order (the shared
 // expert last) and rounded once.  Each wave stages its own row of h as k_q4_dec does, so
-// the only barrier is the one before the sum.
+// the only barrier is the one before the sum.  HBM: 8 routes of 7168 x 2048, 61 MB in 13 us, 4.6 TB/s.
 template <int NG, int U>
 __global__ __launch_bounds__(1024) void k_q4_dec_sum(Q4DecSumArgs A) {
     extern __shared__ __attribute__((aligned(16))) unsigned char staged[];

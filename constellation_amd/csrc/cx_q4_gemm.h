@@ -32,6 +32,15 @@ constexpr int kQ4GemmWaves = 4;
 // k_q4_row_scales) for the MFMAs of all the item's rows; the rows of x go straight from
 // memory to one of two LDS buffers, a column tile ahead.  The buffers are two objects:
 // the compiler then knows that reads of one need not wait for loads into the other.
+//
+// What bounds it: issue.  Beside an MFMA of 16 cycles a wave converts codes (a pack of two codes and
+// a product with the scale for every two weights), reads a fragment of x and waits its turn; with
+// 8 tiles of rows to a conversion and two workgroups a CU the matrix cores are busy 69 % of the time
+// (4096 rows by 4096 x 7168: 192 us, 1.25 PFLOP/s; a library's bf16 product reaches 1.43 on
+// this card).  Fewer rows per item amortise a conversion less: 1024 tokens over 64 experts, gate/up 500
+// us and 60 %.  Steps that led here, at that size (both products and what is around them): x through
+// registers 1476 us, straight to LDS with fragments two steps ahead 1000, outputs turned in LDS 935,
+// equal items and wide conversions 819, long items first 789.
 constexpr int kQ4GemmBuf = kQ4GemmRows * 256;
 
 // s_waitcnt vmcnt(0) lgkmcnt(0), then a barrier: the loads into the other buffer have
@@ -128,7 +137,9 @@ __device__ __forceinline__ void q4_gemm_store(const Q4GemmArgs& L, const f32x4 (
 // XS (e4m3 rows of x, as fp16): each column tile's sums are scaled by the row's x_scale in
 // fp32 before they are added up, with items of up to 64 rows for the second set of sums.
 // The matrix cores' own 8-bit products would be twice as fast, but drop what lies 2^13
-// below the largest product of an instruction, and sums here are kept to fp32.
+// below the largest product of an instruction, and sums here are kept to fp32.  The second set of
+// sums costs a multiply-add per MFMA and 4 values, and half the rows per conversion: 3001
+// rows by 7168 x 2048 in 101 to 116 us, 0.8 to 0.87 PFLOP/s (128 rows and one workgroup a CU: 8 % slower).
 template <int NG, int RTW, int NT, bool XS>
 __device__ __forceinline__ void q4_gemm_tile(const Q4GemmArgs& L, unsigned char* lds0, unsigned char* lds1, const cx_q4_desc& w,
                                              size_t mat, int rb, int ks, int begin, int rows) {

@@ -248,7 +248,7 @@ def test_combine_leaves_out_bad_rows_and_weights(gpu):
 
 
 @pytest.mark.parametrize("dtype,dodt", [(BF, BF), (HF, SF), (SF, SF), (SF, BF)])
-@pytest.mark.parametrize("T,K,H,drop", [(1, 8, 7168, 0.0), (33, 3, 1411, 0.3), (3, 64, 136, 0.2), (130, 1, 1, 0.5), (1030, 9, 72, 0.1)])
+@pytest.mark.parametrize("T,K,H,drop", [(1, 8, 7168, 0.0), (33, 3, 1411, 0.3), (3, 64, 136, 0.2), (130, 1, 1, 0.5), (447, 9, 72, 0.1), (448, 10, 72, 0.1), (1030, 9, 72, 0.1)])
 def test_combine_rows_grad(gpu, T, K, H, drop, dtype, dodt):
     print(f"[rows] grad {T}x{K}x{H} {dtype} {dodt}", flush=True)
     place = sorted_ref(some_ids(H, T, K, 16, drop), 16)[2]
