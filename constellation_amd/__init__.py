@@ -5,7 +5,8 @@ include/cx_moe.h (libcx_moe.so).
 
 Python modules:
   _lib               ctypes binding of the C ABI (no fallback)
-  engine             torch-tensor handles: Context, Expert, Layer
+  engine             torch-tensor handles: Context, Expert, Layer, Q4Matrix and
+                     Q4Layer (4-bit weights); norm, sorted rows and gradients
   moe_layer_runtime  route_token_real / route_tokens: the server's router API
                      (server/moe_layer_runtime.py:232-408) on the HIP router
 
