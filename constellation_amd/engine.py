@@ -491,6 +491,8 @@ class Context:
         d = w.desc
         if w.device != self.device:
             raise ValueError(f"matrix on cuda:{w.device}, context on cuda:{self.device}")
+        if not w._live:
+            raise ValueError("the matrix has been freed")
         if K != d.cols:
             raise ValueError(f"x has {K} columns, the matrix {d.cols}")
         f8 = x.dtype == torch.float8_e4m3fn
@@ -523,6 +525,8 @@ class Context:
         T = x.shape[0]
         K = topk_ids.shape[1] if topk_ids.dim() == 2 else 0
         self._here(x, topk_ids, topk_w)
+        if not all(m._live for m in (layer.gate_up, layer.down, *(layer.shared or ()))):
+            raise ValueError("a matrix of the layer has been freed")
         if x.shape[1] != layer.hidden:
             raise ValueError(f"x has {x.shape[1]} columns, the layer {layer.hidden}")
         if K and (topk_ids.shape != (T, K) or topk_w.shape != (T, K)):

@@ -602,3 +602,58 @@ def test_q4_layer_skewed_routes(gpu, E, shared):
     finally:
         for m in mats:
             m.free()
+
+
+@pytest.mark.parametrize("dtype", [BF, HF, F8])
+@pytest.mark.parametrize("E,N,K,group,counts", [(1, 70, 1023, 64, (1, 4, 5, 16, 17)), (1, 70, 1025, 64, (4, 5, 16, 17)), (1, 70, 1032, 64, (1, 16, 17, 65)),
+                                                (1, 4200, 256, 32, (1, 3, 16)), (5, 48, 136, 32, (5, 6, 80, 81)), (5, 2048, 2048, 128, (5, 6, 81))])
+def test_q4_matmul_on_both_sides_of_its_rules(gpu, E, N, K, group, counts, dtype):
+    """Each kernel at the sizes where another takes over, eager and from a graph replayed between eager calls."""
+    from constellation_amd.engine import Q4Matrix
+    print(f"[q4] rules {E}x{N}x{K} {dtype}", flush=True)
+    codes, scales = make(E + K, E, N, K, group)
+    w = Q4Matrix.pack(codes.cuda(), scales.cuda(), K, group=group)
+    W = dense(codes, scales, K, group)
+    try:
+        for P in counts:
+            x, xs, x64 = make_x(P, P, K, dtype)
+            off = torch.tensor([0] + sorted(torch.randint(0, P + 1, (E - 1,), generator=torch.Generator().manual_seed(P)).tolist()) + [P], dtype=torch.int32)
+            want = torch.cat([x64[a:b] @ W[e].T for e, (a, b) in enumerate(zip(off[:-1].tolist(), off[1:].tolist()))])
+            size = torch.cat([x64[a:b].abs() @ W[e].abs().T for e, (a, b) in enumerate(zip(off[:-1].tolist(), off[1:].tolist()))])
+            xd, sd, offd = x.cuda(), None if xs is None else xs.cuda(), off.cuda() if E > 1 else None
+
+            def call():
+                return gpu.q4_matmul(w, xd, x_scale=sd, offsets=offd, out_dtype=SF)
+            eager = call()
+            near(eager, want, size * (K + 8) * U + TINY[SF], P)
+            torch.cuda.synchronize()
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph):
+                y = call()
+            for _ in range(3):
+                y.zero_()
+                graph.replay()
+                again = call()
+                torch.cuda.synchronize()
+                assert torch.equal(y, eager) and torch.equal(again, eager), P
+        gpu.sync()
+    finally:
+        w.free()
+
+
+def test_q4_matmul_after_free(gpu):
+    """A freed matrix, and a layer that holds one, are refused."""
+    from constellation_amd.engine import Q4Layer, Q4Matrix
+    H, I, E = 64, 32, 2
+    gu, dn = make(1, E, 2 * I, H, 32), make(2, E, H, I, 32)
+    g = Q4Matrix.pack(gu[0].cuda(), gu[1].cuda(), H, group=32, gated=True)
+    d = Q4Matrix.pack(dn[0].cuda(), dn[1].cuda(), I, group=32)
+    layer = Q4Layer(gpu, g, d)
+    x = rand(1, 3, H, dtype=BF).cuda()
+    g.free()
+    g.free()  # once more does nothing
+    with pytest.raises(ValueError, match="freed"):
+        gpu.q4_matmul(g, x, offsets=torch.tensor([0, 1, 3], dtype=torch.int32, device="cuda"))
+    with pytest.raises(ValueError, match="freed"):
+        gpu.moe(layer, x, torch.zeros(3, 1, dtype=torch.int32, device="cuda"), torch.ones(3, 1, device="cuda"))
+    d.free()
