@@ -294,20 +294,24 @@ inline bool q4_routes_ok(int n_tokens, int top_k, int hidden, int inter, int sha
     return n_tokens == 1 && hidden <= kQ4DecCols && inter <= kQ4SumHeld * 512 && top_k + shared <= 16 &&
            q4_sum_lds(inter, top_k + shared) <= 63 * 1024;
 }
-// The kernel of a product by its items' rows.  One matrix and up to 16 rows: few rows (bf16 4096 x 7168,
-// 1 and 4 rows: 7.2 and 8.2 us, decode kernel 8.1 and 11.5; 16 rows 11.7, GEMM at 17 22.7), whose reads of x
-// need whole pieces of 8 columns: otherwise the decode kernel as far as it goes, then, unless columns are
-// few, the GEMM (4096 x 7161, 4 to 16 rows: 22 us, few rows 26 to 42; 1000 x 1411: 13, 12 to 17).  A stack: the decode
-// kernel while matrices have one row on average (64 of 4096 x 7168, 64 rows: 122 us, GEMM 162; 96 rows
-// 173 and 177), then the GEMM (256 rows: 190 us, few rows 310; 1024: 208 and 357), but few rows up to
-// 16 a matrix while all codes are so few that launches decide (8 of 512 x 1024: 9 to 10 us, GEMM
-// 15 to 17; 16 of 1024 x 2048: 15 to 28 and 19 to 22).
-constexpr int64_t kQ4SmallStack = 8 << 20;  // bytes of codes
+// The kernel of a product by its items' rows (us, bf16).
+// Few rows while items of 16 rows, at most one short one per matrix, take fewer than 2^30 multiply-adds: few
+// launches decide there, and beyond it the reads of x from L2 (one matrix of 4096 x 7168, 32 and 48 rows: 20.1
+// and 28.6, GEMM 24.0 and 27.5; 7168 x 2048, 64 rows: 18.6 and 22.0; 1000 x 2048, 128: 10.1 and 25.2; 16 matrices of
+// 1024 x 2048, 96 and 256 rows: 19 and 28, GEMM 22 and 22; 64 of 1024 x 1024, 96 rows: 22 and 17), half of that
+// for many rows in e4m3, which the GEMM takes as they are (512 x 512, 1024 and 2048 rows: 11.6 and 21.7, GEMM
+// 16.0 and 17.4; in bf16 10.5 and 19.7, 24.8 and 26.7); and for up to
+// 16 rows of one matrix of any size (18432 x 7168, 16 rows: 32.8, GEMM at 17 31.1).  Its reads of x need whole
+// pieces of 8 columns: otherwise it is left to short rows (4096 x 7161, 5 to 16 rows: 26 to 42, GEMM 22).
+// The decode kernel while matrices of a stack have one row on average (64 of 4096 x 7168, 64 rows: 122, GEMM 162;
+// 96 rows 173 and 177) and for rows without whole pieces as far as it goes; the GEMM for the rest.
+constexpr double kQ4FewWork = 1 << 30;
 inline int q4_item_rows(int64_t n_rows, int n_mats, int rows, int cols, bool two_sums) {
     const int dec = q4_dec_rows(cols);
     if (dec > 0 && n_rows <= (n_mats > 1 ? n_mats : cols % 8 != 0 ? dec : 0)) return dec;
-    const bool small = n_mats == 1 || (int64_t)n_mats * rows * cols / 2 <= kQ4SmallStack, pieces = cols % 8 == 0 || cols <= 1024;
-    return small && pieces && n_rows <= (int64_t)kTileTok * n_mats ? kTileTok : two_sums ? kQ4GemmRows / 2 : kQ4GemmRows;
+    const int64_t items = n_mats == 1 ? (n_rows + kTileTok - 1) / kTileTok : std::min<int64_t>(n_mats, n_rows) + n_rows / kTileTok;
+    const bool small = (n_mats == 1 && items <= 1) || (double)items * kTileTok * rows * cols < (two_sums && n_rows > 128 ? kQ4FewWork / 2 : kQ4FewWork);
+    return small && (cols % 8 == 0 || cols <= 1024) ? kTileTok : two_sums ? kQ4GemmRows / 2 : kQ4GemmRows;
 }
 // Of a layer, whose second product reads the first one's fp32 rows: the decode kernel or the GEMM.
 inline int q4_layer_rows(int64_t n_rows, int n_mats, int cols) {

@@ -606,7 +606,7 @@ def test_q4_layer_skewed_routes(gpu, E, shared):
 
 @pytest.mark.parametrize("dtype", [BF, HF, F8])
 @pytest.mark.parametrize("E,N,K,group,counts", [(1, 70, 1023, 64, (1, 4, 5, 16, 17)), (1, 70, 1025, 64, (4, 5, 16, 17)), (1, 70, 1032, 64, (1, 16, 17, 65)),
-                                                (1, 4200, 256, 32, (1, 3, 16)), (5, 48, 136, 32, (5, 6, 80, 81)), (5, 2048, 2048, 128, (5, 6, 81))])
+                                                (1, 4200, 256, 32, (1, 3, 16)), (1, 600, 1024, 64, (129, 1740, 1760)), (5, 48, 136, 32, (5, 6, 80, 81)), (5, 2048, 2048, 128, (5, 6, 81))])
 def test_q4_matmul_on_both_sides_of_its_rules(gpu, E, N, K, group, counts, dtype):
     """Each kernel at the sizes where another takes over, eager and from a graph replayed between eager calls."""
     from constellation_amd.engine import Q4Matrix

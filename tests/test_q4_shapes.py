@@ -75,7 +75,8 @@ def test_staged_rows_fit_the_lds(rules):
             assert rules.item(1, 1, 64, cols, 0) == (rows if cols % 8 else 16) and rules.item(8, 8, 64, cols, 0) == rows
             assert rules.layer(1, 1, cols) == rules.layer(rows, 1, cols) == rules.layer(64, 64, cols) == rows
         assert rules.layer(65, 64, cols) == 128 and rules.item(16, 1, 64, cols, 0) == (16 if cols % 8 == 0 or cols <= 1024 else 128)
-        assert rules.item(10 ** 6, 1, 64, cols, 0) == 128 and rules.item(10 ** 6, 1, 64, cols, 1) == 64
+        assert rules.item(16, 1, 1 << 24, 4096, 0) == 16 and rules.item(17, 1, 1 << 24, 4096, 0) == 128
+        assert rules.item(10 ** 8, 1, 64, cols, 0) == 128 and rules.item(10 ** 8, 1, 64, cols, 1) == 64
     for inter in range(1, 2100, 17):
         for k in (1, 2, 8, 9, 15, 16, 17, 64):
             if rules.routes(1, k, 7168, inter, 0):
@@ -86,7 +87,8 @@ def test_staged_rows_fit_the_lds(rules):
 
 def test_stacks_by_their_size(rules):
     """Few rows per matrix: by launches where the codes are few, and without overflow where they are many."""
-    assert rules.item(64, 8, 512, 1024, 0) == 16 and rules.item(129, 8, 512, 1024, 0) == 128
+    assert rules.item(64, 8, 512, 1024, 0) == 16 and rules.item(2000, 8, 512, 1024, 0) == 128
+    assert rules.item(1024, 1, 512, 512, 1) == 16 and rules.item(2048, 1, 512, 512, 1) == 64 and rules.item(2048, 1, 512, 512, 0) == 16
     assert rules.item(600, 64, 4096, 7168, 0) == 128 and rules.item(600, 64, 4096, 7168, 1) == 64
     assert rules.item(5000, 1024, 1 << 24, 1 << 24, 0) == 128
 
