@@ -80,7 +80,7 @@ __device__ __forceinline__ void q4_gemm_store(const Q4GemmArgs& L, const f32x4 (
         const int r = n * 16 + t, p = begin + r;
         xs[n] = 1.0f;
         if (r < rows && (L.order != nullptr || L.x_row_scale != nullptr)) {
-            const int pair = L.order != nullptr ? L.order[p] : p * L.top_k, xr = pair / L.top_k;
+            const int pair = L.order != nullptr ? L.order[p] : p, xr = L.order != nullptr ? pair / L.top_k : p;  // top_k: of an order only
             if (pair < 0 || xr >= L.n_x)
                 xs[n] = 0.0f;
             else if (L.x_row_scale != nullptr)

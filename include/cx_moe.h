@@ -374,7 +374,7 @@ CX_API int cx_q4_free(int device, cx_q4_desc* w);
  * offsets[e] .. offsets[e + 1] - 1 go through matrix e (cx_sort_tokens' offsets,
  * [n_mats + 1]) and the rows behind the last matrix's are zeros; offsets that
  * decrease or leave the rows are cut and reported by cx_ctx_sync.
- * order NULL: row p of y is row p of x.  Otherwise it is row order[p] / top_k
+ * order NULL: row p of y is row p of x, and top_k is not read.  Otherwise it is row order[p] / top_k
  * (cx_sort_tokens' order: the gather needs no launch of its own); a row whose
  * entry is negative or past n_x reads as zeros.
  * scratch: cx_q4_scratch bytes of device memory, 16-byte aligned, of the caller's
