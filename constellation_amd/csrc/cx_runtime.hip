@@ -1558,6 +1558,7 @@ int cx_q4_matmul(cx_ctx* ctx, const cx_q4_desc* w, const void* x, int x_dtype, c
     int rc = check_q4(w);
     if (rc) return rc;
     if (!act16(x_dtype) && x_dtype != CX_DTYPE_E4M3) return fail(CX_EINVAL, "x must be fp16, bf16 or e4m3");
+    if (x_scale && x_dtype != CX_DTYPE_E4M3) return fail(CX_EINVAL, "x_scale comes with e4m3 x only");
     if (!act_any(y_dtype)) return fail(CX_EINVAL, "y must be fp16, bf16 or fp32");
     if (n_rows < 0 || n_x < 0 || (order && top_k < 1)) return fail(CX_EINVAL, "bad n_rows, n_x or top_k");
     if (!order && n_x != n_rows) return fail(CX_EINVAL, "without an order x and y have the same rows (%d and %d)", n_x, n_rows);

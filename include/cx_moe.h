@@ -365,7 +365,8 @@ CX_API int cx_q4_free(int device, cx_q4_desc* w);
 
 /* y = x W^T (gated: silu(x G^T) * (x U^T)), fp32 accumulation of exact products,
  * rounded once.
- * x: [*, cols] fp16, bf16, or e4m3 with x_scale [*, ceil(cols / 128)].
+ * x: [*, cols] fp16, bf16, or e4m3 with x_scale [*, ceil(cols / 128)] (NULL for the
+ * other types).
  * y: [n_rows, rows] (gated: rows / 2) in fp16, bf16 or fp32.  bf16 rows of x
  * may take part as fp16 times a power of two per row: exact but for values below
  * 2^-31 of the row's largest, which are off by less than 2^-39 of that.  All

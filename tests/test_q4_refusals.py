@@ -1,0 +1,40 @@
+"""Arguments of the 4-bit entry points that are refused before anything touches a
+device.  No GPU: the context is memory that none of these calls reads."""
+from __future__ import annotations
+
+import ctypes as C
+
+import pytest
+
+from constellation_amd._lib import BF16, CX_EINVAL, E4M3, FP16, Q4Desc, lib
+
+
+@pytest.fixture(scope="module")
+def held():
+    """Host memory in the place of device buffers: 16-byte aligned, never read."""
+    raw = C.create_string_buffer(1 << 16)
+    return raw, (C.addressof(raw) + 255) // 256 * 256
+
+
+def desc(at, n_mats=1, rows=64, cols=128, group=128, gated=0):
+    d = Q4Desc()
+    d.codes, d.scales = at, at
+    d.n_mats, d.rows, d.cols, d.group, d.gated = n_mats, rows, cols, group, gated
+    return d
+
+
+def refused(rc, text):
+    assert rc == CX_EINVAL and text.encode() in lib().cx_last_error(), (rc, text, lib().cx_last_error())
+
+
+def matmul(at, d, dt=BF16, xs=None, n_x=4, P=4, offsets=None, size=1 << 16):
+    return lib().cx_q4_matmul(at, C.byref(d), at, dt, xs, n_x, None, 1, offsets, P, at, BF16, at, size, None)
+
+
+@pytest.mark.parametrize("dt", [BF16, FP16])
+@pytest.mark.parametrize("rows", [1, 16, 4000])
+def test_x_scale_without_e4m3(held, dt, rows):
+    """Refused for any number of rows: some kernels would read it as a factor of the row."""
+    _, at = held
+    refused(matmul(at, desc(at), dt=dt, xs=at, n_x=rows, P=rows, size=1 << 40), "x_scale comes with e4m3 x only")
+    refused(matmul(at, desc(at), dt=E4M3, xs=None), "NULL buffer")
