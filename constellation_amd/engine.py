@@ -521,14 +521,18 @@ class Context:
                                  cx_dtype(out_dtype), _ptr(scratch), size, self.stream()))
         return y
 
-    def _q4_moe(self, layer: Q4Layer, x, topk_ids, topk_w, y, yf):
-        T = x.shape[0]
-        K = topk_ids.shape[1] if topk_ids.dim() == 2 else 0
-        self._here(x, topk_ids, topk_w)
+    def _q4_ready(self, layer: Q4Layer, x: torch.Tensor, *others: Optional[torch.Tensor]) -> None:
+        """What a call on a 4-bit layer needs of it and of x, before anything is launched."""
+        self._here(x, *others)
         if not all(m._live for m in (layer.gate_up, layer.down, *(layer.shared or ()))):
             raise ValueError("a matrix of the layer has been freed")
-        if x.shape[1] != layer.hidden:
-            raise ValueError(f"x has {x.shape[1]} columns, the layer {layer.hidden}")
+        if x.dim() != 2 or x.shape[1] != layer.hidden:
+            raise ValueError(f"x has {x.shape[-1] if x.dim() else 0} columns in {x.dim()} dimensions, the layer {layer.hidden} in 2")
+
+    def _q4_moe(self, layer: Q4Layer, x, topk_ids, topk_w, y, yf):
+        self._q4_ready(layer, x, topk_ids, topk_w)
+        T = x.shape[0]
+        K = topk_ids.shape[1] if topk_ids.dim() == 2 else 0
         if K and (topk_ids.shape != (T, K) or topk_w.shape != (T, K)):
             raise ValueError(f"routes must be [{T}, top_k]")
         gu, dn = C.byref(layer.gate_up.desc), C.byref(layer.down.desc)
@@ -584,6 +588,22 @@ class Context:
         x = x.contiguous()
         T = x.shape[0]
         out_dtype = out_dtype or x.dtype
+        if isinstance(layer, Q4Layer):  # its router is a launch of its own, before the layer's
+            E, H = layer.n_experts, layer.hidden
+            self._q4_ready(layer, x, w_router, bias, resident, *(out or ()))
+            w_router, bias = w_router.contiguous(), bias.contiguous()
+            resident = None if resident is None else resident.contiguous()
+            if w_router.shape != (E, H):
+                raise ValueError(f"w_router must be [{E}, {H}], not {list(w_router.shape)}")
+            if bias.shape != (E,) or bias.dtype != torch.float32:
+                raise ValueError(f"bias must be fp32 [{E}]")
+            if resident is not None and (resident.shape != (E,) or resident.element_size() != 1):
+                raise ValueError(f"resident must be uint8 [{E}]")
+            for t, n, dts in zip(out or (), (H, H, top_k, top_k), (
+                    (torch.float16, torch.bfloat16), (torch.float32,), (torch.int32,), (torch.float32,))):
+                if t is not None and (t.shape != (T, n) or t.dtype not in dts or not t.is_contiguous()):
+                    raise ValueError(f"out must be contiguous: y [{T}, {H}] in 16 bits, its fp32 copy or None, "
+                                     f"ids int32 and weights fp32 [{T}, {top_k}]")
         if out is None:
             y = torch.empty((T, layer.hidden), dtype=out_dtype, device=x.device)
             yf = torch.empty((T, layer.hidden), dtype=torch.float32, device=x.device) if want_f32 else None
