@@ -524,6 +524,8 @@ class Context:
     def _q4_ready(self, layer: Q4Layer, x: torch.Tensor, *others: Optional[torch.Tensor]) -> None:
         """What a call on a 4-bit layer needs of it and of x, before anything is launched."""
         self._here(x, *others)
+        if layer.gate_up.device != self.device:
+            raise ValueError(f"layer on cuda:{layer.gate_up.device}, context on cuda:{self.device}")
         if not all(m._live for m in (layer.gate_up, layer.down, *(layer.shared or ()))):
             raise ValueError("a matrix of the layer has been freed")
         if x.dim() != 2 or x.shape[1] != layer.hidden:

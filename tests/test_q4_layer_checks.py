@@ -85,9 +85,15 @@ def test_tensors_elsewhere_launch_nothing(ctx, layer):
         ctx.moe_layer(layer, **router())
 
 
-def test_a_freed_layer_launches_nothing(ctx, layer):
+def test_a_freed_or_foreign_layer_launches_nothing(ctx, layer):
     x, ids, w = torch.zeros(T, H, dtype=torch.bfloat16), torch.zeros(T, K, dtype=torch.int32), torch.ones(T, K)
     layer.down._live = False
     for call in (lambda: ctx.moe_layer(layer, **router()), lambda: ctx.moe(layer, x, ids, w)):
         with pytest.raises(ValueError, match="freed"):
+            call()
+    far = engine.Context.__new__(engine.Context)
+    far.device, far.handle = 1, 1
+    there = engine.Q4Layer(far, matrix(E, 2 * I, H, True, 1), matrix(E, H, I, False, 1))
+    for call in (lambda: ctx.moe_layer(there, **router()), lambda: ctx.moe(there, x, ids, w)):
+        with pytest.raises(ValueError, match="layer on cuda:1"):
             call()
