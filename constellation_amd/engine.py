@@ -533,9 +533,8 @@ class Context:
 
     def _q4_moe(self, layer: Q4Layer, x, topk_ids, topk_w, y, yf):
         self._q4_ready(layer, x, topk_ids, topk_w)
-        T = x.shape[0]
-        K = topk_ids.shape[1] if topk_ids.dim() == 2 else 0
-        if K and (topk_ids.shape != (T, K) or topk_w.shape != (T, K)):
+        T, K = x.shape[0], topk_ids.shape[1] if topk_ids.dim() == 2 else -1
+        if topk_ids.shape != (T, K) or topk_w.shape != (T, K):
             raise ValueError(f"routes must be [{T}, top_k]")
         gu, dn = C.byref(layer.gate_up.desc), C.byref(layer.down.desc)
         sg, sd = (C.byref(m.desc) for m in layer.shared) if layer.shared else (None, None)

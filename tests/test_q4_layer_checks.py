@@ -97,3 +97,14 @@ def test_a_freed_or_foreign_layer_launches_nothing(ctx, layer):
     for call in (lambda: ctx.moe_layer(there, **router()), lambda: ctx.moe(there, x, ids, w)):
         with pytest.raises(ValueError, match="layer on cuda:1"):
             call()
+
+
+@pytest.mark.parametrize("ids,w", [(torch.zeros(K, dtype=torch.int32), torch.ones(K)), (torch.zeros(T, K, dtype=torch.int32), torch.ones(T, K + 1)),
+                                   (torch.zeros(T - 1, K, dtype=torch.int32), torch.ones(T - 1, K)), (torch.zeros(T, K, dtype=torch.int32), torch.ones(T)),
+                                   (torch.zeros(T, 0, dtype=torch.int32), torch.ones(T, K))])
+def test_routes_of_another_shape_launch_nothing(ctx, ids, w):
+    """A shared expert beside them does not make them a call without routes."""
+    shared = (matrix(1, 2 * I, H, True), matrix(1, H, I, False))
+    layer = engine.Q4Layer(ctx, matrix(E, 2 * I, H, True), matrix(E, H, I, False), shared)
+    with pytest.raises(ValueError, match="routes must be"):
+        ctx.moe(layer, torch.zeros(T, H, dtype=torch.bfloat16), ids, w)
