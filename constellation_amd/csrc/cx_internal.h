@@ -443,6 +443,7 @@ hipError_t launch_q4_pack(const cx_q4_desc& w, const uint8_t* codes, const uint1
 hipError_t launch_q4_items(const int32_t* offsets, int n_mats, int n_rows, int item_rows, Q4Item* items, int* err_flag,
                            hipStream_t s);
 size_t q4_part_bytes(const cx_q4_desc& w, int64_t n_rows, int n_mats, int item_rows);  // the GEMM's partial sums
+size_t q4_most_part_bytes(const cx_q4_desc& w, int64_t n_rows, int n_mats, int item_rows);  // of any call of up to n_rows rows
 size_t q4_x_scratch(const cx_q4_desc& w, int n_x);  // of products with items of more than 16 rows
 // Given routes, one item per pair: what a layer over a few tokens has instead of a plan.
 struct Q4Routes {

@@ -14,6 +14,11 @@ size_t q4_part_bytes(const cx_q4_desc& w, int64_t n_rows, int n_mats, int item_r
     return s > 1 ? (size_t)s * n_rows * q4_row_tiles(w) * 64 : 0;
 }
 
+size_t q4_most_part_bytes(const cx_q4_desc& w, int64_t n_rows, int n_mats, int item_rows) {
+    if (item_rows <= kTileTok) return 0;
+    return (size_t)q4_gemm_part_rows(q4_row_tiles(w), q4_col_tiles(w), n_rows, n_mats, item_rows) * q4_row_tiles(w) * 64;
+}
+
 hipError_t launch_q4_gemm(const Q4Launch& L, hipStream_t s) {
     Q4GemmArgs a{};
     a.w = L.w;

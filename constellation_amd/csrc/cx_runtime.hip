@@ -825,6 +825,13 @@ Q4Scratch q4_scratch(const cx_q4_desc& w, int x_dtype, int n_x, int n_rows, bool
     return z;
 }
 
+// What covers every call of up to n_x and n_rows rows (the kernels of more rows need no less of x and its scale).
+size_t q4_scratch_most(const cx_q4_desc& w, int x_dtype, int n_x, int n_rows, bool with_offsets) {
+    const Q4Scratch z = q4_scratch(w, x_dtype, n_x, n_rows, with_offsets);
+    return (with_offsets ? align_up(sizeof(Q4Item) * (size_t)q4_most_items(n_rows, w.n_mats, q4_dec_rows(w.cols))) : 0) + (z.part - z.x) +
+           q4_most_part_bytes(w, n_rows, w.n_mats, z.item_rows);
+}
+
 // Scratch of cx_q4_moe.
 struct Q4MoeScratch {
     int64_t pairs, max_items;
@@ -832,22 +839,26 @@ struct Q4MoeScratch {
     size_t items, order, place, x, h, hx, ys, part, bytes;
 };
 
-Q4MoeScratch q4_moe_scratch(const cx_q4_desc& gu, const cx_q4_desc& down, int shared, int n_tokens, int top_k) {
+// most: what covers every call of up to n_tokens tokens.
+Q4MoeScratch q4_moe_scratch(const cx_q4_desc& gu, const cx_q4_desc& down, int shared, int n_tokens, int top_k, bool most) {
     Q4MoeScratch z{};
     z.pairs = (int64_t)n_tokens * (top_k + shared);
     // both products take the same items; in between h is fp32, which the decode kernel and the GEMM read
     z.item_rows = q4_layer_rows(z.pairs, gu.n_mats + shared, std::max(gu.cols, down.cols));
     z.max_items = q4_max_items(z.pairs, gu.n_mats + shared, z.item_rows);
     const bool gemm = z.item_rows > kTileTok;
+    const int64_t listed = most ? q4_most_items(z.pairs, gu.n_mats + shared, q4_dec_rows(std::max(gu.cols, down.cols))) : z.max_items;
     z.items = 0;
-    z.order = z.items + align_up(sizeof(Q4Item) * (size_t)z.max_items);
+    z.order = z.items + align_up(sizeof(Q4Item) * (size_t)listed);
     z.place = z.order + align_up(4 * (size_t)z.pairs);
     z.x = z.place + align_up(4 * (size_t)z.pairs);
     z.h = z.x + (gemm ? q4_x_scratch(gu, n_tokens) : 0);
     z.hx = z.h + align_up(4 * (size_t)z.pairs * down.cols);
     z.ys = z.hx + (gemm ? q4_x_scratch(down, (int)z.pairs) : 0);
     z.part = z.ys + align_up(4 * (size_t)z.pairs * down.rows);
-    auto parts = [&](const cx_q4_desc& w) { return q4_part_bytes(w, z.pairs, w.n_mats + shared, z.item_rows); };
+    auto parts = [&](const cx_q4_desc& w) {
+        return most ? q4_most_part_bytes(w, z.pairs, w.n_mats + shared, z.item_rows) : q4_part_bytes(w, z.pairs, w.n_mats + shared, z.item_rows);
+    };
     z.bytes = z.part + std::max(parts(gu), parts(down));
     return z;
 }
@@ -1547,7 +1558,7 @@ int cx_q4_free(int device, cx_q4_desc* w) {
 
 size_t cx_q4_scratch(const cx_q4_desc* w, int x_dtype, int n_x, int n_rows, int with_offsets) {
     if (!w || w->n_mats < 1 || n_x < 0 || n_rows < 0) return 0;
-    return q4_scratch(*w, x_dtype, n_x, n_rows, with_offsets != 0).bytes;
+    return q4_scratch_most(*w, x_dtype, n_x, n_rows, with_offsets != 0);
 }
 
 int cx_q4_matmul(cx_ctx* ctx, const cx_q4_desc* w, const void* x, int x_dtype, const float* x_scale, int n_x,
@@ -1600,7 +1611,7 @@ int cx_q4_matmul(cx_ctx* ctx, const cx_q4_desc* w, const void* x, int x_dtype, c
 
 size_t cx_q4_moe_scratch(const cx_q4_desc* gate_up, const cx_q4_desc* down, int has_shared, int n_tokens, int top_k) {
     if (!gate_up || !down || gate_up->n_mats < 1 || n_tokens < 0 || top_k < 0) return 0;
-    return q4_moe_scratch(*gate_up, *down, has_shared != 0, n_tokens, top_k).bytes;
+    return q4_moe_scratch(*gate_up, *down, has_shared != 0, n_tokens, top_k, true).bytes;
 }
 
 int cx_q4_moe(cx_ctx* ctx, const cx_q4_desc* gate_up, const cx_q4_desc* down, const cx_q4_desc* shared_gate_up,
@@ -1629,7 +1640,7 @@ int cx_q4_moe(cx_ctx* ctx, const cx_q4_desc* gate_up, const cx_q4_desc* down, co
     if ((int64_t)n_tokens * (top_k + shared) > kMaxPairs) return fail(CX_EINVAL, "too many pairs: n_tokens * top_k must be at most 2^30");
     if (n_tokens == 0) return CX_OK;
     if (!x || !y || (top_k > 0 && (!topk_ids || !topk_w))) return fail(CX_EINVAL, "NULL buffer");
-    const Q4MoeScratch z = q4_moe_scratch(*gate_up, *down, shared, n_tokens, top_k);
+    const Q4MoeScratch z = q4_moe_scratch(*gate_up, *down, shared, n_tokens, top_k, false);
     if (!scratch || scratch_bytes < z.bytes || reinterpret_cast<uintptr_t>(scratch) % 16)
         return fail(CX_EINVAL, "scratch must be %zu bytes, 16-byte aligned", z.bytes);
     if ((rc = set_device(ctx->device))) return rc;

@@ -325,9 +325,12 @@ inline int q4_layer_rows(int64_t n_rows, int n_mats, int cols) {
 // (measured: 0.94, 1.2 and 1.96 with 2, 4 and 8), 1 + nt / 10 times that beside a second one; the
 // partial sums are written and read at 4.5 MB a us, and the launch is 3.
 constexpr int kQ4GemmBlock = 16;  // row tiles of a workgroup
+inline int64_t q4_gemm_items(int64_t n_rows, int n_mats, int item_rows) {
+    return std::max<int64_t>(n_mats > 1 ? std::min<int64_t>(n_mats, n_rows) : 1, (n_rows + item_rows - 1) / item_rows);
+}
 inline int q4_gemm_splits(int row_tiles, int col_tiles, int64_t n_rows, int n_mats, int item_rows) {
     if (n_rows <= 0) return 1;
-    const int64_t items = std::max<int64_t>(n_mats > 1 ? std::min<int64_t>(n_mats, n_rows) : 1, (n_rows + item_rows - 1) / item_rows);
+    const int64_t items = q4_gemm_items(n_rows, n_mats, item_rows);
     const double nt = std::min<double>(item_rows / 16, std::max(2.0, (double)((n_rows + 16 * items - 1) / (16 * items))));
     const int64_t wgs = items * ((row_tiles + kQ4GemmBlock - 1) / kQ4GemmBlock);
     int best = 1;
@@ -341,6 +344,24 @@ inline int q4_gemm_splits(int row_tiles, int col_tiles, int64_t n_rows, int n_ma
     return best;
 }
 
+// The most rows of partial sums (ranges times rows) that a call of up to n_rows rows has: with more rows
+// come fewer ranges, so that a smaller call may need more.  The estimate's items and nt stay the same over an interval
+// of rows; within it only the partial sums' own cost grows with the rows, in proportion to the ranges, so
+// that the ranges are the most at its first row.  Items beyond one per matrix are at least half full, 32 rows, whose
+// partial sums cost 0.0018 us a row tile and more; what ranges can save is less than a round of workgroups, 3.6 us a
+// column tile, so that there are none from 2000 row tiles of items per column tile on.
+inline int64_t q4_gemm_part_rows(int row_tiles, int col_tiles, int64_t n_rows, int n_mats, int item_rows) {
+    int64_t most = 0;
+    for (int64_t n = 1, end; n <= n_rows; n = end + 1) {
+        const int64_t items = q4_gemm_items(n, n_mats, item_rows), nt = std::max<int64_t>(2, (n + 16 * items - 1) / (16 * items));
+        if (items > n_mats && items * row_tiles >= 2000 * (int64_t)col_tiles) break;
+        end = n < n_mats ? n : std::min({n_rows, items * item_rows, items * 16 * nt});
+        const int s = q4_gemm_splits(row_tiles, col_tiles, n, n_mats, item_rows);
+        if (s > 1) most = std::max(most, s * end);
+    }
+    return most;
+}
+
 // Rows of each of the n items that `rows` rows are cut to (the last has what is left): equal
 // ones of whole 16-row tiles, so that the last is not a short one.  n is the least that holds
 // them, so no item is empty: (n - 1) shares are at most (n - 1) * item_rows, fewer than the rows.
@@ -352,6 +373,11 @@ constexpr int q4_item_share(int n, int rows) {
 // most one short item per matrix that has rows, and one of rows without a matrix.
 inline int64_t q4_max_items(int64_t n_rows, int n_mats, int item_rows) {
     return 2 + (n_rows < n_mats ? n_rows : n_mats) + n_rows / item_rows;
+}
+// The same for every call of up to n_rows rows, whatever kernel it takes: none has shorter items than the
+// decode kernel (16 rows where that does not go).
+inline int64_t q4_most_items(int64_t n_rows, int n_mats, int dec_rows) {
+    return q4_max_items(n_rows, n_mats, dec_rows > 0 ? dec_rows : kTileTok);
 }
 
 }  // namespace cx

@@ -293,6 +293,7 @@ class Q4Layer:
         self.gate_up, self.down, self.shared = gate_up, down, shared
         self.n_experts, self.hidden, self.inter = g.n_mats, d.rows, d.cols
         self.experts = [self] * self.n_experts  # every expert of the stack is resident
+        self._scratch: dict = {}  # sizes by tokens and top_k
 
 
 class Context:
@@ -538,7 +539,9 @@ class Context:
             raise ValueError(f"routes must be [{T}, top_k]")
         gu, dn = C.byref(layer.gate_up.desc), C.byref(layer.down.desc)
         sg, sd = (C.byref(m.desc) for m in layer.shared) if layer.shared else (None, None)
-        size = lib().cx_q4_moe_scratch(gu, dn, int(layer.shared is not None), T, K)
+        size = layer._scratch.get((T, K))
+        if size is None:
+            size = layer._scratch[T, K] = lib().cx_q4_moe_scratch(gu, dn, int(layer.shared is not None), T, K)
         scratch = torch.empty(size, dtype=torch.uint8, device=x.device)
         check(lib().cx_q4_moe(self.handle, gu, dn, sg, sd, x.data_ptr(), cx_dtype(x.dtype), T,
                               topk_ids.data_ptr(), topk_w.data_ptr(), K, y.data_ptr(), cx_dtype(y.dtype),

@@ -379,7 +379,8 @@ CX_API int cx_q4_free(int device, cx_q4_desc* w);
  * (cx_sort_tokens' order: the gather needs no launch of its own); a row whose
  * entry is negative or past n_x reads as zeros.
  * scratch: cx_q4_scratch bytes of device memory, 16-byte aligned, of the caller's
- * (NULL where that is 0), in use until the call's work is done. */
+ * (NULL where that is 0), in use until the call's work is done.  What it asks for
+ * covers every call with as many rows or fewer on the same matrix and type of x. */
 CX_API size_t cx_q4_scratch(const cx_q4_desc* w, int x_dtype, int n_x, int n_rows, int with_offsets);
 CX_API int cx_q4_matmul(cx_ctx* ctx, const cx_q4_desc* w, const void* x, int x_dtype, const float* x_scale,
                  int n_x, const int32_t* order, int top_k, const int32_t* offsets, int n_rows,
@@ -395,8 +396,9 @@ CX_API int cx_q4_matmul(cx_ctx* ctx, const cx_q4_desc* w, const void* x, int x_d
  * takes part in the down product as fp16 times a power of two per row (11 bits).
  * n_tokens may be 0; a call whose padded rows of x or h would pass 4 GB in fp16
  * (about 299,000 tokens of 7168, or a million pairs of 2048) is refused.
- * scratch: cx_q4_moe_scratch bytes of the caller's, as above; a captured graph
- * keeps using the scratch it was captured with. */
+ * scratch: cx_q4_moe_scratch bytes of the caller's, as above (enough for every call
+ * with as many tokens or fewer); a captured graph keeps using the scratch it was
+ * captured with. */
 CX_API size_t cx_q4_moe_scratch(const cx_q4_desc* gate_up, const cx_q4_desc* down, int has_shared,
                          int n_tokens, int top_k);
 CX_API int cx_q4_moe(cx_ctx* ctx, const cx_q4_desc* gate_up, const cx_q4_desc* down,
