@@ -49,8 +49,12 @@ def _check_pairs(rows: int, n_tokens: int, top_k: int, weights: Optional[torch.T
         raise ValueError(f"weights must be fp32 [{n_tokens}, {top_k}]")
 
 
-# the current stream's handle without a Stream object around it: a microsecond less a call
-_stream = torch._C._cuda_getCurrentRawStream
+def _stream(device: int) -> int:
+    """The current stream's handle; without a Stream object around it, where torch has
+    that (a microsecond less a call).  Looked up by the call: the module also serves programs
+    whose torch has no GPU build."""
+    raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+    return torch.cuda.current_stream(device).cuda_stream if raw is None else raw(device)
 
 
 def device_count() -> int:
