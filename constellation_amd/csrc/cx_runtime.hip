@@ -800,7 +800,8 @@ int check_rows(cx_ctx* ctx, int n_tokens, int top_k, int64_t width) {
 
 int check_q4(const cx_q4_desc* w) {
     if (!w || !w->codes || !w->scales) return fail(CX_EINVAL, "4-bit descriptor is NULL or empty");
-    if (w->n_mats <= 0 || w->rows <= 0 || w->cols <= 0 || (w->group != 32 && w->group != 64 && w->group != 128) ||
+    // the limits of cx_q4_pack: the plan of a stack's rows has a place in LDS for each of its matrices
+    if (w->n_mats <= 0 || w->rows <= 0 || w->cols <= 0 || w->n_mats > kSortMaxExperts || w->rows > kQ4MaxSide || w->cols > kQ4MaxSide || (w->group != 32 && w->group != 64 && w->group != 128) ||
         (w->gated && w->rows % 2 != 0))
         return fail(CX_EINVAL, "bad 4-bit descriptor");
     return CX_OK;
@@ -1514,7 +1515,7 @@ int cx_q4_pack(int device, const uint8_t* codes, const uint16_t* scales, int n_m
     if (!out) return fail(CX_EINVAL, "NULL out");
     std::memset(out, 0, sizeof(*out));
     if (!codes || !scales) return fail(CX_EINVAL, "NULL buffer");
-    if (n_mats < 1 || n_mats > kSortMaxExperts || rows < 1 || cols < 1 || rows > (1 << 24) || cols > (1 << 24))
+    if (n_mats < 1 || n_mats > kSortMaxExperts || rows < 1 || cols < 1 || rows > kQ4MaxSide || cols > kQ4MaxSide)
         return fail(CX_EINVAL, "bad 4-bit shape (n_mats must be 1..%d, rows and cols 1..2^24)", kSortMaxExperts);
     if (group != 32 && group != 64 && group != 128) return fail(CX_EINVAL, "group must be 32, 64 or 128");
     if (gated && rows % 2 != 0) return fail(CX_EINVAL, "a gated matrix has an even number of rows");

@@ -265,6 +265,7 @@ inline size_t plan_buffer_bytes(int n_tokens, int top_k, int n_experts, int has_
 // ---------------------------------------------------------------------------
 // Rows around the experts and 4-bit products.
 constexpr int kSortMaxExperts = 1024;  // the counts of a workgroup's waves fit its LDS
+constexpr int kQ4MaxSide = 1 << 24;    // rows and columns of a 4-bit matrix
 constexpr int kNormMaxHidden = 65536;  // a row in the registers of 1024 threads, 64 values each
 
 constexpr int kRowThreads = 256;       // workgroup of the gather and combine kernels

@@ -38,3 +38,20 @@ def test_x_scale_without_e4m3(held, dt, rows):
     _, at = held
     refused(matmul(at, desc(at), dt=dt, xs=at, n_x=rows, P=rows, size=1 << 40), "x_scale comes with e4m3 x only")
     refused(matmul(at, desc(at), dt=E4M3, xs=None), "NULL buffer")
+
+
+@pytest.mark.parametrize("field,value", [("n_mats", 1025), ("n_mats", 0), ("n_mats", 1 << 20), ("rows", (1 << 24) + 16), ("cols", (1 << 24) + 128),
+                                         ("rows", 0), ("cols", -1), ("group", 48)])
+def test_descriptors_past_what_is_packed(held, field, value):
+    """A descriptor that cx_q4_pack would not have made: a stack of more than 1024 matrices has no plan."""
+    _, at = held
+    d = desc(at, 4)
+    setattr(d, field, value)
+    refused(matmul(at, d, offsets=at, size=1 << 40), "bad 4-bit descriptor")
+    gu, dn = desc(at, 4, 128, 128, gated=1), desc(at, 4, 128, 64)
+    for w in (gu, dn):
+        keep = getattr(w, field)
+        setattr(w, field, value)
+        refused(lib().cx_q4_moe(at, C.byref(gu), C.byref(dn), None, None, at, BF16, 4, at, at, 2, at, BF16, None, at, 1 << 40, None),
+                "bad 4-bit descriptor")
+        setattr(w, field, keep)
