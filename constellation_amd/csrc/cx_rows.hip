@@ -455,7 +455,7 @@ int gather_width(const GatherArgs& g) {
 
 template <class V>
 hipError_t gather_as(const GatherArgs& g, hipStream_t s) {
-    const int pieces = (int)(g.row_bytes / sizeof(V)), chunks = (pieces + kRowThreads - 1) / kRowThreads;
+    const int pieces = (int)(g.row_bytes / sizeof(V)), chunks = (int)(((int64_t)pieces + kRowThreads - 1) / kRowThreads);
     cx_launch(k_gather_rows<V>, dim3((unsigned)(g.n_tokens * chunks)), dim3(kRowThreads), 0, s, static_cast<const V*>(g.x),
               static_cast<V*>(g.xs), g.place, g.top_k, g.n_tokens * g.top_k, pieces, chunks, g.err_flag);
     return hipGetLastError();

@@ -794,6 +794,7 @@ int check_rows(cx_ctx* ctx, int n_tokens, int top_k, int64_t width) {
     if (!ctx) return fail(CX_EINVAL, "NULL context");
     if (n_tokens < 0 || top_k < 1 || top_k > 64) return fail(CX_EINVAL, "bad n_tokens/top_k");
     if (width <= 0) return fail(CX_EINVAL, "rows must not be empty");
+    if (width > kMaxRowWidth) return fail(CX_EINVAL, "rows must have at most %d columns", kMaxRowWidth);
     if ((int64_t)n_tokens * top_k > kMaxPairs) return fail(CX_EINVAL, "too many pairs: n_tokens * top_k must be at most 2^30");
     return set_device(ctx->device);
 }
@@ -1452,7 +1453,8 @@ int cx_sort_tokens(cx_ctx* ctx, const int32_t* ids, int n_tokens, int top_k, int
 int cx_gather_rows(cx_ctx* ctx, const void* x, size_t row_bytes, const int32_t* place, int n_tokens, int top_k,
                    void* xs, void* stream) {
     DeviceRestore keep;
-    int rc = check_rows(ctx, n_tokens, top_k, row_bytes > 0 && row_bytes <= INT32_MAX ? (int64_t)row_bytes : 0);
+    if (ctx && row_bytes > INT32_MAX) return fail(CX_EINVAL, "rows must have fewer than 2^31 bytes");
+    int rc = check_rows(ctx, n_tokens, top_k, row_bytes > 0);
     if (rc) return rc;
     if (n_tokens == 0) return CX_OK;
     if (!x || !place || !xs) return fail(CX_EINVAL, "NULL buffer");

@@ -270,6 +270,9 @@ constexpr int kNormMaxHidden = 65536;  // a row in the registers of 1024 threads
 
 constexpr int kRowThreads = 256;       // workgroup of the gather and combine kernels
 
+// Columns of a row that is summed: those that the last threads look at, past its end, still fit an int.
+constexpr int kMaxRowWidth = INT32_MAX - 8 * kRowThreads;
+
 // A launch's threads are counted in 32 bits.
 inline bool rows_grid_ok(int64_t workgroups, int threads) { return workgroups * threads < ((int64_t)1 << 32); }
 

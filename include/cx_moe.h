@@ -286,8 +286,9 @@ CX_API int cx_moe_layer(cx_ctx* ctx, const cx_layer* layer,
  * these calls allocates, copies or waits, so all of them can be captured into a
  * graph; they use no scratch, so calls on different streams may overlap.  Rows
  * are contiguous and may start at any address of their type's alignment; rows
- * and widths whose bytes are multiples of 16 take the wide accesses.  A call of
- * no tokens does nothing. */
+ * and widths whose bytes are multiples of 16 take the wide accesses.  A row has
+ * fewer than 2^31 bytes where it is gathered and at most 2^31 - 2049 columns where it
+ * is summed.  A call of no tokens does nothing. */
 
 /* s = x + residual, rounded to x's type (the residual stream); then the RMS norm
  * of s as it was rounded:

@@ -55,3 +55,13 @@ def test_descriptors_past_what_is_packed(held, field, value):
         refused(lib().cx_q4_moe(at, C.byref(gu), C.byref(dn), None, None, at, BF16, 4, at, at, 2, at, BF16, None, at, 1 << 40, None),
                 "bad 4-bit descriptor")
         setattr(w, field, keep)
+
+
+@pytest.mark.parametrize("hidden", [2 ** 31 - 1, 2 ** 31 - 2048])
+def test_rows_whose_columns_do_not_fit_an_int(held, hidden):
+    """A thread looks at up to 2048 columns from its first one on."""
+    _, at = held
+    L = lib()
+    refused(L.cx_combine_rows(at, at, BF16, at, None, None, 1, 1, hidden, at, BF16, None, None), "at most 2147481599 columns")
+    refused(L.cx_combine_rows_grad(at, at, BF16, at, BF16, at, None, 1, 1, hidden, at, None, None), "at most 2147481599 columns")
+    refused(L.cx_gather_rows(at, at, hidden + 2048, at, 1, 1, at, None), "fewer than 2^31 bytes")
