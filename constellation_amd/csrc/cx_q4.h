@@ -212,7 +212,7 @@ __global__ __launch_bounds__(64 * kQ4FewWaves, 2) void k_q4_few(Q4Launch L, int 
         v *= q4_row_scales(w)[(mat * RT + min(rt, RT - 1)) * 16 + r];
         if (L.w.gated) {
             const float up = __shfl_down(v, 8);
-            v = v / (1.0f + __expf(-v)) * up;
+            v = v / (1.0f + expf(-v)) * up;
         }
         const int n = L.w.gated ? rt * 8 + r : rt * 16 + r;
         if (tt < np && rt < RT && n < width && (!L.w.gated || r < 8)) q4_store(L, (size_t)(begin + tt) * width + n, v);

@@ -233,7 +233,7 @@ __global__ __launch_bounds__(64 * kQ4DecWaves) void k_q4_dec(Q4DecArgs A) {
         v *= q4_row_scales(w)[(mat * RT + min(o, RT - 1)) * 16 + r] * row_up[min(tt, A.lds_rows - 1)];
         if (L.w.gated) {
             const float other_half = __shfl_down(v, 8);
-            v = v / (1.0f + __expf(-v)) * other_half;
+            v = v / (1.0f + expf(-v)) * other_half;
         }
         const int n = L.w.gated ? o * 8 + r : o * 16 + r;
         if (tt < np && o < RT && n < width && (!L.w.gated || r < 8)) q4_store(L, (size_t)(begin + tt) * width + n, v);

@@ -99,7 +99,7 @@ __device__ __forceinline__ void q4_gemm_store(const Q4GemmArgs& L, const f32x4 (
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     const float up = __shfl_xor(v[i], 32);
-                    v[i] = v[i] / (1.0f + __expf(-v[i])) * up;
+                    v[i] = v[i] / (1.0f + expf(-v[i])) * up;
                 }
                 c = m * 8 + 4 * (q & 1);
             }
@@ -326,7 +326,7 @@ __global__ __launch_bounds__(256) void k_q4_sum(const float* part, int splits, i
     }
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-        const float v = gated ? a[i] / (1.0f + __expf(-a[i])) * b[i] : a[i];
+        const float v = gated ? a[i] / (1.0f + expf(-a[i])) * b[i] : a[i];
         if (n + i >= width) continue;
         if (y_type == CX_DTYPE_F32)
             static_cast<float*>(y)[p * width + n + i] = v;
