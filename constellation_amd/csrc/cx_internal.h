@@ -434,7 +434,7 @@ struct Q4Launch {
     int64_t max_items;       // of the list, its head included
     void* y;                 // [n_rows, rows] ([n_rows, rows / 2] gated)
     int y_type;              // CX_DTYPE_*
-    void* x_scratch;         // q4_x_scratch bytes
+    void* x_scratch;         // q4_x_scratch bytes (of 2 planes for kQ4F32)
     float* part;             // q4_part_bytes
 };
 size_t q4_code_bytes(const cx_q4_desc& w);
@@ -444,7 +444,7 @@ hipError_t launch_q4_items(const int32_t* offsets, int n_mats, int n_rows, int i
                            hipStream_t s);
 size_t q4_part_bytes(const cx_q4_desc& w, int64_t n_rows, int n_mats, int item_rows);  // the GEMM's partial sums
 size_t q4_most_part_bytes(const cx_q4_desc& w, int64_t n_rows, int n_mats, int item_rows);  // of any call of up to n_rows rows
-size_t q4_x_scratch(const cx_q4_desc& w, int n_x);  // of products with items of more than 16 rows
+size_t q4_x_scratch(const cx_q4_desc& w, int n_x, int planes);  // of products with items of more than 16 rows; planes: 2 of fp32 x
 // Given routes, one item per pair: what a layer over a few tokens has instead of a plan.
 struct Q4Routes {
     const int32_t* ids;    // [n_tokens, top_k]; nullable: no routes, L.items or one matrix

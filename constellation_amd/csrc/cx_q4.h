@@ -39,6 +39,18 @@ __device__ __forceinline__ f16x8 q4_f16(uint32_t w) {
     return f16x8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
 }
 
+// Two fp32 values as two fp16 planes: in x each rounded to 11 bits, in y what that leaves of it,
+// rounded to 11 bits again: together within 2^-23 of the value, or 2^-25 where the rest
+// is below fp16's normal numbers.  Of an infinity or a NaN nothing is left.
+__device__ __forceinline__ uint2 q4_planes(float a, float b) {
+    const uint32_t ha = f16_rne(a), hb = f16_rne(b);
+    auto rest = [](float v, uint32_t h) {
+        const float r = v - static_cast<float>(__builtin_bit_cast(_Float16, static_cast<uint16_t>(h)));
+        return f16_rne(__builtin_fabsf(v) < __builtin_inff() ? r : 0.0f);
+    };
+    return uint2{ha | (hb << 16), rest(a, ha) | (rest(b, hb) << 16)};
+}
+
 // x's columns col .. col + 7 of one row as MFMA operand bits, element by element; columns past
 // the row's end are zeros (the codes there are, too, but a NaN times zero is not).
 template <int XT>

@@ -72,11 +72,12 @@ __global__ __launch_bounds__(256) void k_q4_row_scales(cx_q4_desc w, const uint1
 // Rows of x as fp16 times a power of two per row, in rows of whole 128-column tiles,
 // zeros behind the row.  The row's largest value comes to 2^14 .. 2^15, so bf16
 // values (8 significant bits) are exact down to 2^-31 of it and the others off by less than
-// 2^-39 of it: nothing next to the sums' own 2^-24.  fp32 values are rounded to 11 bits.
+// 2^-39 of it: nothing next to the sums' own 2^-24.  fp32 values come in two planes (q4_planes), 64 columns
+// of the first, then the same of the second.
 //
 // A row is read once, kRowPieces pieces of 8 values a thread in registers (wider rows are read
 // again for what lies behind), 16 bytes at a time where it starts on them.  1024 bf16 rows of 7168 take 9
-// us, 8192 fp32 rows of 2048 22 (100 MB, 4.6 TB/s), 3001 e4m3 rows of 2048 7.
+// us, 8192 fp32 rows of 2048 26 (134 MB, 5.1 TB/s), 3001 e4m3 rows of 2048 7.
 constexpr int kRowPieces = 4;
 
 template <int DT>
@@ -132,7 +133,7 @@ template <int DT>
 __global__ __launch_bounds__(256) void k_q4_rows(const void* x, int cols, int padded, uint16_t* dst, float* scale) {
     __shared__ uint32_t part[4];
     const int tid = threadIdx.x;
-    const size_t row = (size_t)blockIdx.x * cols, out = (size_t)blockIdx.x * padded;
+    const size_t row = (size_t)blockIdx.x * cols, out = (size_t)blockIdx.x * padded * (DT == CX_DTYPE_F32 ? 2 : 1);
     constexpr int kEl = DT == CX_DTYPE_F32 ? 4 : DT == CX_DTYPE_E4M3 ? 1 : 2, kSpan = kRowPieces * 256 * 8;
     const bool vec = cols % 8 == 0 && (reinterpret_cast<uintptr_t>(x) & (kEl == 1 ? 7 : 15)) == 0;
     float v[kRowPieces][8];
@@ -168,9 +169,21 @@ __global__ __launch_bounds__(256) void k_q4_rows(const void* x, int cols, int pa
     }
     auto put = [&](int c, const float (&f)[8]) {
         u32x4 o;
+        if constexpr (DT == CX_DTYPE_F32) {
+            u32x4 lo;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) o[i] = f16_rne(f[2 * i] * up) | (f16_rne(f[2 * i + 1] * up) << 16);
-        *reinterpret_cast<u32x4*>(dst + out + c) = o;
+            for (int i = 0; i < 4; ++i) {
+                const uint2 p = q4_planes(f[2 * i] * up, f[2 * i + 1] * up);
+                o[i] = p.x, lo[i] = p.y;
+            }
+            uint16_t* to = dst + out + c / 64 * 128 + c % 64;
+            *reinterpret_cast<u32x4*>(to) = o;
+            *reinterpret_cast<u32x4*>(to + 64) = lo;
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) o[i] = f16_rne(f[2 * i] * up) | (f16_rne(f[2 * i + 1] * up) << 16);
+            *reinterpret_cast<u32x4*>(dst + out + c) = o;
+        }
     };
 #pragma unroll
     for (int i = 0; i < kRowPieces; ++i)
@@ -276,10 +289,11 @@ bool q4_grid_ok(const Q4Launch& L) {
     const int RT = q4_row_tiles(L.w);
     if (!rows_grid_ok(item_bound(L) * (RT + 16), 1024)) return false;
     return L.item_rows <= kTileTok || (rows_grid_ok(L.n_x, 256) && rows_grid_ok((int64_t)L.n_rows * RT * 4 / 256 + 1, 256) &&
-                                       (int64_t)L.n_x * q4_col_tiles(L.w) * 256 < ((int64_t)1 << 32));  // the GEMM's places in x, in bytes
+                                       // the GEMM's places in x, in bytes; of two planes within an item
+                                       (L.x_type == kQ4F32 ? (int64_t)L.item_rows * 2 : (int64_t)L.n_x) * q4_col_tiles(L.w) * 256 < ((int64_t)1 << 32));
 }
 
-size_t q4_x_scratch(const cx_q4_desc& w, int n_x) { return up256((size_t)n_x * q4_col_tiles(w) * 256) + up256((size_t)n_x * 4); }
+size_t q4_x_scratch(const cx_q4_desc& w, int n_x, int planes) { return up256((size_t)n_x * q4_col_tiles(w) * 256 * planes) + up256((size_t)n_x * 4); }
 
 hipError_t launch_q4_routes(const Q4Launch& L, const Q4Launch& D, const Q4Routes& routes, int n_tokens, void* y, int out_dtype,
                             float* y_f32, hipStream_t s) {
@@ -298,7 +312,7 @@ hipError_t launch_q4(const Q4Launch& L, hipStream_t s) {
         Q4Launch G = L;
         if (L.x_type != kQ4Fp16 || padded != L.w.cols || !dma_aligned(L.x)) {
             uint16_t* x = static_cast<uint16_t*>(L.x_scratch);
-            float* scale = reinterpret_cast<float*>(static_cast<char*>(L.x_scratch) + up256((size_t)L.n_x * padded * 2));
+            float* scale = reinterpret_cast<float*>(static_cast<char*>(L.x_scratch) + up256((size_t)L.n_x * padded * (L.x_type == kQ4F32 ? 4 : 2)));
             auto k = L.x_type == kQ4Bf16   ? k_q4_rows<CX_DTYPE_BF16>
                      : L.x_type == kQ4Fp16 ? k_q4_rows<CX_DTYPE_FP16>
                      : L.x_type == kQ4F32  ? k_q4_rows<CX_DTYPE_F32>

@@ -50,11 +50,13 @@ struct Q4Ring {
 //
 // x is staged once per workgroup as fp16 in LDS: fp16 and e4m3 values as they are, others
 // times the power of two that brings the row's largest value to 2^14 .. 2^15 (bf16 is then
-// exact down to 2^-31 of it; fp32, the h of an expert, is rounded to 11 bits).  The codes
+// exact down to 2^-31 of it).  fp32, the h of an expert, is staged as two planes (q4_planes), whose
+// products are two of the MFMA's 16 columns, so that the second one costs LDS and no time.  The codes
 // times their scales are exact in fp16 (k_q4_row_scales), so the MFMAs sum exact products.
 template <int XT, int NG, int U>
 __global__ __launch_bounds__(64 * kQ4DecWaves) void k_q4_dec(Q4DecArgs A) {
     constexpr bool kScaled = XT == kQ4E4m3;  // a scale per row and column tile
+    constexpr int kPlanes = XT == kQ4F32 ? 2 : 1;
     const Q4Launch& L = A.L;
     __shared__ float row_up[4];
     __shared__ uint32_t tops[4][kQ4DecWaves];
@@ -85,7 +87,7 @@ __global__ __launch_bounds__(64 * kQ4DecWaves) void k_q4_dec(Q4DecArgs A) {
     const cx_q4_desc& w = other ? L.shared : L.w;
     const size_t mat = other ? 0 : (size_t)max(expert, 0);
     const int cols = L.w.cols, pitch = KT * 256 + kQ4LdsPad, rt = block * groups + rg;
-    float* xs_lds = reinterpret_cast<float*>(staged + A.lds_rows * pitch);  // kScaled: [lds_rows][KT]
+    float* xs_lds = reinterpret_cast<float*>(staged + A.lds_rows * pitch);  // kScaled (one plane): [lds_rows][KT]
 
     const size_t tile0 = (mat * RT + min(rt, RT - 1)) * (size_t)KT;
     const int per = (KT + A.splits - 1) / A.splits, k0 = ks * per, k1 = expert < 0 || rt >= RT ? k0 : min(KT, k0 + per);
@@ -175,7 +177,15 @@ __global__ __launch_bounds__(64 * kQ4DecWaves) void k_q4_dec(Q4DecArgs A) {
             const int p = i * 64 * kQ4DecWaves + tid;
             if (p >= KT * 16) continue;
             u32x4 o;
-            if constexpr (XT == kQ4Fp16) {
+            if constexpr (XT == kQ4F32) {
+                u32x4 lo;
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    const uint2 two = q4_planes(__uint_as_float(v[i][2 * k]) * up, __uint_as_float(v[i][2 * k + 1]) * up);
+                    o[k] = two.x, lo[k] = two.y;
+                }
+                *reinterpret_cast<u32x4*>(staged + (r * 2 + 1) * pitch + p * 16) = lo;
+            } else if constexpr (XT == kQ4Fp16) {
                 o = u32x4{v[i][0], v[i][1], v[i][2], v[i][3]};
             } else if constexpr (XT == kQ4E4m3) {
                 o = __builtin_bit_cast(u32x4, cvt8_f16(v[i][0], v[i][1]));
@@ -184,7 +194,7 @@ __global__ __launch_bounds__(64 * kQ4DecWaves) void k_q4_dec(Q4DecArgs A) {
                 for (int k = 0; k < 4; ++k)
                     o[k] = f16_rne(__uint_as_float(bits(i, 2 * k)) * up) | (f16_rne(__uint_as_float(bits(i, 2 * k + 1)) * up) << 16);
             }
-            *reinterpret_cast<u32x4*>(staged + r * pitch + p * 16) = o;
+            *reinterpret_cast<u32x4*>(staged + r * kPlanes * pitch + p * 16) = o;
         }
         if constexpr (kScaled)
             for (int k = tid; k < KT; k += 64 * kQ4DecWaves) xs_lds[r * KT + k] = xr >= 0 ? L.x_scale[(size_t)xr * KT + k] : 0.0f;
@@ -192,8 +202,8 @@ __global__ __launch_bounds__(64 * kQ4DecWaves) void k_q4_dec(Q4DecArgs A) {
     __syncthreads();
 
     // ---- the products; lanes of rows that are not there read another row, whose sums are dropped
-    const int lr = min(t, A.lds_rows - 1);
-    const unsigned char* in = staged + lr * pitch + q * 16;
+    const int lr = kPlanes == 2 ? min(t & 3, A.lds_rows - 1) : min(t, A.lds_rows - 1);
+    const unsigned char* in = staged + (kPlanes == 2 ? lr * 2 + (t >> 2 & 1) : lr) * pitch + q * 16;  // columns 4 .. 7: the second plane
     f32x4 acc[2] = {};
     auto multiply = [&](int kt, int u) {
         u32x4 b[4];
@@ -229,7 +239,10 @@ __global__ __launch_bounds__(64 * kQ4DecWaves) void k_q4_dec(Q4DecArgs A) {
     for (int i = tid; i < groups * 64; i += 64 * kQ4DecWaves) {  // 4 rows x 16 of each row tile
         const int g = i >> 6, o = block * groups + g, tt = (i & 63) >> 4, r = i & 15;
         float v = 0.0f;
-        for (int k = 0; k < A.splits; ++k) v += red[g * A.splits + k][i & 63];
+        for (int k = 0; k < A.splits; ++k) {
+            v += red[g * A.splits + k][i & 63];
+            if constexpr (kPlanes == 2) v += red[g * A.splits + k][64 + (i & 63)];
+        }
         v *= q4_row_scales(w)[(mat * RT + min(o, RT - 1)) * 16 + r] * row_up[min(tt, A.lds_rows - 1)];
         if (L.w.gated) {
             const float other_half = __shfl_down(v, 8);
@@ -242,17 +255,21 @@ __global__ __launch_bounds__(64 * kQ4DecWaves) void k_q4_dec(Q4DecArgs A) {
 
 // The down projections of a token's routes and their weighted sum, for a few tokens: a wave per
 // route, all on the same row tile, whose results are summed in route order (the shared
-// expert last) and rounded once.  Each wave stages its own row of h as k_q4_dec does, so
-// the only barrier is the one before the sum.  HBM: 8 routes of 7168 x 2048, 61 MB in 13 us, 4.6 TB/s.
-template <int NG, int U>
+// expert last) and rounded once.  Each wave stages its own row of h in two planes as k_q4_dec does,
+// 512 columns at a time, so the only barrier is the one before the sum.  Even columns of the MFMA
+// take the first plane, odd ones the second.  HBM: 8 routes of 7168 x 2048, 61 MB in 13.8 us, 4.4 TB/s
+// (13.0 with h rounded to the first plane).
+template <int NG>
 __global__ __launch_bounds__(1024) void k_q4_dec_sum(Q4DecSumArgs A) {
+    constexpr int U = 4;  // column tiles in flight: those of 512 columns
     extern __shared__ __attribute__((aligned(16))) unsigned char staged[];
     const int RT = A.RT, KT = A.KT, tok = blockIdx.x / RT, rt = blockIdx.x - tok * RT;
     const int wave = wave_id(), lane = threadIdx.x & 63, t = lane & 15, q = lane >> 4;
-    const int ke = A.routes.top_k + A.routes.shared, cols = A.w.cols, pitch = KT * 256 + kQ4LdsPad, k = wave;
+    const int ke = A.routes.top_k + A.routes.shared, cols = A.w.cols, pitch = q4_sum_pitch(cols), k = wave;
     float* red = reinterpret_cast<float*>(staged + ke * pitch);  // [ke][16]
     float* weight = red + ke * 16;
     unsigned char* mine = staged + wave * pitch;
+    const int lo_at = min(KT, 4) * 256 + kQ4LdsPad;  // of the second plane
     // in the order of their waits: h's row and the token's other ids, then the weights
     const __amdgpu_buffer_rsrc_t rh = make_rsrc(A.h + ((size_t)tok * ke + k) * cols, (uint32_t)cols * 4);
     u32x4 held[kQ4SumHeld][2];
@@ -293,35 +310,44 @@ __global__ __launch_bounds__(1024) void k_q4_dec_sum(Q4DecSumArgs A) {
     for (int m = 32; m >= 1; m >>= 1) most = max(most, (uint32_t)__shfl_xor((int)most, m));
     const int e = most == 0 ? 127 : min(max((int)(most >> 23) - 14, 1), 253);
     const float up = __uint_as_float((uint32_t)(254 - e) << 23), down = __uint_as_float((uint32_t)e << 23);
-#pragma unroll
-    for (int i = 0; i < kQ4SumHeld; ++i) {
-        const int c = (i * 64 + lane) * 8;
-        if (c >= KT * 128) continue;
-        u32x4 o;
-#pragma unroll
-        for (int d = 0; d < 4; ++d)
-            o[d] = f16_rne(__uint_as_float(held[i][d >> 1][2 * (d & 1)]) * up) | (f16_rne(__uint_as_float(held[i][d >> 1][2 * (d & 1) + 1]) * up) << 16);
-        *reinterpret_cast<u32x4*>(mine + c * 2) = o;
-    }
-    __builtin_amdgcn_wave_barrier();
     f32x4 acc[2] = {};
-    for (int kt = 0; kt < KT; kt += U) {
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            if (kt + u >= KT) break;
+    for (int i = 0; i < kQ4SumHeld; ++i) {  // 512 columns: a piece of 8 a lane
+        const int k0 = i * 4;
+        if (k0 >= KT) break;
+        const int c = lane * 16, part = min(KT - k0, 4) * 256;
+        if (c < part) {
+            u32x4 hi, lo;
+#pragma unroll
+            for (int d = 0; d < 4; ++d) {
+                const uint2 two = q4_planes(__uint_as_float(held[i][d >> 1][2 * (d & 1)]) * up, __uint_as_float(held[i][d >> 1][2 * (d & 1) + 1]) * up);
+                hi[d] = two.x, lo[d] = two.y;
+            }
+            *reinterpret_cast<u32x4*>(mine + c) = hi;
+            *reinterpret_cast<u32x4*>(mine + lo_at + c) = lo;
+        }
+        __builtin_amdgcn_wave_barrier();
+        const unsigned char* in = mine + (t & 1) * lo_at + q * 16;
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            if (k0 + u >= KT) break;
             __builtin_amdgcn_sched_barrier(0);
             u32x4 b[4];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) b[j] = *reinterpret_cast<const u32x4*>(mine + (kt + u) * 256 + j * 64 + q * 16);
+            for (int j = 0; j < 4; ++j) b[j] = *reinterpret_cast<const u32x4*>(in + u * 256 + j * 64);
 #pragma unroll
             for (int j = 0; j < 4; ++j) acc[j & 1] = Mma<true>::mma(ring.weights(u, j), Mma<true>::bits(b[j]), acc[j & 1]);
-            ring.fetch(rw, rs, kt + U + u, u, lane);
+            ring.fetch(rw, rs, k0 + 4 + u, u, lane);
         }
+        __builtin_amdgcn_wave_barrier();
     }
+    f32x4 both = acc[0] + acc[1];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) both[i] += __shfl_xor(both[i], 1);
     if (t == 0) {
         const f32x4 scale = *reinterpret_cast<const f32x4*>(q4_row_scales(w) + tile0 / KT * 16 + 4 * q);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) red[k * 16 + 4 * q + i] = used ? (acc[0][i] + acc[1][i]) * scale[i] * down : 0.0f;
+        for (int i = 0; i < 4; ++i) red[k * 16 + 4 * q + i] = used ? both[i] * scale[i] * down : 0.0f;
     }
     __syncthreads();
     const int n = rt * 16 + threadIdx.x;

@@ -9,7 +9,7 @@ namespace {
 
 template <int XT, int NG>
 hipError_t dec_launch(const Q4DecArgs& A, int64_t items, hipStream_t s) {
-    const size_t lds = std::max<size_t>(q4_dec_lds(A.L.w.cols, A.lds_rows), kQ4DecWaves * 1024);
+    const size_t lds = std::max<size_t>(q4_dec_lds(A.L.w.cols, A.lds_rows * (XT == kQ4F32 ? 2 : 1)), kQ4DecWaves * 1024);
     // A ring of 8: one token through 8 experts takes 42 us with 4 to 8 places, 45 with 14 and 52 with 20 (registers
     // that waves then lack); 4 in the sum's kernel: 41.3 us, 42.2 with 8, 43.3 with 16.
     cx_launch(k_q4_dec<XT, NG, 8>, dim3((unsigned)(items * A.row_blocks)), dim3(64 * kQ4DecWaves), (uint32_t)lds, s, A);
@@ -42,7 +42,7 @@ hipError_t launch_q4_dec(const Q4Launch& L, const Q4Routes* routes, int splits, 
 
 hipError_t launch_q4_dec_sum(const Q4DecSumArgs& A, int n_tokens, hipStream_t s) {
     const int ke = A.routes.top_k + A.routes.shared;
-    auto k = A.w.group == 128 ? k_q4_dec_sum<1, 4> : A.w.group == 64 ? k_q4_dec_sum<2, 4> : k_q4_dec_sum<4, 4>;
+    auto k = A.w.group == 128 ? k_q4_dec_sum<1> : A.w.group == 64 ? k_q4_dec_sum<2> : k_q4_dec_sum<4>;
     cx_launch(k, dim3((unsigned)(n_tokens * A.RT)), dim3(64 * ke), (uint32_t)q4_sum_lds(A.w.cols, ke), s, A);
     return hipGetLastError();
 }

@@ -14,7 +14,7 @@ struct Q4GemmArgs {
     const uint16_t* x;        // [n_x, padded]
     const float* x_row_scale; // nullable [n_x]
     const float* x_scale;     // XS: [n_x, KT]
-    int padded;               // columns of a row of x: KT * 128
+    int padded;               // columns of a row of x: KT * 128, twice that with two planes
     int n_x, n_rows, top_k;
     const int32_t* order;
     const Q4Item* items;
@@ -37,10 +37,11 @@ constexpr int kQ4GemmWaves = 4;
 // a product with the scale for every two weights), reads a fragment of x and waits its turn; with
 // 8 tiles of rows to a conversion and two workgroups a CU the matrix cores are busy 69 % of the time
 // (4096 rows by 4096 x 7168: 192 us, 1.25 PFLOP/s; a library's bf16 product reaches 1.43 on
-// this card).  Fewer rows per item amortise a conversion less: 1024 tokens over 64 experts, gate/up 500
-// us and 60 %.  Steps that led here, at that size (both products and what is around them): x through
-// registers 1476 us, straight to LDS with fragments two steps ahead 1000, outputs turned in LDS 935,
-// equal items and wide conversions 819, long items first 789.
+// this card).  Fewer rows per item amortise a conversion less: 1024 tokens over 64 experts, gate/up 472
+// us and 63 %; the down product, whose h is two planes on one conversion, 439 us and 67 %.  Steps that led here,
+// at that size (both products and what is around them): x through registers 1476 us, straight to LDS with
+// fragments two steps ahead 1000, outputs turned in LDS 935, equal items and wide conversions 819, long
+// items first 789; h in two planes 955 (11 bits of h were too few for fp16 and fp32 outputs).
 constexpr int kQ4GemmBuf = kQ4GemmRows * 256;
 
 // s_waitcnt vmcnt(0) lgkmcnt(0), then a barrier: the loads into the other buffer have
@@ -140,7 +141,11 @@ __device__ __forceinline__ void q4_gemm_store(const Q4GemmArgs& L, const f32x4 (
 // below the largest product of an instruction, and sums here are kept to fp32.  The second set of
 // sums costs a multiply-add per MFMA and 4 values, and half the rows per conversion: 3001
 // rows by 7168 x 2048 in 101 to 116 us, 0.8 to 0.87 PFLOP/s (128 rows and one workgroup a CU: 8 % slower).
-template <int NG, int RTW, int NT, bool XS>
+//
+// PL (fp32 rows of x, the h of a layer, as two fp16 planes; row p of x is row p of y): a buffer holds 64 columns, 8 pieces of a row's first
+// plane and the 8 of its second, so that a buffer and a turn have as many MFMAs as without planes
+// and a conversion serves both planes of all rows.
+template <int NG, int RTW, int NT, bool XS, bool PL>
 __device__ __forceinline__ void q4_gemm_tile(const Q4GemmArgs& L, unsigned char* lds0, unsigned char* lds1, const cx_q4_desc& w,
                                              size_t mat, int rb, int ks, int begin, int rows) {
     const int wave = wave_id(), lane = threadIdx.x & 63, t = lane & 15, q = lane >> 4;
@@ -149,28 +154,31 @@ __device__ __forceinline__ void q4_gemm_tile(const Q4GemmArgs& L, unsigned char*
     // row r gets the row's piece s ^ (r % 16), so that the 16 rows of a fragment lie in
     // 16 different places of the banks.
     const int tr = threadIdx.x >> 4, piece = (threadIdx.x & 15) ^ tr;
+    const uint32_t pitch = (uint32_t)L.padded * 2;
     uint32_t xoff[NT];  // in bytes; rows that do not exist read another and are never stored
 #pragma unroll
     for (int i = 0; i < NT; ++i) {
         const int r = i * 16 + tr;
-        int xr = begin + (r < rows ? r : 0);
-        if (L.order != nullptr) xr = max(L.order[xr], 0) / L.top_k;
-        xoff[i] = (uint32_t)(xr < L.n_x ? xr : 0) * (uint32_t)(L.padded * 2) + piece * 16;
+        int xr = (PL ? 0 : begin) + (r < rows ? r : 0);
+        if (!PL && L.order != nullptr) xr = max(L.order[xr], 0) / L.top_k;
+        xoff[i] = (uint32_t)(PL || xr < L.n_x ? xr : 0) * pitch + piece * 16;
     }
-    const uint8_t* wp[RTW];
-    const uint16_t* sp[RTW];
-#pragma unroll
-    for (int m = 0; m < RTW; ++m) {
-        const int rt = min((rb * kQ4GemmWaves + wave) * RTW + m, L.RT - 1);
-        const size_t tile = (mat * L.RT + rt) * (size_t)KT;
-        wp[m] = w.codes + tile * kQ4Tile;
-        sp[m] = w.scales + tile * 16 * NG;
-    }
-    struct Sc {  // the lane's row's scales of a tile
-        uint32_t d[(NG + 1) / 2];
+    const int rt0 = min((rb * kQ4GemmWaves + wave) * RTW, L.RT - 1), rts = min(RTW, L.RT - rt0);  // row tiles past the matrix: its last one again
+    const size_t tile0 = (mat * L.RT + rt0) * (size_t)KT;
+    const uint8_t* wp = w.codes + tile0 * kQ4Tile;
+    const uint16_t* sp = w.scales + tile0 * 16 * NG;
+    // Loads of a lane's 32-bit place and a scalar one, with planes of the item's own rows: of 64-bit places in each lane
+    // the compiler spilled (with planes 599 us for the down products below, 439 without spills; gate/up 492 and 472).
+    // e4m3 rows, whose launch bounds leave registers, take plain loads (118 us as above, 116).
+    const __amdgpu_buffer_rsrc_t rx = make_rsrc(reinterpret_cast<const char*>(L.x) + (PL ? (size_t)begin * pitch : 0), (PL ? (uint32_t)rows : (uint32_t)L.n_x) * pitch);
+    const __amdgpu_buffer_rsrc_t rw = make_rsrc(wp, (uint32_t)(rts * KT) * kQ4Tile), rs = make_rsrc(sp, (uint32_t)(rts * KT) * 32 * NG);
+    // of a fetch, which is a column tile or, with planes, half of one: the lane's codes, and its row's scales
+    typedef uint32_t Codes __attribute__((ext_vector_type(PL ? 2 : 4)));
+    struct Sc {
+        uint32_t d[PL ? 1 : (NG + 1) / 2];
     };
     f32x4 acc[NT][RTW] = {}, sum[XS ? NT : 1][RTW] = {};
-    u32x4 a[2][RTW];
+    Codes a[2][RTW];
     Sc s[2][RTW];
     uint32_t xso = 0;  // XS: wave 0 brings the rows' scales, a lane each, behind their 64 rows
     if constexpr (XS) {
@@ -179,22 +187,40 @@ __device__ __forceinline__ void q4_gemm_tile(const Q4GemmArgs& L, unsigned char*
         if (L.order != nullptr) xr = max(L.order[xr], 0) / L.top_k;
         xso = (uint32_t)(xr < L.n_x ? xr : 0) * (uint32_t)KT;
     }
-    auto fetch = [&](int kt, auto to, unsigned char* buf) {
+    auto fetch = [&](int part, auto to, unsigned char* buf) {  // part: column tile, with planes its half `to`
 #pragma unroll
-        for (int i = 0; i < NT; ++i)
-            __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(reinterpret_cast<const char*>(L.x) + (size_t)kt * 256 + xoff[i]),
-                                             (__attribute__((address_space(3))) void*)(buf + i * 4096 + wave * 1024), 16, 0, 0);
+        for (int i = 0; i < NT; ++i) {
+            const auto at = (__attribute__((address_space(3))) void*)(buf + i * 4096 + wave * 1024);
+            if constexpr (!XS)
+                __builtin_amdgcn_raw_ptr_buffer_load_lds(rx, at, 16, xoff[i], part * 256, 0, 0);
+            else
+                __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(reinterpret_cast<const char*>(L.x) + (size_t)part * 256 + xoff[i]), at, 16, 0, 0);
+        }
 #pragma unroll
         for (int m = 0; m < RTW; ++m) {
-            a[to][m] = ld16(wp[m] + (size_t)kt * kQ4Tile + (uint32_t)lane * 16);
-            if constexpr (NG == 1)
-                s[to][m].d[0] = (sp[m] + (size_t)kt * 16)[(uint32_t)t];
+            const int tile = min(m, rts - 1) * KT + (PL ? part >> 1 : part);
+            if constexpr (XS) {
+                a[to][m] = ld16(wp + (size_t)tile * kQ4Tile + (uint32_t)lane * 16);
+                if constexpr (NG == 1)
+                    s[to][m].d[0] = (sp + (size_t)tile * 16)[(uint32_t)t];
+                else
+                    s[to][m] = *reinterpret_cast<const Sc*>(sp + (size_t)tile * 16 * NG + (uint32_t)t * NG);
+                continue;
+            }
+            if constexpr (PL)
+                a[to][m] = __builtin_bit_cast(Codes, __builtin_amdgcn_raw_buffer_load_b64(rw, lane * 16 + to * 8, tile * kQ4Tile, 0));
             else
-                s[to][m] = *reinterpret_cast<const Sc*>(sp[m] + (size_t)kt * 16 * NG + (uint32_t)t * NG);
+                a[to][m] = __builtin_bit_cast(Codes, __builtin_amdgcn_raw_buffer_load_b128(rw, lane * 16, tile * kQ4Tile, 0));
+            if constexpr (NG == 1)
+                s[to][m].d[0] = __builtin_amdgcn_raw_buffer_load_b16(rs, t * 2, tile * 32, 0);
+            else if constexpr (NG == 2 || PL)  // the tile's two scales, with planes its half's two of four
+                s[to][m].d[0] = __builtin_amdgcn_raw_buffer_load_b32(rs, t * 2 * NG + (NG == 4 ? to * 4 : 0), tile * 32 * NG, 0);
+            else
+                s[to][m] = __builtin_bit_cast(Sc, __builtin_amdgcn_raw_buffer_load_b64(rs, t * 8, tile * 128, 0));
         }
         if constexpr (XS)
             if (wave == 0)
-                __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(L.x_scale + kt + xso),
+                __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(L.x_scale + part + xso),
                                                  (__attribute__((address_space(3))) void*)(buf + 16384), 4, 0, 0);
     };
     auto scaled_add = [&](const unsigned char* buf, int n) {
@@ -212,25 +238,28 @@ __device__ __forceinline__ void q4_gemm_tile(const Q4GemmArgs& L, unsigned char*
         // Steps of RTW MFMAs on one fragment of x, in this order: the fragment after the
         // next is read and the next columns' weights are converted while they run.
         const unsigned char* in = buf + t * 256;
-        constexpr int kSteps = 4 * NT;
+        constexpr int kSteps = 4 * NT, kOf = PL ? 2 * NT : NT;  // steps that share a conversion: those of all rows, with planes of both
         f16x8 fa[2][RTW];
         u32x4 b[3];
-        auto convert = [&](int j, int m) {
-            const int g = j * NG / 4;
+        auto convert = [&](int j, int m) {  // of the fetch's columns 32 j .. + 31
+            const int g = (PL ? from * 2 + j : j) * NG / 4 - (PL && NG == 4 ? from * 2 : 0);
             const _Float16 sc = __builtin_bit_cast(f16x2, s[from][m].d[g / 2])[g % 2];
             fa[j & 1][m] = q4_f16(a[from][m][j]) * f16x8{sc, sc, sc, sc, sc, sc, sc, sc};
         };
-        auto read = [&](int i) { b[i % 3] = *reinterpret_cast<const u32x4*>(in + i % NT * 4096 + (((i / NT * 4 + q) ^ t) * 16)); };
+        auto read = [&](int i) {
+            const int j = i / kOf, plane = i % kOf / NT;
+            b[i % 3] = *reinterpret_cast<const u32x4*>(in + i % NT * 4096 + ((((plane * 2 + j) * 4 + q) ^ t) * 16));
+        };
         read(0);
         read(1);
 #pragma unroll
         for (int m = 0; m < RTW; ++m) convert(0, m);
 #pragma unroll
         for (int i = 0; i < kSteps; ++i) {
-            const int j = i / NT, n = i % NT;
+            const int j = i / kOf, at = i % kOf, n = i % NT;
             __builtin_amdgcn_sched_barrier(0);
             if (i + 2 < kSteps) read(i + 2);
-            if (j < 3)
+            if (j + 1 < kSteps / kOf && at >= kOf - NT)  // late: registers
 #pragma unroll
                 for (int m = n * RTW / NT; m < (n + 1) * RTW / NT; ++m) convert(j + 1, m);
 #pragma unroll
@@ -250,15 +279,16 @@ __device__ __forceinline__ void q4_gemm_tile(const Q4GemmArgs& L, unsigned char*
     };
     constexpr std::integral_constant<int, 0> even{};
     constexpr std::integral_constant<int, 1> odd{};
-    const int per = (KT + L.splits - 1) / L.splits, k0 = ks * per, k1 = min(KT, k0 + per);
+    constexpr int kParts = PL ? 2 : 1;  // of a column tile
+    const int per = (KT + L.splits - 1) / L.splits, k0 = ks * per * kParts, k1 = min(KT * kParts, k0 + per * kParts);
     if (k0 < k1) fetch(k0, even, lds0);
     q4_gemm_turn();
-    for (int kt = k0; kt < k1; kt += 2) {
-        if (kt + 1 < k1) fetch(kt + 1, odd, lds1);
+    for (int k = k0; k < k1; k += 2) {
+        if (PL || k + 1 < k1) fetch(k + 1, odd, lds1);
         multiply(even, lds0);
         q4_gemm_turn();
-        if (kt + 1 >= k1) break;
-        if (kt + 2 < k1) fetch(kt + 2, even, lds0);
+        if (!PL && k + 1 >= k1) break;
+        if (k + 2 < k1) fetch(k + 2, even, lds0);
         multiply(odd, lds1);
         q4_gemm_turn();
     }
@@ -268,7 +298,7 @@ __device__ __forceinline__ void q4_gemm_tile(const Q4GemmArgs& L, unsigned char*
         q4_gemm_store<RTW, NT>(L, acc, lds0, w, mat, rb, ks, begin, rows);
 }
 
-template <int NG, int RTW, bool XS>
+template <int NG, int RTW, bool XS, bool PL>
 __global__ __launch_bounds__(64 * kQ4GemmWaves, 2) void k_q4_gemm(Q4GemmArgs L) {
     __shared__ __attribute__((aligned(16))) unsigned char lds0[kQ4GemmBuf], lds1[kQ4GemmBuf];
     const int per = L.RB * L.splits, idx = blockIdx.x / per, unit = blockIdx.x - idx * per, ks = unit / L.RB, rb = unit - ks * L.RB;
@@ -295,7 +325,7 @@ __global__ __launch_bounds__(64 * kQ4GemmWaves, 2) void k_q4_gemm(Q4GemmArgs L) 
     const cx_q4_desc& w = other ? L.shared : L.w;
     const size_t mat = other ? 0 : (size_t)expert;
     auto tile = [&](auto nt) {
-        q4_gemm_tile<NG, RTW, nt, XS>(L, lds0, lds1, w, mat, rb, ks, begin, rows);
+        q4_gemm_tile<NG, RTW, nt, XS, PL>(L, lds0, lds1, w, mat, rb, ks, begin, rows);
     };
     if constexpr (!XS) {
         if (rows > 112) return tile(std::integral_constant<int, 8>{});

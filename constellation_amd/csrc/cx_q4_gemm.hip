@@ -29,7 +29,7 @@ hipError_t launch_q4_gemm(const Q4Launch& L, hipStream_t s) {
     a.item_rows = L.item_rows;
     a.RT = q4_row_tiles(L.w);
     a.KT = q4_col_tiles(L.w);
-    a.padded = a.KT * 128;
+    a.padded = a.KT * (L.x_type == kQ4F32 ? 256 : 128);
     a.n_x = L.n_x;
     a.n_rows = L.n_rows;
     a.top_k = L.top_k;
@@ -42,10 +42,12 @@ hipError_t launch_q4_gemm(const Q4Launch& L, hipStream_t s) {
     a.splits = splits_of(L.w, L.n_rows, L.n_mats, L.item_rows);
     a.RB = (a.RT + kQ4GemmWaves * kRtw - 1) / (kQ4GemmWaves * kRtw);
     const int64_t items = L.items != nullptr ? L.max_items : (L.n_rows + L.item_rows - 1) / L.item_rows;
-    const bool xs = L.x_type == kQ4E4m3;
-    auto k = L.w.group == 128  ? (xs ? k_q4_gemm<1, kRtw, true> : k_q4_gemm<1, kRtw, false>)
-             : L.w.group == 64 ? (xs ? k_q4_gemm<2, kRtw, true> : k_q4_gemm<2, kRtw, false>)
-                               : (xs ? k_q4_gemm<4, kRtw, true> : k_q4_gemm<4, kRtw, false>);
+    auto of = [&](auto ng) {
+        return L.x_type == kQ4E4m3 ? k_q4_gemm<ng, kRtw, true, false> : L.x_type == kQ4F32 ? k_q4_gemm<ng, kRtw, false, true> : k_q4_gemm<ng, kRtw, false, false>;
+    };
+    auto k = L.w.group == 128  ? of(std::integral_constant<int, 1>{})
+             : L.w.group == 64 ? of(std::integral_constant<int, 2>{})
+                               : of(std::integral_constant<int, 4>{});
     cx_launch(k, dim3((unsigned)(items * a.RB * a.splits)), dim3(64 * kQ4GemmWaves), 0, s, a);
     if (a.splits > 1) {
         const int width = L.w.gated ? L.w.rows / 2 : L.w.rows, units = (width + 3) / 4;

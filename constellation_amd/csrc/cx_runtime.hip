@@ -822,7 +822,7 @@ Q4Scratch q4_scratch(const cx_q4_desc& w, int x_dtype, int n_x, int n_rows, bool
     z.item_rows = q4_item_rows(n_rows, w.n_mats, w.rows, w.cols, x_dtype == CX_DTYPE_E4M3);
     z.max_items = q4_max_items(n_rows, w.n_mats, z.item_rows);
     z.x = with_offsets ? align_up(sizeof(Q4Item) * (size_t)z.max_items) : 0;
-    z.part = z.x + (z.item_rows > kTileTok ? q4_x_scratch(w, n_x) : 0);
+    z.part = z.x + (z.item_rows > kTileTok ? q4_x_scratch(w, n_x, 1) : 0);
     z.bytes = z.part + q4_part_bytes(w, n_rows, w.n_mats, z.item_rows);
     return z;
 }
@@ -846,17 +846,17 @@ Q4MoeScratch q4_moe_scratch(const cx_q4_desc& gu, const cx_q4_desc& down, int sh
     Q4MoeScratch z{};
     z.pairs = (int64_t)n_tokens * (top_k + shared);
     // both products take the same items; in between h is fp32, which the decode kernel and the GEMM read
-    z.item_rows = q4_layer_rows(z.pairs, gu.n_mats + shared, std::max(gu.cols, down.cols));
+    z.item_rows = q4_layer_rows(z.pairs, gu.n_mats + shared, std::max(gu.cols, down.cols), down.cols);
     z.max_items = q4_max_items(z.pairs, gu.n_mats + shared, z.item_rows);
     const bool gemm = z.item_rows > kTileTok;
-    const int64_t listed = most ? q4_most_items(z.pairs, gu.n_mats + shared, q4_dec_rows(std::max(gu.cols, down.cols))) : z.max_items;
+    const int64_t listed = most ? q4_most_items(z.pairs, gu.n_mats + shared, q4_layer_dec_rows(std::max(gu.cols, down.cols), down.cols)) : z.max_items;
     z.items = 0;
     z.order = z.items + align_up(sizeof(Q4Item) * (size_t)listed);
     z.place = z.order + align_up(4 * (size_t)z.pairs);
     z.x = z.place + align_up(4 * (size_t)z.pairs);
-    z.h = z.x + (gemm ? q4_x_scratch(gu, n_tokens) : 0);
+    z.h = z.x + (gemm ? q4_x_scratch(gu, n_tokens, 1) : 0);
     z.hx = z.h + align_up(4 * (size_t)z.pairs * down.cols);
-    z.ys = z.hx + (gemm ? q4_x_scratch(down, (int)z.pairs) : 0);
+    z.ys = z.hx + (gemm ? q4_x_scratch(down, (int)z.pairs, 2) : 0);
     z.part = z.ys + align_up(4 * (size_t)z.pairs * down.rows);
     auto parts = [&](const cx_q4_desc& w) {
         return most ? q4_most_part_bytes(w, z.pairs, w.n_mats + shared, z.item_rows) : q4_part_bytes(w, z.pairs, w.n_mats + shared, z.item_rows);

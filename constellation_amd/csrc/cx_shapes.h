@@ -289,10 +289,11 @@ inline int q4_dec_rows(int cols) {
     while (rows > 0 && q4_dec_lds(cols, rows) > 63 * 1024) --rows;
     return rows;
 }
-// LDS of the down projections and sum of one token's routes: a staged row, 16 sums and a weight per route, a
-// wave each.
+// LDS of the down projections and sum of one token's routes: up to 512 columns in two planes, 16 sums and a
+// weight per route, a wave each.
 constexpr int kQ4SumHeld = 4;  // 8-value pieces of a row per lane
-inline size_t q4_sum_lds(int cols, int routes) { return (size_t)routes * ((size_t)((cols + 127) / 128) * 256 + kQ4LdsPad + 68); }
+constexpr int q4_sum_pitch(int cols) { return 2 * ((cols > 384 ? 4 : (cols + 127) / 128) * 256 + kQ4LdsPad); }
+inline size_t q4_sum_lds(int cols, int routes) { return (size_t)routes * (q4_sum_pitch(cols) + 68); }
 // A layer on one token's routes, without a plan.
 inline bool q4_routes_ok(int n_tokens, int top_k, int hidden, int inter, int shared) {
     return n_tokens == 1 && hidden <= kQ4DecCols && inter <= kQ4SumHeld * 512 && top_k + shared <= 16 &&
@@ -317,9 +318,15 @@ inline int q4_item_rows(int64_t n_rows, int n_mats, int rows, int cols, bool two
     const bool small = (n_mats == 1 && items <= 1) || (double)items * kTileTok * rows * cols < (two_sums && n_rows > 128 ? kQ4FewWork / 2 : kQ4FewWork);
     return small && (cols % 8 == 0 || cols <= 1024) ? kTileTok : two_sums ? kQ4GemmRows / 2 : kQ4GemmRows;
 }
-// Of a layer, whose second product reads the first one's fp32 rows: the decode kernel or the GEMM.
-inline int q4_layer_rows(int64_t n_rows, int n_mats, int cols) {
-    const int dec = q4_dec_rows(cols);
+// Of a layer of up to `cols` columns, whose second product reads the first one's fp32 rows of `inter` columns, two
+// planes of each: the decode kernel or the GEMM.
+inline int q4_layer_dec_rows(int cols, int inter) {
+    int dec = q4_dec_rows(cols);
+    while (dec > 0 && q4_dec_lds(inter, 2 * dec) > 63 * 1024) --dec;
+    return dec;
+}
+inline int q4_layer_rows(int64_t n_rows, int n_mats, int cols, int inter = 0) {
+    const int dec = q4_layer_dec_rows(cols, inter);
     return dec > 0 && n_rows <= std::max(n_mats, dec) ? dec : kQ4GemmRows;
 }
 

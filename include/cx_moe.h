@@ -394,9 +394,11 @@ CX_API int cx_q4_matmul(cx_ctx* ctx, const cx_q4_desc* w, const void* x, int x_d
  * gate_up: gated [2 * inter, hidden] per expert; down: [hidden, inter] per expert;
  * shared_gate_up / shared_down (nullable, together): the shared expert, stacks of
  * one with the same sizes and groups.  h = silu(gate) * up is kept in fp32 and
- * takes part in the down product as fp16 times a power of two per row (11 bits).
- * n_tokens may be 0; a call whose padded rows of x or h would pass 4 GB in fp16
- * (about 299,000 tokens of 7168, or a million pairs of 2048) is refused.
+ * takes part in the down product as the sum of two fp16 values times a power of two per
+ * row: within 2^-23 of itself, or 2^-39 of its row's largest value.
+ * n_tokens may be 0; a call whose padded rows of x would pass 4 GB in fp16 (about
+ * 299,000 tokens of 7168), or with more items than a launch has (about 1.1 million
+ * pairs at hidden 7168), is refused.
  * scratch: cx_q4_moe_scratch bytes of the caller's, as above (enough for every call
  * with as many tokens or fewer); a captured graph keeps using the scratch it was
  * captured with. */

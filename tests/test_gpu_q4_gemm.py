@@ -165,7 +165,7 @@ DEC_LAYERS = [(1, 15, 20, 256, 136, 1, True), (1, 16, 40, 1000, 64, 0, True), (1
 def test_layers(gpu, T, K, E, H, I, shared, dtype):
     """Layers at the limits of their kernels: many routes, wide rows, wide experts."""
     from constellation_amd.engine import Q4Layer, Q4Matrix
-    from test_gpu_q4 import H_HALF, layer_ref
+    from test_gpu_q4 import layer_ref
     print(f"[q4 gemm] layer {T}x{K} of {E} {H}x{I} shared {shared} {dtype}", flush=True)
     group = 32 if I % 64 else 128
     gu, dn, sg, sd = (make(i + T, n, *s, group) for i, (n, s) in
@@ -183,7 +183,7 @@ def test_layers(gpu, T, K, E, H, I, shared, dtype):
         torch.cuda.synchronize()
         gpu.sync()
         D = [dense(c, s, k, group) for (c, s), k in ((gu, H), (dn, I), (sg, H), (sd, I))]
-        want, tol = layer_ref(x.double(), ids, w, D[0], D[1], H_HALF, (D[2], D[3]) if shared else None)
+        want, tol = layer_ref(x.double(), ids, w, D[0], D[1], 2.0 ** -22, (D[2], D[3]) if shared else None)
         near(yf, want, tol, "fp32")
         near(y, want, rounded(want, tol, dtype), "rounded")
     finally:

@@ -18,6 +18,10 @@ SOURCE = r"""
 using namespace cx;
 extern "C" {
 int splits(int rt, int kt, int64_t rows, int mats, int item) { return q4_gemm_splits(rt, kt, rows, mats, item); }
+int layer_dec(int cols, int inter) { return q4_layer_dec_rows(cols, inter); }
+size_t dec_lds(int cols, int rows) { return q4_dec_lds(cols, rows); }
+size_t sum_lds(int cols, int routes) { return q4_sum_lds(cols, routes); }
+int routes(int k, int h, int i) { return q4_routes_ok(1, k, h, i, 0); }
 int64_t part_rows(int rt, int kt, int64_t rows, int mats, int item) { return q4_gemm_part_rows(rt, kt, rows, mats, item); }
 }
 """
@@ -31,6 +35,7 @@ def rules(tmp_path_factory):
                     "-o", str(d / "parts.so")], check=True)
     L = C.CDLL(str(d / "parts.so"))
     L.part_rows.restype = C.c_int64
+    L.dec_lds.restype = L.sum_lds.restype = C.c_size_t
     L.splits.argtypes = L.part_rows.argtypes = [C.c_int, C.c_int, C.c_int64, C.c_int, C.c_int]
     return L
 
@@ -101,3 +106,15 @@ def test_partial_rows_over_all_smaller_calls(rules):
                 for n in range(9001, 400000, 1117):  # nothing larger where the bound has stopped to look
                     s = rules.splits(rt, kt, n, mats, item)
                     assert s == 1 or s * n <= rules.part_rows(rt, kt, n, mats, item), (rt, kt, mats, item, n)
+
+
+def test_both_planes_of_h_fit_the_lds(rules):
+    for inter in [*range(1, 9000, 61), 2048, 4096, 7168, 8192, 8193]:
+        rows = rules.layer_dec(max(64, inter), inter)
+        assert 0 <= rows <= 4 and (rows > 0) == (inter <= 8192)
+        assert rows == 0 or rules.dec_lds(inter, 2 * rows) <= 64 * 1024 - 256  # beside its static 144 bytes
+        for k in (1, 9, 15, 16):
+            if rules.routes(k, 7168, inter):
+                # two planes of up to 4 column tiles, 16 sums and a weight per route
+                assert rules.sum_lds(inter, k) == k * (2 * (min(-(-inter // 128), 4) * 256 + 64) + 68) <= 64 * 1024
+    assert rules.routes(16, 7168, 2048) and not rules.routes(17, 7168, 2048) and not rules.routes(1, 7168, 2049)
