@@ -49,6 +49,13 @@ def _check_pairs(rows: int, n_tokens: int, top_k: int, weights: Optional[torch.T
         raise ValueError(f"weights must be fp32 [{n_tokens}, {top_k}]")
 
 
+def _outside_autograd(name: str, gradient: str, *tensors: Optional[torch.Tensor]) -> None:
+    """A result without a graph must not pass for one with it."""
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+        raise ValueError(f"{name} records no graph: call it under torch.no_grad() or in an autograd.Function "
+                         f"whose backward is {gradient}")
+
+
 def _stream(device: int) -> int:
     """The current stream's handle; without a Stream object around it, where torch has
     that (a microsecond less a call).  Looked up by the call: the module also serves programs
@@ -432,8 +439,10 @@ class Context:
 
     def gather_rows(self, x: torch.Tensor, place: torch.Tensor) -> torch.Tensor:
         """Rows of x [T, H] (any type) in sorted order [T * K, H]; zeros where a
-        pair has no expert.  Its gradient: combine_rows(dxs, place)."""
+        pair has no expert.  Its gradient: combine_rows(dxs, place), by the caller's
+        autograd.Function (tensors that require grad are refused outside of one)."""
         self._here(x, place)
+        _outside_autograd("gather_rows", "combine_rows(dxs, place)", x)
         T, H = _rows_2d(x)
         K = _places(place, T)
         x = x.contiguous()
@@ -446,8 +455,10 @@ class Context:
                      add: Optional[torch.Tensor] = None,
                      out_dtype: Optional[torch.dtype] = None) -> torch.Tensor:
         """Sorted rows ys [T * K, H] back to tokens: [T, H] in out_dtype (ys's),
-        the sum over k of weights[t, k] * ys[place[t, k]] (+ add[t])."""
+        the sum over k of weights[t, k] * ys[place[t, k]] (+ add[t]).  Its gradient:
+        combine_rows_grad, by the caller's autograd.Function (as gather_rows)."""
         self._here(ys, place, weights, add)
+        _outside_autograd("combine_rows", "combine_rows_grad", ys, weights, add)
         P, H = _rows_2d(ys)
         T = place.shape[0]
         K = _places(place, T)
