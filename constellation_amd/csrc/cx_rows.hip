@@ -684,10 +684,7 @@ hipError_t launch_combine_rows(const CombineArgs& a, hipStream_t s) {
 
 hipError_t launch_combine_grad(const CombineGradArgs& a, hipStream_t s) {
     const bool vec = a.hidden % 8 == 0 && at16(a.ys) && at16(a.dys) && at16(a.dout);
-    // few tokens: a workgroup per route, or there are too few of them (bf16 rows of 7168, 8 a token: 128 tokens 10.4 us,
-    // with a token's routes together 20.0; 384: 22.7 and 27.2; 512: 29.7 and 29.8; 1024: 54 and 43; fp32 rows of
-    // 2001, 6 a token: 128 tokens 5.7 and 8.5, 384: 15.2 and 12.6, 509: 19.0 and 13.7)
-    const int routes = a.n_tokens < 448 ? 1 : 8, splits = (a.top_k + routes - 1) / routes;
+    const int routes = combine_grad_routes((int64_t)a.n_tokens * a.top_k, vec), splits = (a.top_k + routes - 1) / routes;
     auto k = a.ys_dtype == CX_DTYPE_BF16   ? (vec ? k_combine_grad<CX_DTYPE_BF16, true> : k_combine_grad<CX_DTYPE_BF16, false>)
              : a.ys_dtype == CX_DTYPE_FP16 ? (vec ? k_combine_grad<CX_DTYPE_FP16, true> : k_combine_grad<CX_DTYPE_FP16, false>)
                                            : (vec ? k_combine_grad<CX_DTYPE_F32, true> : k_combine_grad<CX_DTYPE_F32, false>);

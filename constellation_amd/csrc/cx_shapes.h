@@ -276,6 +276,15 @@ constexpr int kMaxRowWidth = INT32_MAX - 8 * kRowThreads;
 // A launch's threads are counted in 32 bits.
 inline bool rows_grid_ok(int64_t workgroups, int threads) { return workgroups * threads < ((int64_t)1 << 32); }
 
+// Routes of a token that one workgroup of the combine's gradient takes: one each while workgroups are few, up to eight
+// together, on one read of dout, once there are many.  Where that turns depends on the pairs and on
+// the width of the accesses, little on the rows' bytes (us, one each and together; bf16 rows of 7168, 8 a token: 384
+// tokens 22.4 and 26.7, 512: 28.8 and 29.1, 640: 36.0 and 32.8; 16 a token: 256 tokens 26.1 and 29.2, 384: 36.3 and
+// 35.5; of 1024, 8 a token: 320 tokens 8.2 and 8.4, 512: 11.8 and 9.1; fp32 of 7168, 6 a token: 320 tokens 26.6 and
+// 27.1, 640: 49.0 and 42.2; rows at odd addresses, fp32 of 2001, 6 a token: 256 tokens 9.4 and 9.7, 320: 13.1 and 11.2;
+// bf16 of 2001, 16 a token: 96 tokens 9.0 and 10.3, 128: 11.3 and 10.7).
+inline int combine_grad_routes(int64_t pairs, bool vec) { return pairs < (vec ? 3500 : 1800) ? 1 : 8; }
+
 // Rows of x per work item: up to 4 for the decode kernel, which stages them in LDS; up to 16
 // for the kernel of few rows, which reads them from L2; up to 128 for the GEMM (64 where
 // it keeps a second set of sums).
