@@ -287,10 +287,15 @@ class Q4Layer:
     """A layer of 4-bit experts: `gate_up` a gated stack [E, 2 * inter, hidden],
     `down` a stack [E, hidden, inter], `shared` the shared expert's two (stacks of
     one), if the layer has one.  Context.moe and Context.moe_layer take it in
-    place of a Layer, and so does moe_dispatch.LocalNode."""
+    place of a Layer, and so does moe_dispatch.LocalNode.
+
+    `experts`: the ids of the layer's experts that the stacks hold, in their order,
+    of n_experts in all (one more than the largest); by default 0 .. E - 1.  A route to
+    another expert is left out and reported by Context.sync."""
 
     def __init__(self, ctx: "Context", gate_up: Q4Matrix, down: Q4Matrix,
-                 shared: Optional[tuple[Q4Matrix, Q4Matrix]] = None):
+                 shared: Optional[tuple[Q4Matrix, Q4Matrix]] = None, *,
+                 experts: Optional[Sequence[int]] = None, n_experts: Optional[int] = None):
         g, d = gate_up.desc, down.desc
         if not g.gated or d.gated or g.n_mats != d.n_mats or g.rows != 2 * d.cols or g.cols != d.rows:
             raise ValueError("a layer's matrices must be gated [E, 2 * inter, hidden] and [E, hidden, inter]")
@@ -302,8 +307,21 @@ class Q4Layer:
             raise ValueError("a layer's matrices must be on its context's device")
         self.ctx = ctx
         self.gate_up, self.down, self.shared = gate_up, down, shared
-        self.n_experts, self.hidden, self.inter = g.n_mats, d.rows, d.cols
-        self.experts = [self] * self.n_experts  # every expert of the stack is resident
+        held = list(range(g.n_mats)) if experts is None else [int(e) for e in experts]
+        self.n_experts = max(held) + 1 if n_experts is None and held else n_experts or 0
+        if len(held) != g.n_mats or len(set(held)) != len(held) or min(held) < 0 or max(held) >= self.n_experts:
+            raise ValueError(f"experts must be {g.n_mats} different ids below n_experts")
+        self.hidden, self.inter = d.rows, d.cols
+        self.experts = [None] * self.n_experts  # entry i: who holds expert i here
+        for e in held:
+            self.experts[e] = self
+        # slot in the stacks by id + 1: -1 for no route, one past the stacks for an expert that they do not hold
+        self._slots = None
+        if held != list(range(self.n_experts)):
+            slots = [-1] + [g.n_mats] * (self.n_experts + 1)
+            for i, e in enumerate(held):
+                slots[e + 1] = i
+            self._slots = torch.tensor(slots, dtype=torch.int32, device="cpu" if ctx.device < 0 else f"cuda:{ctx.device}")
         self._scratch: dict = {}  # sizes by tokens and top_k
 
 
@@ -552,6 +570,8 @@ class Context:
         T, K = x.shape[0], topk_ids.shape[1] if topk_ids.dim() == 2 else -1
         if topk_ids.shape != (T, K) or topk_w.shape != (T, K):
             raise ValueError(f"routes must be [{T}, top_k]")
+        if layer._slots is not None:
+            topk_ids = layer._slots[topk_ids.clamp(-1, layer.n_experts).long() + 1]
         gu, dn = C.byref(layer.gate_up.desc), C.byref(layer.down.desc)
         sg, sd = (C.byref(m.desc) for m in layer.shared) if layer.shared else (None, None)
         size = layer._scratch.get((T, K))

@@ -63,7 +63,8 @@ class LocalNode:
 
     layers: layer id -> engine.Layer whose entry i is the layer's local
     expert i (None where not resident here) and whose shared expert, when
-    present, is the layer's shared expert."""
+    present, is the layer's shared expert; or an engine.Q4Layer, whose
+    `experts` say which of the layer's its stacks hold."""
 
     def __init__(self, layers: dict[int, engine.Layer], device: int = 0):
         self.layers = dict(layers)
