@@ -447,10 +447,10 @@ class Context:
         pairs t * K + k sorted by expert (cx_sort_tokens).  ids: any integer type."""
         self._here(ids)
         T, K = _rows_2d(ids)
-        if ids.dtype not in (torch.int32, torch.int64, torch.int16, torch.int8, torch.uint8):
+        if ids.dtype == torch.bool or ids.is_floating_point() or ids.is_complex():
             raise TypeError(f"ids must be integers, not {ids.dtype}")
-        if ids.dtype == torch.int64:  # what does not fit 32 bits names no expert, and must not become one that does
-            ids = ids.clamp(-1, 2 ** 31 - 1)
+        if ids.element_size() >= 4 and ids.dtype != torch.int32:  # what does not fit 32 bits names no expert, and must not become one that does
+            ids = ids.to(torch.int64).clamp(-1, 2 ** 31 - 1)
         ids = ids.to(torch.int32).contiguous()
         order = torch.empty(T * K, dtype=torch.int32, device=ids.device)
         offsets = torch.empty(n_experts + 1, dtype=torch.int32, device=ids.device)

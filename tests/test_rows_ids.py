@@ -27,13 +27,13 @@ def test_ids_past_32_bits_name_no_expert(ctx, seen):  # noqa: F811
     assert seen[0] == [3, 2 ** 31 - 1, -1, -1, 2 ** 31 - 1, 7]
 
 
-@pytest.mark.parametrize("dtype", [torch.int32, torch.int16, torch.int8, torch.uint8])
+@pytest.mark.parametrize("dtype", [torch.int32, torch.int16, torch.int8, torch.uint8, torch.uint16, torch.uint32, torch.uint64, torch.int64])
 def test_smaller_integers(ctx, seen, dtype):  # noqa: F811
     ctx.sort_tokens(torch.tensor([[3, 120]]).to(dtype), 8)
     assert seen[0] == [3, 120]
 
 
-@pytest.mark.parametrize("dtype", [torch.float32, torch.bool, torch.bfloat16, torch.uint32, torch.uint64])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bool, torch.bfloat16, torch.complex64])
 def test_other_types_are_refused(ctx, seen, dtype):  # noqa: F811
     with pytest.raises(TypeError, match="ids must be integers"):
         ctx.sort_tokens(torch.ones(2, 2).to(dtype), 8)
