@@ -86,3 +86,29 @@ def test_an_infinite_h_stays_in_its_token(gpu, T, I):
     finally:
         for m in mats:
             m.free()
+
+
+def test_h_of_more_than_4_gb(gpu):
+    """Places in h past 32 bits: the last rows of a call whose h in two planes takes 4.4 GB."""
+    from constellation_amd.engine import Q4Layer, Q4Matrix
+    from test_gpu_q4 import dense, layer_ref, make, rounded
+    T, K, E, H, I = 67_000, 8, 9, 64, 2048
+    print(f"[q4 h] {T}x{K} of {E} {H}x{I}", flush=True)
+    gu, dn = make(1, E, 2 * I, H, 64), make(2, E, H, I, 128)
+    mats = [Q4Matrix.pack(gu[0].cuda(), gu[1].cuda(), H, group=64, gated=True), Q4Matrix.pack(dn[0].cuda(), dn[1].cuda(), I)]
+    try:
+        layer = Q4Layer(gpu, *mats)
+        x = torch.randn(T, H, device="cuda", generator=torch.Generator("cuda").manual_seed(1)).to(BF)
+        ids = torch.rand(T, E, device="cuda", generator=torch.Generator("cuda").manual_seed(2)).topk(K, dim=1).indices.to(torch.int32)
+        w = torch.rand(T, K, device="cuda", generator=torch.Generator("cuda").manual_seed(3))
+        y, yf = gpu.moe(layer, x, ids, w, want_f32=True)
+        torch.cuda.synchronize()
+        gpu.sync()
+        some = torch.cat((torch.arange(8), torch.arange(T - 24, T), torch.randperm(T, generator=torch.Generator().manual_seed(4))[:16]))
+        want, tol = layer_ref(x.cpu().double()[some], ids.cpu()[some], w.cpu()[some], dense(*gu, H, 64), dense(*dn, I, 128), 2.0 ** -22)
+        near(yf.cpu()[some], want, tol, "fp32")
+        near(y.cpu()[some], want, rounded(want, tol, BF), "rounded")
+    finally:
+        torch.cuda.synchronize()
+        for m in mats:
+            m.free()
