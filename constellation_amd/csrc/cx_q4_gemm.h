@@ -142,9 +142,9 @@ __device__ __forceinline__ void q4_gemm_store(const Q4GemmArgs& L, const f32x4 (
 // sums costs a multiply-add per MFMA and 4 values, and half the rows per conversion: 3001
 // rows by 7168 x 2048 in 101 to 116 us, 0.8 to 0.87 PFLOP/s (128 rows and one workgroup a CU: 8 % slower).
 //
-// PL (fp32 rows of x, the h of a layer, as two fp16 planes; row p of x is row p of y): a buffer holds 64 columns, 8 pieces of a row's first
-// plane and the 8 of its second, so that a buffer and a turn have as many MFMAs as without planes
-// and a conversion serves both planes of all rows.
+// PL (fp32 rows of x, the h of a layer, as two fp16 planes; row p of x is row p of y): a buffer holds 64
+// columns, 8 pieces of a row's first plane and the 8 of its second, so that a buffer and a turn have
+// as many MFMAs as without planes and a conversion serves both planes of all rows.
 template <int NG, int RTW, int NT, bool XS, bool PL>
 __device__ __forceinline__ void q4_gemm_tile(const Q4GemmArgs& L, unsigned char* lds0, unsigned char* lds1, const cx_q4_desc& w,
                                              size_t mat, int rb, int ks, int begin, int rows) {
@@ -169,7 +169,7 @@ __device__ __forceinline__ void q4_gemm_tile(const Q4GemmArgs& L, unsigned char*
     const uint16_t* sp = w.scales + tile0 * 16 * NG;
     // Loads of a lane's 32-bit place and a scalar one, with planes of the item's own rows: of 64-bit places in each lane
     // the compiler spilled (with planes 599 us for the down products below, 439 without spills; gate/up 492 and 472).
-    // e4m3 rows, whose launch bounds leave registers, take plain loads (118 us as above, 116).
+    // e4m3 rows, whose items of 64 rows leave registers, take plain loads (3001 rows by 7168 x 2048: 116 us, 118 with these).
     const __amdgpu_buffer_rsrc_t rx = make_rsrc(reinterpret_cast<const char*>(L.x) + (PL ? (size_t)begin * pitch : 0), (PL ? (uint32_t)rows : (uint32_t)L.n_x) * pitch);
     const __amdgpu_buffer_rsrc_t rw = make_rsrc(wp, (uint32_t)(rts * KT) * kQ4Tile), rs = make_rsrc(sp, (uint32_t)(rts * KT) * 32 * NG);
     // of a fetch, which is a column tile or, with planes, half of one: the lane's codes, and its row's scales

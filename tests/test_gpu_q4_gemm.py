@@ -189,3 +189,25 @@ def test_layers(gpu, T, K, E, H, I, shared, dtype):
     finally:
         for m in mats:
             m.free()
+
+
+@pytest.mark.parametrize("dtype", [BF, HF])
+def test_rows_up_to_the_last_place_in_32_bits(gpu, dtype):
+    """299,000 rows of 7168, whose places in x end just below 4 GB."""
+    from constellation_amd.engine import Q4Matrix
+    T, N, K = 299_000, 24, 7168
+    print(f"[q4 gemm] {T}x{K} by {N} {dtype}", flush=True)
+    codes, scales = make(1, 1, N, K, 128)
+    w = Q4Matrix.pack(codes.cuda(), scales.cuda(), K)
+    try:
+        x = torch.empty(T, K, dtype=dtype, device="cuda")
+        x[:] = torch.randn(1000, K, device="cuda", generator=torch.Generator("cuda").manual_seed(1)).to(dtype).repeat(T // 1000, 1)
+        some = torch.cat((torch.arange(2), torch.arange(T // 2 - 3, T // 2 + 3), torch.arange(T - 20, T)))
+        x[some.cuda()] = rand(2, some.numel(), K, dtype=dtype).cuda()  # rows that are found nowhere else
+        y = gpu.q4_matmul(w, x)
+        torch.cuda.synchronize()
+        want, e = product_ref(x[some.cuda()].cpu().double(), dense(codes, scales, K, 128)[0], False)
+        near(y.cpu()[some], want, rounded(want, e, dtype), dtype)
+    finally:
+        torch.cuda.synchronize()
+        w.free()
