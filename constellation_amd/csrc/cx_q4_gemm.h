@@ -167,9 +167,11 @@ __device__ __forceinline__ void q4_gemm_tile(const Q4GemmArgs& L, unsigned char*
     const size_t tile0 = (mat * L.RT + rt0) * (size_t)KT;
     const uint8_t* wp = w.codes + tile0 * kQ4Tile;
     const uint16_t* sp = w.scales + tile0 * 16 * NG;
-    // Loads of a lane's 32-bit place and a scalar one, with planes of the item's own rows: of 64-bit places in each lane
-    // the compiler spilled (with planes 599 us for the down products below, 439 without spills; gate/up 492 and 472).
-    // e4m3 rows, whose items of 64 rows leave registers, take plain loads (3001 rows by 7168 x 2048: 116 us, 118 with these).
+    // kBounded: loads of a lane's 32-bit place and a scalar one, with planes of the item's own rows, where the compiler
+    // spills otherwise: with planes (down products of 1024 tokens over 64 experts 439 us, 599 with plain loads) and with
+    // the four scales of groups of 32 (1024 rows by 4096 x 7168: 74.6 us, 84.9). The others are faster with plain loads
+    // (4096 rows by 4096 x 7168, groups of 64 and 128: 192 and 193 us, 199 bounded; e4m3, 3001 rows by 7168 x 2048: 108.4, 110.8).
+    constexpr bool kBounded = PL || (NG == 4 && !XS);
     const __amdgpu_buffer_rsrc_t rx = make_rsrc(reinterpret_cast<const char*>(L.x) + (PL ? (size_t)begin * pitch : 0), (PL ? (uint32_t)rows : (uint32_t)L.n_x) * pitch);
     const __amdgpu_buffer_rsrc_t rw = make_rsrc(wp, (uint32_t)(rts * KT) * kQ4Tile), rs = make_rsrc(sp, (uint32_t)(rts * KT) * 32 * NG);
     // of a fetch, which is a column tile or, with planes, half of one: the lane's codes, and its row's scales
@@ -191,7 +193,7 @@ __device__ __forceinline__ void q4_gemm_tile(const Q4GemmArgs& L, unsigned char*
 #pragma unroll
         for (int i = 0; i < NT; ++i) {
             const auto at = (__attribute__((address_space(3))) void*)(buf + i * 4096 + wave * 1024);
-            if constexpr (!XS)
+            if constexpr (kBounded)
                 __builtin_amdgcn_raw_ptr_buffer_load_lds(rx, at, 16, xoff[i], part * 256, 0, 0);
             else
                 __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(reinterpret_cast<const char*>(L.x) + (size_t)part * 256 + xoff[i]), at, 16, 0, 0);
@@ -199,7 +201,7 @@ __device__ __forceinline__ void q4_gemm_tile(const Q4GemmArgs& L, unsigned char*
 #pragma unroll
         for (int m = 0; m < RTW; ++m) {
             const int tile = min(m, rts - 1) * KT + (PL ? part >> 1 : part);
-            if constexpr (XS) {
+            if constexpr (!kBounded) {
                 a[to][m] = ld16(wp + (size_t)tile * kQ4Tile + (uint32_t)lane * 16);
                 if constexpr (NG == 1)
                     s[to][m].d[0] = (sp + (size_t)tile * 16)[(uint32_t)t];
