@@ -35,7 +35,7 @@ constexpr int kQ4GemmWaves = 4;
 //
 // What bounds it: issue.  Beside an MFMA of 16 cycles a wave converts codes (a pack of two codes and
 // a product with the scale for every two weights), reads a fragment of x and waits its turn; with
-// 8 tiles of rows to a conversion and two workgroups a CU the matrix cores are busy 69 % of the time
+// 8 tiles of rows to a conversion and two workgroups a CU the matrix cores are busy 71 % of the time
 // (4096 rows by 4096 x 7168: 192 us, 1.25 PFLOP/s; a library's bf16 product reaches 1.43 on
 // this card).  Fewer rows per item amortise a conversion less: 1024 tokens over 64 experts, gate/up 472
 // us and 63 %; the down product, whose h is two planes on one conversion, 439 us and 67 %.  Steps that led here,
@@ -144,7 +144,9 @@ __device__ __forceinline__ void q4_gemm_store(const Q4GemmArgs& L, const f32x4 (
 //
 // PL (fp32 rows of x, the h of a layer, as two fp16 planes; row p of x is row p of y): a buffer holds 64
 // columns, 8 pieces of a row's first plane and the 8 of its second, so that a buffer and a turn have
-// as many MFMAs as without planes and a conversion serves both planes of all rows.
+// as many MFMAs as without planes and a conversion serves both planes of all rows.  Items of up to 64 rows, whose
+// weights bound them, have a whole column tile of both planes in a buffer instead, and half the turns (16 and 128
+// tokens over 64 experts 342 and 357 us, in halves 349 and 375).
 template <int NG, int RTW, int NT, bool XS, bool PL>
 __device__ __forceinline__ void q4_gemm_tile(const Q4GemmArgs& L, unsigned char* lds0, unsigned char* lds1, const cx_q4_desc& w,
                                              size_t mat, int rb, int ks, int begin, int rows) {
@@ -154,6 +156,8 @@ __device__ __forceinline__ void q4_gemm_tile(const Q4GemmArgs& L, unsigned char*
     // row r gets the row's piece s ^ (r % 16), so that the 16 rows of a fragment lie in
     // 16 different places of the banks.
     const int tr = threadIdx.x >> 4, piece = (threadIdx.x & 15) ^ tr;
+    constexpr bool kHalf = PL && NT > 4;         // a fetch is half a column tile
+    constexpr int kPieces = PL && !kHalf ? 2 : 1;  // 256-byte pieces of a row in a fetch
     const uint32_t pitch = (uint32_t)L.padded * 2;
     uint32_t xoff[NT];  // in bytes; rows that do not exist read another and are never stored
 #pragma unroll
@@ -174,10 +178,10 @@ __device__ __forceinline__ void q4_gemm_tile(const Q4GemmArgs& L, unsigned char*
     constexpr bool kBounded = PL || (NG == 4 && !XS);
     const __amdgpu_buffer_rsrc_t rx = make_rsrc(reinterpret_cast<const char*>(L.x) + (PL ? (size_t)begin * pitch : 0), (PL ? (uint32_t)rows : (uint32_t)L.n_x) * pitch);
     const __amdgpu_buffer_rsrc_t rw = make_rsrc(wp, (uint32_t)(rts * KT) * kQ4Tile), rs = make_rsrc(sp, (uint32_t)(rts * KT) * 32 * NG);
-    // of a fetch, which is a column tile or, with planes, half of one: the lane's codes, and its row's scales
-    typedef uint32_t Codes __attribute__((ext_vector_type(PL ? 2 : 4)));
+    // of a fetch: the lane's codes, and its row's scales
+    typedef uint32_t Codes __attribute__((ext_vector_type(kHalf ? 2 : 4)));
     struct Sc {
-        uint32_t d[PL ? 1 : (NG + 1) / 2];
+        uint32_t d[kHalf ? 1 : (NG + 1) / 2];
     };
     f32x4 acc[NT][RTW] = {}, sum[XS ? NT : 1][RTW] = {};
     Codes a[2][RTW];
@@ -189,18 +193,18 @@ __device__ __forceinline__ void q4_gemm_tile(const Q4GemmArgs& L, unsigned char*
         if (L.order != nullptr) xr = max(L.order[xr], 0) / L.top_k;
         xso = (uint32_t)(xr < L.n_x ? xr : 0) * (uint32_t)KT;
     }
-    auto fetch = [&](int part, auto to, unsigned char* buf) {  // part: column tile, with planes its half `to`
+    auto fetch = [&](int part, auto to, unsigned char* buf) {  // part: column tile (kHalf: its half `to`)
 #pragma unroll
-        for (int i = 0; i < NT; ++i) {
+        for (int i = 0; i < NT * kPieces; ++i) {
             const auto at = (__attribute__((address_space(3))) void*)(buf + i * 4096 + wave * 1024);
             if constexpr (kBounded)
-                __builtin_amdgcn_raw_ptr_buffer_load_lds(rx, at, 16, xoff[i], part * 256, 0, 0);
+                __builtin_amdgcn_raw_ptr_buffer_load_lds(rx, at, 16, xoff[i % NT], (part * kPieces + i / NT) * 256, 0, 0);
             else
                 __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(reinterpret_cast<const char*>(L.x) + (size_t)part * 256 + xoff[i]), at, 16, 0, 0);
         }
 #pragma unroll
         for (int m = 0; m < RTW; ++m) {
-            const int tile = min(m, rts - 1) * KT + (PL ? part >> 1 : part);
+            const int tile = min(m, rts - 1) * KT + (kHalf ? part >> 1 : part);
             if constexpr (!kBounded) {
                 a[to][m] = ld16(wp + (size_t)tile * kQ4Tile + (uint32_t)lane * 16);
                 if constexpr (NG == 1)
@@ -209,13 +213,13 @@ __device__ __forceinline__ void q4_gemm_tile(const Q4GemmArgs& L, unsigned char*
                     s[to][m] = *reinterpret_cast<const Sc*>(sp + (size_t)tile * 16 * NG + (uint32_t)t * NG);
                 continue;
             }
-            if constexpr (PL)
+            if constexpr (kHalf)
                 a[to][m] = __builtin_bit_cast(Codes, __builtin_amdgcn_raw_buffer_load_b64(rw, lane * 16 + to * 8, tile * kQ4Tile, 0));
             else
                 a[to][m] = __builtin_bit_cast(Codes, __builtin_amdgcn_raw_buffer_load_b128(rw, lane * 16, tile * kQ4Tile, 0));
             if constexpr (NG == 1)
                 s[to][m].d[0] = __builtin_amdgcn_raw_buffer_load_b16(rs, t * 2, tile * 32, 0);
-            else if constexpr (NG == 2 || PL)  // the tile's two scales, with planes its half's two of four
+            else if constexpr (NG == 2 || kHalf)  // the tile's two scales, or its half's two of four
                 s[to][m].d[0] = __builtin_amdgcn_raw_buffer_load_b32(rs, t * 2 * NG + (NG == 4 ? to * 4 : 0), tile * 32 * NG, 0);
             else
                 s[to][m] = __builtin_bit_cast(Sc, __builtin_amdgcn_raw_buffer_load_b64(rs, t * 8, tile * 128, 0));
@@ -240,17 +244,17 @@ __device__ __forceinline__ void q4_gemm_tile(const Q4GemmArgs& L, unsigned char*
         // Steps of RTW MFMAs on one fragment of x, in this order: the fragment after the
         // next is read and the next columns' weights are converted while they run.
         const unsigned char* in = buf + t * 256;
-        constexpr int kSteps = 4 * NT, kOf = PL ? 2 * NT : NT;  // steps that share a conversion: those of all rows, with planes of both
+        constexpr int kSteps = 4 * NT * kPieces, kOf = PL ? 2 * NT : NT;  // steps that share a conversion: those of all rows, with planes of both
         f16x8 fa[2][RTW];
         u32x4 b[3];
         auto convert = [&](int j, int m) {  // of the fetch's columns 32 j .. + 31
-            const int g = (PL ? from * 2 + j : j) * NG / 4 - (PL && NG == 4 ? from * 2 : 0);
+            const int g = (kHalf ? from * 2 + j : j) * NG / 4 - (kHalf && NG == 4 ? from * 2 : 0);
             const _Float16 sc = __builtin_bit_cast(f16x2, s[from][m].d[g / 2])[g % 2];
             fa[j & 1][m] = q4_f16(a[from][m][j]) * f16x8{sc, sc, sc, sc, sc, sc, sc, sc};
         };
         auto read = [&](int i) {
-            const int j = i / kOf, plane = i % kOf / NT;
-            b[i % 3] = *reinterpret_cast<const u32x4*>(in + i % NT * 4096 + ((((plane * 2 + j) * 4 + q) ^ t) * 16));
+            const int j = i / kOf, plane = i % kOf / NT, piece = PL ? plane * 2 + j % 2 : j;
+            b[i % 3] = *reinterpret_cast<const u32x4*>(in + ((PL ? j / 2 * NT : 0) + i % NT) * 4096 + (((piece * 4 + q) ^ t) * 16));
         };
         read(0);
         read(1);
@@ -281,15 +285,15 @@ __device__ __forceinline__ void q4_gemm_tile(const Q4GemmArgs& L, unsigned char*
     };
     constexpr std::integral_constant<int, 0> even{};
     constexpr std::integral_constant<int, 1> odd{};
-    constexpr int kParts = PL ? 2 : 1;  // of a column tile
+    constexpr int kParts = kHalf ? 2 : 1;  // of a column tile
     const int per = (KT + L.splits - 1) / L.splits, k0 = ks * per * kParts, k1 = min(KT * kParts, k0 + per * kParts);
     if (k0 < k1) fetch(k0, even, lds0);
     q4_gemm_turn();
     for (int k = k0; k < k1; k += 2) {
-        if (PL || k + 1 < k1) fetch(k + 1, odd, lds1);
+        if (kHalf || k + 1 < k1) fetch(k + 1, odd, lds1);
         multiply(even, lds0);
         q4_gemm_turn();
-        if (!PL && k + 1 >= k1) break;
+        if (!kHalf && k + 1 >= k1) break;
         if (k + 2 < k1) fetch(k + 2, even, lds0);
         multiply(odd, lds1);
         q4_gemm_turn();
