@@ -85,7 +85,8 @@ __device__ __forceinline__ void q4_store(const Q4Launch& L, size_t at, float v) 
 }
 
 // Up to 16 rows of x against RW row tiles of weights per wave: the kernel streams a matrix's
-// weights once per item, and with one row HBM bounds it (18432 x 7168: 70 MB in 22.8 us, 3.1 TB/s; 4096 x
+// weights once per item.  With one row the latency of its loads bounds it, of weights and of x from L2 (18432 x
+// 7168: 70 MB in 22.8 us, 3.1 of the 5 TB/s that the decode kernel reaches on more matrices; 4096 x
 // 7168 in 7.2, of which a launch's ramp and the reduction are half), with 16 the reads of x, as many
 // bytes as four times the weights' codes over RW, from L2 (32 and 11.7 us).  Products are of the bf16
 // (fp16) x as it is with the codes, exact; the scales come to the fp32 sums of their group.
