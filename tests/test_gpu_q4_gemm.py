@@ -211,3 +211,28 @@ def test_rows_up_to_the_last_place_in_32_bits(gpu, dtype):
     finally:
         torch.cuda.synchronize()
         w.free()
+
+
+@pytest.mark.parametrize("dtype,group", [(BF, 32), (HF, 64), (F8, 128)])
+@pytest.mark.parametrize("P,n_x,N,K", [(3, 40, 48, 256), (4, 2, 64, 1030), (16, 5, 48, 512), (70, 9, 50, 264), (33, 200, 40, 1025), (300, 31, 48, 1100)])
+def test_order_of_one_matrix(gpu, P, n_x, N, K, dtype, group):
+    """Rows of one matrix's product by an order alone: some twice, some never, some that are not there."""
+    from constellation_amd.engine import Q4Matrix
+    print(f"[q4 gemm] order of one {P} from {n_x} {N}x{K} {dtype}", flush=True)
+    codes, scales = make(P, 1, N, K, group)
+    w = Q4Matrix.pack(codes.cuda(), scales.cuda(), K, group=group)
+    try:
+        x, xs, x64 = make_x(3, n_x, K, dtype)
+        g = torch.Generator().manual_seed(P)
+        for top_k in (1, 5):
+            order = torch.randint(0, n_x * top_k, (P,), generator=g)
+            order[0], order[-1] = -1 - order[0], n_x * top_k
+            src = torch.where(order < 0, n_x, order // top_k).clamp(max=n_x)
+            rows = torch.cat((x64, torch.zeros(1, K, dtype=torch.float64)))[src]
+            want, e = product_ref(rows, dense(codes, scales, K, group)[0], False)
+            y = gpu.q4_matmul(w, x.cuda(), x_scale=None if xs is None else xs.cuda(), order=order.to(torch.int32).cuda(), top_k=top_k, out_dtype=SF)
+            torch.cuda.synchronize()
+            near(y, want, 2 * e + TINY[SF], top_k)
+            assert not y[0].any() and not y[-1].any()
+    finally:
+        w.free()
