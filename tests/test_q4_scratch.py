@@ -41,7 +41,7 @@ def rules(tmp_path_factory):
 
 
 SIZES = sorted({1, 2, 3, 4, 5, 8, 15, 16, 17, 31, 32, 33, 48, 63, 64, 65, 66, 80, 96, 112, 127, 128, 129, 130, 256, 257, 448, 497, 498, 640, 641,
-                1023, 1024, 1025, 1280, 1281, 1536, 2047, 2048, 2049, 3072, 3073, 4096, 6110, 6111, 6112, 8192, 20000, 1 << 17,
+                1023, 1024, 1025, 1280, 1281, 1536, 2047, 2048, 2049, 2999, 3000, 4096, 6110, 6111, 6112, 8192, 20000, 1 << 17,
                 *range(150, 1500, 53), *range(1500, 12000, 331)})
 
 
