@@ -236,3 +236,28 @@ def test_order_of_one_matrix(gpu, P, n_x, N, K, dtype, group):
             assert not y[0].any() and not y[-1].any()
     finally:
         w.free()
+
+
+def test_scratch_of_the_largest_call_serves_smaller_ones(gpu):
+    """One allocation of what the largest call asks for, at its exact size, under calls of every kernel."""
+    import ctypes as C
+    from constellation_amd._lib import BF16, F32, check, lib
+    from constellation_amd.engine import Q4Matrix
+    print("[q4 gemm] one scratch", flush=True)
+    N, K, most = 7168, 2048, 4096
+    codes, scales = make(1, 1, N, K, 128)
+    w = Q4Matrix.pack(codes.cuda(), scales.cuda(), K)
+    try:
+        size = lib().cx_q4_scratch(C.byref(w.desc), BF16, most, most, 0)
+        scratch = torch.empty(size, dtype=torch.uint8, device="cuda")
+        x = rand(1, most, K, dtype=BF).cuda()
+        for T in (most, 497, 448, 130, 64, 1):
+            want = gpu.q4_matmul(w, x[:T], out_dtype=SF)
+            y = torch.empty(T, N, device="cuda")
+            check(lib().cx_q4_matmul(gpu.handle, C.byref(w.desc), x.data_ptr(), BF16, None, T, None, 1, None, T, y.data_ptr(), F32,
+                                     scratch.data_ptr(), size, gpu.stream()))
+            torch.cuda.synchronize()
+            assert torch.equal(y, want), T
+    finally:
+        torch.cuda.synchronize()
+        w.free()
