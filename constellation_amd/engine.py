@@ -49,6 +49,10 @@ def _check_pairs(rows: int, n_tokens: int, top_k: int, weights: Optional[torch.T
         raise ValueError(f"weights must be fp32 [{n_tokens}, {top_k}]")
 
 
+def _device(index: int) -> torch.device:
+    return torch.device("cuda", index)
+
+
 def _outside_autograd(name: str, gradient: str, *tensors: Optional[torch.Tensor]) -> None:
     """A result without a graph must not pass for one with it."""
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
@@ -321,7 +325,7 @@ class Q4Layer:
             slots = [-1] + [g.n_mats] * (self.n_experts + 1)
             for i, e in enumerate(held):
                 slots[e + 1] = i
-            self._slots = torch.tensor(slots, dtype=torch.int32, device="cpu" if ctx.device < 0 else f"cuda:{ctx.device}")
+            self._slots = torch.tensor(slots, dtype=torch.int32, device=_device(ctx.device))
         self._scratch: dict = {}  # sizes by tokens and top_k
 
 
@@ -670,7 +674,7 @@ class Context:
 
     # -- synthetic data ------------------------------------------------------
     def gen_normal(self, seed: int, stream_id: int, shape, std: float, dtype: torch.dtype):
-        t = torch.empty(shape, dtype=dtype, device=f"cuda:{self.device}")
+        t = torch.empty(shape, dtype=dtype, device=_device(self.device))
         check(lib().cx_gen_normal(self.handle, seed, stream_id, t.numel(), std, cx_dtype(dtype),
                                   t.data_ptr(), self.stream()))
         return t

@@ -35,6 +35,7 @@ def matrix(n, rows, cols, gated, device=-1):
 def ctx(monkeypatch):
     monkeypatch.setattr(engine, "lib", lambda: NoLibrary())
     monkeypatch.setattr(engine, "_stream", lambda device: 0)
+    monkeypatch.setattr(engine, "_device", lambda index: torch.device("cpu"))
     c = engine.Context.__new__(engine.Context)
     c.device, c.handle = -1, 1
     return c
