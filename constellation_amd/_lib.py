@@ -121,6 +121,13 @@ _SIGS = {
     "cx_q4_moe_scratch": (C.c_size_t, [C.POINTER(Q4Desc), C.POINTER(Q4Desc), _I, _I, _I]),
     "cx_q4_moe": (_I, [_P, C.POINTER(Q4Desc), C.POINTER(Q4Desc), C.POINTER(Q4Desc),
                        C.POINTER(Q4Desc), _P, _I, _I, _P, _P, _I, _P, _I, _P, _P, C.c_size_t, _P]),
+    "cx_matmul_scratch": (C.c_size_t, [_I, _I, _I, _I, _I, _I, _I]),
+    "cx_matmul": (_I, [_P, _P, _I, _P, _I, _I, _I, _I, _I, _P, _I, _P, _I, _P, _I, _P, _P, C.c_size_t, _P]),
+    "cx_matmul_grad_scratch": (C.c_size_t, [_I, _I, _I, _I, _I, _I, _I, _I, _I]),
+    "cx_matmul_grad": (_I, [_P, _P, _P, _P, _I, _P, _I, _I, _I, _P, _I, _P, _P, _I, _P, C.c_size_t, _P]),
+    "cx_quantize_i8": (_I, [_P, _P, _I, _I, _I, _P, _P, _P]),
+    "cx_i8_matmul_scratch": (C.c_size_t, [_I, _I, _I, _I, _I, _I]),
+    "cx_i8_matmul": (_I, [_P, _P, _P, _I, _P, _P, _I, _I, _I, _I, _P, _I, _P, _I, _P, _I, _P, C.c_size_t, _P]),
     "cx_gen_fp8_matrix": (_I, [_P, C.c_uint64, C.c_uint64, _I, _I, _I, _I, C.c_float, _P, _P,
                                _P]),
     "cx_gen_normal": (_I, [_P, C.c_uint64, C.c_uint64, C.c_uint64, C.c_float, _I, _P, _P]),

@@ -32,6 +32,9 @@ SOURCES = {
     "cx_runtime.hip": [],
     "cx_expert.hip": [],
     "cx_few.hip": [],
+    "cx_i8.hip": [],
+    "cx_mm.hip": [],
+    "cx_mm_grad.hip": [],
     "cx_pp.hip": [],
     "cx_q4.hip": [],
     "cx_q4_dec.hip": [],

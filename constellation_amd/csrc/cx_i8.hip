@@ -1,0 +1,121 @@
+// cx_i8.hip — rows to 8-bit integers with a scale each, and products of such rows with
+// 8-bit weights: y[p, n] = xs[p] ws[n] sum over k of x[p, k] w[n, k], the sum exact in 32 bits.
+#include "cx_mm.h"
+
+namespace cx {
+namespace {
+
+using Big = MmShape<2, 4, 4, 2>;
+using Small = MmShape<2, 2, 2, 2>;
+
+template <class S, bool GATED, bool DMA>
+hipError_t run(MmLaunch& L, hipStream_t s) {
+    const int out = GATED ? S::BM / 2 : S::BM, width = GATED ? L.rows / 2 : L.rows;
+    L.m_tiles = (width + out - 1) / out;
+    cx_launch(k_mm<MmI8, S, GATED, DMA>, dim3(mm_grid(L, S::BN)), dim3(S::kThreads), 0, s, L);
+    return hipGetLastError();
+}
+
+template <bool GATED>
+hipError_t pick(MmLaunch& L, hipStream_t s) {
+    if (L.cols % 16 != 0 || !mm_at16(L.x) || !mm_at16(L.w)) return run<Small, GATED, false>(L, s);
+    return mm_big(L.n_rows, L.offsets ? L.n_mats : 1, L.rows) ? run<Big, GATED, true>(L, s) : run<Small, GATED, true>(L, s);
+}
+
+constexpr int kI8Threads = 256, kI8Held = 4;  // pieces of 8 values of a row that a thread holds
+
+__device__ __forceinline__ void i8_piece(const void* x, int type, size_t at, int left, bool vec, float (&v)[8]) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = 0.0f;
+    if (left <= 0) return;
+    if (type == CX_DTYPE_F32) {
+        const float* p = static_cast<const float*>(x) + at;
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            if (i < left) v[i] = p[i];
+        return;
+    }
+    const uint16_t* p = static_cast<const uint16_t*>(x) + at;
+    uint32_t h[8] = {};
+    if (vec) {
+        const u32x4 d = ld16(p);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) h[i] = i & 1 ? d[i >> 1] >> 16 : d[i >> 1] & 0xFFFFu;
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            if (i < left) h[i] = p[i];
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+        v[i] = type == CX_DTYPE_BF16 ? __uint_as_float(h[i] << 16) : (float)__builtin_bit_cast(_Float16, (uint16_t)h[i]);
+}
+
+// A row per workgroup: its largest size, then codes from correctly rounded quotients.
+__global__ __launch_bounds__(kI8Threads) void k_quantize_i8(const void* x, int type, int cols, int8_t* q, float* scale) {
+    __shared__ uint32_t part[kI8Threads / 64];
+    constexpr int kSpan = kI8Held * kI8Threads * 8;
+    const int tid = threadIdx.x;
+    const size_t row = (size_t)blockIdx.x * cols;
+    const bool vec = cols % 8 == 0 && (reinterpret_cast<uintptr_t>(x) & 15) == 0, wide = cols % 8 == 0 && (reinterpret_cast<uintptr_t>(q) & 7) == 0;
+    float v[kI8Held][8];
+    uint32_t most = 0;  // as bits: of sizes the larger one has the larger bits, and a NaN is the largest
+    auto take = [&](const float (&f)[8]) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) most = max(most, __float_as_uint(f[i]) & 0x7FFFFFFFu);
+    };
+#pragma unroll
+    for (int i = 0; i < kI8Held; ++i) {
+        const int c = (i * kI8Threads + tid) * 8;
+        i8_piece(x, type, row + c, cols - c, vec, v[i]);
+        take(v[i]);
+    }
+    for (int c = kSpan + tid * 8; c < cols; c += kI8Threads * 8) {
+        float f[8];
+        i8_piece(x, type, row + c, cols - c, vec, f);
+        take(f);
+    }
+#pragma unroll
+    for (int m = 32; m >= 1; m >>= 1) most = max(most, (uint32_t)__shfl_xor((int)most, m));
+    if ((tid & 63) == 0) part[tid >> 6] = most;
+    __syncthreads();
+    most = max(max(part[0], part[1]), max(part[2], part[3]));
+    const float s = most > 0x7F800000u ? __uint_as_float(most) : fmaxf(__uint_as_float(most) / 127.0f, 1e-12f);
+    if (tid == 0) scale[blockIdx.x] = s;
+    auto put = [&](int c, const float (&f)[8]) {
+        uint32_t d[2] = {};
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const float r = rintf(f[i] / s);
+            d[i >> 2] |= ((uint32_t)(r == r ? (int)fminf(fmaxf(r, -127.0f), 127.0f) : 0) & 0xFFu) << (8 * (i & 3));
+        }
+        if (wide) {
+            *reinterpret_cast<uint2*>(q + row + c) = uint2{d[0], d[1]};
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                if (c + i < cols) q[row + c + i] = (int8_t)(d[i >> 2] >> (8 * (i & 3)));
+        }
+    };
+#pragma unroll
+    for (int i = 0; i < kI8Held; ++i) {
+        const int c = (i * kI8Threads + tid) * 8;
+        if (c < cols) put(c, v[i]);
+    }
+    for (int c = kSpan + tid * 8; c < cols; c += kI8Threads * 8) {
+        float f[8];
+        i8_piece(x, type, row + c, cols - c, vec, f);
+        put(c, f);
+    }
+}
+
+}  // namespace
+
+hipError_t launch_mm_i8(MmLaunch L, hipStream_t s) { return L.gated ? pick<true>(L, s) : pick<false>(L, s); }
+
+hipError_t launch_quantize_i8(const void* x, int x_type, int n_rows, int cols, int8_t* q, float* scale, hipStream_t s) {
+    cx_launch(k_quantize_i8, dim3((unsigned)n_rows), dim3(kI8Threads), 0, s, x, x_type, cols, q, scale);
+    return hipGetLastError();
+}
+
+}  // namespace cx

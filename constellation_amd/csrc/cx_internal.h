@@ -494,4 +494,52 @@ hipError_t launch_q4_gemm(const Q4Launch& L, hipStream_t s);
 bool q4_grid_ok(const Q4Launch& L);
 hipError_t launch_q4(const Q4Launch& L, hipStream_t s);
 
+// ---------------------------------------------------------------------------
+// Products with weights as the program holds them (cx_mm.hip, cx_mm_grad.hip, cx_i8.hip).
+constexpr int kMmI8 = 5;  // beside CX_DTYPE_FP16 and _BF16: 8-bit integers, scales per row of x and of the weights
+struct MmLaunch {
+    int type;
+    const void* w;           // [n_mats, rows, cols]
+    const void* x;           // [n_x, cols]
+    const void* dy;          // gradients: [n_rows, rows]
+    const float* x_scale;    // kMmI8 [n_x]
+    const float* w_scale;    // kMmI8 [n_mats, rows]
+    int n_mats, rows, cols;
+    int gated;               // forward: silu of the first half of the rows times the second
+    int n_x, n_rows, top_k;
+    const int32_t* order;    // nullable: row p reads x row order[p] / top_k
+    const int32_t* offsets;  // nullable: all rows belong to matrix 0
+    void* y;                 // forward [n_rows, rows] (gated: rows / 2); at x [n_rows, cols]; at w [n_mats, rows, cols]
+    int y_type;              // CX_DTYPE_*
+    void* pre;               // gated, nullable: the sums themselves [n_rows, rows], in `type`
+    int* err_flag;
+    int m_tiles, by_item;    // tiles in the output's contiguous direction; mm_tile's order
+};
+// Workgroup b runs on XCD b % 8.  by_item: an item's tiles run on one XCD, whose L2 then holds its rows of x (stacks);
+// otherwise tile m of every item does, and its L2 holds the weights (one matrix).
+struct MmTile {
+    int item, m;
+};
+__host__ __device__ inline MmTile mm_tile(unsigned b, int m_tiles, int by_item) {
+    if (by_item) {
+        const int i = (int)(b >> 3);
+        return MmTile{i / m_tiles * 8 + (int)(b & 7), i % m_tiles};
+    }
+    const int pitch = (m_tiles + 7) / 8 * 8;
+    return MmTile{(int)b / pitch, (int)b % pitch};
+}
+inline unsigned mm_grid(MmLaunch& L, int item_rows) {
+    const int64_t items = mm_items(L.n_rows, L.n_mats, L.offsets != nullptr, item_rows);
+    L.by_item = L.offsets != nullptr;
+    return (unsigned)(L.by_item ? (items + 7) / 8 * 8 * L.m_tiles : items * ((L.m_tiles + 7) / 8 * 8));
+}
+inline bool mm_at16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+hipError_t launch_mm(MmLaunch L, hipStream_t s);
+hipError_t launch_mm_i8(MmLaunch L, hipStream_t s);
+hipError_t launch_mm_dx(MmLaunch L, hipStream_t s);
+hipError_t launch_mm_dw(MmLaunch L, hipStream_t s);
+// dpre of silu(g) * u from dh and pre = [g, u], rounded to their type: [n_rows, 2 * inter].
+hipError_t launch_gate_grad(const void* dh, const void* pre, int type, int64_t n_rows, int inter, void* dpre, hipStream_t s);
+hipError_t launch_quantize_i8(const void* x, int x_type, int n_rows, int cols, int8_t* q, float* scale, hipStream_t s);
+
 }  // namespace cx

@@ -1,0 +1,87 @@
+// cx_mm_grad.hip — gradients of the products with 16-bit weights, and of the gate between them.
+#include "cx_mm.h"
+
+namespace cx {
+namespace {
+
+using Big = MmShape<2, 4, 4, 2>;
+using Small = MmShape<2, 2, 2, 2>;
+
+template <class T, class S, bool DMA>
+hipError_t dx(MmLaunch& L, hipStream_t s) {
+    L.m_tiles = (L.cols + S::BM - 1) / S::BM;
+    cx_launch(k_mm_dx<T, S, DMA>, dim3(mm_grid(L, S::BN)), dim3(S::kThreads), 0, s, L);
+    return hipGetLastError();
+}
+
+template <class T, class S, bool DMA>
+hipError_t dw(MmLaunch& L, hipStream_t s) {
+    L.m_tiles = (L.cols + S::BM - 1) / S::BM;
+    const int64_t tiles = (int64_t)L.n_mats * L.m_tiles * ((L.rows + S::BN - 1) / S::BN);
+    cx_launch(k_mm_dw<T, S, DMA>, dim3((unsigned)tiles), dim3(S::kThreads), 0, s, L);
+    return hipGetLastError();
+}
+
+template <class T>
+hipError_t dx_pick(MmLaunch& L, hipStream_t s) {
+    if (L.cols % 8 != 0 || L.rows % 8 != 0 || !mm_at16(L.w) || !mm_at16(L.dy)) return dx<T, Small, false>(L, s);
+    return mm_big(L.n_rows, L.offsets ? L.n_mats : 1, L.cols) ? dx<T, Big, true>(L, s) : dx<T, Small, true>(L, s);
+}
+
+template <class T>
+hipError_t dw_pick(MmLaunch& L, hipStream_t s) {
+    if (L.cols % 8 != 0 || L.rows % 8 != 0 || !mm_at16(L.x) || !mm_at16(L.dy)) return dw<T, Small, false>(L, s);
+    return (int64_t)L.n_mats * ((L.cols + 255) / 256) * ((L.rows + 255) / 256) >= 256 ? dw<T, Big, true>(L, s) : dw<T, Small, true>(L, s);
+}
+
+// h = silu(g) u has dg = dh u sig(g) (1 + g (1 - sig(g))) and du = dh silu(g); each rounded once.  One value
+// of dh, g and u a lane, 8 where rows allow 16-byte accesses.  HBM bounds it.
+template <bool BF, int N>
+__global__ __launch_bounds__(256) void k_gate_grad(const uint16_t* dh, const uint16_t* pre, int64_t n_rows, int inter, uint16_t* dpre) {
+    const int per = (inter + N - 1) / N;
+    const int64_t total = n_rows * per;
+    for (int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x; at < total; at += (int64_t)gridDim.x * 256) {
+        const int64_t p = at / per;
+        const int c = (int)(at - p * per) * N;
+        typedef uint16_t V __attribute__((ext_vector_type(N == 1 ? 2 : N)));
+        auto value = [](uint16_t h) { return BF ? __uint_as_float((uint32_t)h << 16) : (float)__builtin_bit_cast(_Float16, h); };
+        auto round = [](float f) { return (uint16_t)(BF ? bf16_rne(f) : f16_rne(f)); };
+        V d = {}, g = {}, u = {}, a, b;
+        const int64_t o = p * 2 * inter + c;
+        if constexpr (N == 1) {
+            d[0] = dh[p * inter + c], g[0] = pre[o], u[0] = pre[o + inter];
+        } else {
+            d = *reinterpret_cast<const V*>(dh + p * inter + c);
+            g = *reinterpret_cast<const V*>(pre + o);
+            u = *reinterpret_cast<const V*>(pre + o + inter);
+        }
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const float x = value(g[i]), t = value(d[i]), sig = 1.0f / (1.0f + expf(-x));
+            a[i] = round(t * value(u[i]) * sig * (1.0f + x * (1.0f - sig)));
+            b[i] = round(t * x * sig);
+        }
+        if constexpr (N == 1) {
+            dpre[o] = a[0], dpre[o + inter] = b[0];
+        } else {
+            *reinterpret_cast<V*>(dpre + o) = a;
+            *reinterpret_cast<V*>(dpre + o + inter) = b;
+        }
+    }
+}
+
+}  // namespace
+
+hipError_t launch_mm_dx(MmLaunch L, hipStream_t s) { return L.type == CX_DTYPE_BF16 ? dx_pick<MmBf16>(L, s) : dx_pick<MmF16>(L, s); }
+hipError_t launch_mm_dw(MmLaunch L, hipStream_t s) { return L.type == CX_DTYPE_BF16 ? dw_pick<MmBf16>(L, s) : dw_pick<MmF16>(L, s); }
+
+hipError_t launch_gate_grad(const void* dh, const void* pre, int type, int64_t n_rows, int inter, void* dpre, hipStream_t s) {
+    const bool vec = inter % 8 == 0 && mm_at16(dh) && mm_at16(pre) && mm_at16(dpre);
+    const int64_t wgs = (n_rows * ((inter + (vec ? 7 : 0)) / (vec ? 8 : 1)) + 255) / 256;
+    auto k = type == CX_DTYPE_BF16 ? (vec ? k_gate_grad<true, 8> : k_gate_grad<true, 1>) : (vec ? k_gate_grad<false, 8> : k_gate_grad<false, 1>);
+    cx_launch(k, dim3((unsigned)std::min<int64_t>(wgs, 8192)), dim3(256), 0, s, static_cast<const uint16_t*>(dh), static_cast<const uint16_t*>(pre),
+              n_rows, inter, static_cast<uint16_t*>(dpre));
+    return hipGetLastError();
+}
+
+}  // namespace cx

@@ -799,6 +799,48 @@ int check_rows(cx_ctx* ctx, int n_tokens, int top_k, int64_t width) {
     return set_device(ctx->device);
 }
 
+// What the products of a program's own experts ask of their sizes.
+int check_mm(cx_ctx* ctx, int el, int n_mats, int rows, int cols, int gated, const void* offsets, int n_rows) {
+    if (!ctx) return fail(CX_EINVAL, "NULL context");
+    if (n_mats < 1 || n_mats > kSortMaxExperts) return fail(CX_EINVAL, "n_mats must be 1..%d", kSortMaxExperts);
+    if (rows < 1 || cols < 1 || rows > kMmMaxSide || cols > (el == 1 ? kI8MaxCols : kMmMaxSide))
+        return fail(CX_EINVAL, "rows must be 1..%d and cols 1..%d", kMmMaxSide, el == 1 ? kI8MaxCols : kMmMaxSide);
+    if ((uint64_t)rows * cols * el >= (uint64_t)1 << 32) return fail(CX_EINVAL, "a matrix must have fewer than 2^32 bytes");
+    if (gated && rows % 2 != 0) return fail(CX_EINVAL, "a gated matrix has an even number of rows");
+    if (n_rows < 0) return fail(CX_EINVAL, "bad n_rows");
+    if (!offsets && n_mats != 1) return fail(CX_EINVAL, "a stack of %d matrices needs offsets", n_mats);
+    if (!mm_grid_ok(n_rows, n_mats, rows, cols)) return fail(CX_EINVAL, "too many rows or matrices for one launch");
+    return CX_OK;
+}
+
+int check_scratch(size_t need, const void* scratch, size_t bytes) {
+    if (need && (!scratch || bytes < need || reinterpret_cast<uintptr_t>(scratch) % 16))
+        return fail(CX_EINVAL, "scratch must be %zu bytes, 16-byte aligned", need);
+    return CX_OK;
+}
+
+// The forward products in 16 bits (x_scale NULL) and in 8.
+int matmul(cx_ctx* ctx, MmLaunch L, size_t need, void* scratch, size_t scratch_bytes, void* stream) {
+    const int el = L.type == kMmI8 ? 1 : 2;
+    int rc = check_mm(ctx, el, L.n_mats, L.rows, L.cols, L.gated, L.offsets, L.n_rows);
+    if (rc) return rc;
+    if (!act_any(L.y_type)) return fail(CX_EINVAL, "y must be fp16, bf16 or fp32");
+    if (L.pre && !L.gated) return fail(CX_EINVAL, "pre comes with a gated product only");
+    if (L.n_x < 0 || (L.order && L.top_k < 1)) return fail(CX_EINVAL, "bad n_x or top_k");
+    if (!L.order && L.n_x != L.n_rows) return fail(CX_EINVAL, "without an order x and y have the same rows (%d and %d)", L.n_x, L.n_rows);
+    if (L.n_rows == 0) return CX_OK;
+    if (L.n_x == 0) return fail(CX_EINVAL, "x has no rows");
+    if (L.order && (uint64_t)L.n_x * L.cols * el >= (uint64_t)1 << 32) return fail(CX_EINVAL, "rows picked by an order must have fewer than 2^32 bytes in all");
+    if (!L.x || !L.w || !L.y || (el == 1 && (!L.x_scale || !L.w_scale))) return fail(CX_EINVAL, "NULL buffer");
+    if ((rc = check_scratch(need, scratch, scratch_bytes))) return rc;
+    if ((rc = set_device(ctx->device))) return rc;
+    L.err_flag = ctx->err_flag;
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    Span sp(ctx, "matmul", s);
+    CX_HIP(launch_mm(L, s));
+    return CX_OK;
+}
+
 int check_q4(const cx_q4_desc* w) {
     if (!w || !w->codes || !w->scales) return fail(CX_EINVAL, "4-bit descriptor is NULL or empty");
     // the limits of cx_q4_pack: the plan of a stack's rows has a place in LDS for each of its matrices
@@ -1727,6 +1769,131 @@ int cx_q4_moe(cx_ctx* ctx, const cx_q4_desc* gate_up, const cx_q4_desc* down, co
     Span sp(ctx, "combine", s);
     CX_HIP(launch_combine_rows(c, s));
     return CX_OK;
+}
+
+// ---------------------------------------------------------------------------
+// Products of a program's own experts.
+
+size_t cx_matmul_scratch(int dtype, int n_mats, int rows, int cols, int gated, int n_rows, int with_offsets) {
+    (void)dtype, (void)n_mats, (void)rows, (void)cols, (void)gated, (void)n_rows, (void)with_offsets;
+    return 0;
+}
+
+int cx_matmul(cx_ctx* ctx, const void* x, int n_x, const void* w, int dtype, int n_mats, int rows, int cols, int gated,
+              const int32_t* order, int top_k, const int32_t* offsets, int n_rows, void* y, int y_dtype, void* pre,
+              void* scratch, size_t scratch_bytes, void* stream) {
+    DeviceRestore keep;
+    if (!act16(dtype)) return fail(CX_EINVAL, "x and weights must be fp16 or bf16");
+    MmLaunch L{};
+    L.type = dtype;
+    L.w = w;
+    L.x = x;
+    L.n_mats = n_mats;
+    L.rows = rows;
+    L.cols = cols;
+    L.gated = gated != 0;
+    L.n_x = n_x;
+    L.n_rows = n_rows;
+    L.order = order;
+    L.top_k = top_k;
+    L.offsets = offsets;
+    L.y = y;
+    L.y_type = y_dtype;
+    L.pre = pre;
+    return matmul(ctx, L, cx_matmul_scratch(dtype, n_mats, rows, cols, gated, n_rows, offsets != nullptr), scratch, scratch_bytes, stream);
+}
+
+size_t cx_matmul_grad_scratch(int dtype, int n_mats, int rows, int cols, int gated, int n_rows, int with_offsets, int with_dx,
+                              int dw_dtype) {
+    (void)dtype, (void)n_mats, (void)cols, (void)with_offsets, (void)with_dx, (void)dw_dtype;
+    if (rows < 1 || n_rows < 1) return 0;
+    return gated ? ((size_t)n_rows * rows * 2 + 15) / 16 * 16 : 0;
+}
+
+int cx_matmul_grad(cx_ctx* ctx, const void* dy, const void* x, const void* w, int dtype, const void* pre, int n_mats, int rows,
+                   int cols, const int32_t* offsets, int n_rows, void* dx, void* dw, int dw_dtype, void* scratch,
+                   size_t scratch_bytes, void* stream) {
+    DeviceRestore keep;
+    if (!act16(dtype)) return fail(CX_EINVAL, "x and weights must be fp16 or bf16");
+    int rc = check_mm(ctx, 2, n_mats, rows, cols, pre != nullptr, offsets, n_rows);
+    if (rc) return rc;
+    if (!dx && !dw) return fail(CX_EINVAL, "nothing to compute: dx or dw");
+    if (dw && dw_dtype != dtype && dw_dtype != CX_DTYPE_F32) return fail(CX_EINVAL, "dw must be of x's type or fp32");
+    if (n_rows == 0 && !dw) return CX_OK;
+    if ((n_rows > 0 && (!dy || (dw && !x))) || (dx && !w)) return fail(CX_EINVAL, "NULL buffer");
+    const size_t need = cx_matmul_grad_scratch(dtype, n_mats, rows, cols, pre != nullptr, n_rows, offsets != nullptr, dx != nullptr, dw ? dw_dtype : 0);
+    if ((rc = check_scratch(need, scratch, scratch_bytes))) return rc;
+    if ((rc = set_device(ctx->device))) return rc;
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    MmLaunch L{};
+    L.type = dtype;
+    L.w = w;
+    L.x = x;
+    L.dy = dy;
+    L.n_mats = n_mats;
+    L.rows = rows;
+    L.cols = cols;
+    L.n_x = L.n_rows = n_rows;
+    L.offsets = offsets;
+    L.err_flag = ctx->err_flag;
+    Span sp(ctx, "matmul_grad", s);
+    if (pre && n_rows > 0) {
+        CX_HIP(launch_gate_grad(dy, pre, dtype, n_rows, rows / 2, scratch, s));
+        L.dy = scratch;
+    }
+    if (dx && n_rows > 0) {
+        L.y = dx;
+        L.y_type = dtype;
+        CX_HIP(launch_mm_dx(L, s));
+    }
+    if (dw) {
+        L.y = dw;
+        L.y_type = dw_dtype;
+        CX_HIP(launch_mm_dw(L, s));
+    }
+    return CX_OK;
+}
+
+int cx_quantize_i8(cx_ctx* ctx, const void* x, int x_dtype, int n_rows, int cols, int8_t* q, float* scale, void* stream) {
+    DeviceRestore keep;
+    int rc = check_rows(ctx, n_rows, 1, cols);
+    if (rc) return rc;
+    if (!act_any(x_dtype)) return fail(CX_EINVAL, "x must be fp16, bf16 or fp32");
+    if (n_rows == 0) return CX_OK;
+    if (!x || !q || !scale) return fail(CX_EINVAL, "NULL buffer");
+    if (!rows_grid_ok(n_rows, 256)) return fail(CX_EINVAL, "too many rows for one launch");
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    Span sp(ctx, "quantize", s);
+    CX_HIP(launch_quantize_i8(x, x_dtype, n_rows, cols, q, scale, s));
+    return CX_OK;
+}
+
+size_t cx_i8_matmul_scratch(int n_mats, int rows, int cols, int gated, int n_rows, int with_offsets) {
+    return cx_matmul_scratch(kMmI8, n_mats, rows, cols, gated, n_rows, with_offsets);
+}
+
+int cx_i8_matmul(cx_ctx* ctx, const int8_t* x, const float* x_scale, int n_x, const int8_t* w, const float* w_scale, int n_mats,
+                 int rows, int cols, int gated, const int32_t* order, int top_k, const int32_t* offsets, int n_rows, void* y,
+                 int y_dtype, void* scratch, size_t scratch_bytes, void* stream) {
+    DeviceRestore keep;
+    MmLaunch L{};
+    L.type = kMmI8;
+    L.w = w;
+    L.x = x;
+    L.x_scale = x_scale;
+    L.w_scale = w_scale;
+    L.n_mats = n_mats;
+    L.rows = rows;
+    L.cols = cols;
+    L.gated = gated != 0;
+    L.n_x = n_x;
+    L.n_rows = n_rows;
+    L.order = order;
+    L.top_k = top_k;
+    L.offsets = offsets;
+    L.y = y;
+    L.y_type = y_dtype;
+    return matmul(ctx, L, cx_i8_matmul_scratch(n_mats, rows, cols, gated, n_rows, offsets != nullptr), scratch, scratch_bytes, stream);
 }
 
 // ---------------------------------------------------------------------------

@@ -400,4 +400,25 @@ inline int64_t q4_most_items(int64_t n_rows, int n_mats, int dec_rows) {
     return q4_max_items(n_rows, n_mats, dec_rows > 0 ? dec_rows : kTileTok);
 }
 
+// Products with weights as the program holds them.
+constexpr int kMmMaxSide = 1 << 22;  // 256 rows of it lie within 32 bits
+constexpr int kI8MaxCols = 131071;  // 2^14 times that is less than 2^31: sums in 32 bits are exact
+// Rows of each of the n items that `rows` rows are cut to (the last has what is left): equal ones of whole 32-row tiles.
+constexpr int mm_share(int n, int rows) { return n <= 1 ? rows : (rows + 32 * n - 1) / (32 * n) * 32; }
+// Items of up to item_rows rows, those of rows behind the last matrix's included, at most.
+inline int64_t mm_items(int64_t n_rows, int n_mats, bool stack, int item_rows) {
+    if (!stack) return (n_rows + item_rows - 1) / item_rows;
+    return (n_rows < n_mats ? n_rows : n_mats) + n_rows / item_rows + 1;
+}
+
+// Tiles of 256 x 256 where they fill the card, of 128 x 128 otherwise.
+inline bool mm_big(int64_t n_rows, int n_mats, int width) {
+    return (n_rows / 256 + 1) * ((width + 255) / 256) >= 256 && n_rows >= (int64_t)n_mats * 64;
+}
+// Launches stay within 2^32 threads and 2^30 rows, at the smallest tiles and with every matrix's last tile short.
+inline bool mm_grid_ok(int64_t n_rows, int n_mats, int rows, int cols) {
+    const int64_t items = mm_items(n_rows, n_mats, true, 128) + 8, tiles = (std::max(rows, cols) + 63) / 64 + 8;
+    return n_rows <= (1 << 30) && items * tiles < ((int64_t)1 << 24) && n_mats * (((int64_t)rows + 127) / 128) * ((cols + 127) / 128) < ((int64_t)1 << 24);
+}
+
 }  // namespace cx

@@ -563,6 +563,128 @@ class Context:
                                  cx_dtype(out_dtype), _ptr(scratch), size, self.stream()))
         return y
 
+    # -- products of a program's own experts --------------------------------------
+    def _stack(self, w: torch.Tensor, cols: int, offsets, gated: bool = False) -> tuple[int, int]:
+        """(matrices, rows) of weights [rows, cols] or [n_mats, rows, cols]."""
+        if w.dim() not in (2, 3) or w.shape[-1] != cols:
+            raise ValueError(f"weights {tuple(w.shape)} do not take rows of {cols} columns")
+        if not w.is_contiguous():
+            raise ValueError("weights must be contiguous")
+        if gated and w.shape[-2] % 2:
+            raise ValueError("a gated matrix has an even number of rows")
+        E = w.shape[0] if w.dim() == 3 else 1
+        if offsets is None:
+            if E != 1:
+                raise ValueError(f"a stack of {E} matrices needs offsets")
+        elif offsets.dtype != torch.int32 or offsets.shape != (E + 1,) or not offsets.is_contiguous():
+            raise ValueError(f"offsets must be a contiguous int32 vector of {E + 1}")
+        return E, w.shape[-2]
+
+    @staticmethod
+    def _picked(order: Optional[torch.Tensor], rows: int) -> int:
+        if order is None:
+            return rows
+        if order.dtype != torch.int32 or order.dim() != 1 or not order.is_contiguous():
+            raise ValueError("order must be a contiguous int32 vector")
+        return order.shape[0]
+
+    def matmul(self, x: torch.Tensor, w: torch.Tensor, *, gated: bool = False, keep: bool = False,
+               offsets: Optional[torch.Tensor] = None, order: Optional[torch.Tensor] = None, top_k: int = 1,
+               out_dtype: Optional[torch.dtype] = None):
+        """x W^T of 16-bit x [T, K] and weights [N, K] or a stack [E, N, K], whose matrix e takes the
+        rows offsets[e] .. offsets[e + 1] - 1; with `order`, row p is row order[p] // top_k of x
+        (sort_tokens' offsets and order).  gated: the rows of a matrix are a gate and then an up matrix,
+        and the result is silu(x G^T) * (x U^T) [P, N / 2]; with `keep` (result, pre), pre = [x G^T, x U^T]
+        in x's type, which matmul_grad asks for.  Its gradient: matmul_grad, by the caller's autograd.Function
+        (as gather_rows)."""
+        self._here(x, w, offsets, order)
+        _outside_autograd("matmul", "matmul_grad", x, w)
+        T, K = _rows_2d(x)
+        E, N = self._stack(w, K, offsets, gated)
+        if x.dtype not in (torch.float16, torch.bfloat16) or w.dtype != x.dtype:
+            raise TypeError("x and weights must be float16 or bfloat16, of one type")
+        if keep and not gated:
+            raise ValueError("keep is of gated products")
+        P = self._picked(order, T)
+        x = x.contiguous()
+        out_dtype = out_dtype or x.dtype
+        dt = cx_dtype(x.dtype)
+        y = torch.empty((P, N // 2 if gated else N), dtype=out_dtype, device=x.device)
+        pre = torch.empty((P, N), dtype=x.dtype, device=x.device) if keep else None
+        size = lib().cx_matmul_scratch(dt, E, N, K, int(gated), P, int(offsets is not None))
+        scratch = torch.empty(size, dtype=torch.uint8, device=x.device) if size else None
+        check(lib().cx_matmul(self.handle, x.data_ptr(), T, w.data_ptr(), dt, E, N, K, int(gated), _ptr(order), top_k,
+                              _ptr(offsets), P, y.data_ptr(), cx_dtype(out_dtype), _ptr(pre), _ptr(scratch), size,
+                              self.stream()))
+        return (y, pre) if keep else y
+
+    def matmul_grad(self, dy: torch.Tensor, x: torch.Tensor, w: torch.Tensor, *, pre: Optional[torch.Tensor] = None,
+                    offsets: Optional[torch.Tensor] = None, want_dx: bool = True, want_dw: bool = True,
+                    dw_dtype: Optional[torch.dtype] = None):
+        """(dx, dw) of matmul(x, w) without an order: dx in x's type, dw of w's shape in dw_dtype (x's, or fp32),
+        None where it was not wanted.  pre: what a gated product kept; dy is the gradient at its result."""
+        self._here(dy, x, w, pre, offsets)
+        P, K = _rows_2d(x)
+        E, N = self._stack(w, K, offsets, pre is not None)
+        if x.dtype not in (torch.float16, torch.bfloat16) or any(t is not None and t.dtype != x.dtype for t in (dy, w, pre)):
+            raise TypeError("dy, x, weights and pre must be float16 or bfloat16, of one type")
+        if dy.shape != (P, N if pre is None else N // 2):
+            raise ValueError(f"dy must be [{P}, {N if pre is None else N // 2}]")
+        if pre is not None and pre.shape != (P, N):
+            raise ValueError(f"pre must be [{P}, {N}]")
+        if not (want_dx or want_dw):
+            raise ValueError("nothing to compute: want_dx or want_dw")
+        dw_dtype = dw_dtype or x.dtype
+        if dw_dtype not in (x.dtype, torch.float32):
+            raise TypeError("dw must be of x's type or float32")
+        dy, x = dy.contiguous(), x.contiguous()
+        pre = None if pre is None else pre.contiguous()
+        dx = torch.empty_like(x) if want_dx else None
+        dw = torch.empty_like(w, dtype=dw_dtype) if want_dw else None
+        dt, dwt = cx_dtype(x.dtype), cx_dtype(dw_dtype) if want_dw else 0
+        size = lib().cx_matmul_grad_scratch(dt, E, N, K, int(pre is not None), P, int(offsets is not None), int(want_dx), dwt)
+        scratch = torch.empty(size, dtype=torch.uint8, device=x.device) if size else None
+        check(lib().cx_matmul_grad(self.handle, dy.data_ptr(), x.data_ptr(), w.data_ptr(), dt, _ptr(pre), E, N, K,
+                                   _ptr(offsets), P, _ptr(dx), _ptr(dw), dwt, _ptr(scratch), size, self.stream()))
+        return dx, dw
+
+    def quantize_i8(self, x: torch.Tensor):
+        """(q int8, scale fp32 of x's leading shape): rows (the last dimension) of x in 8-bit integers times
+        a scale each.  A weight matrix's channels are its rows."""
+        self._here(x)
+        if x.dim() < 1:
+            raise ValueError("expected rows")
+        x = x.contiguous()
+        q = torch.empty_like(x, dtype=torch.int8)
+        scale = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)
+        check(lib().cx_quantize_i8(self.handle, x.data_ptr(), cx_dtype(x.dtype), scale.numel(), x.shape[-1],
+                                   q.data_ptr(), scale.data_ptr(), self.stream()))
+        return q, scale
+
+    def i8_matmul(self, x: torch.Tensor, x_scale: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, *,
+                  gated: bool = False, offsets: Optional[torch.Tensor] = None, order: Optional[torch.Tensor] = None,
+                  top_k: int = 1, out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+        """x W^T of 8-bit x [T, K] with a scale per row and 8-bit weights [N, K] or [E, N, K] with a scale per
+        channel ([N] or [E, N]), as quantize_i8 makes them, in out_dtype; all else as matmul."""
+        self._here(x, x_scale, w, w_scale, offsets, order)
+        T, K = _rows_2d(x)
+        E, N = self._stack(w, K, offsets, gated)
+        if x.dtype != torch.int8 or w.dtype != torch.int8:
+            raise TypeError("x and weights must be int8")
+        if x_scale.shape != (T,) or x_scale.dtype != torch.float32:
+            raise ValueError(f"x_scale must be fp32 [{T}]")
+        if w_scale.shape != w.shape[:-1] or w_scale.dtype != torch.float32 or not w_scale.is_contiguous():
+            raise ValueError(f"w_scale must be contiguous fp32 {list(w.shape[:-1])}")
+        P = self._picked(order, T)
+        x, x_scale = x.contiguous(), x_scale.contiguous()
+        y = torch.empty((P, N // 2 if gated else N), dtype=out_dtype, device=x.device)
+        size = lib().cx_i8_matmul_scratch(E, N, K, int(gated), P, int(offsets is not None))
+        scratch = torch.empty(size, dtype=torch.uint8, device=x.device) if size else None
+        check(lib().cx_i8_matmul(self.handle, x.data_ptr(), x_scale.data_ptr(), T, w.data_ptr(), w_scale.data_ptr(), E, N, K,
+                                 int(gated), _ptr(order), top_k, _ptr(offsets), P, y.data_ptr(), cx_dtype(out_dtype),
+                                 _ptr(scratch), size, self.stream()))
+        return y
+
     def _q4_ready(self, layer: Q4Layer, x: torch.Tensor, *others: Optional[torch.Tensor]) -> None:
         """What a call on a 4-bit layer needs of it and of x, before anything is launched."""
         self._here(x, *others)

@@ -150,7 +150,7 @@ CX_API int cx_ctx_sync(cx_ctx* ctx, void* stream);
 /* Per-kernel timing with HIP events recorded on the launch stream around
  * every kernel the context launches (kernels: "route", "plan", "gate_up",
  * "down", "combine"; of the calls around the experts "rms_norm", "sort",
- * "gather", "combine", "combine_grad", "q4", and "experts" for a 4-bit layer's
+ * "gather", "combine", "combine_grad", "q4", "matmul", "matmul_grad", "quantize", and "experts" for a 4-bit layer's
  * launches on one token).  cx_ctx_profile(ctx, 1) starts collecting (and clears
  * totals), 0 stops.  cx_ctx_profile_read synchronises on the recorded events
  * and returns the launch count and summed milliseconds of one kernel. */
@@ -409,6 +409,60 @@ CX_API int cx_q4_moe(cx_ctx* ctx, const cx_q4_desc* gate_up, const cx_q4_desc* d
               const void* x, int in_dtype, int n_tokens, const int32_t* topk_ids,
               const float* topk_w, int top_k, void* y, int out_dtype, float* y_f32,
               void* scratch, size_t scratch_bytes, void* stream);
+
+/* ---- products of a program's own experts --------------------------------------
+ * Weights as the program holds them: n_mats row-major matrices [rows, cols] in fp16 or
+ * bf16, or in 8-bit integers with a fp32 scale per row (channel).  No counterpart in the
+ * reference.  Rows are dealt to a stack's matrices as cx_q4_matmul deals them: rows
+ * offsets[e] .. offsets[e + 1] - 1 belong to matrix e (offsets NULL: one matrix, n_mats 1, for
+ * all rows), rows behind the last matrix's are zeros in every output that has such rows, offsets
+ * that decrease or leave the rows are cut and reported by cx_ctx_sync.  None of these
+ * calls allocates, copies or waits, so all of them can be captured into a graph.  Sums are
+ * in fp32 (exact 32-bit integers for 8-bit rows), in an order that depends on sizes alone, and rounded
+ * once.  Buffers may start at any address of their type's alignment; rows and addresses of whole
+ * 16-byte pieces take the fast loads.  n_mats is at most 1024, rows and cols 2^22 (8-bit:
+ * cols 131071), n_rows 2^30, and a matrix has fewer than 2^32 bytes. */
+
+/* y = x W^T.  gated: rows is even and the halves are a gate and an up matrix G, U:
+ * y = silu(x G^T) * (x U^T); pre (nullable, for the gradient) receives [x G^T, x U^T],
+ * [n_rows, rows] in x's type.
+ * x: [n_x, cols] of the weights' type; y: [n_rows, rows] (gated: rows / 2) in fp16, bf16 or
+ * fp32.  order NULL: row p of y is row p of x.  Otherwise it is row order[p] / top_k of x (which
+ * has fewer than 2^32 bytes then); a row whose entry is negative or past n_x reads as zeros.
+ * scratch: cx_matmul_scratch bytes of device memory, 16-byte aligned, of the caller's (NULL where
+ * that is 0), in use until the call's work is done. */
+CX_API size_t cx_matmul_scratch(int dtype, int n_mats, int rows, int cols, int gated, int n_rows, int with_offsets);
+CX_API int cx_matmul(cx_ctx* ctx, const void* x, int n_x, const void* w, int dtype, int n_mats, int rows, int cols,
+              int gated, const int32_t* order, int top_k, const int32_t* offsets, int n_rows, void* y, int y_dtype,
+              void* pre, void* scratch, size_t scratch_bytes, void* stream);
+
+/* The gradients of y = x W^T: dx = dy W [n_rows, cols] in x's type, dw[e] = dy_e^T x_e
+ * [n_mats, rows, cols] in x's type or fp32 (zeros for a matrix without rows); either may be
+ * NULL.  dy: [n_rows, rows] in x's type.
+ * pre given: the product was gated, dy is the gradient at its y, [n_rows, rows / 2], and what takes
+ * dy's place is the gradient at pre = [g, u], rounded to x's type:
+ *   [dy * u * s(g) * (1 + g * (1 - s(g))), dy * g * s(g)],  s the logistic function.
+ * Every row of x takes part once: rows come as they lie, without an order.
+ * scratch: cx_matmul_grad_scratch bytes, as above. */
+CX_API size_t cx_matmul_grad_scratch(int dtype, int n_mats, int rows, int cols, int gated, int n_rows, int with_offsets,
+              int with_dx, int dw_dtype);
+CX_API int cx_matmul_grad(cx_ctx* ctx, const void* dy, const void* x, const void* w, int dtype, const void* pre,
+              int n_mats, int rows, int cols, const int32_t* offsets, int n_rows, void* dx, void* dw, int dw_dtype,
+              void* scratch, size_t scratch_bytes, void* stream);
+
+/* Rows to 8-bit integers with a scale per row:
+ *   scale[t] = max(max |x[t]| / 127, 1e-12),  q = x / scale rounded to the nearest (ties to even)
+ * both quotients correctly rounded in fp32.  x: fp16, bf16 or fp32.  A row with a NaN has a
+ * NaN scale, one with an infinity an infinite one.  The channels of a weight matrix are its rows. */
+CX_API int cx_quantize_i8(cx_ctx* ctx, const void* x, int x_dtype, int n_rows, int cols, int8_t* q, float* scale,
+              void* stream);
+
+/* y[p, n] = x_scale[row(p)] * w_scale[n] * sum over k of x[row(p), k] * w[n, k], gated as above; all
+ * else as cx_matmul.  x: [n_x, cols], w: [n_mats, rows, cols], w_scale: [n_mats, rows]. */
+CX_API size_t cx_i8_matmul_scratch(int n_mats, int rows, int cols, int gated, int n_rows, int with_offsets);
+CX_API int cx_i8_matmul(cx_ctx* ctx, const int8_t* x, const float* x_scale, int n_x, const int8_t* w, const float* w_scale,
+              int n_mats, int rows, int cols, int gated, const int32_t* order, int top_k, const int32_t* offsets,
+              int n_rows, void* y, int y_dtype, void* scratch, size_t scratch_bytes, void* stream);
 
 /* ---- whole-layer wire message ---------------------------------------------
  * MoeLayerRequest (msg_type 42) / MoeLayerResponse (43): one request per
