@@ -1817,7 +1817,7 @@ int cx_matmul_grad(cx_ctx* ctx, const void* dy, const void* x, const void* w, in
     if (!act16(dtype)) return fail(CX_EINVAL, "x and weights must be fp16 or bf16");
     int rc = check_mm(ctx, 2, n_mats, rows, cols, pre != nullptr, offsets, n_rows);
     if (rc) return rc;
-    if (!dx && !dw) return fail(CX_EINVAL, "nothing to compute: dx or dw");
+    if (n_rows > 0 && !dx && !dw) return fail(CX_EINVAL, "nothing to compute: dx or dw");
     if (dw && dw_dtype != dtype && dw_dtype != CX_DTYPE_F32) return fail(CX_EINVAL, "dw must be of x's type or fp32");
     if (n_rows == 0 && !dw) return CX_OK;
     if ((n_rows > 0 && (!dy || (dw && !x))) || (dx && !w)) return fail(CX_EINVAL, "NULL buffer");

@@ -27,10 +27,6 @@ def own(t, odd=False):
     return room[1:].view(t.shape)
 
 
-def pre_tol(want, e, dtype):
-    return rounded(want, e, dtype)
-
-
 # rows, weight rows, columns: a token; widths that pieces of 16 bytes do and do not divide; tiles that end inside
 # their rows, their outputs and their last step; more than one step, odd and even counts of them
 ONE = [(1, 32, 64), (1, 1, 1), (1, 512, 7168), (2, 18, 130), (5, 100, 129), (16, 64, 1000), (17, 130, 384), (33, 34, 8), (40, 66, 72), (64, 256, 640),
@@ -249,12 +245,20 @@ def test_gradients(gpu, P, E, N, K, dtype):
         near(gx, dx, rounded(dx, ex, dtype), "dx")
         near(gw.view(w.shape), dw, rounded(dw, ew, out), "dw")
         assert not gx[held:].any()
-    gpu.sync()
+    if held > P:  # offsets that leave the rows
+        from constellation_amd._lib import CxError
+        with pytest.raises(CxError, match="offset"):
+            gpu.sync()
+    else:
+        gpu.sync()
     only, none = gpu.matmul_grad(dy.cuda(), x.cuda(), wd, offsets=off.to(torch.int32).cuda() if E else None, want_dw=False)
     assert none is None and torch.equal(only, gx)
     none, only = gpu.matmul_grad(dy.cuda(), x.cuda(), wd, offsets=off.to(torch.int32).cuda() if E else None, want_dx=False, dw_dtype=SF)
     assert none is None
     near(only.view(w.shape), dw, rounded(dw, ew, SF), "dw alone")
+    if held > P:
+        with pytest.raises(CxError, match="offset"):
+            gpu.sync()
 
 
 def gate_grad_ref(dh, pre):
