@@ -1,6 +1,6 @@
 // cx_i8.hip — rows to 8-bit integers with a scale each, and products of such rows with
 // 8-bit weights: y[p, n] = xs[p] ws[n] sum over k of x[p, k] w[n, k], the sum exact in 32 bits.
-#include "cx_mm.h"
+#include "cx_mm_few.h"
 
 namespace cx {
 namespace {
@@ -18,7 +18,10 @@ hipError_t run(MmLaunch& L, hipStream_t s) {
 
 template <bool GATED>
 hipError_t pick(MmLaunch& L, hipStream_t s) {
-    if (L.cols % 16 != 0 || !mm_at16(L.x) || !mm_at16(L.w)) return run<Small, GATED, false>(L, s);
+    const bool dma = L.cols % 16 == 0 && mm_at16(L.x) && mm_at16(L.w);
+    const MmFew f = mm_few_form(L.n_rows, L.n_mats, L.rows, L.cols, 1);
+    if (f.rows > 0) return mm_few<MmI8, GATED>(L, f, dma, s);
+    if (!dma) return run<Small, GATED, false>(L, s);
     return mm_big(L.n_rows, L.offsets ? L.n_mats : 1, L.rows) ? run<Big, GATED, true>(L, s) : run<Small, GATED, true>(L, s);
 }
 

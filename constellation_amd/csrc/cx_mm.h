@@ -78,7 +78,8 @@ __device__ __forceinline__ int wave_scan_add(int v, int lane) {
     return v;
 }
 
-// Run idx of up to item_rows rows (uniform in a wave; each wave finds it by itself).
+// Run idx of up to item_rows rows, of whole tiles of TILE (uniform in a wave; each wave finds it by itself).
+template <int TILE>
 __device__ __forceinline__ MmItem mm_item(const int32_t* offsets, int n_mats, int n_rows, int item_rows, int idx) {
     if (offsets == nullptr) {
         const int begin = idx * item_rows;
@@ -95,7 +96,7 @@ __device__ __forceinline__ MmItem mm_item(const int32_t* offsets, int n_mats, in
         if (past != 0) {
             const int l = __builtin_ctzll(past);
             const int r = __shfl(rows, l), m = __shfl(n, l), first = __shfl(end, l) - m, i = idx - first;
-            const int share = mm_share(m, r);  // equal runs
+            const int share = mm_share(m, r, TILE);  // equal runs
             return MmItem{e0 + l, __builtin_amdgcn_readfirstlane(__shfl(begin, l) + i * share), __builtin_amdgcn_readfirstlane(min(share, r - i * share))};
         }
         held = __shfl(top, 63);
@@ -421,7 +422,7 @@ __global__ __launch_bounds__(S::kThreads, 2) void k_mm(MmLaunch L) {
     const MmTile tile = mm_tile(blockIdx.x, L.m_tiles, L.by_item);
     if (L.offsets != nullptr && blockIdx.x == 0 && wave_id() == 0) mm_check(L.offsets, L.n_mats, L.n_rows, L.err_flag);
     if (tile.m >= L.m_tiles) return;
-    const MmItem it = mm_item(L.offsets, L.n_mats, L.n_rows, S::BN, tile.item);
+    const MmItem it = mm_item<32>(L.offsets, L.n_mats, L.n_rows, S::BN, tile.item);
     if (it.rows <= 0) return;
     const int width = GATED ? L.rows / 2 : L.rows, m0 = tile.m * kOut;
     if (it.mat < 0) {
@@ -513,7 +514,7 @@ __global__ __launch_bounds__(S::kThreads, 2) void k_mm_dx(MmLaunch L) {
     const MmTile tile = mm_tile(blockIdx.x, L.m_tiles, L.by_item);
     if (L.offsets != nullptr && blockIdx.x == 0 && wave_id() == 0) mm_check(L.offsets, L.n_mats, L.n_rows, L.err_flag);
     if (tile.m >= L.m_tiles) return;
-    const MmItem it = mm_item(L.offsets, L.n_mats, L.n_rows, S::BN, tile.item);
+    const MmItem it = mm_item<32>(L.offsets, L.n_mats, L.n_rows, S::BN, tile.item);
     if (it.rows <= 0) return;
     const int width = L.cols, m0 = tile.m * S::BM;
     if (it.mat < 0) return mm_clear(L.y, L.y_type, it.begin, it.rows, width, m0, S::BM, S::kThreads);

@@ -1,5 +1,5 @@
 // cx_mm.hip — products with 16-bit weights as the program holds them: plain and gated.
-#include "cx_mm.h"
+#include "cx_mm_few.h"
 
 namespace cx {
 namespace {
@@ -18,6 +18,8 @@ hipError_t run(MmLaunch& L, hipStream_t s) {
 template <class T, bool GATED>
 hipError_t pick(MmLaunch& L, hipStream_t s) {
     const bool dma = L.cols % (16 / T::kEl) == 0 && mm_at16(L.x) && mm_at16(L.w);
+    const MmFew f = mm_few_form(L.n_rows, L.n_mats, L.rows, L.cols, T::kEl);
+    if (f.rows > 0) return mm_few<T, GATED>(L, f, dma, s);
     if (!dma) return run<T, Small, GATED, false>(L, s);
     return mm_big(L.n_rows, L.offsets ? L.n_mats : 1, L.rows) ? run<T, Big, GATED, true>(L, s) : run<T, Small, GATED, true>(L, s);
 }

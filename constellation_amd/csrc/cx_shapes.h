@@ -403,8 +403,9 @@ inline int64_t q4_most_items(int64_t n_rows, int n_mats, int dec_rows) {
 // Products with weights as the program holds them.
 constexpr int kMmMaxSide = 1 << 22;  // 256 rows of it lie within 32 bits
 constexpr int kI8MaxCols = 131071;  // 2^14 times that is less than 2^31: sums in 32 bits are exact
-// Rows of each of the n items that `rows` rows are cut to (the last has what is left): equal ones of whole 32-row tiles.
-constexpr int mm_share(int n, int rows) { return n <= 1 ? rows : (rows + 32 * n - 1) / (32 * n) * 32; }
+// Rows of each of the n items that `rows` rows are cut to (the last has what is left): equal ones of whole
+// tiles of 16 or 32 rows.  n is the least number of items of whole tiles that holds them, so that no item is empty and none is too long.
+constexpr int mm_share(int n, int rows, int tile) { return n <= 1 ? rows : (rows + tile * n - 1) / (tile * n) * tile; }
 // Items of up to item_rows rows, those of rows behind the last matrix's included, at most.
 inline int64_t mm_items(int64_t n_rows, int n_mats, bool stack, int item_rows) {
     if (!stack) return (n_rows + item_rows - 1) / item_rows;
@@ -415,9 +416,26 @@ inline int64_t mm_items(int64_t n_rows, int n_mats, bool stack, int item_rows) {
 inline bool mm_big(int64_t n_rows, int n_mats, int width) {
     return (n_rows / 256 + 1) * ((width + 255) / 256) >= 256 && n_rows >= (int64_t)n_mats * 64;
 }
+// The kernel of few rows: rows of an item, tiles of 16 weight rows a wave, ranges of the columns a workgroup;
+// rows 0: tiles through LDS instead.
+constexpr int kMmFewWaves = 8;
+struct MmFew {
+    int rows, tiles, splits;
+};
+inline MmFew mm_few_form(int64_t n_rows, int n_mats, int rows, int cols, int el) {
+    const int64_t busy = std::min<int64_t>(n_rows, n_mats);
+    const int64_t avg = (n_rows + busy - 1) / std::max<int64_t>(busy, 1);
+    if (avg > 64) return MmFew{0, 0, 0};
+    MmFew f{avg <= 16 ? 16 : avg <= 32 ? 32 : 64, 1, 1};
+    const int64_t tiles = (rows + 15) / 16, items = busy;
+    f.tiles = f.rows > 16 || tiles * items > 1024 ? 2 : 1;
+    const int steps = (cols * el + 127) / 128;
+    while (f.splits < kMmFewWaves && tiles / f.tiles * items * f.splits * 2 <= 4096 && steps / f.splits >= 4) f.splits *= 2;
+    return f;
+}
 // Launches stay within 2^32 threads and 2^30 rows, at the smallest tiles and with every matrix's last tile short.
 inline bool mm_grid_ok(int64_t n_rows, int n_mats, int rows, int cols) {
-    const int64_t items = mm_items(n_rows, n_mats, true, 128) + 8, tiles = (std::max(rows, cols) + 63) / 64 + 8;
+    const int64_t items = mm_items(n_rows, n_mats, true, 16) + 8, tiles = (std::max(rows, cols) + 63) / 64 + 8;
     return n_rows <= (1 << 30) && items * tiles < ((int64_t)1 << 24) && n_mats * (((int64_t)rows + 127) / 128) * ((cols + 127) / 128) < ((int64_t)1 << 24);
 }
 
