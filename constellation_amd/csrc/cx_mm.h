@@ -13,32 +13,25 @@
 
 namespace cx {
 
-typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef int i32x4 __attribute__((ext_vector_type(4)));
-typedef int i32x16 __attribute__((ext_vector_type(16)));
-typedef short s16x4 __attribute__((ext_vector_type(4)));
 
-// v_mfma 32x32 of 16 bytes a lane and operand: lane l holds row (column) l % 32, contraction bytes 16 (l / 32)
-// .. + 15 of 32; a result's element i is row 8 (i / 4) + 4 (l / 32) + i % 4, column l % 32.
+// v_mfma 16x16 of 16 bytes a lane and operand: lane l holds row (column) l % 16, bytes 16 (l / 16) .. + 15 of 64 of the
+// contraction; a result's element i is row 4 (l / 16) + i, column l % 16.
 struct MmBf16 {
     static constexpr int kType = CX_DTYPE_BF16, kEl = 2;
-    typedef f32x16 Acc;
-    static __device__ __forceinline__ Acc mma(u32x4 a, u32x4 b, Acc c) {
-        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
-    }
+    typedef f32x4 Acc;
+    static __device__ __forceinline__ Acc mma(u32x4 a, u32x4 b, Acc c) { return Mma<false>::mma(Mma<false>::bits(a), Mma<false>::bits(b), c); }
 };
 struct MmF16 {
     static constexpr int kType = CX_DTYPE_FP16, kEl = 2;
-    typedef f32x16 Acc;
-    static __device__ __forceinline__ Acc mma(u32x4 a, u32x4 b, Acc c) {
-        return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
-    }
+    typedef f32x4 Acc;
+    static __device__ __forceinline__ Acc mma(u32x4 a, u32x4 b, Acc c) { return Mma<true>::mma(Mma<true>::bits(a), Mma<true>::bits(b), c); }
 };
 struct MmI8 {
     static constexpr int kType = kMmI8, kEl = 1;
-    typedef i32x16 Acc;
+    typedef i32x4 Acc;
     static __device__ __forceinline__ Acc mma(u32x4 a, u32x4 b, Acc c) {
-        return __builtin_amdgcn_mfma_i32_32x32x32_i8(__builtin_bit_cast(i32x4, a), __builtin_bit_cast(i32x4, b), c, 0, 0, 0);
+        return __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(i32x4, a), __builtin_bit_cast(i32x4, b), c, 0, 0, 0);
     }
 };
 
@@ -118,14 +111,16 @@ __device__ __forceinline__ MmItem mm_rows_of(const int32_t* offsets, int n_rows,
 }
 
 // ---------------------------------------------------------------------------
-// A workgroup's tile: WM x WN waves of TM x TN results of 32 x 32.  m is the direction in which the
+// A workgroup's tile: WM x WN waves of TM x TN results of 16 x 16.  m is the direction in which the
 // output is contiguous, n its rows.
-template <int WM_, int WN_, int TM_, int TN_>
+template <int WM_, int WN_, int TM_, int TN_, int SLOTS>
 struct MmShape {
     static constexpr int WM = WM_, WN = WN_, TM = TM_, TN = TN_;
     static constexpr int kWaves = WM * WN, kThreads = 64 * kWaves;
-    static constexpr int BM = WM * TM * 32, BN = WN * TN * 32;
-    static constexpr int kStage = (BM + BN) * 128;  // bytes of LDS of a step of the contraction
+    static constexpr int BM = WM * TM * 16, BN = WN * TN * 16;
+    // LDS: a step of the contraction is 128 bytes of each row (column) of an operand; SLOTS steps of n, one more of m
+    static constexpr int kSlots = SLOTS, kStepM = BM * 128, kStepN = BN * 128, kEndM = (SLOTS + 1) * kStepM;
+    static constexpr int kLds = kEndM + SLOTS * kStepN;
 };
 
 static __device__ __attribute__((aligned(16))) const uint32_t mm_zeros[4] = {};
@@ -135,11 +130,19 @@ struct __attribute__((packed)) MmPacked {
     u32x4 v;
 };
 
+// A pointer that is the same in all lanes, in scalar registers.
+__device__ __forceinline__ const char* mm_uniform(const void* p) {
+    const uint64_t v = (uint64_t)p;
+    return (const char*)((uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)v) | ((uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)(v >> 32)) << 32));
+}
+
 // The pieces of 16 bytes that a thread brings to LDS for one operand of a step, R rows (columns) wide.
-//  TR false: rows that are contiguous in the contraction, 128 bytes of each.  Row r's piece c lies
-//    in place c ^ (r % 8) ^ (r / 8 % 2), so that the 16 rows which a wave reads at a time lie in different banks.
+//  TR false: rows that are contiguous in the contraction, 128 bytes of each: whole lines, as L2 is asked for half of
+//    them one by one (64 bytes of each and twice the steps: 4096 rows by 4096 x 7168, loads alone 159 us, 138 with
+//    lines).  Row r's piece c lies in place c ^ (r % 8) ^ (r / 8 % 2), so that the 16 rows which a wave reads at a time
+//    lie in different banks.
 //  TR true: 64 rows of the contraction, R 16-bit columns of each.  32-byte chunk c of row j lies in place
-//    c ^ 2 (j % 4), for the transposing reads of four rows at a time.
+//    c ^ (2 (j % 4) + j / 8 % 2), for the transposing reads of four rows at a time, by two groups of lanes.
 // Places are 32 bits from a uniform base, which moves with the steps.
 template <int R, int THREADS, int EL, bool TR>
 struct MmSrc {
@@ -158,7 +161,7 @@ struct MmSrc {
     __device__ __forceinline__ void rows(const void* base_, F offset) {
         static_assert(!TR, "");
         const int t = threadIdx.x, c = (t & 7) ^ ((t >> 3) & 7) ^ ((t >> 6) & 1);
-        base = static_cast<const char*>(base_);
+        base = mm_uniform(base_);
         move = 128;
         first = c * (16 / EL);
 #pragma unroll
@@ -169,30 +172,27 @@ struct MmSrc {
         static_assert(TR, "");
         const int t = threadIdx.x, piece = t % (R / 8);
         first = t / (R / 8);
-        const int col = col0 + (((piece >> 1) ^ (2 * (first & 3))) * 2 + (piece & 1)) * 8;
-        base = static_cast<const char*>(base_);
+        const int col = col0 + (((piece >> 1) ^ (2 * (first & 3) + (first >> 3 & 1))) * 2 + (piece & 1)) * 8;
+        base = mm_uniform(base_);
         left = width - col;
         off[0] = (uint32_t)first * (uint32_t)width * 2 + (left > 0 ? col * 2 : 0);
         gap = (uint32_t)kStepRows * (uint32_t)width * 2;
         move = (size_t)width * 128;
     }
-    __device__ __forceinline__ const char* piece(int i, int k) const {
-        return base + (size_t)k * move + (TR ? off[0] + (uint32_t)i * gap : off[TR ? 0 : i]);
+    // Piece i of the step that starts at `from`.
+    __device__ __forceinline__ const char* piece(int i, const char* from) const { return from + (TR ? off[0] + (uint32_t)i * gap : off[TR ? 0 : i]); }
+    __device__ __forceinline__ const char* step(int k) const { return base + (size_t)k * move; }
+    // Straight to LDS, piece i of a step that starts at `from`, to `lds` + the wave's part: whole pieces that start on 16
+    // bytes.  It takes `from` from scalar registers and the lane's 32-bit place as it is: with a sum of 64 bits before
+    // each load, loads took as much issue as MFMAs.
+    __device__ __forceinline__ void fetch(unsigned char* lds, int i, const char* from) const {
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(make_rsrc(from, 0xFFFFFFFFu), (__attribute__((address_space(3))) void*)(lds + i * THREADS * 16), 16,
+                                                 (int)(TR ? off[0] + (uint32_t)i * gap : off[TR ? 0 : i]), 0, 0, 0);
     }
-    // Straight to LDS: whole pieces that start on 16 bytes.  What lies past the contraction's n elements is zeros.
-    __device__ __forceinline__ void fetch(unsigned char* lds, int k, int n) const {
-        auto bring = [&](int i, const char* q) {
-            __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)q,
-                                             (__attribute__((address_space(3))) void*)(lds + i * THREADS * 16 + wave_id() * 1024), 16, 0, 0);
-        };
-        if ((k + 1) * kStep <= n) {
-#pragma unroll
-            for (int i = 0; i < P; ++i) bring(i, piece(i, k));
-        } else {
-#pragma unroll
-            for (int i = 0; i < P; ++i)
-                bring(i, k * kStep + first + (TR ? i * kStepRows : 0) < n ? piece(i, k) : reinterpret_cast<const char*>(mm_zeros));
-        }
+    // The same for any step k: what lies past the contraction's n elements is zeros.
+    __device__ __forceinline__ void fetch_to(unsigned char* lds, int i, int k, int n) const {
+        const char* q = k * kStep + first + (TR ? i * kStepRows : 0) < n ? piece(i, step(k)) : reinterpret_cast<const char*>(mm_zeros);
+        __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)q, (__attribute__((address_space(3))) void*)(lds + i * THREADS * 16), 16, 0, 0);
     }
     // Through registers: rows of any width at any address.
     __device__ __forceinline__ void load(u32x4 (&v)[P], int k, int n) const {
@@ -200,7 +200,7 @@ struct MmSrc {
 #pragma unroll
         for (int i = 0; i < P; ++i) {
             const int have = TR ? (k * kStep + first + i * kStepRows < n ? left : 0) : n - k * kStep - first;
-            const char* q = piece(i, k);
+            const char* q = piece(i, step(k));
             v[i] = u32x4{};
             if (have >= kWhole) {
                 v[i] = ((const __attribute__((address_space(1))) MmPacked*)q)->v;
@@ -222,148 +222,260 @@ struct MmSrc {
     }
 };
 
-// A wave's fragments of an operand, T of 32 rows (columns) from row r0 of the tile on.
-template <int R, int T, bool TR>
+__device__ __forceinline__ uint32_t mm_lds_addr(const unsigned char* p) {
+    return (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) unsigned char*)p;
+}
+
+// Fragment reads are written as asm: of plain loads the compiler cannot tell which slot a pending direct load
+// writes, and waits for all of them.  Every output is an operand of mm_wait, so it stays live and unread until the
+// read has landed.
+template <int OFF>
+__device__ __forceinline__ void mm_read16(u32x4& v, uint32_t at) {
+    static_assert(OFF >= 0 && OFF < 65536, "offset field");
+    asm volatile("ds_read_b128 %0, %1 offset:%2" : "=v"(v) : "v"(at), "i"(OFF));
+}
+template <int OFF>
+__device__ __forceinline__ void mm_read_tr(uint64_t& v, uint32_t at) {
+    static_assert(OFF >= 0 && OFF < 65536, "offset field");
+    asm volatile("ds_read_b64_tr_b16 %0, %1 offset:%2" : "=v"(v) : "v"(at), "i"(OFF));
+}
+
+// f(integral_constant 0), ..., f(integral_constant N - 1)
+template <int N, int I = 0, class F>
+__device__ __forceinline__ void mm_each(F f) {
+    if constexpr (I < N) {
+        f(std::integral_constant<int, I>{});
+        mm_each<N, I + 1>(f);
+    }
+}
+
+// A wave's fragments of an operand, T tiles of 16 rows (columns) from row r0 of the tile on, of 64 bytes (32 rows) of the
+// contraction: the halves S of a step.  TR: the four rows' halves of a fragment are reads of their own.
+template <int R, bool TR, int T>
 struct MmFrag {
-    uint32_t at[TR ? T : 4];
-    __device__ __forceinline__ MmFrag(int r0) {
-        const int l = threadIdx.x & 63;
+    static constexpr int kReads = TR ? 2 : 1, kPlaces = TR ? T : 2;
+    union Held {
+        u32x4 v;
+        uint64_t h[2];
+    };
+    uint32_t at[kPlaces];
+    __device__ __forceinline__ MmFrag(int r0, uint32_t lds) {
+        const int l = threadIdx.x & 63, g = l >> 4, i = l & 15;
         if constexpr (TR) {
-            const int g = l >> 4, i = l & 15;
 #pragma unroll
             for (int t = 0; t < T; ++t)
-                at[t] = (8 * (g >> 1) + (i >> 2)) * R * 2 + (((r0 / 16 + 2 * t + (g & 1)) ^ (2 * (i >> 2))) * 32) + (i & 3) * 8;
+                at[t] = lds + (8 * g + (i >> 2)) * R * 2 + (((r0 / 16 + t) ^ (2 * (i >> 2) + (g & 1))) * 32) + (i & 3) * 8;
         } else {
-            const int key = (l & 7) ^ ((l >> 3) & 1);
+            const int key = (i & 7) ^ (i >> 3);
 #pragma unroll
-            for (int s = 0; s < 4; ++s) at[s] = (r0 + (l & 31)) * 128 + (((2 * s + (l >> 5)) ^ key) * 16);
+            for (int s = 0; s < 2; ++s) at[s] = lds + (r0 + i) * 128 + (((4 * s + g) ^ key) * 16);
         }
     }
-    __device__ __forceinline__ void read(u32x4 (&f)[T], const unsigned char* lds, int s) const {
-#pragma unroll
-        for (int t = 0; t < T; ++t) {
-            if constexpr (TR) {
-                union {
-                    s16x4 h[2];
-                    u32x4 v;
-                } u;
-#pragma unroll
-                for (int h = 0; h < 2; ++h)
-                    u.h[h] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(lds + at[t] + (16 * s + 4 * h) * R * 2));
-                f[t] = u.v;
-            } else {
-                f[t] = *reinterpret_cast<const u32x4*>(lds + at[s] + t * 4096);
-            }
+    template <int S, int I>
+    __device__ __forceinline__ void read(Held& f, uint32_t slot) const {
+        if constexpr (TR) {
+            mm_read_tr<32 * S * R * 2>(f.h[0], at[I] + slot);
+            mm_read_tr<(32 * S + 4) * R * 2>(f.h[1], at[I] + slot);
+        } else {
+            mm_read16<I * 2048>(f.v, at[S] + slot);
         }
     }
 };
 
-// s_waitcnt vmcnt(0) lgkmcnt(0), then a barrier: what was fetched is there, and no wave still reads what was
-// read before.
-__device__ __forceinline__ void mm_turn() {
-    __builtin_amdgcn_s_waitcnt(0x70);
-    __builtin_amdgcn_s_barrier();
-    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
+// All LDS reads and writes of the wave have landed, those into the N fragments of `f` among them.
+template <int N, class H>
+__device__ __forceinline__ void mm_wait(H (&f)[N]) {
+#if defined(__HIP_DEVICE_COMPILE__)
+    asm volatile("s_waitcnt lgkmcnt(0)" : "+v"(f[0].v));
+#pragma unroll
+    for (int i = 1; i < N; ++i) asm volatile("" : "+v"(f[i].v));
+#endif
 }
 
-// acc[m][n] += A B over `steps` steps of 128 bytes (64 rows) of a contraction of n elements.  Steps go through two
-// buffers of LDS, which are two objects: the compiler then knows that reads of one need not wait for loads into the
-// other.  A step is four MFMA depths; the fragments of a depth are read while the depth before multiplies,
-// and a step's last depth multiplies while the next step's first fragments are read, behind the barrier.
+__device__ __forceinline__ void mm_barrier() {
+    __builtin_amdgcn_sched_barrier(0);
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
+}
+
+// acc[m][n] += A B over steps k0 .. k1 - 1 of 128 bytes (64 rows) of a contraction of n elements.
+//
+// Steps go through two rings of slots in LDS.  A step is four depths, both halves of the wave's m against all of its n for
+// both halves of the contraction; the fragments of a depth are read while the depth before it multiplies.  Before a step's last depth the wave waits for the next step's loads and passes the
+// barrier, behind which no wave reads this step any more; its last depth then multiplies while the next step's first
+// fragments are read.  Loads into the slots that became free go out one by one between MFMAs: of B at once, of A, whose ring is
+// a slot longer, during the next step.  With two slots of both (4096 rows by 4096 x 7168 in 241 us) the last loads came too late, and half lines
+// with five slots asked L2 for twice as much (271).
 template <class T, class S, bool AT, bool BT, bool DMA>
 __device__ __forceinline__ void mm_core(const MmSrc<S::BM, S::kThreads, T::kEl, AT>& a, const MmSrc<S::BN, S::kThreads, T::kEl, BT>& b,
-                                        int n, int k0, int k1, unsigned char* lds0, unsigned char* lds1, typename T::Acc (&acc)[S::TM][S::TN]) {
-    constexpr int kB = S::BM * 128;
+                                        int n, int k0, int k1, unsigned char* lds, typename T::Acc (&acc)[S::TM][S::TN]) {
+    typedef MmFrag<S::BM, AT, S::TM> FA;
+    typedef MmFrag<S::BN, BT, S::TN> FB;
+    constexpr int kLoadsA = S::BM * 8 / S::kThreads, kLoadsB = S::BN * 8 / S::kThreads;
+    constexpr int kHalf = S::TM / 2, kMma = kHalf * S::TN;
     const int wave = wave_id();
-    const MmFrag<S::BM, S::TM, AT> fa(wave % S::WM * S::TM * 32);
-    const MmFrag<S::BN, S::TN, BT> fb(wave / S::WM * S::TN * 32);
+    const FA fa(wave % S::WM * S::TM * 16, mm_lds_addr(lds));
+    const FB fb(wave / S::WM * S::TN * 16, mm_lds_addr(lds) + S::kEndM);
 #pragma unroll
     for (int m = 0; m < S::TM; ++m)
 #pragma unroll
         for (int t = 0; t < S::TN; ++t) acc[m][t] = typename T::Acc{};
     if (k0 >= k1) return;
     u32x4 va[MmSrc<S::BM, S::kThreads, T::kEl, AT>::P], vb[MmSrc<S::BN, S::kThreads, T::kEl, BT>::P];  // DMA: not used
-    auto fetch = [&](int k, unsigned char* buf) {
+    unsigned char *lds_b = lds + S::kEndM, *to_a = lds + wave * 1024, *to_b = lds_b + wave * 1024;
+    typename FA::Held xa[2][kHalf];  // of the depth and the next
+    typename FB::Held xb[2][S::TN];  // of the half of the contraction and the next
+    const char *pa = a.step(k0 + S::kSlots), *pb = b.step(k0 + S::kSlots - 1);  // of the next loads
+    // depth D of step k multiplies; the next one's fragments are read from slots `ra` and `rb` beside it, and a share of
+    // the loads that slots became free for goes out: B's in depths 3 and 0, A's in 1 and 2, evenly.  STEADY: they are of
+    // whole steps.
+    auto depth = [&](auto d, auto steady, int k, uint32_t ra, uint32_t rb, int to) {
+        constexpr int D = decltype(d)::value, N = (D + 1) & 3;
+        constexpr bool B = D == 3 || D == 0;
+        constexpr int kShare = (B ? kLoadsB : kLoadsA) / 2, kFirst = D == 0 || D == 2 ? kShare : 0, kGap = kMma / kShare;
+        constexpr int kReads = kHalf + (N & 1 ? 0 : S::TN);  // the next depth's half of m, and n where its half of the contraction is new
+        static_assert(kShare * kGap == kMma, "loads between MFMAs");
+        const int step = D == 0 ? k + S::kSlots - 1 : k + S::kSlots;
+        __builtin_amdgcn_s_setprio(1);
+        mm_each<kMma>([&](auto i) {
+            constexpr int m = i.value / S::TN, t = i.value % S::TN;
+            mm_each<kReads>([&](auto r) {  // at the first half of the MFMAs, evenly
+                if constexpr (r.value * (kMma / 2) / kReads == i.value) {
+                    if constexpr (r.value < kHalf)
+                        fa.template read<N / 2, N % 2 * kHalf + r.value>(xa[N % 2][r.value], ra);
+                    else
+                        fb.template read<N / 2, r.value - kHalf>(xb[N / 2][r.value - kHalf], rb);
+                }
+            });
+            if constexpr (DMA && i.value % kGap == 0) {
+                constexpr int j = kFirst + i.value / kGap;
+                if constexpr (decltype(steady)::value) {
+                    if constexpr (B)
+                        b.fetch(to_b + to, j, pb);
+                    else
+                        a.fetch(to_a + to, j, pa);
+                } else if (step < k1) {
+                    if constexpr (B)
+                        b.fetch_to(to_b + to, j, step, n);
+                    else
+                        a.fetch_to(to_a + to, j, step, n);
+                }
+            }
+            typename T::Acc& sum = acc[D % 2 * kHalf + m][t];
+            sum = T::mma(xa[D % 2][m].v, xb[D / 2][t].v, sum);
+            __builtin_amdgcn_sched_barrier(0);
+        });
+        __builtin_amdgcn_s_setprio(0);
+        mm_wait(xa[N % 2]);
+        if constexpr (N % 2 == 0) mm_wait(xb[N / 2]);
+    };
+    constexpr std::integral_constant<int, 0> d0{};
+    constexpr std::integral_constant<int, 1> d1{};
+    constexpr std::integral_constant<int, 2> d2{};
+    constexpr std::integral_constant<int, 3> d3{};
+    // step k + 1 has landed when only the loads of later steps are in flight
+    auto arrived = [&](int k) {
+        const int later = k1 - 2 - k;
+        if (later >= S::kSlots - 1)
+            vm_wait<(S::kSlots - 1) * kLoadsA + (S::kSlots - 2) * kLoadsB>();
+        else if (S::kSlots > 3 && later == 2)
+            vm_wait<2 * (kLoadsA + kLoadsB)>();
+        else if (S::kSlots > 2 && later == 1)
+            vm_wait<kLoadsA + kLoadsB>();
+        else
+            vm_wait<0>();
+    };
+    static_assert(S::kSlots >= 2 && S::kSlots <= 4, "arrived()");
+    if constexpr (DMA) {
+#pragma unroll
+        for (int i = 0; i < S::kSlots; ++i) {
+            if (k0 + i >= k1) break;
+#pragma unroll
+            for (int j = 0; j < kLoadsA; ++j) a.fetch_to(to_a + i * S::kStepM, j, k0 + i, n);
+#pragma unroll
+            for (int j = 0; j < (i < S::kSlots - 1 ? kLoadsB : kLoadsB / 2); ++j) b.fetch_to(to_b + i * S::kStepN, j, k0 + i, n);
+        }
+        if (k1 - k0 >= S::kSlots)
+            vm_wait<(S::kSlots - 1) * kLoadsA + (S::kSlots - 2) * kLoadsB + kLoadsB / 2>();
+        else
+            vm_wait<0>();
+    } else {
+        a.load(va, k0, n);
+        b.load(vb, k0, n);
+        a.put(lds, va);
+        b.put(lds_b, vb);
+        if (k0 + 1 < k1) {
+            a.load(va, k0 + 1, n);
+            b.load(vb, k0 + 1, n);
+        }
+        __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0)
+    }
+    mm_barrier();
+    mm_each<kHalf>([&](auto r) { fa.template read<0, r.value>(xa[0][r.value], 0); });
+    mm_each<S::TN>([&](auto r) { fb.template read<0, r.value>(xb[0][r.value], 0); });
+    mm_wait(xa[0]);
+    mm_wait(xb[0]);
+    int sa = 0, sb = 0, was_a = S::kEndM - S::kStepM, was_b = (S::kSlots - 1) * S::kStepN;  // slots of the step, and of the one before it
+    auto step = [&](auto steady, int k) {
+        const int na = sa + S::kStepM == S::kEndM ? 0 : sa + S::kStepM, nb = sb + S::kStepN == S::kSlots * S::kStepN ? 0 : sb + S::kStepN;
+        depth(d0, steady, k, sa, sb, was_b);
+        pb += b.move;
+        depth(d1, steady, k, sa, sb, was_a);
+        if (!DMA && k + 1 < k1) {
+            a.put(lds + na, va);
+            b.put(lds_b + nb, vb);
+        }
+        depth(d2, steady, k, sa, sb, was_a);
+        pa += a.move;
         if constexpr (DMA) {
-            a.fetch(buf, k, n);
-            b.fetch(buf + kB, k, n);
-        } else {
-            a.load(va, k, n);
-            b.load(vb, k, n);
+            if constexpr (decltype(steady)::value)
+                vm_wait<(S::kSlots - 1) * kLoadsA + (S::kSlots - 2) * kLoadsB>();
+            else
+                arrived(k);
         }
-    };
-    auto put = [&](unsigned char* buf) {
-        if constexpr (!DMA) {
-            a.put(buf, va);
-            b.put(buf + kB, vb);
+        mm_barrier();
+        if (!DMA && k + 2 < k1) {
+            a.load(va, k + 2, n);
+            b.load(vb, k + 2, n);
         }
-    };
-    u32x4 xa[2][S::TM], xb[2][S::TN];
-    auto read = [&](int s, const unsigned char* buf) {
-        fa.read(xa[s & 1], buf, s);
-        fb.read(xb[s & 1], buf + kB, s);
-    };
-    auto multiply = [&](int s) {
+        __builtin_amdgcn_sched_barrier(0);
+        depth(d3, steady, k, na, nb, sb);  // past the last step it reads what lies in the rings, not used
+#if defined(__HIP_DEVICE_COMPILE__)  // keeps the sums where they are: no copies of them at the loop's end
 #pragma unroll
         for (int m = 0; m < S::TM; ++m)
 #pragma unroll
-            for (int t = 0; t < S::TN; ++t) acc[m][t] = T::mma(xa[s & 1][m], xb[s & 1][t], acc[m][t]);
-#if defined(__HIP_DEVICE_COMPILE__)  // keeps the sums where they are: no copies of them at the loop's end
-        if (s == 3)
-#pragma unroll
-            for (int m = 0; m < S::TM; ++m)
-#pragma unroll
-                for (int t = 0; t < S::TN; ++t) asm volatile("" : "+v"(acc[m][t]));
+            for (int t = 0; t < S::TN; ++t) asm volatile("" : "+v"(acc[m][t]));
 #endif
+        was_a = sa;
+        was_b = sb;
+        sa = na;
+        sb = nb;
     };
-    auto step = [&](int k, unsigned char* buf, unsigned char* other) {
-        if (!DMA && k + 1 < k1) fetch(k + 1, other);
-#pragma unroll
-        for (int s = 0; s < 3; ++s) {
-            __builtin_amdgcn_sched_barrier(0);
-            read(s + 1, buf);
-            multiply(s);
-        }
-        __builtin_amdgcn_sched_barrier(0);
-        if (!DMA && k + 1 < k1) put(other);
-        mm_turn();
-        if (DMA && k + 2 < k1) fetch(k + 2, buf);
-        if (k + 1 < k1) read(0, other);
-        multiply(3);
-    };
-    fetch(k0, lds0);
-    put(lds0);
-    mm_turn();
-    if (DMA && k0 + 1 < k1) fetch(k0 + 1, lds1);
-    read(0, lds0);
     int k = k0;
-    for (; k + 1 < k1; k += 2) {
-        step(k, lds0, lds1);
-        step(k + 1, lds1, lds0);
-    }
-    if (k < k1) step(k, lds0, lds1);
+    if constexpr (DMA)
+        for (const int whole = min(k1, n / MmSrc<S::BM, S::kThreads, T::kEl, AT>::kStep); k + S::kSlots < whole; ++k) step(std::true_type{}, k);
+    for (; k < k1; ++k) step(std::false_type{}, k);
+    mm_barrier();
 }
 
-// 32 rows of W * 32 outputs, from a wave's results through its own part of LDS, so that it stores whole lines.
-// v: results whose m is consecutive; row(n) is where in `out` row n starts (elements), < 0: not stored.
-template <int W, class F>
-__device__ __forceinline__ void mm_put(const f32x16 (&v)[W], float* turn, void* out, int type, bool vec, int m0, int width, F row) {
-    constexpr int kChunks = W * 8;  // of four floats
-    const int l = threadIdx.x & 63, n = l & 31;
+// 16 rows of W * 16 outputs, from a wave's results through its own part of LDS (W KB), so that it stores whole lines.
+// v(w, i): element i of result w, whose m follow each other; row(n) is where in `out` row n starts (elements), < 0: not stored.
+template <int W, class V, class F>
+__device__ __forceinline__ void mm_put(V v, float* turn, void* out, int type, bool vec, int m0, int width, F row) {
+    constexpr int kChunks = W * 4;  // of four floats
+    const int l = threadIdx.x & 63, n = l & 15;
 #pragma unroll
     for (int w = 0; w < W; ++w)
-#pragma unroll
-        for (int g = 0; g < 4; ++g) {
-            const int c = w * 8 + 2 * g + (l >> 5);
-            *reinterpret_cast<f32x4*>(turn + n * W * 32 + (c ^ (n & (kChunks - 1))) * 4) = f32x4{v[w][4 * g], v[w][4 * g + 1], v[w][4 * g + 2], v[w][4 * g + 3]};
-        }
+        *reinterpret_cast<f32x4*>(turn + n * W * 16 + ((w * 4 + (l >> 4)) ^ (n & (kChunks - 1))) * 4) = f32x4{v(w, 0), v(w, 1), v(w, 2), v(w, 3)};
     __builtin_amdgcn_wave_barrier();
-    const int per = type == CX_DTYPE_F32 ? 4 : 8, lanes = W * 32 / per;  // columns of a lane's store, lanes of a row
-    for (int i = l; i < 32 * lanes; i += 64) {
+    const int per = type == CX_DTYPE_F32 ? 4 : 8, lanes = W * 16 / per;  // columns of a lane's store, lanes of a row
+    for (int i = l; i < 16 * lanes; i += 64) {
         const int r = i / lanes, c = (i - r * lanes) * per, left = width - m0 - c;
         const int64_t at = row(r);
         if (at < 0 || left <= 0) continue;
-        const float* src = turn + r * W * 32;
+        const float* src = turn + r * W * 16;
         const f32x4 a = *reinterpret_cast<const f32x4*>(src + ((c / 4) ^ (r & (kChunks - 1))) * 4);
         if (type == CX_DTYPE_F32) {
             float* y = static_cast<float*>(out) + at + m0 + c;
@@ -416,13 +528,13 @@ __device__ __forceinline__ bool mm_vec(const void* p, int width, int type) {
 // half per wave, so that both factors of an output meet in one lane.
 template <class T, class S, bool GATED, bool DMA>
 __global__ __launch_bounds__(S::kThreads, 2) void k_mm(MmLaunch L) {
-    __shared__ __attribute__((aligned(16))) unsigned char lds0[S::kStage], lds1[S::kStage];
-    static_assert(S::kWaves * 8192 <= S::kStage, "turned results");
+    __shared__ __attribute__((aligned(16))) unsigned char lds[S::kLds];
+    static_assert(S::kWaves * S::TM * 1024 <= S::kLds, "turned results");
     constexpr int kOut = GATED ? S::BM / 2 : S::BM;  // columns of y
     const MmTile tile = mm_tile(blockIdx.x, L.m_tiles, L.by_item);
     if (L.offsets != nullptr && blockIdx.x == 0 && wave_id() == 0) mm_check(L.offsets, L.n_mats, L.n_rows, L.err_flag);
     if (tile.m >= L.m_tiles) return;
-    const MmItem it = mm_item<32>(L.offsets, L.n_mats, L.n_rows, S::BN, tile.item);
+    const MmItem it = mm_item<16>(L.offsets, L.n_mats, L.n_rows, S::BN, tile.item);
     if (it.rows <= 0) return;
     const int width = GATED ? L.rows / 2 : L.rows, m0 = tile.m * kOut;
     if (it.mat < 0) {
@@ -438,7 +550,7 @@ __global__ __launch_bounds__(S::kThreads, 2) void k_mm(MmLaunch L) {
     // weight rows from the tile's first on; those past the matrix are its last one again, and not stored
     constexpr int half = S::TM / 2;  // gated: results of gate rows
     a.rows(static_cast<const char*>(L.w) + ((size_t)it.mat * L.rows + m0) * pitch, [&](int r) {
-        const int n = GATED ? min(m0 + (r / (S::TM * 32) * half + r / 32 % half) * 32 + r % 32, width - 1) + (r / 32 % S::TM < half ? 0 : width)
+        const int n = GATED ? min(m0 + (r / (S::TM * 16) * half + r / 16 % half) * 16 + r % 16, width - 1) + (r / 16 % S::TM < half ? 0 : width)
                             : min(m0 + r, width - 1);
         return (uint32_t)(n - m0) * (uint32_t)pitch;
     });
@@ -452,57 +564,44 @@ __global__ __launch_bounds__(S::kThreads, 2) void k_mm(MmLaunch L) {
     const int x0 = L.order == nullptr ? it.begin : 0;
     b.rows(static_cast<const char*>(L.x) + (size_t)x0 * pitch, [&](int r) { return (uint32_t)(max(source(r), x0) - x0) * (uint32_t)pitch; });
     typename T::Acc acc[S::TM][S::TN];
-    mm_core<T, S, false, false, DMA>(a, b, L.cols, 0, (L.cols + 128 / T::kEl - 1) / (128 / T::kEl), lds0, lds1, acc);
+    mm_core<T, S, false, false, DMA>(a, b, L.cols, 0, (L.cols + 128 / T::kEl - 1) / (128 / T::kEl), lds, acc);
     // results to y
-    const int wave = wave_id(), l = threadIdx.x & 63, wm = wave % S::WM, n0 = wave / S::WM * S::TN * 32;
-    float* turn = reinterpret_cast<float*>(lds0 + wave * 8192);
-    f32x16 v[S::TM];
+    const int wave = wave_id(), l = threadIdx.x & 63, wm = wave % S::WM, n0 = wave / S::WM * S::TN * 16;
+    float* turn = reinterpret_cast<float*>(lds + wave * S::TM * 1024);
+    const int mw = m0 + wm * (GATED ? half : S::TM) * 16;  // of the wave
+    f32x4 ws[T::kEl == 1 ? S::TM : 1];
+    if constexpr (T::kEl == 1) {
+#pragma unroll
+        for (int m = 0; m < S::TM; ++m)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int c = 4 * (l >> 4) + i;
+                ws[m][i] = L.w_scale[(size_t)it.mat * L.rows + (GATED ? min(mw + m % half * 16 + c, width - 1) + (m < half ? 0 : width) : min(mw + m * 16 + c, width - 1))];
+            }
+    }
+    const bool vec = mm_vec(L.y, width, L.y_type), pvec = GATED && L.pre != nullptr && mm_vec(L.pre, width, T::kType);
 #pragma unroll
     for (int t = 0; t < S::TN; ++t) {
-        const int nt = n0 + t * 32;
+        const int nt = n0 + t * 16;
         if (nt >= it.rows) break;
-        const int xr = source(nt + (l & 31));
+        const int xr = source(nt + (l & 15));
         const float xs = T::kEl == 1 ? (xr < 0 ? 0.0f : L.x_scale[xr]) : 1.0f;
-#pragma unroll
-        for (int m = 0; m < S::TM; ++m) {
-#pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                float f = (float)acc[m][t][i];
-                if constexpr (T::kEl == 1) {
-                    const int c = 8 * (i >> 2) + 4 * (l >> 5) + (i & 3);
-                    const int n = GATED ? min(m0 + (wm * half + m % half) * 32 + c, width - 1) + (m < half ? 0 : width)
-                                        : min(m0 + (wm * S::TM + m) * 32 + c, width - 1);
-                    f = f * xs * L.w_scale[(size_t)it.mat * L.rows + n];
-                }
-                v[m][i] = xr < 0 ? 0.0f : f;
-            }
-        }
+        auto value = [&](int m, int i) {
+            float f = (float)acc[m][t][i];
+            if constexpr (T::kEl == 1) f = f * xs * ws[m][i];
+            return xr < 0 ? 0.0f : f;
+        };
         auto row = [&](int64_t w, int64_t off) {
             return [=](int r) { return nt + r < it.rows ? (int64_t)(it.begin + nt + r) * w + off : (int64_t)-1; };
         };
         if constexpr (GATED) {
-            f32x16 g[half], u[half], h[half];
-#pragma unroll
-            for (int m = 0; m < half; ++m) {
-                g[m] = v[m];
-                u[m] = v[half + m];
-#pragma unroll
-                for (int i = 0; i < 16; ++i) h[m][i] = mm_silu(g[m][i]) * u[m][i];
-            }
-            const int mw = m0 + wm * half * 32;
             if (L.pre != nullptr) {
-                const bool vec = mm_vec(L.pre, width, T::kType);
-                mm_put<half>(g, turn, L.pre, T::kType, vec, mw, width, row(2 * (int64_t)width, 0));
-                mm_put<half>(u, turn, L.pre, T::kType, vec, mw, width, row(2 * (int64_t)width, width));
+                mm_put<half>([&](int w, int i) { return value(w, i); }, turn, L.pre, T::kType, pvec, mw, width, row(2 * (int64_t)width, 0));
+                mm_put<half>([&](int w, int i) { return value(half + w, i); }, turn, L.pre, T::kType, pvec, mw, width, row(2 * (int64_t)width, width));
             }
-            mm_put<half>(h, turn, L.y, L.y_type, mm_vec(L.y, width, L.y_type), mw, width, row(width, 0));
+            mm_put<half>([&](int w, int i) { return mm_silu(value(w, i)) * value(half + w, i); }, turn, L.y, L.y_type, vec, mw, width, row(width, 0));
         } else {
-            const bool vec = mm_vec(L.y, width, L.y_type);
-#pragma unroll
-            for (int m = 0; m < S::TM; m += 2) {
-                f32x16 o[2] = {v[m], v[m + 1]};
-                mm_put<2>(o, turn, L.y, L.y_type, vec, m0 + (wm * S::TM + m) * 32, width, row(width, 0));
-            }
+            mm_put<S::TM>(value, turn, L.y, L.y_type, vec, mw, width, row(width, 0));
         }
     }
 }
@@ -510,11 +609,11 @@ __global__ __launch_bounds__(S::kThreads, 2) void k_mm(MmLaunch L) {
 // The gradient at x.  m: columns of the weights, read across their rows; n: rows of dy.
 template <class T, class S, bool DMA>
 __global__ __launch_bounds__(S::kThreads, 2) void k_mm_dx(MmLaunch L) {
-    __shared__ __attribute__((aligned(16))) unsigned char lds0[S::kStage], lds1[S::kStage];
+    __shared__ __attribute__((aligned(16))) unsigned char lds[S::kLds];
     const MmTile tile = mm_tile(blockIdx.x, L.m_tiles, L.by_item);
     if (L.offsets != nullptr && blockIdx.x == 0 && wave_id() == 0) mm_check(L.offsets, L.n_mats, L.n_rows, L.err_flag);
     if (tile.m >= L.m_tiles) return;
-    const MmItem it = mm_item<32>(L.offsets, L.n_mats, L.n_rows, S::BN, tile.item);
+    const MmItem it = mm_item<16>(L.offsets, L.n_mats, L.n_rows, S::BN, tile.item);
     if (it.rows <= 0) return;
     const int width = L.cols, m0 = tile.m * S::BM;
     if (it.mat < 0) return mm_clear(L.y, L.y_type, it.begin, it.rows, width, m0, S::BM, S::kThreads);
@@ -522,28 +621,24 @@ __global__ __launch_bounds__(S::kThreads, 2) void k_mm_dx(MmLaunch L) {
     MmSrc<S::BN, S::kThreads, 2, false> b;
     a.cols(static_cast<const char*>(L.w) + (size_t)it.mat * L.rows * L.cols * 2, m0, width);
     b.rows(static_cast<const char*>(L.dy) + (size_t)it.begin * L.rows * 2, [&](int r) { return (uint32_t)min(r, it.rows - 1) * (uint32_t)L.rows * 2; });
-    f32x16 acc[S::TM][S::TN];
-    mm_core<T, S, true, false, DMA>(a, b, L.rows, 0, (L.rows + 63) / 64, lds0, lds1, acc);
-    const int wave = wave_id(), n0 = wave / S::WM * S::TN * 32;
-    float* turn = reinterpret_cast<float*>(lds0 + wave * 8192);
+    f32x4 acc[S::TM][S::TN];
+    mm_core<T, S, true, false, DMA>(a, b, L.rows, 0, (L.rows + 63) / 64, lds, acc);
+    const int wave = wave_id(), n0 = wave / S::WM * S::TN * 16;
+    float* turn = reinterpret_cast<float*>(lds + wave * S::TM * 1024);
     const bool vec = mm_vec(L.y, width, L.y_type);
 #pragma unroll
     for (int t = 0; t < S::TN; ++t) {
-        const int nt = n0 + t * 32;
+        const int nt = n0 + t * 16;
         if (nt >= it.rows) break;
-#pragma unroll
-        for (int m = 0; m < S::TM; m += 2) {
-            f32x16 o[2] = {acc[m][t], acc[m + 1][t]};
-            mm_put<2>(o, turn, L.y, L.y_type, vec, m0 + (wave % S::WM * S::TM + m) * 32, width,
+        mm_put<S::TM>([&](int m, int i) { return acc[m][t][i]; }, turn, L.y, L.y_type, vec, m0 + wave % S::WM * S::TM * 16, width,
                       [&](int r) { return nt + r < it.rows ? (int64_t)(it.begin + nt + r) * width : (int64_t)-1; });
-        }
     }
 }
 
 // The gradient at the weights of each matrix.  m: their columns; n: their rows.
 template <class T, class S, bool DMA>
 __global__ __launch_bounds__(S::kThreads, 2) void k_mm_dw(MmLaunch L) {
-    __shared__ __attribute__((aligned(16))) unsigned char lds0[S::kStage], lds1[S::kStage];
+    __shared__ __attribute__((aligned(16))) unsigned char lds[S::kLds];
     if (L.offsets != nullptr && blockIdx.x == 0 && wave_id() == 0) mm_check(L.offsets, L.n_mats, L.n_rows, L.err_flag);
     const int n_tiles = (L.rows + S::BN - 1) / S::BN, per = n_tiles * L.m_tiles, mat = blockIdx.x / per, i = blockIdx.x - mat * per;
     const int n0 = i / L.m_tiles * S::BN, m0 = (i - i / L.m_tiles * L.m_tiles) * S::BM;
@@ -552,21 +647,17 @@ __global__ __launch_bounds__(S::kThreads, 2) void k_mm_dw(MmLaunch L) {
     MmSrc<S::BN, S::kThreads, 2, true> b;
     a.cols(static_cast<const char*>(L.x) + (size_t)it.begin * L.cols * 2, m0, L.cols);
     b.cols(static_cast<const char*>(L.dy) + (size_t)it.begin * L.rows * 2, n0, L.rows);
-    f32x16 acc[S::TM][S::TN];
-    mm_core<T, S, true, true, DMA>(a, b, it.rows, 0, (it.rows + 63) / 64, lds0, lds1, acc);
-    const int wave = wave_id(), nw = n0 + wave / S::WM * S::TN * 32;
-    float* turn = reinterpret_cast<float*>(lds0 + wave * 8192);
+    f32x4 acc[S::TM][S::TN];
+    mm_core<T, S, true, true, DMA>(a, b, it.rows, 0, (it.rows + 63) / 64, lds, acc);
+    const int wave = wave_id(), nw = n0 + wave / S::WM * S::TN * 16;
+    float* turn = reinterpret_cast<float*>(lds + wave * S::TM * 1024);
     const bool vec = mm_vec(L.y, L.cols, L.y_type);
 #pragma unroll
     for (int t = 0; t < S::TN; ++t)
-#pragma unroll
-        for (int m = 0; m < S::TM; m += 2) {
-            f32x16 o[2] = {acc[m][t], acc[m + 1][t]};
-            mm_put<2>(o, turn, L.y, L.y_type, vec, m0 + (wave % S::WM * S::TM + m) * 32, L.cols, [&](int r) {
-                const int n = nw + t * 32 + r;
-                return n < L.rows ? ((int64_t)mat * L.rows + n) * L.cols : (int64_t)-1;
-            });
-        }
+        mm_put<S::TM>([&](int m, int i) { return acc[m][t][i]; }, turn, L.y, L.y_type, vec, m0 + wave % S::WM * S::TM * 16, L.cols, [&](int r) {
+            const int n = nw + t * 16 + r;
+            return n < L.rows ? ((int64_t)mat * L.rows + n) * L.cols : (int64_t)-1;
+        });
 }
 
 }  // namespace cx

@@ -4,8 +4,8 @@
 namespace cx {
 namespace {
 
-using Big = MmShape<2, 4, 4, 2>;
-using Small = MmShape<2, 2, 2, 2>;
+using Big = MmShape<2, 4, 8, 4, 2>;
+using Small = MmShape<2, 2, 4, 4, 2>;
 
 template <class T, class S, bool GATED, bool DMA>
 hipError_t run(MmLaunch& L, hipStream_t s) {

@@ -6,24 +6,6 @@
 
 namespace cx {
 
-// 16 x 16 products of 16 bytes a lane: lane l holds row l % 16, piece l / 16 of 64 bytes; a result's
-// element i is weight row 4 (l / 16) + i, row l % 16 of x.
-template <class T>
-struct MmTile16 {
-    typedef f32x4 Acc;
-    static __device__ __forceinline__ Acc mma(u32x4 a, u32x4 b, Acc c) {
-        return T::kType == CX_DTYPE_BF16 ? Mma<false>::mma(Mma<false>::bits(a), Mma<false>::bits(b), c)
-                                         : Mma<true>::mma(Mma<true>::bits(a), Mma<true>::bits(b), c);
-    }
-};
-template <>
-struct MmTile16<MmI8> {
-    typedef i32x4 Acc;
-    static __device__ __forceinline__ Acc mma(u32x4 a, u32x4 b, Acc c) {
-        return __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(i32x4, a), __builtin_bit_cast(i32x4, b), c, 0, 0, 0);
-    }
-};
-
 // 16 bytes of a row, `have` elements of which exist.  VEC: all or none of them, at an address that 16 divides.
 template <int EL, bool VEC>
 __device__ __forceinline__ u32x4 mm_piece(const char* q, int have) {
@@ -51,7 +33,7 @@ __device__ __forceinline__ u32x4 mm_piece(const char* q, int have) {
 // U that it multiplies, of weights and of up to 16 NB rows of x, which come from L2.
 template <class T, int NB, int RW, bool GATED, bool VEC>
 __global__ __launch_bounds__(64 * kMmFewWaves, 2) void k_mm_few(MmLaunch L, int splits, int row_blocks) {
-    typedef typename MmTile16<T>::Acc Acc;
+    typedef typename T::Acc Acc;
     constexpr int EL = T::kEl, kStep = 128 / EL, U = !VEC ? 1 : NB == 1 && RW == 1 ? 4 : NB * RW <= 4 ? 2 : 1;
     __shared__ __attribute__((aligned(16))) uint32_t red[kMmFewWaves][RW][NB][256];
     const int idx = blockIdx.x / row_blocks, block = blockIdx.x - idx * row_blocks;
@@ -114,7 +96,7 @@ __global__ __launch_bounds__(64 * kMmFewWaves, 2) void k_mm_few(MmLaunch L, int 
                 for (int b = 0; b < NB; ++b) {
                     if (b > 0 && 16 * b >= it.rows) break;
 #pragma unroll
-                    for (int m = 0; m < RW; ++m) acc[m][b] = MmTile16<T>::mma(a[from][u][m][j], x[from][u][b][j], acc[m][b]);
+                    for (int m = 0; m < RW; ++m) acc[m][b] = T::mma(a[from][u][m][j], x[from][u][b][j], acc[m][b]);
                 }
         }
     };
