@@ -5,24 +5,20 @@
 namespace cx {
 namespace {
 
-using Big = MmShape<2, 4, 8, 4, 2>;
-using Small = MmShape<2, 2, 4, 4, 2>;
-
 template <class S, bool GATED, bool DMA>
 hipError_t run(MmLaunch& L, hipStream_t s) {
     const int out = GATED ? S::BM / 2 : S::BM, width = GATED ? L.rows / 2 : L.rows;
     L.m_tiles = (width + out - 1) / out;
-    cx_launch(k_mm<MmI8, S, GATED, DMA>, dim3(mm_grid(L, S::BN)), dim3(S::kThreads), 0, s, L);
+    cx_launch(k_mm<MmI8, S, GATED, DMA>, dim3(mm_grid(L)), dim3(S::kThreads), 0, s, L);
     return hipGetLastError();
 }
 
 template <bool GATED>
 hipError_t pick(MmLaunch& L, hipStream_t s) {
-    const bool dma = L.cols % 16 == 0 && mm_at16(L.x) && mm_at16(L.w);
-    const MmFew f = mm_few_form(L.n_rows, L.n_mats, L.rows, L.cols, 1);
-    if (f.rows > 0) return mm_few<MmI8, GATED>(L, f, dma, s);
-    if (!dma) return run<Small, GATED, false>(L, s);
-    return mm_big(L.n_rows, L.offsets ? L.n_mats : 1, L.rows) ? run<Big, GATED, true>(L, s) : run<Small, GATED, true>(L, s);
+    const bool wide = mm_wide(L);
+    if (L.form.kind == 0) return mm_few<MmI8, GATED>(L, wide, s);
+    const hipError_t e = !wide ? run<MmSmall, GATED, false>(L, s) : L.form.kind == 2 ? run<MmBig, GATED, true>(L, s) : run<MmSmall, GATED, true>(L, s);
+    return e != hipSuccess || L.splits == 1 ? e : launch_mm_sum(L, L.rows, GATED, s);
 }
 
 constexpr int kI8Threads = 256, kI8Held = 4;  // pieces of 8 values of a row that a thread holds

@@ -513,7 +513,10 @@ struct MmLaunch {
     int y_type;              // CX_DTYPE_*
     void* pre;               // gated, nullable: the sums themselves [n_rows, rows], in `type`
     int* err_flag;
+    MmForm form;
+    float* part;             // splits > 1: [splits][n_rows][rows] (at x: cols), sums of fp32, or of integers as their bits
     int m_tiles, by_item;    // tiles in the output's contiguous direction; mm_tile's order
+    int item_rows, splits;
 };
 // Workgroup b runs on XCD b % 8.  by_item: an item's tiles run on one XCD, whose L2 then holds its rows of x (stacks);
 // otherwise tile m of every item does, and its L2 holds the weights (one matrix).
@@ -528,14 +531,20 @@ __host__ __device__ inline MmTile mm_tile(unsigned b, int m_tiles, int by_item) 
     const int pitch = (m_tiles + 7) / 8 * 8;
     return MmTile{(int)b / pitch, (int)b % pitch};
 }
-inline unsigned mm_grid(MmLaunch& L, int item_rows) {
-    const int64_t items = mm_items(L.n_rows, L.n_mats, L.offsets != nullptr, item_rows);
+inline unsigned mm_grid(MmLaunch& L) {
+    L.item_rows = L.form.item_rows;
+    L.splits = L.form.splits;
     L.by_item = L.offsets != nullptr;
-    return (unsigned)(L.by_item ? (items + 7) / 8 * 8 * L.m_tiles : items * ((L.m_tiles + 7) / 8 * 8));
+    const int64_t items = mm_items(L.n_rows, L.n_mats, L.offsets != nullptr, L.item_rows), m = (int64_t)L.m_tiles * L.splits;
+    return (unsigned)(L.by_item ? (items + 7) / 8 * 8 * m : items * ((m + 7) / 8 * 8));
 }
 inline bool mm_at16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+// Whole pieces of 16 bytes, which go straight to LDS.
+inline bool mm_wide(const MmLaunch& L) { return L.cols % (L.type == kMmI8 ? 16 : 8) == 0 && mm_at16(L.x) && mm_at16(L.w); }
+inline bool mm_wide_dx(const MmLaunch& L) { return L.cols % 8 == 0 && L.rows % 8 == 0 && mm_at16(L.w) && mm_at16(L.dy); }
 hipError_t launch_mm(MmLaunch L, hipStream_t s);
 hipError_t launch_mm_i8(MmLaunch L, hipStream_t s);
+hipError_t launch_mm_sum(const MmLaunch& L, int out, bool gated, hipStream_t s);
 hipError_t launch_mm_dx(MmLaunch L, hipStream_t s);
 hipError_t launch_mm_dw(MmLaunch L, hipStream_t s);
 // dpre of silu(g) * u from dh and pre = [g, u], rounded to their type: [n_rows, 2 * inter].

@@ -334,9 +334,8 @@ __device__ __forceinline__ void mm_core(const MmSrc<S::BM, S::kThreads, T::kEl, 
     auto depth = [&](auto d, auto steady, int k, uint32_t ra, uint32_t rb, int to) {
         constexpr int D = decltype(d)::value, N = (D + 1) & 3;
         constexpr bool B = D == 3 || D == 0;
-        constexpr int kShare = (B ? kLoadsB : kLoadsA) / 2, kFirst = D == 0 || D == 2 ? kShare : 0, kGap = kMma / kShare;
+        constexpr int kAll = B ? kLoadsB : kLoadsA, kFirst = D == 0 || D == 2 ? (kAll + 1) / 2 : 0, kShare = D == 0 || D == 2 ? kAll / 2 : (kAll + 1) / 2;
         constexpr int kReads = kHalf + (N & 1 ? 0 : S::TN);  // the next depth's half of m, and n where its half of the contraction is new
-        static_assert(kShare * kGap == kMma, "loads between MFMAs");
         const int step = D == 0 ? k + S::kSlots - 1 : k + S::kSlots;
         __builtin_amdgcn_s_setprio(1);
         mm_each<kMma>([&](auto i) {
@@ -349,20 +348,22 @@ __device__ __forceinline__ void mm_core(const MmSrc<S::BM, S::kThreads, T::kEl, 
                         fb.template read<N / 2, r.value - kHalf>(xb[N / 2][r.value - kHalf], rb);
                 }
             });
-            if constexpr (DMA && i.value % kGap == 0) {
-                constexpr int j = kFirst + i.value / kGap;
-                if constexpr (decltype(steady)::value) {
-                    if constexpr (B)
-                        b.fetch(to_b + to, j, pb);
-                    else
-                        a.fetch(to_a + to, j, pa);
-                } else if (step < k1) {
-                    if constexpr (B)
-                        b.fetch_to(to_b + to, j, step, n);
-                    else
-                        a.fetch_to(to_a + to, j, step, n);
-                }
-            }
+            if constexpr (DMA)
+                mm_each<kShare>([&](auto r) {
+                    constexpr int j = kFirst + r.value;
+                    if constexpr (r.value * kMma / kShare != i.value) return;
+                    if constexpr (decltype(steady)::value) {
+                        if constexpr (B)
+                            b.fetch(to_b + to, j, pb);
+                        else
+                            a.fetch(to_a + to, j, pa);
+                    } else if (step < k1) {
+                        if constexpr (B)
+                            b.fetch_to(to_b + to, j, step, n);
+                        else
+                            a.fetch_to(to_a + to, j, step, n);
+                    }
+                });
             typename T::Acc& sum = acc[D % 2 * kHalf + m][t];
             sum = T::mma(xa[D % 2][m].v, xb[D / 2][t].v, sum);
             __builtin_amdgcn_sched_barrier(0);
@@ -395,10 +396,10 @@ __device__ __forceinline__ void mm_core(const MmSrc<S::BM, S::kThreads, T::kEl, 
 #pragma unroll
             for (int j = 0; j < kLoadsA; ++j) a.fetch_to(to_a + i * S::kStepM, j, k0 + i, n);
 #pragma unroll
-            for (int j = 0; j < (i < S::kSlots - 1 ? kLoadsB : kLoadsB / 2); ++j) b.fetch_to(to_b + i * S::kStepN, j, k0 + i, n);
+            for (int j = 0; j < (i < S::kSlots - 1 ? kLoadsB : (kLoadsB + 1) / 2); ++j) b.fetch_to(to_b + i * S::kStepN, j, k0 + i, n);
         }
         if (k1 - k0 >= S::kSlots)
-            vm_wait<(S::kSlots - 1) * kLoadsA + (S::kSlots - 2) * kLoadsB + kLoadsB / 2>();
+            vm_wait<(S::kSlots - 1) * kLoadsA + (S::kSlots - 2) * kLoadsB + (kLoadsB + 1) / 2>();
         else
             vm_wait<0>();
     } else {
@@ -524,26 +525,53 @@ __device__ __forceinline__ bool mm_vec(const void* p, int width, int type) {
 }
 
 // ---------------------------------------------------------------------------
+// A shape with the fewest tiles in n that hold `rows`: a short item multiplies less.
+template <class S, int TN = 1, class F>
+__device__ __forceinline__ void mm_fit(int rows, F f) {
+    if constexpr (TN < S::TN) {
+        if (rows > S::WN * TN * 16) return mm_fit<S, TN + 1>(rows, f);
+    }
+    f(MmShape<S::WM, S::WN, S::TM, TN, S::kSlots>{});
+}
+
+// This workgroup's tile, range of the contraction and run of rows; false: none, or one of rows behind the last matrix,
+// which are cleared.
+struct MmWork {
+    MmItem it;
+    int m0, ks;
+};
+__device__ __forceinline__ bool mm_work(const MmLaunch& L, int tile_cols, int width, int threads, bool halves, MmWork* w) {
+    const MmTile tile = mm_tile(blockIdx.x, L.m_tiles * L.splits, L.by_item);
+    if (L.offsets != nullptr && blockIdx.x == 0 && wave_id() == 0) mm_check(L.offsets, L.n_mats, L.n_rows, L.err_flag);
+    if (tile.m >= L.m_tiles * L.splits) return false;
+    w->it = mm_item<16>(L.offsets, L.n_mats, L.n_rows, L.item_rows, tile.item);
+    w->ks = tile.m / L.m_tiles;
+    w->m0 = (tile.m - w->ks * L.m_tiles) * tile_cols;
+    if (w->it.rows <= 0) return false;
+    if (w->it.mat >= 0) return true;
+    if (L.splits == 1) {  // otherwise with the sums
+        mm_clear(L.y, L.y_type, w->it.begin, w->it.rows, width, w->m0, tile_cols, threads);
+        if (halves && L.pre != nullptr)
+            for (int h = 0; h < 2; ++h)
+                for (int r = 0; r < w->it.rows; ++r) mm_clear(L.pre, L.type, 2 * (int64_t)(w->it.begin + r) + h, 1, width, w->m0, tile_cols, threads);
+    }
+    return false;
+}
+
+// The row of x of row p (in the order, if there is one), < 0: none.
+__device__ __forceinline__ int mm_row_of_x(const MmLaunch& L, int p) {
+    if (L.order == nullptr) return p;
+    const int pair = L.order[p], xr = pair / L.top_k;
+    return pair < 0 || xr >= L.n_x ? -1 : xr;
+}
+
 // Forward.  m: weight rows; a gated tile has TM / 2 results of gate rows and the same rows of the up
 // half per wave, so that both factors of an output meet in one lane.
 template <class T, class S, bool GATED, bool DMA>
-__global__ __launch_bounds__(S::kThreads, 2) void k_mm(MmLaunch L) {
-    __shared__ __attribute__((aligned(16))) unsigned char lds[S::kLds];
+__device__ __forceinline__ void mm_forward(const MmLaunch& L, const MmWork& work, unsigned char* lds) {
     static_assert(S::kWaves * S::TM * 1024 <= S::kLds, "turned results");
-    constexpr int kOut = GATED ? S::BM / 2 : S::BM;  // columns of y
-    const MmTile tile = mm_tile(blockIdx.x, L.m_tiles, L.by_item);
-    if (L.offsets != nullptr && blockIdx.x == 0 && wave_id() == 0) mm_check(L.offsets, L.n_mats, L.n_rows, L.err_flag);
-    if (tile.m >= L.m_tiles) return;
-    const MmItem it = mm_item<16>(L.offsets, L.n_mats, L.n_rows, S::BN, tile.item);
-    if (it.rows <= 0) return;
-    const int width = GATED ? L.rows / 2 : L.rows, m0 = tile.m * kOut;
-    if (it.mat < 0) {
-        mm_clear(L.y, L.y_type, it.begin, it.rows, width, m0, kOut, S::kThreads);
-        if (GATED && L.pre != nullptr)
-            for (int h = 0; h < 2; ++h)
-                for (int r = 0; r < it.rows; ++r) mm_clear(L.pre, T::kType, 2 * (int64_t)(it.begin + r) + h, 1, width, m0, kOut, S::kThreads);
-        return;
-    }
+    const MmItem it = work.it;
+    const int width = GATED ? L.rows / 2 : L.rows, m0 = work.m0;
     MmSrc<S::BM, S::kThreads, T::kEl, false> a;
     MmSrc<S::BN, S::kThreads, T::kEl, false> b;
     const size_t pitch = (size_t)L.cols * T::kEl;
@@ -554,21 +582,41 @@ __global__ __launch_bounds__(S::kThreads, 2) void k_mm(MmLaunch L) {
                             : min(m0 + r, width - 1);
         return (uint32_t)(n - m0) * (uint32_t)pitch;
     });
-    // the row of x of row r of the item, < 0: none, and row 0 is read in its place
-    auto source = [&](int r) {
-        const int p = it.begin + min(r, it.rows - 1);
-        if (L.order == nullptr) return p;
-        const int pair = L.order[p], xr = pair / L.top_k;
-        return pair < 0 || xr >= L.n_x ? -1 : xr;
-    };
+    // a row that is not there reads row 0, and its results are zeros
     const int x0 = L.order == nullptr ? it.begin : 0;
-    b.rows(static_cast<const char*>(L.x) + (size_t)x0 * pitch, [&](int r) { return (uint32_t)(max(source(r), x0) - x0) * (uint32_t)pitch; });
+    b.rows(static_cast<const char*>(L.x) + (size_t)x0 * pitch, [&](int r) {
+        return (uint32_t)(max(mm_row_of_x(L, it.begin + min(r, it.rows - 1)), x0) - x0) * (uint32_t)pitch;
+    });
     typename T::Acc acc[S::TM][S::TN];
-    mm_core<T, S, false, false, DMA>(a, b, L.cols, 0, (L.cols + 128 / T::kEl - 1) / (128 / T::kEl), lds, acc);
+    const int steps = (L.cols + 128 / T::kEl - 1) / (128 / T::kEl), per = (steps + L.splits - 1) / L.splits, k0 = work.ks * per;
+    mm_core<T, S, false, false, DMA>(a, b, L.cols, k0, min(steps, k0 + per), lds, acc);
     // results to y
     const int wave = wave_id(), l = threadIdx.x & 63, wm = wave % S::WM, n0 = wave / S::WM * S::TN * 16;
     float* turn = reinterpret_cast<float*>(lds + wave * S::TM * 1024);
     const int mw = m0 + wm * (GATED ? half : S::TM) * 16;  // of the wave
+    auto row = [&](int nt, int64_t w, int64_t off) {
+        return [=](int r) { return nt + r < it.rows ? (int64_t)(it.begin + nt + r) * w + off : (int64_t)-1; };
+    };
+    if (L.splits > 1) {  // sums as they are, of this range of the contraction
+        float* part = L.part + (size_t)work.ks * L.n_rows * L.rows;
+        const bool vec = mm_vec(part, width, CX_DTYPE_F32);
+#pragma unroll
+        for (int t = 0; t < S::TN; ++t) {
+            const int nt = n0 + t * 16;
+            if (nt >= it.rows) break;
+            auto bits = [&](int m, int i) {
+                const auto e = acc[m][t][i];  // of an element itself __builtin_bit_cast takes its vector's first
+                return __builtin_bit_cast(float, e);
+            };
+            if constexpr (GATED) {
+                mm_put<half>(bits, turn, part, CX_DTYPE_F32, vec, mw, width, row(nt, L.rows, 0));
+                mm_put<half>([&](int w, int i) { return bits(half + w, i); }, turn, part, CX_DTYPE_F32, vec, mw, width, row(nt, L.rows, width));
+            } else {
+                mm_put<S::TM>(bits, turn, part, CX_DTYPE_F32, vec, mw, width, row(nt, L.rows, 0));
+            }
+        }
+        return;
+    }
     f32x4 ws[T::kEl == 1 ? S::TM : 1];
     if constexpr (T::kEl == 1) {
 #pragma unroll
@@ -584,55 +632,65 @@ __global__ __launch_bounds__(S::kThreads, 2) void k_mm(MmLaunch L) {
     for (int t = 0; t < S::TN; ++t) {
         const int nt = n0 + t * 16;
         if (nt >= it.rows) break;
-        const int xr = source(nt + (l & 15));
+        const int xr = mm_row_of_x(L, it.begin + min(nt + (l & 15), it.rows - 1));
         const float xs = T::kEl == 1 ? (xr < 0 ? 0.0f : L.x_scale[xr]) : 1.0f;
         auto value = [&](int m, int i) {
             float f = (float)acc[m][t][i];
             if constexpr (T::kEl == 1) f = f * xs * ws[m][i];
             return xr < 0 ? 0.0f : f;
         };
-        auto row = [&](int64_t w, int64_t off) {
-            return [=](int r) { return nt + r < it.rows ? (int64_t)(it.begin + nt + r) * w + off : (int64_t)-1; };
-        };
         if constexpr (GATED) {
             if (L.pre != nullptr) {
-                mm_put<half>([&](int w, int i) { return value(w, i); }, turn, L.pre, T::kType, pvec, mw, width, row(2 * (int64_t)width, 0));
-                mm_put<half>([&](int w, int i) { return value(half + w, i); }, turn, L.pre, T::kType, pvec, mw, width, row(2 * (int64_t)width, width));
+                mm_put<half>([&](int w, int i) { return value(w, i); }, turn, L.pre, T::kType, pvec, mw, width, row(nt, 2 * (int64_t)width, 0));
+                mm_put<half>([&](int w, int i) { return value(half + w, i); }, turn, L.pre, T::kType, pvec, mw, width, row(nt, 2 * (int64_t)width, width));
             }
-            mm_put<half>([&](int w, int i) { return mm_silu(value(w, i)) * value(half + w, i); }, turn, L.y, L.y_type, vec, mw, width, row(width, 0));
+            mm_put<half>([&](int w, int i) { return mm_silu(value(w, i)) * value(half + w, i); }, turn, L.y, L.y_type, vec, mw, width, row(nt, width, 0));
         } else {
-            mm_put<S::TM>(value, turn, L.y, L.y_type, vec, mw, width, row(width, 0));
+            mm_put<S::TM>(value, turn, L.y, L.y_type, vec, mw, width, row(nt, width, 0));
         }
     }
 }
 
+template <class T, class S, bool GATED, bool DMA>
+__global__ __launch_bounds__(S::kThreads, 2) void k_mm(MmLaunch L) {
+    __shared__ __attribute__((aligned(16))) unsigned char lds[S::kLds];
+    MmWork work;
+    if (!mm_work(L, GATED ? S::BM / 2 : S::BM, GATED ? L.rows / 2 : L.rows, S::kThreads, GATED, &work)) return;
+    mm_fit<S>(work.it.rows, [&](auto s) { mm_forward<T, decltype(s), GATED, DMA>(L, work, lds); });
+}
+
 // The gradient at x.  m: columns of the weights, read across their rows; n: rows of dy.
 template <class T, class S, bool DMA>
-__global__ __launch_bounds__(S::kThreads, 2) void k_mm_dx(MmLaunch L) {
-    __shared__ __attribute__((aligned(16))) unsigned char lds[S::kLds];
-    const MmTile tile = mm_tile(blockIdx.x, L.m_tiles, L.by_item);
-    if (L.offsets != nullptr && blockIdx.x == 0 && wave_id() == 0) mm_check(L.offsets, L.n_mats, L.n_rows, L.err_flag);
-    if (tile.m >= L.m_tiles) return;
-    const MmItem it = mm_item<16>(L.offsets, L.n_mats, L.n_rows, S::BN, tile.item);
-    if (it.rows <= 0) return;
-    const int width = L.cols, m0 = tile.m * S::BM;
-    if (it.mat < 0) return mm_clear(L.y, L.y_type, it.begin, it.rows, width, m0, S::BM, S::kThreads);
+__device__ __forceinline__ void mm_dx(const MmLaunch& L, const MmWork& work, unsigned char* lds) {
+    const MmItem it = work.it;
+    const int width = L.cols, m0 = work.m0;
     MmSrc<S::BM, S::kThreads, 2, true> a;
     MmSrc<S::BN, S::kThreads, 2, false> b;
     a.cols(static_cast<const char*>(L.w) + (size_t)it.mat * L.rows * L.cols * 2, m0, width);
     b.rows(static_cast<const char*>(L.dy) + (size_t)it.begin * L.rows * 2, [&](int r) { return (uint32_t)min(r, it.rows - 1) * (uint32_t)L.rows * 2; });
     f32x4 acc[S::TM][S::TN];
-    mm_core<T, S, true, false, DMA>(a, b, L.rows, 0, (L.rows + 63) / 64, lds, acc);
+    const int steps = (L.rows + 63) / 64, per = (steps + L.splits - 1) / L.splits, k0 = work.ks * per;
+    mm_core<T, S, true, false, DMA>(a, b, L.rows, k0, min(steps, k0 + per), lds, acc);
     const int wave = wave_id(), n0 = wave / S::WM * S::TN * 16;
     float* turn = reinterpret_cast<float*>(lds + wave * S::TM * 1024);
-    const bool vec = mm_vec(L.y, width, L.y_type);
+    void* out = L.splits > 1 ? L.part + (size_t)work.ks * L.n_rows * width : L.y;
+    const int type = L.splits > 1 ? CX_DTYPE_F32 : L.y_type;
+    const bool vec = mm_vec(out, width, type);
 #pragma unroll
     for (int t = 0; t < S::TN; ++t) {
         const int nt = n0 + t * 16;
         if (nt >= it.rows) break;
-        mm_put<S::TM>([&](int m, int i) { return acc[m][t][i]; }, turn, L.y, L.y_type, vec, m0 + wave % S::WM * S::TM * 16, width,
+        mm_put<S::TM>([&](int m, int i) { return acc[m][t][i]; }, turn, out, type, vec, m0 + wave % S::WM * S::TM * 16, width,
                       [&](int r) { return nt + r < it.rows ? (int64_t)(it.begin + nt + r) * width : (int64_t)-1; });
     }
+}
+
+template <class T, class S, bool DMA>
+__global__ __launch_bounds__(S::kThreads, 2) void k_mm_dx(MmLaunch L) {
+    __shared__ __attribute__((aligned(16))) unsigned char lds[S::kLds];
+    MmWork work;
+    if (!mm_work(L, S::BM, L.cols, S::kThreads, false, &work)) return;
+    mm_fit<S>(work.it.rows, [&](auto s) { mm_dx<T, decltype(s), DMA>(L, work, lds); });
 }
 
 // The gradient at the weights of each matrix.  m: their columns; n: their rows.
@@ -659,5 +717,9 @@ __global__ __launch_bounds__(S::kThreads, 2) void k_mm_dw(MmLaunch L) {
             return n < L.rows ? ((int64_t)mat * L.rows + n) * L.cols : (int64_t)-1;
         });
 }
+
+// Tiles of m and of n in waves, by the launch's form: 256 or 128 in m; n as in MmForm.
+using MmBig = MmShape<2, 4, 8, 4, 2>;
+using MmSmall = MmShape<2, 2, 4, 4, 2>;
 
 }  // namespace cx

@@ -158,12 +158,11 @@ hipError_t mm_few_run(MmLaunch& L, int splits, bool vec, hipStream_t s) {
     return hipGetLastError();
 }
 
-// f: of mm_few_form.
 template <class T, bool GATED>
-hipError_t mm_few(MmLaunch& L, MmFew f, bool vec, hipStream_t s) {
-    if (f.rows == 16) return f.tiles == 1 ? mm_few_run<T, 1, 1, GATED>(L, f.splits, vec, s) : mm_few_run<T, 1, 2, GATED>(L, f.splits, vec, s);
-    if (f.rows == 32) return mm_few_run<T, 2, 2, GATED>(L, f.splits, vec, s);
-    return mm_few_run<T, 4, 2, GATED>(L, f.splits, vec, s);
+hipError_t mm_few(MmLaunch& L, bool vec, hipStream_t s) {
+    const MmForm f = L.form;
+    if (f.item_rows == 16) return f.tiles == 1 ? mm_few_run<T, 1, 1, GATED>(L, f.splits, vec, s) : mm_few_run<T, 1, 2, GATED>(L, f.splits, vec, s);
+    return mm_few_run<T, 2, 2, GATED>(L, f.splits, vec, s);
 }
 
 }  // namespace cx

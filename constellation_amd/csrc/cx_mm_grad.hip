@@ -4,13 +4,10 @@
 namespace cx {
 namespace {
 
-using Big = MmShape<2, 4, 8, 4, 2>;
-using Small = MmShape<2, 2, 4, 4, 2>;
-
 template <class T, class S, bool DMA>
 hipError_t dx(MmLaunch& L, hipStream_t s) {
     L.m_tiles = (L.cols + S::BM - 1) / S::BM;
-    cx_launch(k_mm_dx<T, S, DMA>, dim3(mm_grid(L, S::BN)), dim3(S::kThreads), 0, s, L);
+    cx_launch(k_mm_dx<T, S, DMA>, dim3(mm_grid(L)), dim3(S::kThreads), 0, s, L);
     return hipGetLastError();
 }
 
@@ -24,14 +21,14 @@ hipError_t dw(MmLaunch& L, hipStream_t s) {
 
 template <class T>
 hipError_t dx_pick(MmLaunch& L, hipStream_t s) {
-    if (L.cols % 8 != 0 || L.rows % 8 != 0 || !mm_at16(L.w) || !mm_at16(L.dy)) return dx<T, Small, false>(L, s);
-    return mm_big(L.n_rows, L.offsets ? L.n_mats : 1, L.cols) ? dx<T, Big, true>(L, s) : dx<T, Small, true>(L, s);
+    const hipError_t e = !mm_wide_dx(L) ? dx<T, MmSmall, false>(L, s) : L.form.kind == 2 ? dx<T, MmBig, true>(L, s) : dx<T, MmSmall, true>(L, s);
+    return e != hipSuccess || L.splits == 1 ? e : launch_mm_sum(L, L.cols, false, s);
 }
 
 template <class T>
 hipError_t dw_pick(MmLaunch& L, hipStream_t s) {
-    if (L.cols % 8 != 0 || L.rows % 8 != 0 || !mm_at16(L.x) || !mm_at16(L.dy)) return dw<T, Small, false>(L, s);
-    return (int64_t)L.n_mats * ((L.cols + 255) / 256) * ((L.rows + 255) / 256) >= 256 ? dw<T, Big, true>(L, s) : dw<T, Small, true>(L, s);
+    if (L.cols % 8 != 0 || L.rows % 8 != 0 || !mm_at16(L.x) || !mm_at16(L.dy)) return dw<T, MmSmall, false>(L, s);
+    return (int64_t)L.n_mats * ((L.cols + 255) / 256) * ((L.rows + 255) / 256) >= 256 ? dw<T, MmBig, true>(L, s) : dw<T, MmSmall, true>(L, s);
 }
 
 // h = silu(g) u has dg = dh u sig(g) (1 + g (1 - sig(g))) and du = dh silu(g); each rounded once.  One value

@@ -819,6 +819,12 @@ int check_scratch(size_t need, const void* scratch, size_t bytes) {
     return CX_OK;
 }
 
+// How a forward product is cut, and its partial sums; the same whether or not its rows turn out to be whole pieces.
+MmForm mm_forward_form(int el, int n_mats, int rows, int cols, int n_rows, bool stack) {
+    return mm_form(n_rows, n_mats, stack, rows, (int64_t)cols * el, cols % (16 / el) == 0, true);
+}
+size_t mm_part_bytes(const MmForm& f, int64_t n_rows, int64_t out) { return f.kind > 0 && f.splits > 1 ? (size_t)f.splits * n_rows * out * 4 : 0; }
+
 // The forward products in 16 bits (x_scale NULL) and in 8.
 int matmul(cx_ctx* ctx, MmLaunch L, size_t need, void* scratch, size_t scratch_bytes, void* stream) {
     const int el = L.type == kMmI8 ? 1 : 2;
@@ -835,6 +841,9 @@ int matmul(cx_ctx* ctx, MmLaunch L, size_t need, void* scratch, size_t scratch_b
     if ((rc = check_scratch(need, scratch, scratch_bytes))) return rc;
     if ((rc = set_device(ctx->device))) return rc;
     L.err_flag = ctx->err_flag;
+    L.form = mm_forward_form(el, L.n_mats, L.rows, L.cols, L.n_rows, L.offsets != nullptr);
+    L.part = static_cast<float*>(scratch);
+    if (!mm_wide(L) && L.form.kind == 2) L.form = MmForm{1, 128, L.form.splits, 1};
     hipStream_t s = static_cast<hipStream_t>(stream);
     Span sp(ctx, "matmul", s);
     CX_HIP(launch_mm(L, s));
@@ -1775,8 +1784,9 @@ int cx_q4_moe(cx_ctx* ctx, const cx_q4_desc* gate_up, const cx_q4_desc* down, co
 // Products of a program's own experts.
 
 size_t cx_matmul_scratch(int dtype, int n_mats, int rows, int cols, int gated, int n_rows, int with_offsets) {
-    (void)dtype, (void)n_mats, (void)rows, (void)cols, (void)gated, (void)n_rows, (void)with_offsets;
-    return 0;
+    (void)gated;
+    if (n_mats < 1 || rows < 1 || cols < 1 || n_rows < 1) return 0;
+    return mm_part_bytes(mm_forward_form(dtype == kMmI8 ? 1 : 2, n_mats, rows, cols, n_rows, with_offsets != 0), n_rows, rows);
 }
 
 int cx_matmul(cx_ctx* ctx, const void* x, int n_x, const void* w, int dtype, int n_mats, int rows, int cols, int gated,
@@ -1803,11 +1813,29 @@ int cx_matmul(cx_ctx* ctx, const void* x, int n_x, const void* w, int dtype, int
     return matmul(ctx, L, cx_matmul_scratch(dtype, n_mats, rows, cols, gated, n_rows, offsets != nullptr), scratch, scratch_bytes, stream);
 }
 
+namespace {
+// The gradient's scratch: the gradient at pre, then dx's partial sums.
+struct GradScratch {
+    MmForm dx;
+    size_t part, bytes;
+};
+GradScratch grad_scratch(int n_mats, int rows, int cols, bool gated, int n_rows, bool stack, bool with_dx) {
+    GradScratch z{};
+    z.part = gated ? ((size_t)n_rows * rows * 2 + 15) / 16 * 16 : 0;
+    z.bytes = z.part;
+    if (with_dx) {
+        z.dx = mm_form(n_rows, n_mats, stack, cols, (int64_t)rows * 2, rows % 8 == 0 && cols % 8 == 0, false);
+        z.bytes += mm_part_bytes(z.dx, n_rows, cols);
+    }
+    return z;
+}
+}  // namespace
+
 size_t cx_matmul_grad_scratch(int dtype, int n_mats, int rows, int cols, int gated, int n_rows, int with_offsets, int with_dx,
                               int dw_dtype) {
-    (void)dtype, (void)n_mats, (void)cols, (void)with_offsets, (void)with_dx, (void)dw_dtype;
-    if (rows < 1 || n_rows < 1) return 0;
-    return gated ? ((size_t)n_rows * rows * 2 + 15) / 16 * 16 : 0;
+    (void)dtype, (void)dw_dtype;
+    if (n_mats < 1 || rows < 1 || cols < 1 || n_rows < 1) return 0;
+    return grad_scratch(n_mats, rows, cols, gated != 0, n_rows, with_offsets != 0, with_dx != 0).bytes;
 }
 
 int cx_matmul_grad(cx_ctx* ctx, const void* dy, const void* x, const void* w, int dtype, const void* pre, int n_mats, int rows,
@@ -1821,8 +1849,8 @@ int cx_matmul_grad(cx_ctx* ctx, const void* dy, const void* x, const void* w, in
     if (dw && dw_dtype != dtype && dw_dtype != CX_DTYPE_F32) return fail(CX_EINVAL, "dw must be of x's type or fp32");
     if (n_rows == 0 && !dw) return CX_OK;
     if ((n_rows > 0 && (!dy || (dw && !x))) || (dx && !w)) return fail(CX_EINVAL, "NULL buffer");
-    const size_t need = cx_matmul_grad_scratch(dtype, n_mats, rows, cols, pre != nullptr, n_rows, offsets != nullptr, dx != nullptr, dw ? dw_dtype : 0);
-    if ((rc = check_scratch(need, scratch, scratch_bytes))) return rc;
+    const GradScratch z = n_rows > 0 ? grad_scratch(n_mats, rows, cols, pre != nullptr, n_rows, offsets != nullptr, dx != nullptr) : GradScratch{};
+    if ((rc = check_scratch(z.bytes, scratch, scratch_bytes))) return rc;
     if ((rc = set_device(ctx->device))) return rc;
     hipStream_t s = static_cast<hipStream_t>(stream);
     MmLaunch L{};
@@ -1844,6 +1872,9 @@ int cx_matmul_grad(cx_ctx* ctx, const void* dy, const void* x, const void* w, in
     if (dx && n_rows > 0) {
         L.y = dx;
         L.y_type = dtype;
+        L.form = z.dx;
+        L.part = reinterpret_cast<float*>(static_cast<char*>(scratch) + z.part);
+        if (!mm_wide_dx(L) && L.form.kind == 2) L.form = MmForm{1, 128, L.form.splits, 1};
         CX_HIP(launch_mm_dx(L, s));
     }
     if (dw) {

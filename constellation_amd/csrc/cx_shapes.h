@@ -412,27 +412,51 @@ inline int64_t mm_items(int64_t n_rows, int n_mats, bool stack, int item_rows) {
     return (n_rows < n_mats ? n_rows : n_mats) + n_rows / item_rows + 1;
 }
 
-// Tiles of 256 x 256 where they fill the card, of 128 x 128 otherwise.
-inline bool mm_big(int64_t n_rows, int n_mats, int width) {
-    return (n_rows / 256 + 1) * ((width + 255) / 256) >= 256 && n_rows >= (int64_t)n_mats * 64;
-}
-// The kernel of few rows: rows of an item, tiles of 16 weight rows a wave, ranges of the columns a workgroup;
-// rows 0: tiles through LDS instead.
-constexpr int kMmFewWaves = 8;
-struct MmFew {
-    int rows, tiles, splits;
+// How a product (or the gradient at x) is cut.
+struct MmForm {
+    int kind;       // 0: few rows, weights without LDS; 1: tiles of 128 in m; 2: of 256
+    int item_rows;  // rows of x an item has, at most
+    int splits;     // ranges of the contraction: kind 0 within a workgroup, otherwise with partial sums
+    int tiles;      // kind 0: tiles of 16 weight rows a wave
 };
-inline MmFew mm_few_form(int64_t n_rows, int n_mats, int rows, int cols, int el) {
-    const int64_t busy = std::min<int64_t>(n_rows, n_mats);
-    const int64_t avg = (n_rows + busy - 1) / std::max<int64_t>(busy, 1);
-    if (avg > 64) return MmFew{0, 0, 0};
-    MmFew f{avg <= 16 ? 16 : avg <= 32 ? 32 : 64, 1, 1};
-    const int64_t tiles = (rows + 15) / 16, items = busy;
-    f.tiles = f.rows > 16 || tiles * items > 1024 ? 2 : 1;
-    const int steps = (cols * el + 127) / 128;
-    while (f.splits < kMmFewWaves && tiles / f.tiles * items * f.splits * 2 <= 4096 && steps / f.splits >= 4) f.splits *= 2;
+constexpr int kMmFewWaves = 8;
+
+inline MmForm mm_few_form(int item_rows, int64_t busy, int rows, int steps) {
+    MmForm f{0, item_rows, 1, 1};
+    const int64_t tiles = (rows + 15) / 16;
+    f.tiles = item_rows > 16 || tiles * busy > 1024 ? 2 : 1;
+    while (f.splits < kMmFewWaves && tiles / f.tiles * busy * f.splits * 2 <= 4096 && steps / f.splits >= 4) f.splits *= 2;
     return f;
 }
+
+// out: the output's width, in which tiles of 128 or 256 lie (of a gated product the weights' rows); depth: bytes of the
+// contraction; wide: whole pieces of 16 bytes; few: the kernel of few rows is there.
+inline MmForm mm_form(int64_t n_rows, int n_mats, bool stack, int64_t out, int64_t depth, bool wide, bool few) {
+    const int64_t busy = std::max<int64_t>(1, std::min<int64_t>(n_rows, n_mats)), avg = (n_rows + busy - 1) / busy;
+    const int64_t steps = (depth + 127) / 128;
+    if (few && avg <= 16) return mm_few_form(16, busy, (int)out, (int)steps);
+    MmForm best{1, 128, 1, 1};
+    double least = -1;
+    for (int kind = wide ? 2 : 1; kind >= 1; --kind) {
+        const int unit = kind == 2 ? 64 : 32;
+        for (int tn = 4; tn >= 1; --tn) {
+            const int rows = unit * tn;
+            if (tn > 1 && avg <= rows - unit) continue;
+            const int64_t items = stack ? std::max<int64_t>(busy, (n_rows + rows - 1) / rows + busy / 2) : (n_rows + rows - 1) / rows;
+            const int64_t tiles = items * ((out + 128 * kind - 1) / (128 * kind));
+            const double step = kind == 2 ? 0.45 + 0.25 * tn : 0.3 + 0.09 * tn, beside = kind == 2 ? 1 : 1.6;
+            for (int s = 1; s <= 16 && (s == 1 || (steps / s >= 4 && n_rows * out <= 1 << 26)); s *= 2) {
+                const int64_t wgs = tiles * s, slots = kind == 2 ? 256 : 512;
+                const double per = (double)((steps + s - 1) / s) * step * (wgs > 256 ? beside : 1) + (kind == 2 ? 6 : 4);
+                const double rounds = wgs <= slots ? 1 : wgs > 4 * slots ? (double)wgs / slots + 0.4 : (double)((wgs + slots - 1) / slots);
+                const double cost = rounds * per + (s > 1 ? 4 + 2.0 * s * (double)n_rows * out * 4 / 4.5e6 : 0);
+                if (least < 0 || cost < least) least = cost, best = MmForm{kind, rows, s, 1};
+            }
+        }
+    }
+    return best;
+}
+
 // Launches stay within 2^32 threads and 2^30 rows, at the smallest tiles and with every matrix's last tile short.
 inline bool mm_grid_ok(int64_t n_rows, int n_mats, int rows, int cols) {
     const int64_t items = mm_items(n_rows, n_mats, true, 16) + 8, tiles = (std::max(rows, cols) + 63) / 64 + 8;
