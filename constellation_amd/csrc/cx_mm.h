@@ -461,24 +461,27 @@ __device__ __forceinline__ void mm_core(const MmSrc<S::BM, S::kThreads, T::kEl, 
     mm_barrier();
 }
 
+// Two values rounded to 16 bits, by the hardware's conversions (nearest even, NaN stay NaN).
+__device__ __forceinline__ uint32_t mm_round2(float a, float b, bool bf) {
+    typedef float f32x2 __attribute__((ext_vector_type(2)));
+    const f32x2 v = {a, b};
+    return bf ? __builtin_bit_cast(uint32_t, __builtin_convertvector(v, bf16x2)) : __builtin_bit_cast(uint32_t, __builtin_convertvector(v, f16x2));
+}
+
 // 16 rows of W * 16 outputs, from a wave's results through its own part of LDS (W KB), so that it stores whole lines.
 // v(w, i): element i of result w, whose m follow each other; row(n) is where in `out` row n starts (elements), < 0: not stored.
-template <int W, class V, class F>
-__device__ __forceinline__ void mm_put(V v, float* turn, void* out, int type, bool vec, int m0, int width, F row) {
-    constexpr int kChunks = W * 4;  // of four floats
-    const int l = threadIdx.x & 63, n = l & 15;
+template <int W, bool WIDE, class F>
+__device__ __forceinline__ void mm_put_rows(const float* turn, void* out, bool bf, bool vec, int m0, int width, F row) {
+    constexpr int kChunks = W * 4, kPer = WIDE ? 4 : 8, kLanes = W * 16 / kPer;  // columns of a lane's store, lanes of a row
+    const int l = threadIdx.x & 63;
 #pragma unroll
-    for (int w = 0; w < W; ++w)
-        *reinterpret_cast<f32x4*>(turn + n * W * 16 + ((w * 4 + (l >> 4)) ^ (n & (kChunks - 1))) * 4) = f32x4{v(w, 0), v(w, 1), v(w, 2), v(w, 3)};
-    __builtin_amdgcn_wave_barrier();
-    const int per = type == CX_DTYPE_F32 ? 4 : 8, lanes = W * 16 / per;  // columns of a lane's store, lanes of a row
-    for (int i = l; i < 16 * lanes; i += 64) {
-        const int r = i / lanes, c = (i - r * lanes) * per, left = width - m0 - c;
+    for (int i = 0; i < 16 * kLanes / 64; ++i) {
+        const int r = (i * 64 + l) / kLanes, c = (i * 64 + l) % kLanes * kPer, left = width - m0 - c;
         const int64_t at = row(r);
         if (at < 0 || left <= 0) continue;
         const float* src = turn + r * W * 16;
         const f32x4 a = *reinterpret_cast<const f32x4*>(src + ((c / 4) ^ (r & (kChunks - 1))) * 4);
-        if (type == CX_DTYPE_F32) {
+        if constexpr (WIDE) {
             float* y = static_cast<float*>(out) + at + m0 + c;
             if (vec) {
                 *reinterpret_cast<f32x4*>(y) = a;
@@ -489,19 +492,31 @@ __device__ __forceinline__ void mm_put(V v, float* turn, void* out, int type, bo
             }
         } else {
             const f32x4 b = *reinterpret_cast<const f32x4*>(src + ((c / 4 + 1) ^ (r & (kChunks - 1))) * 4);
-            uint32_t h[8];
-#pragma unroll
-            for (int k = 0; k < 4; ++k) h[k] = cast_out(a[k], type), h[4 + k] = cast_out(b[k], type);
+            const u32x4 h = {mm_round2(a[0], a[1], bf), mm_round2(a[2], a[3], bf), mm_round2(b[0], b[1], bf), mm_round2(b[2], b[3], bf)};
             uint16_t* y = static_cast<uint16_t*>(out) + at + m0 + c;
             if (vec) {
-                *reinterpret_cast<u32x4*>(y) = u32x4{h[0] | (h[1] << 16), h[2] | (h[3] << 16), h[4] | (h[5] << 16), h[6] | (h[7] << 16)};
+                *reinterpret_cast<u32x4*>(y) = h;
             } else {
 #pragma unroll
                 for (int k = 0; k < 8; ++k)
-                    if (k < left) y[k] = (uint16_t)h[k];
+                    if (k < left) y[k] = (uint16_t)(h[k / 2] >> (16 * (k & 1)));
             }
         }
     }
+}
+
+template <int W, class V, class F>
+__device__ __forceinline__ void mm_put(V v, float* turn, void* out, int type, bool vec, int m0, int width, F row) {
+    constexpr int kChunks = W * 4;  // of four floats
+    const int l = threadIdx.x & 63, n = l & 15;
+#pragma unroll
+    for (int w = 0; w < W; ++w)
+        *reinterpret_cast<f32x4*>(turn + n * W * 16 + ((w * 4 + (l >> 4)) ^ (n & (kChunks - 1))) * 4) = f32x4{v(w, 0), v(w, 1), v(w, 2), v(w, 3)};
+    __builtin_amdgcn_wave_barrier();
+    if (type == CX_DTYPE_F32)
+        mm_put_rows<W, true>(turn, out, false, vec, m0, width, row);
+    else
+        mm_put_rows<W, false>(turn, out, type == CX_DTYPE_BF16, vec, m0, width, row);
     __builtin_amdgcn_wave_barrier();
 }
 
