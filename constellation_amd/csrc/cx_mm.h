@@ -141,20 +141,22 @@ __device__ __forceinline__ const char* mm_uniform(const void* p) {
 //    them one by one (64 bytes of each and twice the steps: 4096 rows by 4096 x 7168, loads alone 159 us, 138 with
 //    lines).  Row r's piece c lies in place c ^ (r % 8) ^ (r / 8 % 2), so that the 16 rows which a wave reads at a time
 //    lie in different banks.
-//  TR true: 64 rows of the contraction, R 16-bit columns of each.  32-byte chunk c of row j lies in place
+//  TR true: ROWS rows of the contraction, R 16-bit columns of each.  32-byte chunk c of row j lies in place
 //    c ^ (2 (j % 4) + j / 8 % 2), for the transposing reads of four rows at a time, by two groups of lanes.
 // Places are 32 bits from a uniform base, which moves with the steps.
-template <int R, int THREADS, int EL, bool TR>
+template <int R, int THREADS, int EL, bool TR, int ROWS = 64>
 struct MmSrc {
-    static constexpr int P = R * 8 / THREADS;
+    static constexpr int P = R * (TR ? ROWS : 64) / 8 / THREADS;
     static constexpr int kStepRows = THREADS * 8 / R;  // TR: rows between a thread's pieces
-    static constexpr int kStep = 128 / EL;             // elements of the contraction in a step
+    static constexpr int kStep = TR ? ROWS : 128 / EL;  // elements of the contraction in a step
+    static constexpr int kAlt = TR && kStepRows == 8 ? 2 : 1;  // TR: pieces that lie in different places of their rows
+    static_assert(!TR || kStepRows % 8 == 0, "swizzle");
     const char* base;
-    uint32_t off[TR ? 1 : P];
+    uint32_t off[TR ? kAlt : P];
     uint32_t gap;  // TR: bytes between a thread's pieces
     size_t move;   // bytes between steps
     int first;     // place in the step's contraction of the thread's pieces' first element (TR: of its first piece)
-    int left;      // TR: elements from the piece's first to the row's end
+    int left[kAlt];  // TR: elements from the piece's first to the row's end
 
     // offset(r): bytes from base to row r
     template <class F>
@@ -172,22 +174,26 @@ struct MmSrc {
         static_assert(TR, "");
         const int t = threadIdx.x, piece = t % (R / 8);
         first = t / (R / 8);
-        const int col = col0 + (((piece >> 1) ^ (2 * (first & 3) + (first >> 3 & 1))) * 2 + (piece & 1)) * 8;
         base = mm_uniform(base_);
-        left = width - col;
-        off[0] = (uint32_t)first * (uint32_t)width * 2 + (left > 0 ? col * 2 : 0);
+#pragma unroll
+        for (int i = 0; i < kAlt; ++i) {
+            const int row = first + i * kStepRows, col = col0 + (((piece >> 1) ^ (2 * (row & 3) + (row >> 3 & 1))) * 2 + (piece & 1)) * 8;
+            left[i] = width - col;
+            off[i] = (uint32_t)first * (uint32_t)width * 2 + (left[i] > 0 ? col * 2 : 0);
+        }
         gap = (uint32_t)kStepRows * (uint32_t)width * 2;
-        move = (size_t)width * 128;
+        move = (size_t)width * 2 * ROWS;
     }
+    __device__ __forceinline__ uint32_t place(int i) const { return TR ? off[i % kAlt] + (uint32_t)i * gap : off[TR ? 0 : i]; }
     // Piece i of the step that starts at `from`.
-    __device__ __forceinline__ const char* piece(int i, const char* from) const { return from + (TR ? off[0] + (uint32_t)i * gap : off[TR ? 0 : i]); }
+    __device__ __forceinline__ const char* piece(int i, const char* from) const { return from + place(i); }
     __device__ __forceinline__ const char* step(int k) const { return base + (size_t)k * move; }
     // Straight to LDS, piece i of a step that starts at `from`, to `lds` + the wave's part: whole pieces that start on 16
     // bytes.  It takes `from` from scalar registers and the lane's 32-bit place as it is: with a sum of 64 bits before
     // each load, loads took as much issue as MFMAs.
     __device__ __forceinline__ void fetch(unsigned char* lds, int i, const char* from) const {
         __builtin_amdgcn_raw_ptr_buffer_load_lds(make_rsrc(from, 0xFFFFFFFFu), (__attribute__((address_space(3))) void*)(lds + i * THREADS * 16), 16,
-                                                 (int)(TR ? off[0] + (uint32_t)i * gap : off[TR ? 0 : i]), 0, 0, 0);
+                                                 (int)place(i), 0, 0, 0);
     }
     // The same for any step k: what lies past the contraction's n elements is zeros.
     __device__ __forceinline__ void fetch_to(unsigned char* lds, int i, int k, int n) const {
@@ -199,7 +205,7 @@ struct MmSrc {
         constexpr int kWhole = 16 / EL;
 #pragma unroll
         for (int i = 0; i < P; ++i) {
-            const int have = TR ? (k * kStep + first + i * kStepRows < n ? left : 0) : n - k * kStep - first;
+            const int have = TR ? (k * kStep + first + i * kStepRows < n ? left[i % kAlt] : 0) : n - k * kStep - first;
             const char* q = piece(i, step(k));
             v[i] = u32x4{};
             if (have >= kWhole) {
@@ -459,6 +465,123 @@ __device__ __forceinline__ void mm_core(const MmSrc<S::BM, S::kThreads, T::kEl, 
         for (const int whole = min(k1, n / MmSrc<S::BM, S::kThreads, T::kEl, AT>::kStep); k + S::kSlots < whole; ++k) step(std::true_type{}, k);
     for (; k < k1; ++k) step(std::false_type{}, k);
     mm_barrier();
+}
+
+// The same for the gradient at the weights, whose operands both lie across the contraction: steps of 32 rows, which are whole lines
+// all the same, so that three of them for 256 x 128 results leave room for a second workgroup on the CU.  A matrix's share of
+// rows is short and its results are many: one workgroup stores while the other multiplies (32 matrices of 4096 x 7168, 512 rows
+// each: with one of 256 x 256 results a CU 1215 us, of which 370 were stores that nothing ran beside).
+template <class S>
+struct MmShort {
+    static constexpr int kSlots = 3, kStepM = S::BM * 64, kStepN = S::BN * 64, kStep = kStepM + kStepN, kLds = kSlots * kStep;
+    typedef MmSrc<S::BM, S::kThreads, 2, true, 32> A;
+    typedef MmSrc<S::BN, S::kThreads, 2, true, 32> B;
+};
+template <class T, class S>
+__device__ __forceinline__ void mm_core_short(const typename MmShort<S>::A& a, const typename MmShort<S>::B& b, int n, unsigned char* lds,
+                                              typename T::Acc (&acc)[S::TM][S::TN]) {
+    typedef MmShort<S> H;
+    typedef MmFrag<S::BM, true, S::TM> FA;
+    typedef MmFrag<S::BN, true, S::TN> FB;
+    constexpr int kHalf = S::TM / 2, kMma = kHalf * S::TN, kLoads = H::A::P + H::B::P, kLate = kLoads / 2;
+    const int wave = wave_id(), k1 = (n + 31) / 32;
+    const FA fa(wave % S::WM * S::TM * 16, mm_lds_addr(lds));
+    const FB fb(wave / S::WM * S::TN * 16, mm_lds_addr(lds) + H::kStepM);
+#pragma unroll
+    for (int m = 0; m < S::TM; ++m)
+#pragma unroll
+        for (int t = 0; t < S::TN; ++t) acc[m][t] = typename T::Acc{};
+    if (k1 == 0) return;
+    unsigned char* to = lds + wave * 1024;
+    // load j of a step: A's first
+    auto load = [&](auto steady, int j, int k, const char* pa, const char* pb, int slot) {
+        if constexpr (decltype(steady)::value) {
+            if (j < H::A::P)
+                a.fetch(to + slot, j, pa);
+            else
+                b.fetch(to + slot + H::kStepM, j - H::A::P, pb);
+        } else if (k < k1) {
+            if (j < H::A::P)
+                a.fetch_to(to + slot, j, k, n);
+            else
+                b.fetch_to(to + slot + H::kStepM, j - H::A::P, k, n);
+        }
+    };
+#pragma unroll
+    for (int i = 0; i < 3; ++i)
+#pragma unroll
+        for (int j = 0; j < (i < 2 ? kLoads : kLoads - kLate); ++j) load(std::false_type{}, j, i, nullptr, nullptr, i * H::kStep);
+    if (k1 >= 3)
+        vm_wait<2 * kLoads - kLate>();
+    else
+        vm_wait<0>();
+    mm_barrier();
+    typename FA::Held xa[2][kHalf];
+    typename FB::Held xb[2][S::TN];
+    mm_each<kHalf>([&](auto r) { fa.template read<0, r.value>(xa[0][r.value], 0); });
+    mm_each<S::TN>([&](auto r) { fb.template read<0, r.value>(xb[0][r.value], 0); });
+    mm_wait(xa[0]);
+    mm_wait(xb[0]);
+    int slot = 0, was = 2 * H::kStep;
+    const char *pa = a.step(2), *pb = b.step(2);  // of the next loads
+    // half D of m of step k, whose n is in xb[Q]; beside it the fragments of the next half (from slot `from`) and a share of the loads
+    // of step k + 2 or k + 3
+    auto half = [&](auto d, auto q, auto steady, int k, uint32_t from, int slot_to) {
+        constexpr int D = decltype(d)::value, Q = decltype(q)::value, kReads = kHalf + (D == 1 ? S::TN : 0), kShare = D == 1 ? kLoads - kLate : kLate;
+        __builtin_amdgcn_s_setprio(1);
+        mm_each<kMma>([&](auto i) {
+            constexpr int m = i.value / S::TN, t = i.value % S::TN;
+            mm_each<kReads>([&](auto r) {
+                if constexpr (r.value * (kMma / 2) / kReads == i.value) {
+                    if constexpr (r.value < kHalf)
+                        fa.template read<0, (1 - D) * kHalf + r.value>(xa[1 - D][r.value], from);
+                    else
+                        fb.template read<0, r.value - kHalf>(xb[1 - Q][r.value - kHalf], from);
+                }
+            });
+            mm_each<kShare>([&](auto r) {
+                if constexpr (r.value * kMma / kShare == i.value) load(steady, (D == 1 ? 0 : kLoads - kLate) + r.value, k + 2 + D, pa, pb, slot_to);
+            });
+            typename T::Acc& sum = acc[D * kHalf + m][t];
+            sum = T::mma(xa[D][m].v, xb[Q][t].v, sum);
+            __builtin_amdgcn_sched_barrier(0);
+        });
+        __builtin_amdgcn_s_setprio(0);
+        mm_wait(xa[1 - D]);
+        if constexpr (D == 1) mm_wait(xb[1 - Q]);
+    };
+    constexpr std::integral_constant<int, 0> d0{};
+    constexpr std::integral_constant<int, 1> d1{};
+    auto step = [&](auto q, auto steady, int k) {
+        const int next = slot == 2 * H::kStep ? 0 : slot + H::kStep;
+        half(d0, q, steady, k, slot, was);
+        pa += a.move;
+        pb += b.move;
+        if (decltype(steady)::value || k + 2 < k1)
+            vm_wait<kLoads>();
+        else
+            vm_wait<0>();
+        mm_barrier();
+        half(d1, q, steady, k, next, slot);  // past the last step it reads what lies in the ring, not used
+#if defined(__HIP_DEVICE_COMPILE__)  // keeps the sums where they are: no copies of them at the loop's end
+#pragma unroll
+        for (int m = 0; m < S::TM; ++m)
+#pragma unroll
+            for (int t = 0; t < S::TN; ++t) asm volatile("" : "+v"(acc[m][t]));
+#endif
+        was = slot;
+        slot = next;
+    };
+    int k = 0;
+    for (const int whole = n / 32; k + 4 < whole; k += 2) {
+        step(d0, std::true_type{}, k);
+        step(d1, std::true_type{}, k + 1);
+    }
+    for (; k + 1 < k1; k += 2) {
+        step(d0, std::false_type{}, k);
+        step(d1, std::false_type{}, k + 1);
+    }
+    if (k < k1) step(d0, std::false_type{}, k);
 }
 
 // Two values rounded to 16 bits, by the hardware's conversions (nearest even, NaN stay NaN).
@@ -733,8 +856,40 @@ __global__ __launch_bounds__(S::kThreads, 2) void k_mm_dw(MmLaunch L) {
         });
 }
 
+// The same with short steps, two workgroups a CU.
+template <class T, class S>
+__global__ __launch_bounds__(S::kThreads, 2) void k_mm_dw_short(MmLaunch L) {
+    __shared__ __attribute__((aligned(16))) unsigned char lds[MmShort<S>::kLds];
+    static_assert(S::kWaves * S::TM * 1024 <= MmShort<S>::kLds, "turned results");
+    if (L.offsets != nullptr && blockIdx.x == 0 && wave_id() == 0) mm_check(L.offsets, L.n_mats, L.n_rows, L.err_flag);
+    // tiles of a matrix in blocks of eight in n, down m; XCD b % 8 takes 64 in turn, which share operands in its L2
+    const int n_tiles = (L.rows + S::BN - 1) / S::BN, per = n_tiles * L.m_tiles;
+    const int64_t total = (int64_t)L.n_mats * per, x = blockIdx.x & 7, i = blockIdx.x >> 3, tile = (i / 64 * 8 + x) * 64 + i % 64;
+    if (tile >= total) return;
+    const int mat = (int)(tile / per), j = (int)(tile - (int64_t)mat * per), block = j / (8 * L.m_tiles), r = j - block * 8 * L.m_tiles, wide = min(8, n_tiles - block * 8);
+    const int m0 = r / wide * S::BM, n0 = (block * 8 + r % wide) * S::BN;
+    const MmItem it = mm_rows_of(L.offsets, L.n_rows, mat);
+    typename MmShort<S>::A a;
+    typename MmShort<S>::B b;
+    a.cols(static_cast<const char*>(L.x) + (size_t)it.begin * L.cols * 2, m0, L.cols);
+    b.cols(static_cast<const char*>(L.dy) + (size_t)it.begin * L.rows * 2, n0, L.rows);
+    f32x4 acc[S::TM][S::TN];
+    mm_core_short<T, S>(a, b, it.rows, lds, acc);
+    const int wave = wave_id(), nw = n0 + wave / S::WM * S::TN * 16;
+    mm_barrier();
+    float* turn = reinterpret_cast<float*>(lds + wave * S::TM * 1024);
+    const bool vec = mm_vec(L.y, L.cols, L.y_type);
+#pragma unroll
+    for (int t = 0; t < S::TN; ++t)
+        mm_put<S::TM>([&](int m, int i) { return acc[m][t][i]; }, turn, L.y, L.y_type, vec, m0 + wave % S::WM * S::TM * 16, L.cols, [&](int r) {
+            const int n = nw + t * 16 + r;
+            return n < L.rows ? ((int64_t)mat * L.rows + n) * L.cols : (int64_t)-1;
+        });
+}
+
 // Tiles of m and of n in waves, by the launch's form: 256 or 128 in m; n as in MmForm.
 using MmBig = MmShape<2, 4, 8, 4, 2>;
 using MmSmall = MmShape<2, 2, 4, 4, 2>;
+using MmMid = MmShape<2, 2, 8, 4, 2>;  // of the gradient at the weights
 
 }  // namespace cx
