@@ -53,6 +53,15 @@ class Q4Desc(C.Structure):
     ]
 
 
+class I8LayerDesc(C.Structure):
+    """cx_i8_layer: stacks of 8-bit experts as the program holds them."""
+    _fields_ = [
+        ("gate_up", C.c_void_p), ("gate_up_scale", C.c_void_p), ("down", C.c_void_p), ("down_scale", C.c_void_p),
+        ("n_mats", C.c_int32), ("hidden", C.c_int32), ("inter", C.c_int32), ("shared", C.c_int32),
+        ("reserved", C.c_int32 * 4),
+    ]
+
+
 class MoeLayerRequestInfo(C.Structure):
     """cx_moe_layer_request_info: header fields of a MoeLayerRequest body."""
     _fields_ = [
@@ -128,6 +137,8 @@ _SIGS = {
     "cx_quantize_i8": (_I, [_P, _P, _I, _I, _I, _P, _P, _P]),
     "cx_i8_matmul_scratch": (C.c_size_t, [_I, _I, _I, _I, _I, _I]),
     "cx_i8_matmul": (_I, [_P, _P, _P, _I, _P, _P, _I, _I, _I, _I, _P, _I, _P, _I, _P, _I, _P, C.c_size_t, _P]),
+    "cx_i8_moe_scratch": (C.c_size_t, [C.POINTER(I8LayerDesc), _I, _I]),
+    "cx_i8_moe": (_I, [_P, C.POINTER(I8LayerDesc), _P, _I, _I, _P, _P, _I, _P, _I, _P, _P, C.c_size_t, _P]),
     "cx_gen_fp8_matrix": (_I, [_P, C.c_uint64, C.c_uint64, _I, _I, _I, _I, C.c_float, _P, _P,
                                _P]),
     "cx_gen_normal": (_I, [_P, C.c_uint64, C.c_uint64, C.c_uint64, C.c_float, _I, _P, _P]),

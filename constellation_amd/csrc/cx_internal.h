@@ -369,7 +369,7 @@ struct SortArgs {
     int n_tokens, top_k, n_experts;
     int shared;            // 1: every token also goes to a shared expert, as route top_k and expert n_experts
     int32_t* order;        // [n_tokens * (top_k + shared)]
-    int32_t* offsets;      // nullable [n_experts + 1]
+    int32_t* offsets;      // nullable [n_experts + shared + 1]
     int32_t* place;        // [n_tokens, top_k + shared]
     Q4Item* items;         // nullable: runs of up to item_rows rows of one expert
     int item_rows;

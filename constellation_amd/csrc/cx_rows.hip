@@ -365,7 +365,7 @@ __global__ __launch_bounds__(kSortThreads) void k_sort_tokens(SortArgs a) {
     const int none = a.shared ? a.n_tokens : 0;
     if (blockIdx.x == 0) {
         if (a.offsets != nullptr)
-            for (int e = tid; e <= NK; e += kSortThreads) a.offsets[e] = first[e];
+            for (int e = tid; e <= NK + a.shared; e += kSortThreads) a.offsets[e] = e <= NK ? first[e] : shared_row + none;
         if (a.items != nullptr) {
             const int more = (none + a.item_rows - 1) / a.item_rows;  // of the shared expert, whose items are the longest
             q4_put_items(a.items + 1, more, NK, shared_row, none, tid, kSortThreads);

@@ -1927,6 +1927,143 @@ int cx_i8_matmul(cx_ctx* ctx, const int8_t* x, const float* x_scale, int n_x, co
     return matmul(ctx, L, cx_i8_matmul_scratch(n_mats, rows, cols, gated, n_rows, offsets != nullptr), scratch, scratch_bytes, stream);
 }
 
+namespace {
+struct I8MoeScratch {
+    int64_t pairs;
+    size_t order, offsets, place, q, q_scale, h, hq, h_scale, ys, part, bytes;
+};
+I8MoeScratch i8_moe_scratch(const cx_i8_layer& w, int64_t n_tokens, int top_k) {
+    I8MoeScratch z{};
+    size_t at = 0;
+    auto take = [&](size_t n) {
+        const size_t was = at;
+        at += (n + 255) / 256 * 256;
+        return was;
+    };
+    z.pairs = n_tokens * (top_k + (w.shared != 0));
+    const size_t p = (size_t)z.pairs;
+    z.order = take(p * 4);
+    z.offsets = take(((size_t)w.n_mats + 1) * 4);
+    z.place = take(p * 4);
+    z.q = take((size_t)n_tokens * w.hidden);
+    z.q_scale = take((size_t)n_tokens * 4);
+    z.h = take(p * w.inter * 4);
+    z.hq = take(p * w.inter);
+    z.h_scale = take(p * 4);
+    z.ys = take(p * w.hidden * 4);
+    z.part = take(std::max(mm_part_bytes(mm_forward_form(1, w.n_mats, 2 * w.inter, w.hidden, (int)z.pairs, true), z.pairs, 2 * w.inter),
+                           mm_part_bytes(mm_forward_form(1, w.n_mats, w.hidden, w.inter, (int)z.pairs, true), z.pairs, w.hidden)));
+    z.bytes = at;
+    return z;
+}
+}  // namespace
+
+size_t cx_i8_moe_scratch(const cx_i8_layer* w, int n_tokens, int top_k) {
+    if (!w || w->n_mats < 1 || w->hidden < 1 || w->inter < 1 || w->inter > kMmMaxSide / 2 || n_tokens < 1 || top_k < 0 || top_k > 64 ||
+        (int64_t)n_tokens * (top_k + 1) > kMaxPairs)
+        return 0;
+    return i8_moe_scratch(*w, n_tokens, top_k).bytes;
+}
+
+int cx_i8_moe(cx_ctx* ctx, const cx_i8_layer* w, const void* x, int in_dtype, int n_tokens, const int32_t* topk_ids,
+              const float* topk_w, int top_k, void* y, int out_dtype, float* y_f32, void* scratch, size_t scratch_bytes,
+              void* stream) {
+    DeviceRestore keep;
+    if (!ctx) return fail(CX_EINVAL, "NULL context");
+    if (!w || !w->gate_up || !w->gate_up_scale || !w->down || !w->down_scale) return fail(CX_EINVAL, "8-bit layer is NULL or empty");
+    if (!act16(in_dtype) || !act16(out_dtype)) return fail(CX_EINVAL, "dtypes must be fp16/bf16");
+    const int shared = w->shared != 0;
+    if (n_tokens < 0 || top_k < 0 || top_k > 64 || top_k + shared < 1) return fail(CX_EINVAL, "bad n_tokens/top_k");
+    if ((int64_t)n_tokens * (top_k + shared) > kMaxPairs) return fail(CX_EINVAL, "too many pairs: n_tokens * top_k must be at most 2^30");
+    if (w->n_mats <= shared) return fail(CX_EINVAL, "a layer needs a routed expert");
+    const int pairs = n_tokens * (top_k + shared);
+    if (w->inter < 1 || w->inter > kMmMaxSide / 2) return fail(CX_EINVAL, "inter must be 1..%d", kMmMaxSide / 2);
+    int rc = check_mm(ctx, 1, w->n_mats, 2 * w->inter, w->hidden, 1, w, pairs);
+    if (rc || (rc = check_mm(ctx, 1, w->n_mats, w->hidden, w->inter, 0, w, pairs))) return rc;
+    if ((uint64_t)n_tokens * w->hidden >= (uint64_t)1 << 32) return fail(CX_EINVAL, "x must have fewer than 2^32 values");
+    if (n_tokens == 0) return CX_OK;
+    if (!x || !y || (top_k > 0 && (!topk_ids || !topk_w))) return fail(CX_EINVAL, "NULL buffer");
+    const I8MoeScratch z = i8_moe_scratch(*w, n_tokens, top_k);
+    if ((rc = check_scratch(z.bytes, scratch, scratch_bytes))) return rc;
+    if ((rc = set_device(ctx->device))) return rc;
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    char* m = static_cast<char*>(scratch);
+    SortArgs a{};
+    a.ids = topk_ids;
+    a.weights = topk_w;
+    a.n_tokens = n_tokens;
+    a.top_k = top_k;
+    a.n_experts = w->n_mats - shared;
+    a.shared = shared;
+    a.order = reinterpret_cast<int32_t*>(m + z.order);
+    a.offsets = reinterpret_cast<int32_t*>(m + z.offsets);
+    a.place = reinterpret_cast<int32_t*>(m + z.place);
+    a.err_flag = ctx->err_flag;
+    CombineArgs c{};
+    c.ys = m + z.ys;
+    c.ys_dtype = CX_DTYPE_F32;
+    c.place = a.place;
+    c.weights = topk_w;
+    c.weights_step = top_k;
+    c.out_dtype = out_dtype;
+    c.n_tokens = n_tokens;
+    c.top_k = top_k + shared;
+    c.n_rows = pairs;
+    c.hidden = w->hidden;
+    c.out = y;
+    c.out_f32 = y_f32;
+    c.err_flag = ctx->err_flag;
+    if (!rows_grid_ok(pairs, 256) || !rows_grid_ok(combine_workgroups(c), kRowThreads)) return fail(CX_EINVAL, "too many rows for one launch");
+    MmLaunch L{};
+    L.type = kMmI8;
+    L.n_mats = w->n_mats;
+    L.n_rows = pairs;
+    L.offsets = a.offsets;
+    L.err_flag = ctx->err_flag;
+    L.y_type = CX_DTYPE_F32;
+    L.part = reinterpret_cast<float*>(m + z.part);
+    auto product = [&](const int8_t* weights, const float* scales, int rows, int cols, bool gated, const char* q, const char* qs, int n_x,
+                       const int32_t* order, char* out) {
+        L.w = weights;
+        L.w_scale = scales;
+        L.rows = rows;
+        L.cols = cols;
+        L.gated = gated;
+        L.x = q;
+        L.x_scale = reinterpret_cast<const float*>(qs);
+        L.n_x = n_x;
+        L.order = order;
+        L.top_k = top_k + shared;
+        L.y = out;
+        L.form = mm_forward_form(1, L.n_mats, rows, cols, pairs, true);
+        if (!mm_wide(L) && L.form.kind == 2) L.form = MmForm{1, 128, L.form.splits, 1};
+        return launch_mm(L, s);
+    };
+    {
+        Span sp(ctx, "plan", s);
+        CX_HIP(launch_sort_tokens(a, s));
+    }
+    {
+        Span sp(ctx, "quantize", s);
+        CX_HIP(launch_quantize_i8(x, in_dtype, n_tokens, w->hidden, reinterpret_cast<int8_t*>(m + z.q), reinterpret_cast<float*>(m + z.q_scale), s));
+    }
+    {
+        Span sp(ctx, "gate_up", s);
+        CX_HIP(product(w->gate_up, w->gate_up_scale, 2 * w->inter, w->hidden, true, m + z.q, m + z.q_scale, n_tokens, a.order, m + z.h));
+    }
+    {
+        Span sp(ctx, "quantize", s);
+        CX_HIP(launch_quantize_i8(m + z.h, CX_DTYPE_F32, pairs, w->inter, reinterpret_cast<int8_t*>(m + z.hq), reinterpret_cast<float*>(m + z.h_scale), s));
+    }
+    {
+        Span sp(ctx, "down", s);
+        CX_HIP(product(w->down, w->down_scale, w->hidden, w->inter, false, m + z.hq, m + z.h_scale, pairs, nullptr, m + z.ys));
+    }
+    Span sp(ctx, "combine", s);
+    CX_HIP(launch_combine_rows(c, s));
+    return CX_OK;
+}
+
 // ---------------------------------------------------------------------------
 // Whole-layer wire message (MoeLayerRequest / MoeLayerResponse, cx_moe.h).
 

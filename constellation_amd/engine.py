@@ -12,7 +12,7 @@ from typing import NamedTuple, Optional, Sequence, Union
 import numpy as np
 import torch
 
-from ._lib import (BF16, E4M3, F32, FP16, CxError, DeviceInfo, ExpertDesc, MoeLayerRequestInfo,
+from ._lib import (BF16, E4M3, F32, FP16, CxError, DeviceInfo, ExpertDesc, I8LayerDesc, MoeLayerRequestInfo,
                    Q4Desc, check, lib)
 
 _TORCH_TO_CX = {torch.float16: FP16, torch.bfloat16: BF16, torch.float32: F32}
@@ -287,7 +287,27 @@ class Q4Matrix:
             self._live = False
 
 
-class Q4Layer:
+class _OwnLayer:
+    """What Context.moe needs of a layer whose stacks hold some of the layer's experts."""
+
+    def _hold(self, n_mats: int, experts: Optional[Sequence[int]], n_experts: Optional[int]) -> None:
+        held = list(range(n_mats)) if experts is None else [int(e) for e in experts]
+        self.n_experts = max(held) + 1 if n_experts is None and held else n_experts or 0
+        if len(held) != n_mats or len(set(held)) != len(held) or min(held) < 0 or max(held) >= self.n_experts:
+            raise ValueError(f"experts must be {n_mats} different ids below n_experts")
+        self.experts = [None] * self.n_experts  # entry i: who holds expert i here
+        for e in held:
+            self.experts[e] = self
+        # slot in the stacks by id + 1: -1 for no route, one past the stacks for an expert that they do not hold
+        self._slots = None
+        if held != list(range(self.n_experts)):
+            slots = [-1] + [n_mats] * (self.n_experts + 1)
+            for i, e in enumerate(held):
+                slots[e + 1] = i
+            self._slots = torch.tensor(slots, dtype=torch.int32, device=_device(self.ctx.device))
+
+
+class Q4Layer(_OwnLayer):
     """A layer of 4-bit experts: `gate_up` a gated stack [E, 2 * inter, hidden],
     `down` a stack [E, hidden, inter], `shared` the shared expert's two (stacks of
     one), if the layer has one.  Context.moe and Context.moe_layer take it in
@@ -311,22 +331,46 @@ class Q4Layer:
             raise ValueError("a layer's matrices must be on its context's device")
         self.ctx = ctx
         self.gate_up, self.down, self.shared = gate_up, down, shared
-        held = list(range(g.n_mats)) if experts is None else [int(e) for e in experts]
-        self.n_experts = max(held) + 1 if n_experts is None and held else n_experts or 0
-        if len(held) != g.n_mats or len(set(held)) != len(held) or min(held) < 0 or max(held) >= self.n_experts:
-            raise ValueError(f"experts must be {g.n_mats} different ids below n_experts")
         self.hidden, self.inter = d.rows, d.cols
-        self.experts = [None] * self.n_experts  # entry i: who holds expert i here
-        for e in held:
-            self.experts[e] = self
-        # slot in the stacks by id + 1: -1 for no route, one past the stacks for an expert that they do not hold
-        self._slots = None
-        if held != list(range(self.n_experts)):
-            slots = [-1] + [g.n_mats] * (self.n_experts + 1)
-            for i, e in enumerate(held):
-                slots[e + 1] = i
-            self._slots = torch.tensor(slots, dtype=torch.int32, device=_device(ctx.device))
+        self._hold(g.n_mats, experts, n_experts)
         self._scratch: dict = {}  # sizes by tokens and top_k
+
+
+class I8Layer(_OwnLayer):
+    """A layer of experts with 8-bit weights and a scale per channel, as quantize_i8 makes them of the rows of
+    `gate_up` [E, 2 * inter, hidden] (a gate and then an up matrix) and `down` [E, hidden, inter].  With `shared` the
+    last of the stacks' experts is the layer's shared one.  Context.moe and Context.moe_layer take it in place of a
+    Layer, and so does moe_dispatch.LocalNode.  `experts`, `n_experts`: as Q4Layer's, of the routed experts.  The
+    layer keeps the tensors."""
+
+    def __init__(self, ctx: "Context", gate_up: torch.Tensor, gate_up_scale: torch.Tensor, down: torch.Tensor,
+                 down_scale: torch.Tensor, *, shared: bool = False, experts: Optional[Sequence[int]] = None,
+                 n_experts: Optional[int] = None):
+        ctx._here(gate_up, gate_up_scale, down, down_scale)
+        if gate_up.dim() != 3 or down.dim() != 3 or gate_up.shape != (down.shape[0], 2 * down.shape[2], down.shape[1]):
+            raise ValueError("a layer's matrices must be [E, 2 * inter, hidden] and [E, hidden, inter]")
+        if gate_up.dtype != torch.int8 or down.dtype != torch.int8:
+            raise TypeError("weights must be int8")
+        for t, of in ((gate_up_scale, gate_up), (down_scale, down)):
+            if t.shape != of.shape[:2] or t.dtype != torch.float32:
+                raise ValueError(f"scales must be fp32 {list(of.shape[:2])}, one for each row")
+        if not all(t.is_contiguous() for t in (gate_up, gate_up_scale, down, down_scale)):
+            raise ValueError("weights and scales must be contiguous")
+        if down.shape[0] <= int(shared):
+            raise ValueError("a layer needs a routed expert")
+        self.ctx = ctx
+        self.gate_up, self.gate_up_scale, self.down, self.down_scale = gate_up, gate_up_scale, down, down_scale
+        self.shared = self if shared else None
+        E, self.hidden, self.inter = down.shape
+        self.desc = I8LayerDesc(gate_up.data_ptr(), gate_up_scale.data_ptr(), down.data_ptr(), down_scale.data_ptr(), E,
+                                self.hidden, self.inter, int(shared))
+        self._hold(E - int(shared), experts, n_experts)
+        self._scratch: dict = {}  # sizes by tokens and top_k
+
+    @classmethod
+    def quantize(cls, ctx: "Context", gate_up: torch.Tensor, down: torch.Tensor, **kw) -> "I8Layer":
+        """From 16- or 32-bit weights, as a program trains them (matmul)."""
+        return cls(ctx, *ctx.quantize_i8(gate_up), *ctx.quantize_i8(down), **kw)
 
 
 class Context:
@@ -685,26 +729,36 @@ class Context:
                                  _ptr(scratch), size, self.stream()))
         return y
 
-    def _q4_ready(self, layer: Q4Layer, x: torch.Tensor, *others: Optional[torch.Tensor]) -> None:
-        """What a call on a 4-bit layer needs of it and of x, before anything is launched."""
+    def _own_ready(self, layer: _OwnLayer, x: torch.Tensor, *others: Optional[torch.Tensor]) -> None:
+        """What a call on a 4- or 8-bit layer needs of it and of x, before anything is launched."""
         self._here(x, *others)
-        if layer.gate_up.device != self.device:
+        if isinstance(layer, I8Layer):
+            self._here(layer.gate_up)
+        elif layer.gate_up.device != self.device:
             raise ValueError(f"layer on cuda:{layer.gate_up.device}, context on cuda:{self.device}")
-        if not all(m._live for m in (layer.gate_up, layer.down, *(layer.shared or ()))):
+        elif not all(m._live for m in (layer.gate_up, layer.down, *(layer.shared or ()))):
             raise ValueError("a matrix of the layer has been freed")
         if x.dim() != 2 or x.shape[1] != layer.hidden:
             raise ValueError(f"x has {x.shape[-1] if x.dim() else 0} columns in {x.dim()} dimensions, the layer {layer.hidden} in 2")
 
-    def _q4_moe(self, layer: Q4Layer, x, topk_ids, topk_w, y, yf):
-        self._q4_ready(layer, x, topk_ids, topk_w)
+    def _own_moe(self, layer: _OwnLayer, x, topk_ids, topk_w, y, yf):
+        self._own_ready(layer, x, topk_ids, topk_w)
         T, K = x.shape[0], topk_ids.shape[1] if topk_ids.dim() == 2 else -1
         if topk_ids.shape != (T, K) or topk_w.shape != (T, K):
             raise ValueError(f"routes must be [{T}, top_k]")
         if layer._slots is not None:
             topk_ids = layer._slots[topk_ids.clamp(-1, layer.n_experts).long() + 1]
+        size = layer._scratch.get((T, K))
+        if isinstance(layer, I8Layer):
+            if size is None:
+                size = layer._scratch[T, K] = lib().cx_i8_moe_scratch(C.byref(layer.desc), T, K)
+            scratch = torch.empty(size, dtype=torch.uint8, device=x.device)
+            check(lib().cx_i8_moe(self.handle, C.byref(layer.desc), x.data_ptr(), cx_dtype(x.dtype), T, topk_ids.data_ptr(),
+                                  topk_w.data_ptr(), K, y.data_ptr(), cx_dtype(y.dtype), _ptr(yf), scratch.data_ptr(), size,
+                                  self.stream()))
+            return
         gu, dn = C.byref(layer.gate_up.desc), C.byref(layer.down.desc)
         sg, sd = (C.byref(m.desc) for m in layer.shared) if layer.shared else (None, None)
-        size = layer._scratch.get((T, K))
         if size is None:
             size = layer._scratch[T, K] = lib().cx_q4_moe_scratch(gu, dn, int(layer.shared is not None), T, K)
         scratch = torch.empty(size, dtype=torch.uint8, device=x.device)
@@ -713,7 +767,7 @@ class Context:
                               _ptr(yf), scratch.data_ptr(), size, self.stream()))
 
     # -- grouped MoE -----------------------------------------------------------
-    def moe(self, layer: Union[Layer, Q4Layer], x: torch.Tensor, topk_ids: torch.Tensor, topk_w: torch.Tensor, *,
+    def moe(self, layer: Union[Layer, Q4Layer, I8Layer], x: torch.Tensor, topk_ids: torch.Tensor, topk_w: torch.Tensor, *,
             out_dtype: Optional[torch.dtype] = None, want_f32: bool = False,
             prefill: Optional[bool] = None):
         x = x.contiguous()
@@ -727,8 +781,8 @@ class Context:
         fn = lib().cx_moe_prefill if prefill else lib().cx_moe_decode
         ids = topk_ids.to(torch.int32).contiguous()
         w = topk_w.to(torch.float32).contiguous()
-        if isinstance(layer, Q4Layer):
-            self._q4_moe(layer, x, ids, w, y, yf)
+        if isinstance(layer, _OwnLayer):
+            self._own_moe(layer, x, ids, w, y, yf)
             return (y, yf) if want_f32 else y
         check(fn(self.handle, layer.handle, x.data_ptr(), cx_dtype(x.dtype), T, ids.data_ptr(),
                  w.data_ptr(), K, y.data_ptr(), cx_dtype(out_dtype), _ptr(yf), self.stream()))
@@ -750,16 +804,16 @@ class Context:
                                              out.ctypes.data, out.size, C.byref(n)))
         return out[:n.value].tobytes()
 
-    def moe_layer(self, layer: Union[Layer, Q4Layer], x: torch.Tensor, w_router: torch.Tensor, bias: torch.Tensor, *,
+    def moe_layer(self, layer: Union[Layer, Q4Layer, I8Layer], x: torch.Tensor, w_router: torch.Tensor, bias: torch.Tensor, *,
                   resident: Optional[torch.Tensor] = None, n_group: int = 8, topk_group: int = 4,
                   top_k: int = 8, norm_topk_prob: bool = True, routed_scaling_factor: float = 2.5,
                   out_dtype: Optional[torch.dtype] = None, want_f32: bool = False, out=None):
         x = x.contiguous()
         T = x.shape[0]
         out_dtype = out_dtype or x.dtype
-        if isinstance(layer, Q4Layer):  # its router is a launch of its own, before the layer's
+        if isinstance(layer, _OwnLayer):  # its router is a launch of its own, before the layer's
             E, H = layer.n_experts, layer.hidden
-            self._q4_ready(layer, x, w_router, bias, resident, *(out or ()))
+            self._own_ready(layer, x, w_router, bias, resident, *(out or ()))
             w_router, bias = w_router.contiguous(), bias.contiguous()
             resident = None if resident is None else resident.contiguous()
             if w_router.shape != (E, H):
@@ -780,12 +834,12 @@ class Context:
             w = torch.empty((T, top_k), dtype=torch.float32, device=x.device)
         else:
             y, yf, ids, w = out
-        if isinstance(layer, Q4Layer):
+        if isinstance(layer, _OwnLayer):
             check(lib().cx_route(self.handle, x.data_ptr(), cx_dtype(x.dtype), w_router.data_ptr(),
                                  cx_dtype(w_router.dtype), bias.data_ptr(), _ptr(resident), T, layer.hidden,
                                  layer.n_experts, n_group, topk_group, top_k, int(norm_topk_prob),
                                  routed_scaling_factor, ids.data_ptr(), w.data_ptr(), self.stream()))
-            self._q4_moe(layer, x, ids, w, y, yf)
+            self._own_moe(layer, x, ids, w, y, yf)
             return y, yf, ids, w
         check(lib().cx_moe_layer(self.handle, layer.handle, x.data_ptr(), cx_dtype(x.dtype), T,
                                  w_router.data_ptr(), cx_dtype(w_router.dtype), bias.data_ptr(),

@@ -16,7 +16,8 @@ each node once:
     layer id): cx_moe_decode / cx_moe_prefill on the device tensors, with no
     host copy.  When one local node holds every expert of the layer,
     run_moe_layer_batched routes and computes in one cx_moe_layer call.  A
-    layer may be an engine.Q4Layer (4-bit experts): cx_q4_moe.
+    layer may be an engine.Q4Layer (4-bit experts, cx_q4_moe) or an
+    engine.I8Layer (8-bit experts, cx_i8_moe).
   * RemoteNode — an expert node reached through a caller-supplied transport
     (a function from one framed request to one framed reply, or a socket to
     a worker port): one MoeLayerRequest (msg 42, v1 framing
@@ -63,7 +64,7 @@ class LocalNode:
 
     layers: layer id -> engine.Layer whose entry i is the layer's local
     expert i (None where not resident here) and whose shared expert, when
-    present, is the layer's shared expert; or an engine.Q4Layer, whose
+    present, is the layer's shared expert; or an engine.Q4Layer or I8Layer, whose
     `experts` say which of the layer's its stacks hold."""
 
     def __init__(self, layers: dict[int, engine.Layer], device: int = 0):

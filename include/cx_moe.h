@@ -464,6 +464,25 @@ CX_API int cx_i8_matmul(cx_ctx* ctx, const int8_t* x, const float* x_scale, int 
               int n_mats, int rows, int cols, int gated, const int32_t* order, int top_k, const int32_t* offsets,
               int n_rows, void* y, int y_dtype, void* scratch, size_t scratch_bytes, void* stream);
 
+/* A layer of 8-bit experts on given routes, as cx_q4_moe does it for 4-bit ones: same outputs, order of sums
+ * (route order, shared expert last) and route checks.  Stacks of n_mats experts as the program holds
+ * them: gate_up [n_mats, 2 * inter, hidden], down [n_mats, hidden, inter], a fp32 scale per row of each; with
+ * `shared` the last of them is the shared expert and the others are the routed ones.  Rows of x, and of
+ * h = silu(gate) * up (fp32), become 8-bit integers as cx_quantize_i8 makes them.
+ * scratch: cx_i8_moe_scratch bytes of the caller's, as above. */
+typedef struct cx_i8_layer {
+    const int8_t* gate_up;
+    const float* gate_up_scale;
+    const int8_t* down;
+    const float* down_scale;
+    int32_t n_mats, hidden, inter, shared;
+    int32_t reserved[4]; /* zero */
+} cx_i8_layer;
+CX_API size_t cx_i8_moe_scratch(const cx_i8_layer* layer, int n_tokens, int top_k);
+CX_API int cx_i8_moe(cx_ctx* ctx, const cx_i8_layer* layer, const void* x, int in_dtype, int n_tokens, const int32_t* topk_ids,
+              const float* topk_w, int top_k, void* y, int out_dtype, float* y_f32, void* scratch, size_t scratch_bytes,
+              void* stream);
+
 /* ---- whole-layer wire message ---------------------------------------------
  * MoeLayerRequest (msg_type 42) / MoeLayerResponse (43): one request per
  * node per layer instead of one InferRequest per selected expert, sent
