@@ -5,19 +5,18 @@
 namespace cx {
 namespace {
 
-template <class S, bool GATED, bool DMA>
+template <class S, bool GATED>
 hipError_t run(MmLaunch& L, hipStream_t s) {
     const int out = GATED ? S::BM / 2 : S::BM, width = GATED ? L.rows / 2 : L.rows;
     L.m_tiles = (width + out - 1) / out;
-    cx_launch(k_mm<MmI8, S, GATED, DMA>, dim3(mm_grid(L)), dim3(S::kThreads), 0, s, L);
+    cx_launch(k_mm<MmI8, S, GATED>, dim3(mm_grid(L)), dim3(S::kThreads), 0, s, L);
     return hipGetLastError();
 }
 
 template <bool GATED>
 hipError_t pick(MmLaunch& L, hipStream_t s) {
-    const bool wide = mm_wide(L);
-    if (L.form.kind == 0) return mm_few<MmI8, GATED>(L, wide, s);
-    const hipError_t e = !wide ? run<MmSmall, GATED, false>(L, s) : L.form.kind == 2 ? run<MmBig, GATED, true>(L, s) : run<MmSmall, GATED, true>(L, s);
+    if (L.form.kind == 0) return mm_few<MmI8, GATED>(L, L.cols % 16 == 0, s);
+    const hipError_t e = L.form.kind == 2 ? run<MmBig, GATED>(L, s) : run<MmSmall, GATED>(L, s);
     return e != hipSuccess || L.splits == 1 ? e : launch_mm_sum(L, L.rows, GATED, s);
 }
 

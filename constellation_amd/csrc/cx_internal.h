@@ -515,6 +515,8 @@ struct MmLaunch {
     int* err_flag;
     MmForm form;
     float* part;             // splits > 1: [splits][n_rows][rows] (at x: cols), sums of fp32, or of integers as their bits
+    int x_pitch, w_pitch, dy_pitch;  // elements between rows
+    void *pad_x, *pad_w;     // forward: where rows go that are not whole pieces of 16 bytes (NULL: they are)
     int m_tiles, by_item;    // tiles in the output's contiguous direction; mm_tile's order
     int item_rows, splits;
 };
@@ -539,16 +541,23 @@ inline unsigned mm_grid(MmLaunch& L) {
     return (unsigned)(L.by_item ? (items + 7) / 8 * 8 * m : items * ((m + 7) / 8 * 8));
 }
 inline bool mm_at16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
-// Whole pieces of 16 bytes, which go straight to LDS.
-inline bool mm_wide(const MmLaunch& L) { return L.cols % (L.type == kMmI8 ? 16 : 8) == 0 && mm_at16(L.x) && mm_at16(L.w); }
-inline bool mm_wide_dx(const MmLaunch& L) { return L.cols % 8 == 0 && L.rows % 8 == 0 && mm_at16(L.w) && mm_at16(L.dy); }
+// Rows of `cols` elements to rows of `pitch`, zeros behind them; of the matrices (mat_rows rows each) that have rows.
+struct MmPad {
+    const void* src;
+    void* dst;
+    int el, cols, pitch;
+    int64_t rows;            // in all
+    const int32_t* offsets;  // nullable: matrices without rows of x are left out
+    int mat_rows;
+};
+hipError_t launch_mm_pad(const MmPad& p, hipStream_t s);
 hipError_t launch_mm(MmLaunch L, hipStream_t s);
 hipError_t launch_mm_i8(MmLaunch L, hipStream_t s);
 hipError_t launch_mm_sum(const MmLaunch& L, int out, bool gated, hipStream_t s);
 hipError_t launch_mm_dx(MmLaunch L, hipStream_t s);
 hipError_t launch_mm_dw(MmLaunch L, hipStream_t s);
-// dpre of silu(g) * u from dh and pre = [g, u], rounded to their type: [n_rows, 2 * inter].
-hipError_t launch_gate_grad(const void* dh, const void* pre, int type, int64_t n_rows, int inter, void* dpre, hipStream_t s);
+// dpre of silu(g) * u from dh and pre = [g, u], rounded to their type: [n_rows, 2 * inter], rows `pitch` apart, zeros behind them.
+hipError_t launch_gate_grad(const void* dh, const void* pre, int type, int64_t n_rows, int inter, void* dpre, int pitch, hipStream_t s);
 hipError_t launch_quantize_i8(const void* x, int x_type, int n_rows, int cols, int8_t* q, float* scale, hipStream_t s);
 
 }  // namespace cx

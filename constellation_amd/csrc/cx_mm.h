@@ -125,11 +125,6 @@ struct MmShape {
 
 static __device__ __attribute__((aligned(16))) const uint32_t mm_zeros[4] = {};
 
-// 16 bytes at any alignment.
-struct __attribute__((packed)) MmPacked {
-    u32x4 v;
-};
-
 // A pointer that is the same in all lanes, in scalar registers.
 __device__ __forceinline__ const char* mm_uniform(const void* p) {
     const uint64_t v = (uint64_t)p;
@@ -156,7 +151,6 @@ struct MmSrc {
     uint32_t gap;  // TR: bytes between a thread's pieces
     size_t move;   // bytes between steps
     int first;     // place in the step's contraction of the thread's pieces' first element (TR: of its first piece)
-    int left[kAlt];  // TR: elements from the piece's first to the row's end
 
     // offset(r): bytes from base to row r
     template <class F>
@@ -169,8 +163,8 @@ struct MmSrc {
 #pragma unroll
         for (int i = 0; i < P; ++i) off[i] = offset(i * (THREADS / 8) + (t >> 3)) + c * 16;
     }
-    // columns col0 .. of a matrix `width` wide; those past it read others, and their results are not stored
-    __device__ __forceinline__ void cols(const void* base_, int col0, int width) {
+    // columns col0 .. of a matrix `width` wide, rows `pitch` apart; those past it read others, and their results are not stored
+    __device__ __forceinline__ void cols(const void* base_, int pitch, int col0, int width) {
         static_assert(TR, "");
         const int t = threadIdx.x, piece = t % (R / 8);
         first = t / (R / 8);
@@ -178,11 +172,10 @@ struct MmSrc {
 #pragma unroll
         for (int i = 0; i < kAlt; ++i) {
             const int row = first + i * kStepRows, col = col0 + (((piece >> 1) ^ (2 * (row & 3) + (row >> 3 & 1))) * 2 + (piece & 1)) * 8;
-            left[i] = width - col;
-            off[i] = (uint32_t)first * (uint32_t)width * 2 + (left[i] > 0 ? col * 2 : 0);
+            off[i] = (uint32_t)first * (uint32_t)pitch * 2 + (col < width ? col * 2 : 0);
         }
-        gap = (uint32_t)kStepRows * (uint32_t)width * 2;
-        move = (size_t)width * 2 * ROWS;
+        gap = (uint32_t)kStepRows * (uint32_t)pitch * 2;
+        move = (size_t)pitch * 2 * ROWS;
     }
     __device__ __forceinline__ uint32_t place(int i) const { return TR ? off[i % kAlt] + (uint32_t)i * gap : off[TR ? 0 : i]; }
     // Piece i of the step that starts at `from`.
@@ -199,32 +192,6 @@ struct MmSrc {
     __device__ __forceinline__ void fetch_to(unsigned char* lds, int i, int k, int n) const {
         const char* q = k * kStep + first + (TR ? i * kStepRows : 0) < n ? piece(i, step(k)) : reinterpret_cast<const char*>(mm_zeros);
         __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)q, (__attribute__((address_space(3))) void*)(lds + i * THREADS * 16), 16, 0, 0);
-    }
-    // Through registers: rows of any width at any address.
-    __device__ __forceinline__ void load(u32x4 (&v)[P], int k, int n) const {
-        constexpr int kWhole = 16 / EL;
-#pragma unroll
-        for (int i = 0; i < P; ++i) {
-            const int have = TR ? (k * kStep + first + i * kStepRows < n ? left[i % kAlt] : 0) : n - k * kStep - first;
-            const char* q = piece(i, step(k));
-            v[i] = u32x4{};
-            if (have >= kWhole) {
-                v[i] = ((const __attribute__((address_space(1))) MmPacked*)q)->v;
-            } else if (have > 0) {
-#pragma unroll
-                for (int e = 0; e < kWhole - 1; ++e) {
-                    if (e >= have) continue;
-                    if constexpr (EL == 1)
-                        v[i][e / 4] |= (uint32_t)reinterpret_cast<const uint8_t*>(q)[e] << (8 * (e & 3));
-                    else
-                        v[i][e / 2] |= (uint32_t)reinterpret_cast<const uint16_t*>(q)[e] << (16 * (e & 1));
-                }
-            }
-        }
-    }
-    __device__ __forceinline__ void put(unsigned char* lds, const u32x4 (&v)[P]) const {
-#pragma unroll
-        for (int i = 0; i < P; ++i) *reinterpret_cast<u32x4*>(lds + (i * THREADS + threadIdx.x) * 16) = v[i];
     }
 };
 
@@ -314,7 +281,7 @@ __device__ __forceinline__ void mm_barrier() {
 // fragments are read.  Loads into the slots that became free go out one by one between MFMAs: of B at once, of A, whose ring is
 // a slot longer, during the next step.  With two slots of both (4096 rows by 4096 x 7168 in 241 us) the last loads came too late, and half lines
 // with five slots asked L2 for twice as much (271).
-template <class T, class S, bool AT, bool BT, bool DMA>
+template <class T, class S, bool AT, bool BT>
 __device__ __forceinline__ void mm_core(const MmSrc<S::BM, S::kThreads, T::kEl, AT>& a, const MmSrc<S::BN, S::kThreads, T::kEl, BT>& b,
                                         int n, int k0, int k1, unsigned char* lds, typename T::Acc (&acc)[S::TM][S::TN]) {
     typedef MmFrag<S::BM, AT, S::TM> FA;
@@ -329,7 +296,6 @@ __device__ __forceinline__ void mm_core(const MmSrc<S::BM, S::kThreads, T::kEl, 
 #pragma unroll
         for (int t = 0; t < S::TN; ++t) acc[m][t] = typename T::Acc{};
     if (k0 >= k1) return;
-    u32x4 va[MmSrc<S::BM, S::kThreads, T::kEl, AT>::P], vb[MmSrc<S::BN, S::kThreads, T::kEl, BT>::P];  // DMA: not used
     unsigned char *lds_b = lds + S::kEndM, *to_a = lds + wave * 1024, *to_b = lds_b + wave * 1024;
     typename FA::Held xa[2][kHalf];  // of the depth and the next
     typename FB::Held xb[2][S::TN];  // of the half of the contraction and the next
@@ -354,22 +320,21 @@ __device__ __forceinline__ void mm_core(const MmSrc<S::BM, S::kThreads, T::kEl, 
                         fb.template read<N / 2, r.value - kHalf>(xb[N / 2][r.value - kHalf], rb);
                 }
             });
-            if constexpr (DMA)
-                mm_each<kShare>([&](auto r) {
-                    constexpr int j = kFirst + r.value;
-                    if constexpr (r.value * kMma / kShare != i.value) return;
-                    if constexpr (decltype(steady)::value) {
-                        if constexpr (B)
-                            b.fetch(to_b + to, j, pb);
-                        else
-                            a.fetch(to_a + to, j, pa);
-                    } else if (step < k1) {
-                        if constexpr (B)
-                            b.fetch_to(to_b + to, j, step, n);
-                        else
-                            a.fetch_to(to_a + to, j, step, n);
-                    }
-                });
+            mm_each<kShare>([&](auto r) {
+                constexpr int j = kFirst + r.value;
+                if constexpr (r.value * kMma / kShare != i.value) return;
+                if constexpr (decltype(steady)::value) {
+                    if constexpr (B)
+                        b.fetch(to_b + to, j, pb);
+                    else
+                        a.fetch(to_a + to, j, pa);
+                } else if (step < k1) {
+                    if constexpr (B)
+                        b.fetch_to(to_b + to, j, step, n);
+                    else
+                        a.fetch_to(to_a + to, j, step, n);
+                }
+            });
             typename T::Acc& sum = acc[D % 2 * kHalf + m][t];
             sum = T::mma(xa[D % 2][m].v, xb[D / 2][t].v, sum);
             __builtin_amdgcn_sched_barrier(0);
@@ -395,30 +360,18 @@ __device__ __forceinline__ void mm_core(const MmSrc<S::BM, S::kThreads, T::kEl, 
             vm_wait<0>();
     };
     static_assert(S::kSlots >= 2 && S::kSlots <= 4, "arrived()");
-    if constexpr (DMA) {
 #pragma unroll
-        for (int i = 0; i < S::kSlots; ++i) {
-            if (k0 + i >= k1) break;
+    for (int i = 0; i < S::kSlots; ++i) {
+        if (k0 + i >= k1) break;
 #pragma unroll
-            for (int j = 0; j < kLoadsA; ++j) a.fetch_to(to_a + i * S::kStepM, j, k0 + i, n);
+        for (int j = 0; j < kLoadsA; ++j) a.fetch_to(to_a + i * S::kStepM, j, k0 + i, n);
 #pragma unroll
-            for (int j = 0; j < (i < S::kSlots - 1 ? kLoadsB : (kLoadsB + 1) / 2); ++j) b.fetch_to(to_b + i * S::kStepN, j, k0 + i, n);
-        }
-        if (k1 - k0 >= S::kSlots)
-            vm_wait<(S::kSlots - 1) * kLoadsA + (S::kSlots - 2) * kLoadsB + (kLoadsB + 1) / 2>();
-        else
-            vm_wait<0>();
-    } else {
-        a.load(va, k0, n);
-        b.load(vb, k0, n);
-        a.put(lds, va);
-        b.put(lds_b, vb);
-        if (k0 + 1 < k1) {
-            a.load(va, k0 + 1, n);
-            b.load(vb, k0 + 1, n);
-        }
-        __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0)
+        for (int j = 0; j < (i < S::kSlots - 1 ? kLoadsB : (kLoadsB + 1) / 2); ++j) b.fetch_to(to_b + i * S::kStepN, j, k0 + i, n);
     }
+    if (k1 - k0 >= S::kSlots)
+        vm_wait<(S::kSlots - 1) * kLoadsA + (S::kSlots - 2) * kLoadsB + (kLoadsB + 1) / 2>();
+    else
+        vm_wait<0>();
     mm_barrier();
     mm_each<kHalf>([&](auto r) { fa.template read<0, r.value>(xa[0][r.value], 0); });
     mm_each<S::TN>([&](auto r) { fb.template read<0, r.value>(xb[0][r.value], 0); });
@@ -430,23 +383,13 @@ __device__ __forceinline__ void mm_core(const MmSrc<S::BM, S::kThreads, T::kEl, 
         depth(d0, steady, k, sa, sb, was_b);
         pb += b.move;
         depth(d1, steady, k, sa, sb, was_a);
-        if (!DMA && k + 1 < k1) {
-            a.put(lds + na, va);
-            b.put(lds_b + nb, vb);
-        }
         depth(d2, steady, k, sa, sb, was_a);
         pa += a.move;
-        if constexpr (DMA) {
-            if constexpr (decltype(steady)::value)
-                vm_wait<(S::kSlots - 1) * kLoadsA + (S::kSlots - 2) * kLoadsB>();
-            else
-                arrived(k);
-        }
+        if constexpr (decltype(steady)::value)
+            vm_wait<(S::kSlots - 1) * kLoadsA + (S::kSlots - 2) * kLoadsB>();
+        else
+            arrived(k);
         mm_barrier();
-        if (!DMA && k + 2 < k1) {
-            a.load(va, k + 2, n);
-            b.load(vb, k + 2, n);
-        }
         __builtin_amdgcn_sched_barrier(0);
         depth(d3, steady, k, na, nb, sb);  // past the last step it reads what lies in the rings, not used
 #if defined(__HIP_DEVICE_COMPILE__)  // keeps the sums where they are: no copies of them at the loop's end
@@ -461,8 +404,7 @@ __device__ __forceinline__ void mm_core(const MmSrc<S::BM, S::kThreads, T::kEl, 
         sb = nb;
     };
     int k = k0;
-    if constexpr (DMA)
-        for (const int whole = min(k1, n / MmSrc<S::BM, S::kThreads, T::kEl, AT>::kStep); k + S::kSlots < whole; ++k) step(std::true_type{}, k);
+    for (const int whole = min(k1, n / MmSrc<S::BM, S::kThreads, T::kEl, AT>::kStep); k + S::kSlots < whole; ++k) step(std::true_type{}, k);
     for (; k < k1; ++k) step(std::false_type{}, k);
     mm_barrier();
 }
@@ -597,33 +539,33 @@ template <int W, bool WIDE, class F>
 __device__ __forceinline__ void mm_put_rows(const float* turn, void* out, bool bf, bool vec, int m0, int width, F row) {
     constexpr int kChunks = W * 4, kPer = WIDE ? 4 : 8, kLanes = W * 16 / kPer;  // columns of a lane's store, lanes of a row
     const int l = threadIdx.x & 63;
+    if (!vec) {  // a column a lane, so that a store's lanes are neighbours
+#pragma unroll 4
+        for (int i = 0; i < W * 4; ++i) {
+            const int r = (i * 64 + l) / (W * 16), c = (i * 64 + l) % (W * 16);
+            const int64_t at = row(r);
+            if (at < 0 || c >= width - m0) continue;
+            const float f = turn[r * W * 16 + ((c / 4) ^ (r & (kChunks - 1))) * 4 + c % 4];
+            if constexpr (WIDE)
+                static_cast<float*>(out)[at + m0 + c] = f;
+            else
+                static_cast<uint16_t*>(out)[at + m0 + c] = (uint16_t)mm_round2(f, 0.0f, bf);
+        }
+        return;
+    }
 #pragma unroll
     for (int i = 0; i < 16 * kLanes / 64; ++i) {
-        const int r = (i * 64 + l) / kLanes, c = (i * 64 + l) % kLanes * kPer, left = width - m0 - c;
+        const int r = (i * 64 + l) / kLanes, c = (i * 64 + l) % kLanes * kPer;
         const int64_t at = row(r);
-        if (at < 0 || left <= 0) continue;
+        if (at < 0 || c >= width - m0) continue;
         const float* src = turn + r * W * 16;
         const f32x4 a = *reinterpret_cast<const f32x4*>(src + ((c / 4) ^ (r & (kChunks - 1))) * 4);
         if constexpr (WIDE) {
-            float* y = static_cast<float*>(out) + at + m0 + c;
-            if (vec) {
-                *reinterpret_cast<f32x4*>(y) = a;
-            } else {
-#pragma unroll
-                for (int k = 0; k < 4; ++k)
-                    if (k < left) y[k] = a[k];
-            }
+            *reinterpret_cast<f32x4*>(static_cast<float*>(out) + at + m0 + c) = a;
         } else {
             const f32x4 b = *reinterpret_cast<const f32x4*>(src + ((c / 4 + 1) ^ (r & (kChunks - 1))) * 4);
-            const u32x4 h = {mm_round2(a[0], a[1], bf), mm_round2(a[2], a[3], bf), mm_round2(b[0], b[1], bf), mm_round2(b[2], b[3], bf)};
-            uint16_t* y = static_cast<uint16_t*>(out) + at + m0 + c;
-            if (vec) {
-                *reinterpret_cast<u32x4*>(y) = h;
-            } else {
-#pragma unroll
-                for (int k = 0; k < 8; ++k)
-                    if (k < left) y[k] = (uint16_t)(h[k / 2] >> (16 * (k & 1)));
-            }
+            *reinterpret_cast<u32x4*>(static_cast<uint16_t*>(out) + at + m0 + c) =
+                u32x4{mm_round2(a[0], a[1], bf), mm_round2(a[2], a[3], bf), mm_round2(b[0], b[1], bf), mm_round2(b[2], b[3], bf)};
         }
     }
 }
@@ -705,14 +647,14 @@ __device__ __forceinline__ int mm_row_of_x(const MmLaunch& L, int p) {
 
 // Forward.  m: weight rows; a gated tile has TM / 2 results of gate rows and the same rows of the up
 // half per wave, so that both factors of an output meet in one lane.
-template <class T, class S, bool GATED, bool DMA>
+template <class T, class S, bool GATED>
 __device__ __forceinline__ void mm_forward(const MmLaunch& L, const MmWork& work, unsigned char* lds) {
     static_assert(S::kWaves * S::TM * 1024 <= S::kLds, "turned results");
     const MmItem it = work.it;
     const int width = GATED ? L.rows / 2 : L.rows, m0 = work.m0;
     MmSrc<S::BM, S::kThreads, T::kEl, false> a;
     MmSrc<S::BN, S::kThreads, T::kEl, false> b;
-    const size_t pitch = (size_t)L.cols * T::kEl;
+    const size_t pitch = (size_t)L.w_pitch * T::kEl, x_pitch = (size_t)L.x_pitch * T::kEl;
     // weight rows from the tile's first on; those past the matrix are its last one again, and not stored
     constexpr int half = S::TM / 2;  // gated: results of gate rows
     a.rows(static_cast<const char*>(L.w) + ((size_t)it.mat * L.rows + m0) * pitch, [&](int r) {
@@ -722,12 +664,12 @@ __device__ __forceinline__ void mm_forward(const MmLaunch& L, const MmWork& work
     });
     // a row that is not there reads row 0, and its results are zeros
     const int x0 = L.order == nullptr ? it.begin : 0;
-    b.rows(static_cast<const char*>(L.x) + (size_t)x0 * pitch, [&](int r) {
-        return (uint32_t)(max(mm_row_of_x(L, it.begin + min(r, it.rows - 1)), x0) - x0) * (uint32_t)pitch;
+    b.rows(static_cast<const char*>(L.x) + (size_t)x0 * x_pitch, [&](int r) {
+        return (uint32_t)(max(mm_row_of_x(L, it.begin + min(r, it.rows - 1)), x0) - x0) * (uint32_t)x_pitch;
     });
     typename T::Acc acc[S::TM][S::TN];
     const int steps = (L.cols + 128 / T::kEl - 1) / (128 / T::kEl), per = (steps + L.splits - 1) / L.splits, k0 = work.ks * per;
-    mm_core<T, S, false, false, DMA>(a, b, L.cols, k0, min(steps, k0 + per), lds, acc);
+    mm_core<T, S, false, false>(a, b, L.cols, k0, min(steps, k0 + per), lds, acc);
     // results to y
     const int wave = wave_id(), l = threadIdx.x & 63, wm = wave % S::WM, n0 = wave / S::WM * S::TN * 16;
     float* turn = reinterpret_cast<float*>(lds + wave * S::TM * 1024);
@@ -789,26 +731,26 @@ __device__ __forceinline__ void mm_forward(const MmLaunch& L, const MmWork& work
     }
 }
 
-template <class T, class S, bool GATED, bool DMA>
+template <class T, class S, bool GATED>
 __global__ __launch_bounds__(S::kThreads, 2) void k_mm(MmLaunch L) {
     __shared__ __attribute__((aligned(16))) unsigned char lds[S::kLds];
     MmWork work;
     if (!mm_work(L, GATED ? S::BM / 2 : S::BM, GATED ? L.rows / 2 : L.rows, S::kThreads, GATED, &work)) return;
-    mm_fit<S>(work.it.rows, [&](auto s) { mm_forward<T, decltype(s), GATED, DMA>(L, work, lds); });
+    mm_fit<S>(work.it.rows, [&](auto s) { mm_forward<T, decltype(s), GATED>(L, work, lds); });
 }
 
 // The gradient at x.  m: columns of the weights, read across their rows; n: rows of dy.
-template <class T, class S, bool DMA>
+template <class T, class S>
 __device__ __forceinline__ void mm_dx(const MmLaunch& L, const MmWork& work, unsigned char* lds) {
     const MmItem it = work.it;
     const int width = L.cols, m0 = work.m0;
     MmSrc<S::BM, S::kThreads, 2, true> a;
     MmSrc<S::BN, S::kThreads, 2, false> b;
-    a.cols(static_cast<const char*>(L.w) + (size_t)it.mat * L.rows * L.cols * 2, m0, width);
-    b.rows(static_cast<const char*>(L.dy) + (size_t)it.begin * L.rows * 2, [&](int r) { return (uint32_t)min(r, it.rows - 1) * (uint32_t)L.rows * 2; });
+    a.cols(static_cast<const char*>(L.w) + (size_t)it.mat * L.rows * L.w_pitch * 2, L.w_pitch, m0, width);
+    b.rows(static_cast<const char*>(L.dy) + (size_t)it.begin * L.dy_pitch * 2, [&](int r) { return (uint32_t)min(r, it.rows - 1) * (uint32_t)L.dy_pitch * 2; });
     f32x4 acc[S::TM][S::TN];
     const int steps = (L.rows + 63) / 64, per = (steps + L.splits - 1) / L.splits, k0 = work.ks * per;
-    mm_core<T, S, true, false, DMA>(a, b, L.rows, k0, min(steps, k0 + per), lds, acc);
+    mm_core<T, S, true, false>(a, b, L.rows, k0, min(steps, k0 + per), lds, acc);
     const int wave = wave_id(), n0 = wave / S::WM * S::TN * 16;
     float* turn = reinterpret_cast<float*>(lds + wave * S::TM * 1024);
     void* out = L.splits > 1 ? L.part + (size_t)work.ks * L.n_rows * width : L.y;
@@ -823,16 +765,16 @@ __device__ __forceinline__ void mm_dx(const MmLaunch& L, const MmWork& work, uns
     }
 }
 
-template <class T, class S, bool DMA>
+template <class T, class S>
 __global__ __launch_bounds__(S::kThreads, 2) void k_mm_dx(MmLaunch L) {
     __shared__ __attribute__((aligned(16))) unsigned char lds[S::kLds];
     MmWork work;
     if (!mm_work(L, S::BM, L.cols, S::kThreads, false, &work)) return;
-    mm_fit<S>(work.it.rows, [&](auto s) { mm_dx<T, decltype(s), DMA>(L, work, lds); });
+    mm_fit<S>(work.it.rows, [&](auto s) { mm_dx<T, decltype(s)>(L, work, lds); });
 }
 
 // The gradient at the weights of each matrix.  m: their columns; n: their rows.
-template <class T, class S, bool DMA>
+template <class T, class S>
 __global__ __launch_bounds__(S::kThreads, 2) void k_mm_dw(MmLaunch L) {
     __shared__ __attribute__((aligned(16))) unsigned char lds[S::kLds];
     if (L.offsets != nullptr && blockIdx.x == 0 && wave_id() == 0) mm_check(L.offsets, L.n_mats, L.n_rows, L.err_flag);
@@ -841,10 +783,10 @@ __global__ __launch_bounds__(S::kThreads, 2) void k_mm_dw(MmLaunch L) {
     const MmItem it = mm_rows_of(L.offsets, L.n_rows, mat);
     MmSrc<S::BM, S::kThreads, 2, true> a;
     MmSrc<S::BN, S::kThreads, 2, true> b;
-    a.cols(static_cast<const char*>(L.x) + (size_t)it.begin * L.cols * 2, m0, L.cols);
-    b.cols(static_cast<const char*>(L.dy) + (size_t)it.begin * L.rows * 2, n0, L.rows);
+    a.cols(static_cast<const char*>(L.x) + (size_t)it.begin * L.x_pitch * 2, L.x_pitch, m0, L.cols);
+    b.cols(static_cast<const char*>(L.dy) + (size_t)it.begin * L.dy_pitch * 2, L.dy_pitch, n0, L.rows);
     f32x4 acc[S::TM][S::TN];
-    mm_core<T, S, true, true, DMA>(a, b, it.rows, 0, (it.rows + 63) / 64, lds, acc);
+    mm_core<T, S, true, true>(a, b, it.rows, 0, (it.rows + 63) / 64, lds, acc);
     const int wave = wave_id(), nw = n0 + wave / S::WM * S::TN * 16;
     float* turn = reinterpret_cast<float*>(lds + wave * S::TM * 1024);
     const bool vec = mm_vec(L.y, L.cols, L.y_type);
@@ -871,8 +813,8 @@ __global__ __launch_bounds__(S::kThreads, 2) void k_mm_dw_short(MmLaunch L) {
     const MmItem it = mm_rows_of(L.offsets, L.n_rows, mat);
     typename MmShort<S>::A a;
     typename MmShort<S>::B b;
-    a.cols(static_cast<const char*>(L.x) + (size_t)it.begin * L.cols * 2, m0, L.cols);
-    b.cols(static_cast<const char*>(L.dy) + (size_t)it.begin * L.rows * 2, n0, L.rows);
+    a.cols(static_cast<const char*>(L.x) + (size_t)it.begin * L.x_pitch * 2, L.x_pitch, m0, L.cols);
+    b.cols(static_cast<const char*>(L.dy) + (size_t)it.begin * L.dy_pitch * 2, L.dy_pitch, n0, L.rows);
     f32x4 acc[S::TM][S::TN];
     mm_core_short<T, S>(a, b, it.rows, lds, acc);
     const int wave = wave_id(), nw = n0 + wave / S::WM * S::TN * 16;

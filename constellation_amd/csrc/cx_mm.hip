@@ -5,19 +5,18 @@
 namespace cx {
 namespace {
 
-template <class T, class S, bool GATED, bool DMA>
+template <class T, class S, bool GATED>
 hipError_t run(MmLaunch& L, hipStream_t s) {
     const int out = GATED ? S::BM / 2 : S::BM, width = GATED ? L.rows / 2 : L.rows;
     L.m_tiles = (width + out - 1) / out;
-    cx_launch(k_mm<T, S, GATED, DMA>, dim3(mm_grid(L)), dim3(S::kThreads), 0, s, L);
+    cx_launch(k_mm<T, S, GATED>, dim3(mm_grid(L)), dim3(S::kThreads), 0, s, L);
     return hipGetLastError();
 }
 
 template <class T, bool GATED>
 hipError_t pick(MmLaunch& L, hipStream_t s) {
-    const bool wide = mm_wide(L);
-    if (L.form.kind == 0) return mm_few<T, GATED>(L, wide, s);
-    const hipError_t e = !wide ? run<T, MmSmall, GATED, false>(L, s) : L.form.kind == 2 ? run<T, MmBig, GATED, true>(L, s) : run<T, MmSmall, GATED, true>(L, s);
+    if (L.form.kind == 0) return mm_few<T, GATED>(L, L.cols % 8 == 0, s);
+    const hipError_t e = L.form.kind == 2 ? run<T, MmBig, GATED>(L, s) : run<T, MmSmall, GATED>(L, s);
     return e != hipSuccess || L.splits == 1 ? e : launch_mm_sum(L, L.rows, GATED, s);
 }
 
@@ -95,7 +94,29 @@ __global__ __launch_bounds__(256) void k_mm_sum(MmLaunch L, int out, int gated, 
     put(L.y, L.y_type, (int64_t)p * width + c, v[0]);
 }
 
+// A piece of 16 bytes of a row a lane.
+template <int EL>
+__global__ __launch_bounds__(256) void k_mm_pad(MmPad p) {
+    const int per = p.pitch / (16 / EL);
+    const int64_t total = p.rows * per;
+    for (int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x; at < total; at += (int64_t)gridDim.x * 256) {
+        const int64_t row = total <= 0xFFFFFFFFll ? (uint32_t)at / (uint32_t)per : at / per;
+        if (p.offsets != nullptr) {
+            const int64_t mat = row / p.mat_rows;
+            if (p.offsets[mat + 1] <= 0 || p.offsets[mat + 1] <= p.offsets[mat]) continue;  // cut offsets give it no rows either
+        }
+        const int c = (int)(at - row * per) * (16 / EL);
+        static_cast<u32x4*>(p.dst)[at] = mm_piece<EL, false>(static_cast<const char*>(p.src) + (row * p.cols + c) * EL, p.cols - c);
+    }
+}
+
 }  // namespace
+
+hipError_t launch_mm_pad(const MmPad& p, hipStream_t s) {
+    const int64_t wgs = (p.rows * (p.pitch / (16 / p.el)) + 255) / 256;
+    cx_launch(p.el == 1 ? k_mm_pad<1> : k_mm_pad<2>, dim3((unsigned)std::min<int64_t>(wgs, 16384)), dim3(256), 0, s, p);
+    return hipGetLastError();
+}
 
 hipError_t launch_mm_sum(const MmLaunch& L, int out, bool gated, hipStream_t s) {
     const int chunks = ((gated ? out / 2 : out) + 1023) / 1024;
@@ -104,6 +125,17 @@ hipError_t launch_mm_sum(const MmLaunch& L, int out, bool gated, hipStream_t s) 
 }
 
 hipError_t launch_mm(MmLaunch L, hipStream_t s) {
+    const int el = L.type == kMmI8 ? 1 : 2;
+    L.x_pitch = L.w_pitch = L.cols;
+    if (L.pad_w != nullptr) {
+        const int pitch = mm_pitch(L.cols, el);
+        hipError_t e = launch_mm_pad(MmPad{L.x, L.pad_x, el, L.cols, pitch, L.n_x, nullptr, 1}, s);
+        if (e == hipSuccess) e = launch_mm_pad(MmPad{L.w, L.pad_w, el, L.cols, pitch, (int64_t)L.n_mats * L.rows, L.offsets, L.rows}, s);
+        if (e != hipSuccess) return e;
+        L.x = L.pad_x;
+        L.w = L.pad_w;
+        L.x_pitch = L.w_pitch = pitch;
+    }
     if (L.type == CX_DTYPE_BF16) return L.gated ? pick<MmBf16, true>(L, s) : pick<MmBf16, false>(L, s);
     if (L.type == CX_DTYPE_FP16) return L.gated ? pick<MmF16, true>(L, s) : pick<MmF16, false>(L, s);
     return launch_mm_i8(L, s);

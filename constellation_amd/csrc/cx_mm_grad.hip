@@ -4,18 +4,18 @@
 namespace cx {
 namespace {
 
-template <class T, class S, bool DMA>
+template <class T, class S>
 hipError_t dx(MmLaunch& L, hipStream_t s) {
     L.m_tiles = (L.cols + S::BM - 1) / S::BM;
-    cx_launch(k_mm_dx<T, S, DMA>, dim3(mm_grid(L)), dim3(S::kThreads), 0, s, L);
+    cx_launch(k_mm_dx<T, S>, dim3(mm_grid(L)), dim3(S::kThreads), 0, s, L);
     return hipGetLastError();
 }
 
-template <class T, class S, bool DMA>
+template <class T, class S>
 hipError_t dw(MmLaunch& L, hipStream_t s) {
     L.m_tiles = (L.cols + S::BM - 1) / S::BM;
     const int64_t tiles = (int64_t)L.n_mats * L.m_tiles * ((L.rows + S::BN - 1) / S::BN);
-    cx_launch(k_mm_dw<T, S, DMA>, dim3((unsigned)tiles), dim3(S::kThreads), 0, s, L);
+    cx_launch(k_mm_dw<T, S>, dim3((unsigned)tiles), dim3(S::kThreads), 0, s, L);
     return hipGetLastError();
 }
 
@@ -29,23 +29,22 @@ hipError_t dw_short(MmLaunch& L, hipStream_t s) {
 
 template <class T>
 hipError_t dx_pick(MmLaunch& L, hipStream_t s) {
-    const hipError_t e = !mm_wide_dx(L) ? dx<T, MmSmall, false>(L, s) : L.form.kind == 2 ? dx<T, MmBig, true>(L, s) : dx<T, MmSmall, true>(L, s);
+    const hipError_t e = L.form.kind == 2 ? dx<T, MmBig>(L, s) : dx<T, MmSmall>(L, s);
     return e != hipSuccess || L.splits == 1 ? e : launch_mm_sum(L, L.cols, false, s);
 }
 
 template <class T>
 hipError_t dw_pick(MmLaunch& L, hipStream_t s) {
-    if (L.cols % 8 != 0 || L.rows % 8 != 0 || !mm_at16(L.x) || !mm_at16(L.dy)) return dw<T, MmSmall, false>(L, s);
     const int64_t tiles = (int64_t)L.n_mats * ((L.cols + 255) / 256) * ((L.rows + 255) / 256);
-    if (tiles < 256) return dw<T, MmSmall, true>(L, s);
+    if (tiles < 256) return dw<T, MmSmall>(L, s);
     // 4096 x 7168: 32 matrices with 512 rows each 1162 us with short steps and 1215 with long ones, one with 2048 109 and 100
-    return L.n_rows < (int64_t)L.n_mats * 1024 ? dw_short<T, MmMid>(L, s) : dw<T, MmBig, true>(L, s);
+    return L.n_rows < (int64_t)L.n_mats * 1024 ? dw_short<T, MmMid>(L, s) : dw<T, MmBig>(L, s);
 }
 
 // h = silu(g) u has dg = dh u sig(g) (1 + g (1 - sig(g))) and du = dh silu(g); each rounded once.  One value
 // of dh, g and u a lane, 8 where rows allow 16-byte accesses.  HBM bounds it.
 template <bool BF, int N>
-__global__ __launch_bounds__(256) void k_gate_grad(const uint16_t* dh, const uint16_t* pre, int64_t n_rows, int inter, uint16_t* dpre) {
+__global__ __launch_bounds__(256) void k_gate_grad(const uint16_t* dh, const uint16_t* pre, int64_t n_rows, int inter, uint16_t* dpre, int pitch) {
     const int per = (inter + N - 1) / N;
     const int64_t total = n_rows * per;
     for (int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x; at < total; at += (int64_t)gridDim.x * 256) {
@@ -55,7 +54,7 @@ __global__ __launch_bounds__(256) void k_gate_grad(const uint16_t* dh, const uin
         auto value = [](uint16_t h) { return BF ? __uint_as_float((uint32_t)h << 16) : (float)__builtin_bit_cast(_Float16, h); };
         auto round = [](float f) { return (uint16_t)(BF ? bf16_rne(f) : f16_rne(f)); };
         V d = {}, g = {}, u = {}, a, b;
-        const int64_t o = p * 2 * inter + c;
+        const int64_t o = p * 2 * inter + c, to = p * pitch + c;
         if constexpr (N == 1) {
             d[0] = dh[p * inter + c], g[0] = pre[o], u[0] = pre[o + inter];
         } else {
@@ -70,11 +69,13 @@ __global__ __launch_bounds__(256) void k_gate_grad(const uint16_t* dh, const uin
             b[i] = round(t * x * sig);
         }
         if constexpr (N == 1) {
-            dpre[o] = a[0], dpre[o + inter] = b[0];
+            dpre[to] = a[0], dpre[to + inter] = b[0];
         } else {
-            *reinterpret_cast<V*>(dpre + o) = a;
-            *reinterpret_cast<V*>(dpre + o + inter) = b;
+            *reinterpret_cast<V*>(dpre + to) = a;
+            *reinterpret_cast<V*>(dpre + to + inter) = b;
         }
+        if (c == 0)
+            for (int i = 2 * inter; i < pitch; ++i) dpre[p * pitch + i] = 0;
     }
 }
 
@@ -83,12 +84,12 @@ __global__ __launch_bounds__(256) void k_gate_grad(const uint16_t* dh, const uin
 hipError_t launch_mm_dx(MmLaunch L, hipStream_t s) { return L.type == CX_DTYPE_BF16 ? dx_pick<MmBf16>(L, s) : dx_pick<MmF16>(L, s); }
 hipError_t launch_mm_dw(MmLaunch L, hipStream_t s) { return L.type == CX_DTYPE_BF16 ? dw_pick<MmBf16>(L, s) : dw_pick<MmF16>(L, s); }
 
-hipError_t launch_gate_grad(const void* dh, const void* pre, int type, int64_t n_rows, int inter, void* dpre, hipStream_t s) {
+hipError_t launch_gate_grad(const void* dh, const void* pre, int type, int64_t n_rows, int inter, void* dpre, int pitch, hipStream_t s) {
     const bool vec = inter % 8 == 0 && mm_at16(dh) && mm_at16(pre) && mm_at16(dpre);
     const int64_t wgs = (n_rows * ((inter + (vec ? 7 : 0)) / (vec ? 8 : 1)) + 255) / 256;
     auto k = type == CX_DTYPE_BF16 ? (vec ? k_gate_grad<true, 8> : k_gate_grad<true, 1>) : (vec ? k_gate_grad<false, 8> : k_gate_grad<false, 1>);
     cx_launch(k, dim3((unsigned)std::min<int64_t>(wgs, 8192)), dim3(256), 0, s, static_cast<const uint16_t*>(dh), static_cast<const uint16_t*>(pre),
-              n_rows, inter, static_cast<uint16_t*>(dpre));
+              n_rows, inter, static_cast<uint16_t*>(dpre), pitch);
     return hipGetLastError();
 }
 

@@ -805,7 +805,7 @@ int check_mm(cx_ctx* ctx, int el, int n_mats, int rows, int cols, int gated, con
     if (n_mats < 1 || n_mats > kSortMaxExperts) return fail(CX_EINVAL, "n_mats must be 1..%d", kSortMaxExperts);
     if (rows < 1 || cols < 1 || rows > kMmMaxSide || cols > (el == 1 ? kI8MaxCols : kMmMaxSide))
         return fail(CX_EINVAL, "rows must be 1..%d and cols 1..%d", kMmMaxSide, el == 1 ? kI8MaxCols : kMmMaxSide);
-    if ((uint64_t)rows * cols * el >= (uint64_t)1 << 32) return fail(CX_EINVAL, "a matrix must have fewer than 2^32 bytes");
+    if ((uint64_t)rows * mm_pitch(cols, el) * el >= (uint64_t)1 << 32) return fail(CX_EINVAL, "a matrix must have fewer than 2^32 bytes");
     if (gated && rows % 2 != 0) return fail(CX_EINVAL, "a gated matrix has an even number of rows");
     if (n_rows < 0) return fail(CX_EINVAL, "bad n_rows");
     if (!offsets && n_mats != 1) return fail(CX_EINVAL, "a stack of %d matrices needs offsets", n_mats);
@@ -819,14 +819,33 @@ int check_scratch(size_t need, const void* scratch, size_t bytes) {
     return CX_OK;
 }
 
-// How a forward product is cut, and its partial sums; the same whether or not its rows turn out to be whole pieces.
-MmForm mm_forward_form(int el, int n_mats, int rows, int cols, int n_rows, bool stack) {
-    return mm_form(n_rows, n_mats, stack, rows, (int64_t)cols * el, cols % (16 / el) == 0, true);
+size_t up256(size_t v) { return (v + 255) / 256 * 256; }
+size_t mm_part_bytes(const MmForm& f, int64_t n_rows, int64_t out) { return f.kind > 0 && f.splits > 1 ? up256((size_t)f.splits * n_rows * out * 4) : 0; }
+size_t mm_pad_bytes(int64_t rows, int cols, int el) { return cols % (16 / el) ? up256((size_t)rows * mm_pitch(cols, el) * el) : 0; }
+
+// How a forward product is cut, and its scratch: partial sums, and copies of rows that are not whole pieces.
+struct MmPlan {
+    MmForm form;
+    size_t x, w, bytes;  // partial sums come first
+};
+MmPlan mm_plan(int el, int64_t n_x, int n_mats, int rows, int cols, int64_t n_rows, bool stack) {
+    MmPlan p{mm_form(n_rows, n_mats, stack, rows, (int64_t)cols * el, true), 0, 0, 0};
+    if (p.form.kind == 0) return p;
+    p.x = mm_part_bytes(p.form, n_rows, rows);
+    p.w = p.x + mm_pad_bytes(n_x, cols, el);
+    p.bytes = p.w + mm_pad_bytes((int64_t)n_mats * rows, cols, el);
+    return p;
 }
-size_t mm_part_bytes(const MmForm& f, int64_t n_rows, int64_t out) { return f.kind > 0 && f.splits > 1 ? (size_t)f.splits * n_rows * out * 4 : 0; }
+void use_plan(const MmPlan& p, void* scratch, MmLaunch* L) {
+    char* m = static_cast<char*>(scratch);
+    L->form = p.form;
+    L->part = reinterpret_cast<float*>(m);
+    L->pad_x = p.w > p.x ? m + p.x : nullptr;
+    L->pad_w = p.bytes > p.w ? m + p.w : nullptr;
+}
 
 // The forward products in 16 bits (x_scale NULL) and in 8.
-int matmul(cx_ctx* ctx, MmLaunch L, size_t need, void* scratch, size_t scratch_bytes, void* stream) {
+int matmul(cx_ctx* ctx, MmLaunch L, void* scratch, size_t scratch_bytes, void* stream) {
     const int el = L.type == kMmI8 ? 1 : 2;
     int rc = check_mm(ctx, el, L.n_mats, L.rows, L.cols, L.gated, L.offsets, L.n_rows);
     if (rc) return rc;
@@ -836,14 +855,14 @@ int matmul(cx_ctx* ctx, MmLaunch L, size_t need, void* scratch, size_t scratch_b
     if (!L.order && L.n_x != L.n_rows) return fail(CX_EINVAL, "without an order x and y have the same rows (%d and %d)", L.n_x, L.n_rows);
     if (L.n_rows == 0) return CX_OK;
     if (L.n_x == 0) return fail(CX_EINVAL, "x has no rows");
-    if (L.order && (uint64_t)L.n_x * L.cols * el >= (uint64_t)1 << 32) return fail(CX_EINVAL, "rows picked by an order must have fewer than 2^32 bytes in all");
+    if (L.order && (uint64_t)L.n_x * mm_pitch(L.cols, el) * el >= (uint64_t)1 << 32) return fail(CX_EINVAL, "rows picked by an order must have fewer than 2^32 bytes in all");
     if (!L.x || !L.w || !L.y || (el == 1 && (!L.x_scale || !L.w_scale))) return fail(CX_EINVAL, "NULL buffer");
-    if ((rc = check_scratch(need, scratch, scratch_bytes))) return rc;
+    if (!mm_at16(L.x) || !mm_at16(L.w)) return fail(CX_EINVAL, "x and weights must start on 16 bytes");
+    const MmPlan p = mm_plan(el, L.n_x, L.n_mats, L.rows, L.cols, L.n_rows, L.offsets != nullptr);
+    if ((rc = check_scratch(p.bytes, scratch, scratch_bytes))) return rc;
     if ((rc = set_device(ctx->device))) return rc;
     L.err_flag = ctx->err_flag;
-    L.form = mm_forward_form(el, L.n_mats, L.rows, L.cols, L.n_rows, L.offsets != nullptr);
-    L.part = static_cast<float*>(scratch);
-    if (!mm_wide(L) && L.form.kind == 2) L.form = MmForm{1, 128, L.form.splits, 1};
+    use_plan(p, scratch, &L);
     hipStream_t s = static_cast<hipStream_t>(stream);
     Span sp(ctx, "matmul", s);
     CX_HIP(launch_mm(L, s));
@@ -1783,10 +1802,10 @@ int cx_q4_moe(cx_ctx* ctx, const cx_q4_desc* gate_up, const cx_q4_desc* down, co
 // ---------------------------------------------------------------------------
 // Products of a program's own experts.
 
-size_t cx_matmul_scratch(int dtype, int n_mats, int rows, int cols, int gated, int n_rows, int with_offsets) {
-    (void)gated;
-    if (n_mats < 1 || rows < 1 || cols < 1 || n_rows < 1) return 0;
-    return mm_part_bytes(mm_forward_form(dtype == kMmI8 ? 1 : 2, n_mats, rows, cols, n_rows, with_offsets != 0), n_rows, rows);
+size_t cx_matmul_scratch(int dtype, int n_x, int n_mats, int rows, int cols, int n_rows, int with_offsets) {
+    (void)dtype;  // both have two bytes
+    if (n_x < 1 || n_mats < 1 || rows < 1 || cols < 1 || n_rows < 1) return 0;
+    return mm_plan(2, n_x, n_mats, rows, cols, n_rows, with_offsets != 0).bytes;
 }
 
 int cx_matmul(cx_ctx* ctx, const void* x, int n_x, const void* w, int dtype, int n_mats, int rows, int cols, int gated,
@@ -1810,21 +1829,23 @@ int cx_matmul(cx_ctx* ctx, const void* x, int n_x, const void* w, int dtype, int
     L.y = y;
     L.y_type = y_dtype;
     L.pre = pre;
-    return matmul(ctx, L, cx_matmul_scratch(dtype, n_mats, rows, cols, gated, n_rows, offsets != nullptr), scratch, scratch_bytes, stream);
+    return matmul(ctx, L, scratch, scratch_bytes, stream);
 }
 
 namespace {
-// The gradient's scratch: the gradient at pre, then dx's partial sums.
+// The gradient's scratch: the gradient at pre, or copies of dy's rows; copies of x's and of the weights'; dx's partial sums.
 struct GradScratch {
     MmForm dx;
-    size_t part, bytes;
+    size_t x, w, part, bytes;  // dy's rows come first
 };
-GradScratch grad_scratch(int n_mats, int rows, int cols, bool gated, int n_rows, bool stack, bool with_dx) {
+GradScratch grad_scratch(int n_mats, int rows, int cols, bool gated, int64_t n_rows, bool stack, bool with_dx, bool with_dw) {
     GradScratch z{};
-    z.part = gated ? ((size_t)n_rows * rows * 2 + 15) / 16 * 16 : 0;
+    z.x = gated ? up256((size_t)n_rows * mm_pitch(rows, 2) * 2) : mm_pad_bytes(n_rows, rows, 2);
+    z.w = z.x + (with_dw ? mm_pad_bytes(n_rows, cols, 2) : 0);
+    z.part = z.w + (with_dx ? mm_pad_bytes((int64_t)n_mats * rows, cols, 2) : 0);
     z.bytes = z.part;
     if (with_dx) {
-        z.dx = mm_form(n_rows, n_mats, stack, cols, (int64_t)rows * 2, rows % 8 == 0 && cols % 8 == 0, false);
+        z.dx = mm_form(n_rows, n_mats, stack, cols, (int64_t)rows * 2, false);
         z.bytes += mm_part_bytes(z.dx, n_rows, cols);
     }
     return z;
@@ -1832,10 +1853,10 @@ GradScratch grad_scratch(int n_mats, int rows, int cols, bool gated, int n_rows,
 }  // namespace
 
 size_t cx_matmul_grad_scratch(int dtype, int n_mats, int rows, int cols, int gated, int n_rows, int with_offsets, int with_dx,
-                              int dw_dtype) {
-    (void)dtype, (void)dw_dtype;
+                              int with_dw) {
+    (void)dtype;
     if (n_mats < 1 || rows < 1 || cols < 1 || n_rows < 1) return 0;
-    return grad_scratch(n_mats, rows, cols, gated != 0, n_rows, with_offsets != 0, with_dx != 0).bytes;
+    return grad_scratch(n_mats, rows, cols, gated != 0, n_rows, with_offsets != 0, with_dx != 0, with_dw != 0).bytes;
 }
 
 int cx_matmul_grad(cx_ctx* ctx, const void* dy, const void* x, const void* w, int dtype, const void* pre, int n_mats, int rows,
@@ -1849,7 +1870,8 @@ int cx_matmul_grad(cx_ctx* ctx, const void* dy, const void* x, const void* w, in
     if (dw && dw_dtype != dtype && dw_dtype != CX_DTYPE_F32) return fail(CX_EINVAL, "dw must be of x's type or fp32");
     if (n_rows == 0 && !dw) return CX_OK;
     if ((n_rows > 0 && (!dy || (dw && !x))) || (dx && !w)) return fail(CX_EINVAL, "NULL buffer");
-    const GradScratch z = n_rows > 0 ? grad_scratch(n_mats, rows, cols, pre != nullptr, n_rows, offsets != nullptr, dx != nullptr) : GradScratch{};
+    if (!mm_at16(dy) || (dw && !mm_at16(x)) || (dx && !mm_at16(w))) return fail(CX_EINVAL, "dy, x and weights must start on 16 bytes");
+    const GradScratch z = n_rows > 0 ? grad_scratch(n_mats, rows, cols, pre != nullptr, n_rows, offsets != nullptr, dx != nullptr, dw != nullptr) : GradScratch{};
     if ((rc = check_scratch(z.bytes, scratch, scratch_bytes))) return rc;
     if ((rc = set_device(ctx->device))) return rc;
     hipStream_t s = static_cast<hipStream_t>(stream);
@@ -1865,16 +1887,34 @@ int cx_matmul_grad(cx_ctx* ctx, const void* dy, const void* x, const void* w, in
     L.offsets = offsets;
     L.err_flag = ctx->err_flag;
     Span sp(ctx, "matmul_grad", s);
-    if (pre && n_rows > 0) {
-        CX_HIP(launch_gate_grad(dy, pre, dtype, n_rows, rows / 2, scratch, s));
-        L.dy = scratch;
+    char* m = static_cast<char*>(scratch);
+    L.x_pitch = L.w_pitch = cols;
+    L.dy_pitch = rows;
+    if (n_rows > 0) {
+        const int rp = mm_pitch(rows, 2), cp = mm_pitch(cols, 2);
+        if (pre) {
+            CX_HIP(launch_gate_grad(dy, pre, dtype, n_rows, rows / 2, m, rp, s));
+            L.dy = m;
+        } else if (rp != rows) {
+            CX_HIP(launch_mm_pad(MmPad{dy, m, 2, rows, rp, n_rows, nullptr, 1}, s));
+            L.dy = m;
+        }
+        L.dy_pitch = rp;
+        if (cp != cols && dw) {
+            CX_HIP(launch_mm_pad(MmPad{x, m + z.x, 2, cols, cp, n_rows, nullptr, 1}, s));
+            L.x = m + z.x;
+        }
+        if (cp != cols && dx) {
+            CX_HIP(launch_mm_pad(MmPad{w, m + z.w, 2, cols, cp, (int64_t)n_mats * rows, offsets, rows}, s));
+            L.w = m + z.w;
+        }
+        L.x_pitch = L.w_pitch = cp;
     }
     if (dx && n_rows > 0) {
         L.y = dx;
         L.y_type = dtype;
         L.form = z.dx;
-        L.part = reinterpret_cast<float*>(static_cast<char*>(scratch) + z.part);
-        if (!mm_wide_dx(L) && L.form.kind == 2) L.form = MmForm{1, 128, L.form.splits, 1};
+        L.part = reinterpret_cast<float*>(m + z.part);
         CX_HIP(launch_mm_dx(L, s));
     }
     if (dw) {
@@ -1899,8 +1939,9 @@ int cx_quantize_i8(cx_ctx* ctx, const void* x, int x_dtype, int n_rows, int cols
     return CX_OK;
 }
 
-size_t cx_i8_matmul_scratch(int n_mats, int rows, int cols, int gated, int n_rows, int with_offsets) {
-    return cx_matmul_scratch(kMmI8, n_mats, rows, cols, gated, n_rows, with_offsets);
+size_t cx_i8_matmul_scratch(int n_x, int n_mats, int rows, int cols, int n_rows, int with_offsets) {
+    if (n_x < 1 || n_mats < 1 || rows < 1 || cols < 1 || n_rows < 1) return 0;
+    return mm_plan(1, n_x, n_mats, rows, cols, n_rows, with_offsets != 0).bytes;
 }
 
 int cx_i8_matmul(cx_ctx* ctx, const int8_t* x, const float* x_scale, int n_x, const int8_t* w, const float* w_scale, int n_mats,
@@ -1924,13 +1965,14 @@ int cx_i8_matmul(cx_ctx* ctx, const int8_t* x, const float* x_scale, int n_x, co
     L.offsets = offsets;
     L.y = y;
     L.y_type = y_dtype;
-    return matmul(ctx, L, cx_i8_matmul_scratch(n_mats, rows, cols, gated, n_rows, offsets != nullptr), scratch, scratch_bytes, stream);
+    return matmul(ctx, L, scratch, scratch_bytes, stream);
 }
 
 namespace {
 struct I8MoeScratch {
     int64_t pairs;
-    size_t order, offsets, place, q, q_scale, h, hq, h_scale, ys, part, bytes;
+    size_t order, offsets, place, q, q_scale, h, hq, h_scale, ys, product, bytes;
+    MmPlan gate_up, down;
 };
 I8MoeScratch i8_moe_scratch(const cx_i8_layer& w, int64_t n_tokens, int top_k) {
     I8MoeScratch z{};
@@ -1951,8 +1993,9 @@ I8MoeScratch i8_moe_scratch(const cx_i8_layer& w, int64_t n_tokens, int top_k) {
     z.hq = take(p * w.inter);
     z.h_scale = take(p * 4);
     z.ys = take(p * w.hidden * 4);
-    z.part = take(std::max(mm_part_bytes(mm_forward_form(1, w.n_mats, 2 * w.inter, w.hidden, (int)z.pairs, true), z.pairs, 2 * w.inter),
-                           mm_part_bytes(mm_forward_form(1, w.n_mats, w.hidden, w.inter, (int)z.pairs, true), z.pairs, w.hidden)));
+    z.gate_up = mm_plan(1, n_tokens, w.n_mats, 2 * w.inter, w.hidden, z.pairs, true);
+    z.down = mm_plan(1, z.pairs, w.n_mats, w.hidden, w.inter, z.pairs, true);
+    z.product = take(std::max(z.gate_up.bytes, z.down.bytes));
     z.bytes = at;
     return z;
 }
@@ -1980,9 +2023,10 @@ int cx_i8_moe(cx_ctx* ctx, const cx_i8_layer* w, const void* x, int in_dtype, in
     if (w->inter < 1 || w->inter > kMmMaxSide / 2) return fail(CX_EINVAL, "inter must be 1..%d", kMmMaxSide / 2);
     int rc = check_mm(ctx, 1, w->n_mats, 2 * w->inter, w->hidden, 1, w, pairs);
     if (rc || (rc = check_mm(ctx, 1, w->n_mats, w->hidden, w->inter, 0, w, pairs))) return rc;
-    if ((uint64_t)n_tokens * w->hidden >= (uint64_t)1 << 32) return fail(CX_EINVAL, "x must have fewer than 2^32 values");
+    if ((uint64_t)n_tokens * mm_pitch(w->hidden, 1) >= (uint64_t)1 << 32) return fail(CX_EINVAL, "x must have fewer than 2^32 values");
     if (n_tokens == 0) return CX_OK;
     if (!x || !y || (top_k > 0 && (!topk_ids || !topk_w))) return fail(CX_EINVAL, "NULL buffer");
+    if (!mm_at16(w->gate_up) || !mm_at16(w->down)) return fail(CX_EINVAL, "weights must start on 16 bytes");
     const I8MoeScratch z = i8_moe_scratch(*w, n_tokens, top_k);
     if ((rc = check_scratch(z.bytes, scratch, scratch_bytes))) return rc;
     if ((rc = set_device(ctx->device))) return rc;
@@ -2021,9 +2065,9 @@ int cx_i8_moe(cx_ctx* ctx, const cx_i8_layer* w, const void* x, int in_dtype, in
     L.offsets = a.offsets;
     L.err_flag = ctx->err_flag;
     L.y_type = CX_DTYPE_F32;
-    L.part = reinterpret_cast<float*>(m + z.part);
     auto product = [&](const int8_t* weights, const float* scales, int rows, int cols, bool gated, const char* q, const char* qs, int n_x,
-                       const int32_t* order, char* out) {
+                       const int32_t* order, char* out, const MmPlan& plan) {
+        use_plan(plan, m + z.product, &L);
         L.w = weights;
         L.w_scale = scales;
         L.rows = rows;
@@ -2035,8 +2079,6 @@ int cx_i8_moe(cx_ctx* ctx, const cx_i8_layer* w, const void* x, int in_dtype, in
         L.order = order;
         L.top_k = top_k + shared;
         L.y = out;
-        L.form = mm_forward_form(1, L.n_mats, rows, cols, pairs, true);
-        if (!mm_wide(L) && L.form.kind == 2) L.form = MmForm{1, 128, L.form.splits, 1};
         return launch_mm(L, s);
     };
     {
@@ -2049,7 +2091,7 @@ int cx_i8_moe(cx_ctx* ctx, const cx_i8_layer* w, const void* x, int in_dtype, in
     }
     {
         Span sp(ctx, "gate_up", s);
-        CX_HIP(product(w->gate_up, w->gate_up_scale, 2 * w->inter, w->hidden, true, m + z.q, m + z.q_scale, n_tokens, a.order, m + z.h));
+        CX_HIP(product(w->gate_up, w->gate_up_scale, 2 * w->inter, w->hidden, true, m + z.q, m + z.q_scale, n_tokens, a.order, m + z.h, z.gate_up));
     }
     {
         Span sp(ctx, "quantize", s);
@@ -2057,7 +2099,7 @@ int cx_i8_moe(cx_ctx* ctx, const cx_i8_layer* w, const void* x, int in_dtype, in
     }
     {
         Span sp(ctx, "down", s);
-        CX_HIP(product(w->down, w->down_scale, w->hidden, w->inter, false, m + z.hq, m + z.h_scale, pairs, nullptr, m + z.ys));
+        CX_HIP(product(w->down, w->down_scale, w->hidden, w->inter, false, m + z.hq, m + z.h_scale, pairs, nullptr, m + z.ys, z.down));
     }
     Span sp(ctx, "combine", s);
     CX_HIP(launch_combine_rows(c, s));

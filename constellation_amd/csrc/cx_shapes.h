@@ -412,6 +412,9 @@ inline int64_t mm_items(int64_t n_rows, int n_mats, bool stack, int item_rows) {
     return (n_rows < n_mats ? n_rows : n_mats) + n_rows / item_rows + 1;
 }
 
+// Rows that go through LDS are whole pieces of 16 bytes; others are copied to rows of this many elements first.
+constexpr int mm_pitch(int cols, int el) { return (cols + 16 / el - 1) / (16 / el) * (16 / el); }
+
 // How a product (or the gradient at x) is cut.
 struct MmForm {
     int kind;       // 0: few rows, weights without LDS; 1: tiles of 128 in m; 2: of 256
@@ -430,14 +433,14 @@ inline MmForm mm_few_form(int item_rows, int64_t busy, int rows, int steps) {
 }
 
 // out: the output's width, in which tiles of 128 or 256 lie (of a gated product the weights' rows); depth: bytes of the
-// contraction; wide: whole pieces of 16 bytes; few: the kernel of few rows is there.
-inline MmForm mm_form(int64_t n_rows, int n_mats, bool stack, int64_t out, int64_t depth, bool wide, bool few) {
+// contraction; few: the kernel of few rows is there.
+inline MmForm mm_form(int64_t n_rows, int n_mats, bool stack, int64_t out, int64_t depth, bool few) {
     const int64_t busy = std::max<int64_t>(1, std::min<int64_t>(n_rows, n_mats)), avg = (n_rows + busy - 1) / busy;
     const int64_t steps = (depth + 127) / 128;
     if (few && avg <= 16) return mm_few_form(16, busy, (int)out, (int)steps);
     MmForm best{1, 128, 1, 1};
     double least = -1;
-    for (int kind = wide ? 2 : 1; kind >= 1; --kind) {
+    for (int kind = 2; kind >= 1; --kind) {
         const int unit = kind == 2 ? 64 : 32;
         for (int tn = 4; tn >= 1; --tn) {
             const int rows = unit * tn;

@@ -36,6 +36,12 @@ def _rows_2d(t: torch.Tensor) -> tuple[int, int]:
     return t.shape[0], t.shape[1]
 
 
+def _at16(t: torch.Tensor) -> torch.Tensor:
+    """t, or a copy of it, contiguous and from an address that 16 divides on."""
+    t = t.contiguous()
+    return t if t.data_ptr() % 16 == 0 else t.clone()
+
+
 def _places(place: torch.Tensor, n_tokens: int) -> int:
     if place.dtype != torch.int32 or place.dim() != 2 or place.shape[0] != n_tokens or not place.is_contiguous():
         raise ValueError(f"place must be contiguous int32 [{n_tokens}, top_k]")
@@ -354,8 +360,8 @@ class I8Layer(_OwnLayer):
         for t, of in ((gate_up_scale, gate_up), (down_scale, down)):
             if t.shape != of.shape[:2] or t.dtype != torch.float32:
                 raise ValueError(f"scales must be fp32 {list(of.shape[:2])}, one for each row")
-        if not all(t.is_contiguous() for t in (gate_up, gate_up_scale, down, down_scale)):
-            raise ValueError("weights and scales must be contiguous")
+        if not all(t.is_contiguous() for t in (gate_up, gate_up_scale, down, down_scale)) or (gate_up.data_ptr() | down.data_ptr()) % 16:
+            raise ValueError("weights and scales must be contiguous, weights from an address that 16 divides on")
         if down.shape[0] <= int(shared):
             raise ValueError("a layer needs a routed expert")
         self.ctx = ctx
@@ -650,12 +656,12 @@ class Context:
         if keep and not gated:
             raise ValueError("keep is of gated products")
         P = self._picked(order, T)
-        x = x.contiguous()
+        x, w = _at16(x), _at16(w)
         out_dtype = out_dtype or x.dtype
         dt = cx_dtype(x.dtype)
         y = torch.empty((P, N // 2 if gated else N), dtype=out_dtype, device=x.device)
         pre = torch.empty((P, N), dtype=x.dtype, device=x.device) if keep else None
-        size = lib().cx_matmul_scratch(dt, E, N, K, int(gated), P, int(offsets is not None))
+        size = lib().cx_matmul_scratch(dt, T, E, N, K, P, int(offsets is not None))
         scratch = torch.empty(size, dtype=torch.uint8, device=x.device) if size else None
         check(lib().cx_matmul(self.handle, x.data_ptr(), T, w.data_ptr(), dt, E, N, K, int(gated), _ptr(order), top_k,
                               _ptr(offsets), P, y.data_ptr(), cx_dtype(out_dtype), _ptr(pre), _ptr(scratch), size,
@@ -681,12 +687,13 @@ class Context:
         dw_dtype = dw_dtype or x.dtype
         if dw_dtype not in (x.dtype, torch.float32):
             raise TypeError("dw must be of x's type or float32")
-        dy, x = dy.contiguous(), x.contiguous()
+        dy, x, w = _at16(dy), _at16(x), _at16(w)
         pre = None if pre is None else pre.contiguous()
         dx = torch.empty_like(x) if want_dx else None
         dw = torch.empty_like(w, dtype=dw_dtype) if want_dw else None
         dt, dwt = cx_dtype(x.dtype), cx_dtype(dw_dtype) if want_dw else 0
-        size = lib().cx_matmul_grad_scratch(dt, E, N, K, int(pre is not None), P, int(offsets is not None), int(want_dx), dwt)
+        size = lib().cx_matmul_grad_scratch(dt, E, N, K, int(pre is not None), P, int(offsets is not None), int(want_dx),
+                                             int(want_dw))
         scratch = torch.empty(size, dtype=torch.uint8, device=x.device) if size else None
         check(lib().cx_matmul_grad(self.handle, dy.data_ptr(), x.data_ptr(), w.data_ptr(), dt, _ptr(pre), E, N, K,
                                    _ptr(offsets), P, _ptr(dx), _ptr(dw), dwt, _ptr(scratch), size, self.stream()))
@@ -720,9 +727,9 @@ class Context:
         if w_scale.shape != w.shape[:-1] or w_scale.dtype != torch.float32 or not w_scale.is_contiguous():
             raise ValueError(f"w_scale must be contiguous fp32 {list(w.shape[:-1])}")
         P = self._picked(order, T)
-        x, x_scale = x.contiguous(), x_scale.contiguous()
+        x, w, x_scale = _at16(x), _at16(w), x_scale.contiguous()
         y = torch.empty((P, N // 2 if gated else N), dtype=out_dtype, device=x.device)
-        size = lib().cx_i8_matmul_scratch(E, N, K, int(gated), P, int(offsets is not None))
+        size = lib().cx_i8_matmul_scratch(T, E, N, K, P, int(offsets is not None))
         scratch = torch.empty(size, dtype=torch.uint8, device=x.device) if size else None
         check(lib().cx_i8_matmul(self.handle, x.data_ptr(), x_scale.data_ptr(), T, w.data_ptr(), w_scale.data_ptr(), E, N, K,
                                  int(gated), _ptr(order), top_k, _ptr(offsets), P, y.data_ptr(), cx_dtype(out_dtype),

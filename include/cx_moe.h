@@ -419,8 +419,9 @@ CX_API int cx_q4_moe(cx_ctx* ctx, const cx_q4_desc* gate_up, const cx_q4_desc* d
  * that decrease or leave the rows are cut and reported by cx_ctx_sync.  None of these
  * calls allocates, copies or waits, so all of them can be captured into a graph.  Sums are
  * in fp32 (exact 32-bit integers for 8-bit rows), in an order that depends on sizes alone, and rounded
- * once.  Buffers may start at any address of their type's alignment; rows and addresses of whole
- * 16-byte pieces take the fast loads.  n_mats is at most 1024, rows and cols 2^22 (8-bit:
+ * once.  x, weights and dy start on 16 bytes, other buffers at any address of their type's
+ * alignment; rows that are no whole 16-byte pieces are copied to such rows in the scratch, but for
+ * few rows of x.  n_mats is at most 1024, rows and cols 2^22 (8-bit:
  * cols 131071), n_rows 2^30, and a matrix has fewer than 2^32 bytes. */
 
 /* y = x W^T.  gated: rows is even and the halves are a gate and an up matrix G, U:
@@ -431,7 +432,7 @@ CX_API int cx_q4_moe(cx_ctx* ctx, const cx_q4_desc* gate_up, const cx_q4_desc* d
  * has fewer than 2^32 bytes then); a row whose entry is negative or past n_x reads as zeros.
  * scratch: cx_matmul_scratch bytes of device memory, 16-byte aligned, of the caller's (NULL where
  * that is 0), in use until the call's work is done. */
-CX_API size_t cx_matmul_scratch(int dtype, int n_mats, int rows, int cols, int gated, int n_rows, int with_offsets);
+CX_API size_t cx_matmul_scratch(int dtype, int n_x, int n_mats, int rows, int cols, int n_rows, int with_offsets);
 CX_API int cx_matmul(cx_ctx* ctx, const void* x, int n_x, const void* w, int dtype, int n_mats, int rows, int cols,
               int gated, const int32_t* order, int top_k, const int32_t* offsets, int n_rows, void* y, int y_dtype,
               void* pre, void* scratch, size_t scratch_bytes, void* stream);
@@ -445,7 +446,7 @@ CX_API int cx_matmul(cx_ctx* ctx, const void* x, int n_x, const void* w, int dty
  * Every row of x takes part once: rows come as they lie, without an order.
  * scratch: cx_matmul_grad_scratch bytes, as above. */
 CX_API size_t cx_matmul_grad_scratch(int dtype, int n_mats, int rows, int cols, int gated, int n_rows, int with_offsets,
-              int with_dx, int dw_dtype);
+              int with_dx, int with_dw);
 CX_API int cx_matmul_grad(cx_ctx* ctx, const void* dy, const void* x, const void* w, int dtype, const void* pre,
               int n_mats, int rows, int cols, const int32_t* offsets, int n_rows, void* dx, void* dw, int dw_dtype,
               void* scratch, size_t scratch_bytes, void* stream);
@@ -459,7 +460,7 @@ CX_API int cx_quantize_i8(cx_ctx* ctx, const void* x, int x_dtype, int n_rows, i
 
 /* y[p, n] = x_scale[row(p)] * w_scale[n] * sum over k of x[row(p), k] * w[n, k], gated as above; all
  * else as cx_matmul.  x: [n_x, cols], w: [n_mats, rows, cols], w_scale: [n_mats, rows]. */
-CX_API size_t cx_i8_matmul_scratch(int n_mats, int rows, int cols, int gated, int n_rows, int with_offsets);
+CX_API size_t cx_i8_matmul_scratch(int n_x, int n_mats, int rows, int cols, int n_rows, int with_offsets);
 CX_API int cx_i8_matmul(cx_ctx* ctx, const int8_t* x, const float* x_scale, int n_x, const int8_t* w, const float* w_scale,
               int n_mats, int rows, int cols, int gated, const int32_t* order, int top_k, const int32_t* offsets,
               int n_rows, void* y, int y_dtype, void* scratch, size_t scratch_bytes, void* stream);

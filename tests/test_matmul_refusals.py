@@ -66,6 +66,8 @@ def test_forward(at, call):
     refused(call(at, y_dtype=E4M3), "y must be")
     refused(call(at, y=None), "NULL buffer")
     refused(call(at, w=None), "NULL buffer")
+    refused(call(at, x=at + 2), "start on 16 bytes")
+    refused(call(at, w=at + 2), "start on 16 bytes")
     refused(call(at, order=at, n_x=1 << 30, cols=512), "2^32 bytes in all")
     assert call(at, n_rows=0, n_x=0, x=None, y=None, w=None) == CX_OK
 
@@ -81,17 +83,20 @@ def test_of_one_kind(at):
     refused(grad(at, dx=None, dw=None), "nothing to compute")
     refused(grad(at, dy=None), "NULL buffer")
     refused(grad(at, pre=at, rows=63), "even number")
+    refused(grad(at, dy=at + 8), "start on 16 bytes")
     refused(grad(at, pre=at, size=16), "scratch must be")
     assert grad(at, n_rows=0, dw=None, dx=None, x=None, dy=None) == CX_OK
 
 
 def test_scratch(at):
     """What the size call asks for is asked of the caller, whole and aligned."""
-    need = lib().cx_matmul_scratch(BF16, 1, 4096, 7168, 0, 256, 0)
+    need = lib().cx_matmul_scratch(BF16, 256, 1, 4096, 7168, 256, 0)
     assert need > 0
     for bad in (dict(scratch=None), dict(size=need - 1), dict(scratch=at + 8)):
         refused(matmul(at, rows=4096, cols=7168, n_rows=256, n_x=256, **{**dict(size=need), **bad}), f"scratch must be {need} bytes")
-    assert lib().cx_matmul_scratch(BF16, 0, 1, 1, 0, 1, 0) == 0 and lib().cx_matmul_scratch(BF16, 1, 1, 1, 0, 0, 0) == 0
+    assert lib().cx_matmul_scratch(BF16, 1, 0, 1, 1, 1, 0) == 0 and lib().cx_matmul_scratch(BF16, 1, 1, 1, 1, 0, 0) == 0
+    # rows of x and of the weights that are no whole pieces of 16 bytes: copies of both
+    assert lib().cx_matmul_scratch(BF16, 4000, 1, 100, 9, 4000, 0) >= (4000 + 100) * 16 * 2
 
 
 def test_quantize_refuses(at):

@@ -20,8 +20,8 @@ using namespace cx;
 extern "C" {
 int share(int n, int rows, int tile) { return mm_share(n, rows, tile); }
 int64_t items(int64_t rows, int mats, int stack, int item) { return mm_items(rows, mats, stack, item); }
-int64_t form(int64_t rows, int mats, int stack, int64_t out, int64_t depth, int wide, int few) {
-    const MmForm f = mm_form(rows, mats, stack, out, depth, wide, few);
+int64_t form(int64_t rows, int mats, int stack, int64_t out, int64_t depth, int few) {
+    const MmForm f = mm_form(rows, mats, stack, out, depth, few);
     return ((int64_t)f.kind << 48) | ((int64_t)f.item_rows << 32) | ((int64_t)f.splits << 16) | f.tiles;
 }
 int grid_ok(int64_t rows, int mats, int n, int k) { return mm_grid_ok(rows, mats, n, k); }
@@ -38,13 +38,13 @@ def rules(tmp_path_factory):
     L = C.CDLL(str(d / "rules.so"))
     L.items.restype = L.form.restype = C.c_int64
     L.items.argtypes = [C.c_int64, C.c_int, C.c_int, C.c_int]
-    L.form.argtypes = [C.c_int64, C.c_int, C.c_int, C.c_int64, C.c_int64, C.c_int, C.c_int]
+    L.form.argtypes = [C.c_int64, C.c_int, C.c_int, C.c_int64, C.c_int64, C.c_int]
     L.grid_ok.argtypes = [C.c_int64, C.c_int, C.c_int, C.c_int]
     return L
 
 
-def form(rules, P, E, out, depth, wide, few):
-    v = rules.form(P, max(1, E), int(E > 0), out, depth, int(wide), int(few))
+def form(rules, P, E, out, depth, few):
+    v = rules.form(P, max(1, E), int(E > 0), out, depth, int(few))
     return v >> 48, v >> 32 & 0xFFFF, v >> 16 & 0xFFFF, v & 0xFFFF
 
 
@@ -75,16 +75,15 @@ def test_forms_are_what_the_kernels_take(rules):
         for E in (0, 1, 8, 64, 1024):
             for out in (1, 30, 256, 4096, 20000):
                 for depth in (2, 100, 4096, 14336):
-                    for wide in (False, True):
-                        for few in (False, True):
-                            kind, rows, splits, tiles = form(rules, P, E, out, depth, wide, few)
-                            assert kind in ((0, 1, 2) if wide else (0, 1)) and (few or kind > 0)
-                            if kind == 0:
-                                assert rows == 16 and tiles in (1, 2) and splits in (1, 2, 4, 8)
-                            else:
-                                unit = 64 if kind == 2 else 32
-                                assert rows % unit == 0 and 1 <= rows // unit <= 4 and 1 <= splits <= 16
-                            assert rules.grid_ok(P, max(1, E), out, max(1, depth // 2)) or P * out > 1 << 30 or P >= 1 << 20 or E == 1024
+                    for few in (False, True):
+                        kind, rows, splits, tiles = form(rules, P, E, out, depth, few)
+                        assert kind in (0, 1, 2) and (few or kind > 0)
+                        if kind == 0:
+                            assert rows == 16 and tiles in (1, 2) and splits in (1, 2, 4, 8)
+                        else:
+                            unit = 64 if kind == 2 else 32
+                            assert rows % unit == 0 and 1 <= rows // unit <= 4 and 1 <= splits <= 16
+                        assert rules.grid_ok(P, max(1, E), out, max(1, depth // 2)) or P * out > 1 << 30 or P >= 1 << 20 or E == 1024
 
 
 def test_tests_reach_every_kernel(rules):
@@ -94,19 +93,18 @@ def test_tests_reach_every_kernel(rules):
     for sizes in (ONE, STACK, FORWARD):
         for s in sizes:
             P, E, N, K = s if len(s) == 4 else (s[0], 0, s[1], s[2])
-            kind, rows, splits, _ = form(rules, P, E, N, K * 2, K % 8 == 0, True)
+            kind, rows, splits, _ = form(rules, P, E, N, K * 2, True)
             seen.add((kind, splits > 1))
     assert {(0, False), (0, True), (1, False), (1, True), (2, False), (2, True)} <= seen, seen
     seen = set()
     for P, E, N, K in [*GRADS, *LARGE_GRADS]:
-        kind, rows, splits, _ = form(rules, P, E, K, N * 2, N % 8 == 0 and K % 8 == 0, False)
+        kind, rows, splits, _ = form(rules, P, E, K, N * 2, False)
         seen.add((kind, splits > 1))
     assert {(1, False), (1, True), (2, False)} <= seen, seen
     # the gradient at the weights: tiles of 128 and 256, and short steps, by cx_mm_grad.hip's rule
     seen = set()
     for P, E, N, K in [*GRADS, *LARGE_GRADS]:
-        if N % 8 == 0 and K % 8 == 0:
-            mats = max(1, E)
-            many = mats * -(-K // 256) * -(-N // 256) >= 256
-            seen.add("small" if not many else "short" if P < mats * 1024 else "long")
+        mats = max(1, E)
+        many = mats * -(-K // 256) * -(-N // 256) >= 256
+        seen.add("small" if not many else "short" if P < mats * 1024 else "long")
     assert seen == {"small", "short", "long"}
