@@ -71,8 +71,7 @@ __device__ __forceinline__ int wave_scan_add(int v, int lane) {
     return v;
 }
 
-// Run idx of up to item_rows rows, of whole tiles of TILE (uniform in a wave; each wave finds it by itself).
-template <int TILE>
+// Run idx of up to item_rows rows, of whole tiles of 16 (uniform in a wave; each wave finds it by itself).
 __device__ __forceinline__ MmItem mm_item(const int32_t* offsets, int n_mats, int n_rows, int item_rows, int idx) {
     if (offsets == nullptr) {
         const int begin = idx * item_rows;
@@ -89,7 +88,7 @@ __device__ __forceinline__ MmItem mm_item(const int32_t* offsets, int n_mats, in
         if (past != 0) {
             const int l = __builtin_ctzll(past);
             const int r = __shfl(rows, l), m = __shfl(n, l), first = __shfl(end, l) - m, i = idx - first;
-            const int share = mm_share(m, r, TILE);  // equal runs
+            const int share = mm_share(m, r);  // equal runs
             return MmItem{e0 + l, __builtin_amdgcn_readfirstlane(__shfl(begin, l) + i * share), __builtin_amdgcn_readfirstlane(min(share, r - i * share))};
         }
         held = __shfl(top, 63);
@@ -624,7 +623,7 @@ __device__ __forceinline__ bool mm_work(const MmLaunch& L, int tile_cols, int wi
     const MmTile tile = mm_tile(blockIdx.x, L.m_tiles * L.splits, L.by_item);
     if (L.offsets != nullptr && blockIdx.x == 0 && wave_id() == 0) mm_check(L.offsets, L.n_mats, L.n_rows, L.err_flag);
     if (tile.m >= L.m_tiles * L.splits) return false;
-    w->it = mm_item<16>(L.offsets, L.n_mats, L.n_rows, L.item_rows, tile.item);
+    w->it = mm_item(L.offsets, L.n_mats, L.n_rows, L.item_rows, tile.item);
     w->ks = tile.m / L.m_tiles;
     w->m0 = (tile.m - w->ks * L.m_tiles) * tile_cols;
     if (w->it.rows <= 0) return false;

@@ -35,16 +35,16 @@ __device__ __forceinline__ u32x4 mm_piece(const char* q, int have) {
 // A workgroup's 8 waves are `splits` ranges of the columns times 8 / splits groups of RW tiles of 16 weight
 // rows (gated: 8 gate rows and the same 8 up rows, so that both factors of an output meet in two lanes of
 // a wave); the ranges' sums are added in order.  A wave has U steps of 128 bytes of its rows in flight ahead of the
-// U that it multiplies, of weights and of up to 16 NB rows of x, which come from L2.
-template <class T, int NB, int RW, bool GATED, bool VEC>
+// U that it multiplies, of weights and of up to 16 rows of x, which come from L2.
+template <class T, int RW, bool GATED, bool VEC>
 __global__ __launch_bounds__(64 * kMmFewWaves, 2) void k_mm_few(MmLaunch L, int splits, int row_blocks) {
     typedef typename T::Acc Acc;
-    constexpr int EL = T::kEl, kStep = 128 / EL, U = !VEC ? 1 : NB == 1 && RW == 1 ? 4 : NB * RW <= 4 ? 2 : 1;
-    __shared__ __attribute__((aligned(16))) uint32_t red[kMmFewWaves][RW][NB][256];
+    constexpr int EL = T::kEl, kStep = 128 / EL, U = !VEC ? 1 : RW == 1 ? 4 : 2;
+    __shared__ __attribute__((aligned(16))) uint32_t red[kMmFewWaves][RW][256];
     const int idx = blockIdx.x / row_blocks, block = blockIdx.x - idx * row_blocks;
     const int wave = wave_id(), lane = threadIdx.x & 63, t = lane & 15, q = lane >> 4;
     if (L.offsets != nullptr && blockIdx.x == 0 && wave == kMmFewWaves - 1) mm_check(L.offsets, L.n_mats, L.n_rows, L.err_flag);
-    const MmItem it = mm_item<16>(L.offsets, L.n_mats, L.n_rows, 16 * NB, idx);
+    const MmItem it = mm_item(L.offsets, L.n_mats, L.n_rows, 16, idx);
     if (it.rows <= 0) return;
     const int groups = kMmFewWaves / splits, rg = wave / splits, ks = wave - rg * splits;
     constexpr int kCols = GATED ? 8 : 16;  // outputs of a tile
@@ -64,17 +64,16 @@ __global__ __launch_bounds__(64 * kMmFewWaves, 2) void k_mm_few(MmLaunch L, int 
         return pair < 0 || xr >= L.n_x ? -1 : xr;
     };
     const size_t pitch = (size_t)L.cols * EL;
-    const char *wp[RW], *xp[NB];
+    const char *wp[RW];
 #pragma unroll
     for (int m = 0; m < RW; ++m) {
         const int r = (tile0 + m) * kCols + t % kCols, n = min(r, width - 1) + (GATED && t >= 8 ? width : 0);  // rows past the matrix: its last one again
         wp[m] = static_cast<const char*>(L.w) + ((size_t)it.mat * L.rows + n) * pitch + q * 16;
     }
-#pragma unroll
-    for (int b = 0; b < NB; ++b) xp[b] = static_cast<const char*>(L.x) + (size_t)max(source(16 * b + t), 0) * pitch + q * 16;
+    const char* xp = static_cast<const char*>(L.x) + (size_t)max(source(t), 0) * pitch + q * 16;
     const int steps = (L.cols + kStep - 1) / kStep, per = (steps + splits - 1) / splits, k0 = ks * per, k1 = tile0 >= tiles ? 0 : min(steps, k0 + per);
-    u32x4 a[2][U][RW][2], x[2][U][NB][2];
-    Acc acc[RW][NB] = {};
+    u32x4 a[2][U][RW][2], x[2][U][2];
+    Acc acc[RW] = {};
     auto fetch = [&](int k, auto to) {  // past the range: its last step again, not multiplied
 #pragma unroll
         for (int u = 0; u < U; ++u) {
@@ -85,9 +84,7 @@ __global__ __launch_bounds__(64 * kMmFewWaves, 2) void k_mm_few(MmLaunch L, int 
                 const size_t at = (size_t)kk * 128 + j * 64;
 #pragma unroll
                 for (int m = 0; m < RW; ++m) a[to][u][m][j] = mm_piece<EL, VEC>(wp[m] + at, have);
-#pragma unroll
-                for (int b = 0; b < NB; ++b)
-                    if (b == 0 || 16 * b < it.rows) x[to][u][b][j] = mm_piece<EL, VEC>(xp[b] + at, have);
+                x[to][u][j] = mm_piece<EL, VEC>(xp + at, have);
             }
         }
     };
@@ -98,11 +95,7 @@ __global__ __launch_bounds__(64 * kMmFewWaves, 2) void k_mm_few(MmLaunch L, int 
 #pragma unroll
             for (int j = 0; j < 2; ++j)
 #pragma unroll
-                for (int b = 0; b < NB; ++b) {
-                    if (b > 0 && 16 * b >= it.rows) break;
-#pragma unroll
-                    for (int m = 0; m < RW; ++m) acc[m][b] = T::mma(a[from][u][m][j], x[from][u][b][j], acc[m][b]);
-                }
+                for (int m = 0; m < RW; ++m) acc[m] = T::mma(a[from][u][m][j], x[from][u][j], acc[m]);
         }
     };
     constexpr std::integral_constant<int, 0> even{};
@@ -116,9 +109,7 @@ __global__ __launch_bounds__(64 * kMmFewWaves, 2) void k_mm_few(MmLaunch L, int 
         multiply(k + U, odd);
     }
 #pragma unroll
-    for (int m = 0; m < RW; ++m)
-#pragma unroll
-        for (int b = 0; b < NB; ++b) *reinterpret_cast<u32x4*>(&red[wave][m][b][t * 16 + q * 4]) = __builtin_bit_cast(u32x4, acc[m][b]);
+    for (int m = 0; m < RW; ++m) *reinterpret_cast<u32x4*>(&red[wave][m][t * 16 + q * 4]) = __builtin_bit_cast(u32x4, acc[m]);
     __syncthreads();
     // outputs: 16 lanes have a tile's 16 sums of one row of x
     auto put = [](void* y, int type, int64_t at, float f) {
@@ -127,19 +118,19 @@ __global__ __launch_bounds__(64 * kMmFewWaves, 2) void k_mm_few(MmLaunch L, int 
         else
             static_cast<uint16_t*>(y)[at] = (uint16_t)cast_out(f, type);
     };
-    for (int i = threadIdx.x; i < groups * RW * NB * 256; i += 64 * kMmFewWaves) {
+    for (int i = threadIdx.x; i < groups * RW * 256; i += 64 * kMmFewWaves) {
         // neighbours: the sums of a tile, the tiles of the group, the rows of x
-        const int r = i & 15, m = i / 16 % RW, g = i / (16 * RW) % groups, row = i / (16 * RW * groups), b = row >> 4;
+        const int r = i & 15, m = i / 16 % RW, g = i / (16 * RW) % groups, row = i / (16 * RW * groups);
         if (row >= it.rows) break;
         const int xr = source(row), c = ((block * groups + g) * RW + m) * kCols + r % kCols, n = min(c, width - 1) + (GATED && r >= 8 ? width : 0);
         float v;
         if constexpr (EL == 1) {
             int s = 0;
-            for (int k = 0; k < splits; ++k) s += (int)red[g * splits + k][m][b][(row & 15) * 16 + r];
+            for (int k = 0; k < splits; ++k) s += (int)red[g * splits + k][m][row * 16 + r];
             v = (float)s * (xr < 0 ? 0.0f : L.x_scale[xr]) * L.w_scale[(size_t)it.mat * L.rows + n];
         } else {
             v = 0.0f;
-            for (int k = 0; k < splits; ++k) v += __uint_as_float(red[g * splits + k][m][b][(row & 15) * 16 + r]);
+            for (int k = 0; k < splits; ++k) v += __uint_as_float(red[g * splits + k][m][row * 16 + r]);
         }
         if (xr < 0) v = 0.0f;
         const int64_t p = it.begin + row;
@@ -153,21 +144,19 @@ __global__ __launch_bounds__(64 * kMmFewWaves, 2) void k_mm_few(MmLaunch L, int 
     }
 }
 
-template <class T, int NB, int RW, bool GATED>
-hipError_t mm_few_run(MmLaunch& L, int splits, bool vec, hipStream_t s) {
-    const int kCols = GATED ? 8 : 16, width = GATED ? L.rows / 2 : L.rows, per = kMmFewWaves / splits * RW;
+template <class T, int RW, bool GATED>
+hipError_t mm_few_run(MmLaunch& L, bool vec, hipStream_t s) {
+    const int kCols = GATED ? 8 : 16, width = GATED ? L.rows / 2 : L.rows, splits = L.form.splits, per = kMmFewWaves / splits * RW;
     const int blocks = ((width + kCols - 1) / kCols + per - 1) / per;
-    const int64_t items = mm_items(L.n_rows, L.n_mats, L.offsets != nullptr, 16 * NB);
-    cx_launch(vec ? k_mm_few<T, NB, RW, GATED, true> : k_mm_few<T, NB, RW, GATED, false>, dim3((unsigned)(items * blocks)), dim3(64 * kMmFewWaves), 0, s, L,
+    const int64_t items = mm_items(L.n_rows, L.n_mats, L.offsets != nullptr, 16);
+    cx_launch(vec ? k_mm_few<T, RW, GATED, true> : k_mm_few<T, RW, GATED, false>, dim3((unsigned)(items * blocks)), dim3(64 * kMmFewWaves), 0, s, L,
               splits, blocks);
     return hipGetLastError();
 }
 
 template <class T, bool GATED>
 hipError_t mm_few(MmLaunch& L, bool vec, hipStream_t s) {
-    const MmForm f = L.form;
-    if (f.item_rows == 16) return f.tiles == 1 ? mm_few_run<T, 1, 1, GATED>(L, f.splits, vec, s) : mm_few_run<T, 1, 2, GATED>(L, f.splits, vec, s);
-    return mm_few_run<T, 2, 2, GATED>(L, f.splits, vec, s);
+    return L.form.tiles == 1 ? mm_few_run<T, 1, GATED>(L, vec, s) : mm_few_run<T, 2, GATED>(L, vec, s);
 }
 
 }  // namespace cx

@@ -404,8 +404,8 @@ inline int64_t q4_most_items(int64_t n_rows, int n_mats, int dec_rows) {
 constexpr int kMmMaxSide = 1 << 22;  // 256 rows of it lie within 32 bits
 constexpr int kI8MaxCols = 131071;  // 2^14 times that is less than 2^31: sums in 32 bits are exact
 // Rows of each of the n items that `rows` rows are cut to (the last has what is left): equal ones of whole
-// tiles of 16 or 32 rows.  n is the least number of items of whole tiles that holds them, so that no item is empty and none is too long.
-constexpr int mm_share(int n, int rows, int tile) { return n <= 1 ? rows : (rows + tile * n - 1) / (tile * n) * tile; }
+// tiles of 16 rows.  n is the least number of items of whole tiles that holds them, so that no item is empty and none is too long.
+constexpr int mm_share(int n, int rows) { return n <= 1 ? rows : (rows + 16 * n - 1) / (16 * n) * 16; }
 // Items of up to item_rows rows, those of rows behind the last matrix's included, at most.
 inline int64_t mm_items(int64_t n_rows, int n_mats, bool stack, int item_rows) {
     if (!stack) return (n_rows + item_rows - 1) / item_rows;
@@ -424,10 +424,10 @@ struct MmForm {
 };
 constexpr int kMmFewWaves = 8;
 
-inline MmForm mm_few_form(int item_rows, int64_t busy, int rows, int steps) {
-    MmForm f{0, item_rows, 1, 1};
+inline MmForm mm_few_form(int64_t busy, int rows, int steps) {
+    MmForm f{0, 16, 1, 1};
     const int64_t tiles = (rows + 15) / 16;
-    f.tiles = item_rows > 16 || tiles * busy > 1024 ? 2 : 1;
+    f.tiles = tiles * busy > 1024 ? 2 : 1;
     while (f.splits < kMmFewWaves && tiles / f.tiles * busy * f.splits * 2 <= 4096 && steps / f.splits >= 4) f.splits *= 2;
     return f;
 }
@@ -437,7 +437,7 @@ inline MmForm mm_few_form(int item_rows, int64_t busy, int rows, int steps) {
 inline MmForm mm_form(int64_t n_rows, int n_mats, bool stack, int64_t out, int64_t depth, bool few) {
     const int64_t busy = std::max<int64_t>(1, std::min<int64_t>(n_rows, n_mats)), avg = (n_rows + busy - 1) / busy;
     const int64_t steps = (depth + 127) / 128;
-    if (few && avg <= 16) return mm_few_form(16, busy, (int)out, (int)steps);
+    if (few && avg <= 16) return mm_few_form(busy, (int)out, (int)steps);
     MmForm best{1, 128, 1, 1};
     double least = -1;
     for (int kind = 2; kind >= 1; --kind) {

@@ -18,7 +18,7 @@ SOURCE = r"""
 #include "cx_shapes.h"
 using namespace cx;
 extern "C" {
-int share(int n, int rows, int tile) { return mm_share(n, rows, tile); }
+int share(int n, int rows) { return mm_share(n, rows); }
 int64_t items(int64_t rows, int mats, int stack, int item) { return mm_items(rows, mats, stack, item); }
 int64_t form(int64_t rows, int mats, int stack, int64_t out, int64_t depth, int few) {
     const MmForm f = mm_form(rows, mats, stack, out, depth, few);
@@ -52,7 +52,7 @@ def form(rules, P, E, out, depth, few):
 def test_items_cover_the_rows_once(rules, cap):
     for rows in list(range(1, 12 * cap, 1 if cap < 64 else 5)) + [97 * cap - 1, 97 * cap, 97 * cap + 1, 1 << 20]:
         n = -(-rows // cap)
-        share = rules.share(n, rows, 16)
+        share = rules.share(n, rows)
         assert 1 <= share <= cap and 0 < rows - (n - 1) * share <= share, (rows, n, share)
 
 
