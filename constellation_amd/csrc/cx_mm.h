@@ -124,6 +124,11 @@ struct MmShape {
 
 static __device__ __attribute__((aligned(16))) const uint32_t mm_zeros[4] = {};
 
+// 16 bytes at any alignment.
+struct __attribute__((packed)) MmPacked {
+    u32x4 v;
+};
+
 // A pointer that is the same in all lanes, in scalar registers.
 __device__ __forceinline__ const char* mm_uniform(const void* p) {
     const uint64_t v = (uint64_t)p;
@@ -538,33 +543,34 @@ template <int W, bool WIDE, class F>
 __device__ __forceinline__ void mm_put_rows(const float* turn, void* out, bool bf, bool vec, int m0, int width, F row) {
     constexpr int kChunks = W * 4, kPer = WIDE ? 4 : 8, kLanes = W * 16 / kPer;  // columns of a lane's store, lanes of a row
     const int l = threadIdx.x & 63;
-    if (!vec) {  // a column a lane, so that a store's lanes are neighbours
-#pragma unroll 4
-        for (int i = 0; i < W * 4; ++i) {
-            const int r = (i * 64 + l) / (W * 16), c = (i * 64 + l) % (W * 16);
-            const int64_t at = row(r);
-            if (at < 0 || c >= width - m0) continue;
-            const float f = turn[r * W * 16 + ((c / 4) ^ (r & (kChunks - 1))) * 4 + c % 4];
-            if constexpr (WIDE)
-                static_cast<float*>(out)[at + m0 + c] = f;
-            else
-                static_cast<uint16_t*>(out)[at + m0 + c] = (uint16_t)mm_round2(f, 0.0f, bf);
-        }
-        return;
-    }
 #pragma unroll
     for (int i = 0; i < 16 * kLanes / 64; ++i) {
-        const int r = (i * 64 + l) / kLanes, c = (i * 64 + l) % kLanes * kPer;
+        const int r = (i * 64 + l) / kLanes, c = (i * 64 + l) % kLanes * kPer, left = width - m0 - c;
         const int64_t at = row(r);
-        if (at < 0 || c >= width - m0) continue;
+        if (at < 0 || left <= 0) continue;
         const float* src = turn + r * W * 16;
         const f32x4 a = *reinterpret_cast<const f32x4*>(src + ((c / 4) ^ (r & (kChunks - 1))) * 4);
+        u32x4 v;
         if constexpr (WIDE) {
-            *reinterpret_cast<f32x4*>(static_cast<float*>(out) + at + m0 + c) = a;
+            v = __builtin_bit_cast(u32x4, a);
         } else {
             const f32x4 b = *reinterpret_cast<const f32x4*>(src + ((c / 4 + 1) ^ (r & (kChunks - 1))) * 4);
-            *reinterpret_cast<u32x4*>(static_cast<uint16_t*>(out) + at + m0 + c) =
-                u32x4{mm_round2(a[0], a[1], bf), mm_round2(a[2], a[3], bf), mm_round2(b[0], b[1], bf), mm_round2(b[2], b[3], bf)};
+            v = u32x4{mm_round2(a[0], a[1], bf), mm_round2(a[2], a[3], bf), mm_round2(b[0], b[1], bf), mm_round2(b[2], b[3], bf)};
+        }
+        char* y = static_cast<char*>(out) + (at + m0 + c) * (WIDE ? 4 : 2);
+        if (vec) {
+            *reinterpret_cast<u32x4*>(y) = v;
+        } else if (left >= kPer) {
+            ((__attribute__((address_space(1))) MmPacked*)y)->v = v;
+        } else {
+#pragma unroll
+            for (int k = 0; k < kPer - 1; ++k) {
+                if (k >= left) continue;
+                if constexpr (WIDE)
+                    reinterpret_cast<uint32_t*>(y)[k] = v[k];
+                else
+                    reinterpret_cast<uint16_t*>(y)[k] = (uint16_t)(v[k / 2] >> (16 * (k & 1)));
+            }
         }
     }
 }

@@ -6,11 +6,6 @@
 
 namespace cx {
 
-// 16 bytes at any alignment.
-struct __attribute__((packed)) MmPacked {
-    u32x4 v;
-};
-
 // 16 bytes of a row, `have` elements of which exist.  VEC: all or none of them, at an address that 16 divides.
 template <int EL, bool VEC>
 __device__ __forceinline__ u32x4 mm_piece(const char* q, int have) {
