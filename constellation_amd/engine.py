@@ -645,7 +645,8 @@ class Context:
         rows offsets[e] .. offsets[e + 1] - 1; with `order`, row p is row order[p] // top_k of x
         (sort_tokens' offsets and order).  gated: the rows of a matrix are a gate and then an up matrix,
         and the result is silu(x G^T) * (x U^T) [P, N / 2]; with `keep` (result, pre), pre = [x G^T, x U^T]
-        in x's type, which matmul_grad asks for.  Its gradient: matmul_grad, by the caller's autograd.Function
+        in x's type, which matmul_grad asks for.  Weights that start on no multiple of 16 bytes are copied at each
+        call.  Its gradient: matmul_grad, by the caller's autograd.Function
         (as gather_rows)."""
         self._here(x, w, offsets, order)
         _outside_autograd("matmul", "matmul_grad", x, w)

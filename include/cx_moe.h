@@ -417,7 +417,7 @@ CX_API int cx_q4_moe(cx_ctx* ctx, const cx_q4_desc* gate_up, const cx_q4_desc* d
  * offsets[e] .. offsets[e + 1] - 1 belong to matrix e (offsets NULL: one matrix, n_mats 1, for
  * all rows), rows behind the last matrix's are zeros in every output that has such rows, offsets
  * that decrease or leave the rows are cut and reported by cx_ctx_sync.  None of these
- * calls allocates, copies or waits, so all of them can be captured into a graph.  Sums are
+ * calls allocates, waits or reads device memory from the host, so all of them can be captured into a graph.  Sums are
  * in fp32 (exact 32-bit integers for 8-bit rows), in an order that depends on sizes alone, and rounded
  * once.  x, weights and dy start on 16 bytes, other buffers at any address of their type's
  * alignment; rows that are no whole 16-byte pieces are copied to such rows in the scratch, but for

@@ -71,7 +71,7 @@ def test_item_bound_holds_for_any_deal(rules, cap):
 
 
 def test_forms_are_what_the_kernels_take(rules):
-    for P in (1, 2, 15, 16, 17, 40, 64, 65, 100, 333, 1000, 4096, 20000, 1 << 20):
+    for P in (1, 2, 15, 16, 17, 40, 64, 65, 100, 333, 1000, 4096, 20000, 1 << 20, 1 << 24):
         for E in (0, 1, 8, 64, 1024):
             for out in (1, 30, 256, 4096, 20000):
                 for depth in (2, 100, 4096, 14336):
@@ -83,6 +83,7 @@ def test_forms_are_what_the_kernels_take(rules):
                         else:
                             unit = 64 if kind == 2 else 32
                             assert rows % unit == 0 and 1 <= rows // unit <= 4 and 1 <= splits <= 16
+                            assert splits == 1 or P * -(-out // 1024) < 1 << 24  # workgroups of the sums
                         assert rules.grid_ok(P, max(1, E), out, max(1, depth // 2)) or P * out > 1 << 30 or P >= 1 << 20 or E == 1024
 
 
