@@ -432,6 +432,13 @@ inline MmForm mm_few_form(int64_t busy, int rows, int steps) {
     return f;
 }
 
+// The cost of a form is estimated, in us: a step of a tile, tiles beside each other on a CU, rounds of workgroups, and the
+// partial sums' way through memory.  Rows by 4096 x 7168 gated, us: 40 rows with tiles of 128 59, in 4 ranges 25 (tiles of
+// 256: 88, 33); 256 rows 71, 32 (145, 52); 512 rows 71, 44 (142, 54); 1024 rows 72, 79 (141, 67); 2048 rows 110, 149
+// (141, 128); 4096 rows 209, 344 (172, 289).  32 matrices of 4096 x 7168, 16384 rows, at x: 1302 (964).
+// Few rows: up to 16 a matrix on average.  8 rows 17 (through LDS in 4 ranges 24), 16 rows 20 (24), 24 rows 32 (24).  The
+// host does not know how rows are dealt: where one matrix of many gets them all, its weights are read once for each 16.
+//
 // out: the output's width, in which tiles of 128 or 256 lie (of a gated product the weights' rows); depth: bytes of the
 // contraction; few: the kernel of few rows is there.
 inline MmForm mm_form(int64_t n_rows, int n_mats, bool stack, int64_t out, int64_t depth, bool few) {
