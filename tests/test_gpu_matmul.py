@@ -196,6 +196,12 @@ def test_quantize(gpu, T, K, dtype):
         assert torch.equal(q.cpu(), torch.round(x.float() / scale[:, None]).to(I8))
 
 
+@pytest.mark.parametrize("dtype", [BF, SF])
+@pytest.mark.parametrize("T,K", [(2050, 2048), (2049, 1001), (5, 512), (6, 513)])
+def test_quantize_many_rows(gpu, T, K, dtype):
+    test_quantize(gpu, T, K, dtype)
+
+
 def test_quantize_rows_that_are_not_finite(gpu):
     x = rand(1, 5, 200)
     x[1, 3], x[2, 199], x[3, 0] = float("nan"), float("inf"), -float("inf")
@@ -367,6 +373,41 @@ def test_offsets_out_of_order_are_cut_and_reported(gpu):
         gx, gw = gpu.matmul_grad(y, x.cuda(), w.cuda(), offsets=good)
         assert torch.equal(dx, gx) and torch.equal(dw, gw)
         gpu.sync()
+
+
+def test_offsets_of_odd_rows(gpu):
+    """Rows that are copied first: a first offset past the second gives matrix 0 the rows from 0 on; and a captured call, whose
+    matrices with rows are others at each replay."""
+    from constellation_amd._lib import CxError
+    E, N, K, P = 4, 41, 67, 100
+    x, w, dy = rand(1, P, K, dtype=BF).cuda(), rand(2, E, N, K, dtype=BF, std=0.1).cuda(), rand(3, P, N, dtype=BF).cuda()
+    off = torch.tensor([0, 5, 20, 30, 40], dtype=torch.int32, device="cuda")
+
+    def step():
+        return (gpu.matmul(x, w, offsets=off), *gpu.matmul_grad(dy, x, w, offsets=off))
+    want = step()
+    gpu.sync()
+    off[0] = 7
+    bad = step()
+    with pytest.raises(CxError, match="offset"):
+        gpu.sync()
+    assert all(torch.equal(a, b) for a, b in zip(bad, want))
+    off[0] = 0
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = step()
+    for cut in ([0, 0, 100, 100, 100], [0, 100, 100, 100, 100], [0, 25, 25, 25, 99], [0, 0, 0, 0, 0], [0, 5, 20, 30, 40]):
+        print(f"[mm] offsets {cut}", flush=True)
+        off.copy_(torch.tensor(cut, dtype=torch.int32))
+        want = step()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(held, want)), cut
+        y = torch.zeros(P, N, dtype=torch.float64)
+        for e in range(E):
+            y[cut[e]:cut[e + 1]] = x[cut[e]:cut[e + 1]].cpu().double() @ w[e].cpu().double().T
+        assert torch.allclose(want[0].cpu().double(), y, rtol=2.0 ** -8, atol=2.0 ** -12)
+    gpu.sync()
 
 
 def test_replays_and_streams(gpu):
