@@ -59,11 +59,11 @@ def _device(index: int) -> torch.device:
     return torch.device("cuda", index)
 
 
-def _outside_autograd(name: str, gradient: str, *tensors: Optional[torch.Tensor]) -> None:
-    """A result without a graph must not pass for one with it."""
+def _outside_autograd(name: str, gradient: Optional[str], *tensors: Optional[torch.Tensor]) -> None:
+    """A result without a graph must not pass for one with it.  gradient: the call that a backward makes, if there is one."""
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
-        raise ValueError(f"{name} records no graph: call it under torch.no_grad() or in an autograd.Function "
-                         f"whose backward is {gradient}")
+        raise ValueError(f"{name} records no graph: call it under torch.no_grad()" +
+                         (f" or in an autograd.Function whose backward is {gradient}" if gradient else ""))
 
 
 def _stream(device: int) -> int:
@@ -375,8 +375,8 @@ class I8Layer(_OwnLayer):
 
     @classmethod
     def quantize(cls, ctx: "Context", gate_up: torch.Tensor, down: torch.Tensor, **kw) -> "I8Layer":
-        """From 16- or 32-bit weights, as a program trains them (matmul)."""
-        return cls(ctx, *ctx.quantize_i8(gate_up), *ctx.quantize_i8(down), **kw)
+        """From 16- or 32-bit weights, as a program trains them (matmul), as they are at the moment."""
+        return cls(ctx, *ctx.quantize_i8(gate_up.detach()), *ctx.quantize_i8(down.detach()), **kw)
 
 
 class Context:
@@ -702,8 +702,10 @@ class Context:
 
     def quantize_i8(self, x: torch.Tensor):
         """(q int8, scale fp32 of x's leading shape): rows (the last dimension) of x in 8-bit integers times
-        a scale each.  A weight matrix's channels are its rows."""
+        a scale each.  A weight matrix's channels are its rows.  It has no gradient: an x that requires grad is refused
+        where a graph is recorded."""
         self._here(x)
+        _outside_autograd("quantize_i8", None, x)
         if x.dim() < 1:
             raise ValueError("expected rows")
         x = x.contiguous()
@@ -717,8 +719,10 @@ class Context:
                   gated: bool = False, offsets: Optional[torch.Tensor] = None, order: Optional[torch.Tensor] = None,
                   top_k: int = 1, out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
         """x W^T of 8-bit x [T, K] with a scale per row and 8-bit weights [N, K] or [E, N, K] with a scale per
-        channel ([N] or [E, N]), as quantize_i8 makes them, in out_dtype; all else as matmul."""
+        channel ([N] or [E, N]), as quantize_i8 makes them, in out_dtype; all else as matmul.  It has no gradient: scales
+        that require grad are refused where a graph is recorded."""
         self._here(x, x_scale, w, w_scale, offsets, order)
+        _outside_autograd("i8_matmul", None, x_scale, w_scale)
         T, K = _rows_2d(x)
         E, N = self._stack(w, K, offsets, gated)
         if x.dtype != torch.int8 or w.dtype != torch.int8:
