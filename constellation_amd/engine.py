@@ -673,8 +673,11 @@ class Context:
                     offsets: Optional[torch.Tensor] = None, want_dx: bool = True, want_dw: bool = True,
                     dw_dtype: Optional[torch.dtype] = None):
         """(dx, dw) of matmul(x, w) without an order: dx in x's type, dw of w's shape in dw_dtype (x's, or fp32),
-        None where it was not wanted.  pre: what a gated product kept; dy is the gradient at its result."""
+        None where it was not wanted.  pre: what a gated product kept; dy is the gradient at its result.  There is no
+        gradient of the gradients: tensors that require grad are refused where a graph is recorded (a backward under
+        once_differentiable is not)."""
         self._here(dy, x, w, pre, offsets)
+        _outside_autograd("matmul_grad", None, dy, x, w, pre)
         P, K = _rows_2d(x)
         E, N = self._stack(w, K, offsets, pre is not None)
         if x.dtype not in (torch.float16, torch.bfloat16) or any(t is not None and t.dtype != x.dtype for t in (dy, w, pre)):

@@ -54,3 +54,10 @@ def test_a_layer_takes_trained_weights(ctx):  # noqa: F811
     """Served weights are a program's parameters: the layer's codes are theirs at that moment, and no step of a graph."""
     with pytest.raises(Called, match="cx_quantize_i8"):
         I8Layer.quantize(ctx, z(E, 2 * N, K).requires_grad_(), z(E, K, N).requires_grad_())
+
+
+@pytest.mark.parametrize("which", ["dy", "x", "w", "pre"])
+def test_no_second_gradient_is_lost(ctx, which):  # noqa: F811
+    """In a backward that is itself recorded (create_graph) or outside of one."""
+    t = {"dy": z(T, N // 2), "x": z(T, K), "w": z(N, K), "pre": z(T, N)}
+    refuses(lambda: ctx.matmul_grad(t["dy"], t["x"], t["w"], pre=t["pre"]), t, which)
