@@ -64,6 +64,12 @@ def _outside_autograd(name: str, gradient: Optional[str], *tensors: Optional[tor
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
         raise ValueError(f"{name} records no graph: call it under torch.no_grad()" +
                          (f" or in an autograd.Function whose backward is {gradient}" if gradient else ""))
+    # forward mode, which no_grad does not stop: tangents are looked for (a microsecond) where there may be some
+    fwd = torch.autograd.forward_ad
+    if getattr(fwd, "_current_level", 0) >= 0 and torch._C._is_fwd_grad_enabled() and any(
+            t is not None and fwd.unpack_dual(t).tangent is not None for t in tensors):
+        raise ValueError(f"{name} records no graph, and a tensor has a tangent of forward mode: call it on primals or in an "
+                         f"autograd.Function with a jvp")
 
 
 def _stream(device: int) -> int:

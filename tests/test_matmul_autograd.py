@@ -61,3 +61,39 @@ def test_no_second_gradient_is_lost(ctx, which):  # noqa: F811
     """In a backward that is itself recorded (create_graph) or outside of one."""
     t = {"dy": z(T, N // 2), "x": z(T, K), "w": z(N, K), "pre": z(T, N)}
     refuses(lambda: ctx.matmul_grad(t["dy"], t["x"], t["w"], pre=t["pre"]), t, which)
+
+
+@pytest.mark.parametrize("make,which", [(quantize, "x"), (i8, "x_scale"), (i8, "w_scale"),
+                                        (lambda c: (t := {"x": z(T, K), "w": z(N, K)}, lambda: c.matmul(t["x"], t["w"])), "x"),
+                                        (lambda c: (t := {"x": z(T, K), "w": z(N, K)}, lambda: c.matmul(t["x"], t["w"])), "w"),
+                                        (lambda c: (t := {"dy": z(T, N), "x": z(T, K)}, lambda: c.matmul_grad(t["dy"], t["x"], z(N, K))), "dy"),
+                                        (lambda c: (t := {"x": z(T, K)}, lambda: c.gather_rows(t["x"], torch.arange(T, dtype=torch.int32).view(T, 1))), "x")])
+def test_no_tangent_is_lost(ctx, make, which):  # noqa: F811
+    """Forward mode: a tensor with a tangent, at any mode of the backward one."""
+    fwd = torch.autograd.forward_ad
+    t, call = make(ctx)
+    plain = t[which]
+    with fwd.dual_level():
+        with pytest.raises(Called):  # a level alone is no tangent
+            call()
+        t[which] = fwd.make_dual(plain, torch.ones_like(plain))
+        with pytest.raises(ValueError, match="records no graph"):
+            call()
+        with torch.no_grad(), pytest.raises(ValueError, match="records no graph"):
+            call()
+
+        class Own(torch.autograd.Function):  # whose jvp has the tangents
+            @staticmethod
+            def forward(fn, v):
+                t[which] = v
+                with pytest.raises(Called):
+                    call()
+                return v.clone()
+
+            @staticmethod
+            def jvp(fn, dv):
+                return dv.clone()
+        Own.apply(t[which])
+    t[which] = plain
+    with pytest.raises(Called):
+        call()
