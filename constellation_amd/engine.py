@@ -36,6 +36,12 @@ def _rows_2d(t: torch.Tensor) -> tuple[int, int]:
     return t.shape[0], t.shape[1]
 
 
+def _fit32(*counts: int) -> None:
+    """The C ABI's counts are ints; a larger one would arrive as another."""
+    if max(counts) > 2 ** 31 - 1:
+        raise ValueError(f"{max(counts)}: rows, columns, matrices and top_k must fit 32 bits")
+
+
 def _at16(t: torch.Tensor) -> torch.Tensor:
     """t, or a copy of it, contiguous and from an address that 16 divides on."""
     t = t.contiguous()
@@ -370,6 +376,7 @@ class I8Layer(_OwnLayer):
             raise ValueError("weights and scales must be contiguous, weights from an address that 16 divides on")
         if down.shape[0] <= int(shared):
             raise ValueError("a layer needs a routed expert")
+        _fit32(*gate_up.shape, *down.shape)
         self.ctx = ctx
         self.gate_up, self.gate_up_scale, self.down, self.down_scale = gate_up, gate_up_scale, down, down_scale
         self.shared = self if shared else None
@@ -663,6 +670,7 @@ class Context:
         if keep and not gated:
             raise ValueError("keep is of gated products")
         P = self._picked(order, T)
+        _fit32(T, K, E, N, P, top_k)
         x, w = _at16(x), _at16(w)
         out_dtype = out_dtype or x.dtype
         dt = cx_dtype(x.dtype)
@@ -694,6 +702,7 @@ class Context:
             raise ValueError(f"pre must be [{P}, {N}]")
         if not (want_dx or want_dw):
             raise ValueError("nothing to compute: want_dx or want_dw")
+        _fit32(P, K, E, N)
         dw_dtype = dw_dtype or x.dtype
         if dw_dtype not in (x.dtype, torch.float32):
             raise TypeError("dw must be of x's type or float32")
@@ -717,6 +726,7 @@ class Context:
         _outside_autograd("quantize_i8", None, x)
         if x.dim() < 1:
             raise ValueError("expected rows")
+        _fit32(x.shape[:-1].numel(), x.shape[-1])
         x = x.contiguous()
         q = torch.empty_like(x, dtype=torch.int8)
         scale = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)
@@ -741,6 +751,7 @@ class Context:
         if w_scale.shape != w.shape[:-1] or w_scale.dtype != torch.float32 or not w_scale.is_contiguous():
             raise ValueError(f"w_scale must be contiguous fp32 {list(w.shape[:-1])}")
         P = self._picked(order, T)
+        _fit32(T, K, E, N, P, top_k)
         x, w, x_scale = _at16(x), _at16(w), x_scale.contiguous()
         y = torch.empty((P, N // 2 if gated else N), dtype=out_dtype, device=x.device)
         size = lib().cx_i8_matmul_scratch(T, E, N, K, P, int(offsets is not None))
@@ -761,12 +772,14 @@ class Context:
             raise ValueError("a matrix of the layer has been freed")
         if x.dim() != 2 or x.shape[1] != layer.hidden:
             raise ValueError(f"x has {x.shape[-1] if x.dim() else 0} columns in {x.dim()} dimensions, the layer {layer.hidden} in 2")
+        _fit32(x.shape[0])
 
     def _own_moe(self, layer: _OwnLayer, x, topk_ids, topk_w, y, yf):
         self._own_ready(layer, x, topk_ids, topk_w)
         T, K = x.shape[0], topk_ids.shape[1] if topk_ids.dim() == 2 else -1
         if topk_ids.shape != (T, K) or topk_w.shape != (T, K):
             raise ValueError(f"routes must be [{T}, top_k]")
+        _fit32(K)
         if layer._slots is not None:
             topk_ids = layer._slots[topk_ids.clamp(-1, layer.n_experts).long() + 1]
         size = layer._scratch.get((T, K))
