@@ -7,9 +7,7 @@ namespace {
 
 template <class S, bool GATED>
 hipError_t run(MmLaunch& L, hipStream_t s) {
-    const int out = GATED ? S::BM / 2 : S::BM, width = GATED ? L.rows / 2 : L.rows;
-    L.m_tiles = (width + out - 1) / out;
-    cx_launch(k_mm<MmI8, S, GATED>, dim3(mm_grid(L)), dim3(S::kThreads), 0, s, L);
+    cx_launch(k_mm<MmI8, S, GATED>, dim3(mm_grid(L, L.rows)), dim3(S::kThreads), 0, s, L);
     return hipGetLastError();
 }
 

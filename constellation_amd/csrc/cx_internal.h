@@ -533,12 +533,12 @@ __host__ __device__ inline MmTile mm_tile(unsigned b, int m_tiles, int by_item) 
     const int pitch = (m_tiles + 7) / 8 * 8;
     return MmTile{(int)b / pitch, (int)b % pitch};
 }
-inline unsigned mm_grid(MmLaunch& L) {
+inline unsigned mm_grid(MmLaunch& L, int64_t out) {
     L.item_rows = L.form.item_rows;
     L.splits = L.form.splits;
     L.by_item = L.offsets != nullptr;
-    const int64_t items = mm_items(L.n_rows, L.n_mats, L.offsets != nullptr, L.item_rows), m = (int64_t)L.m_tiles * L.splits;
-    return (unsigned)(L.by_item ? (items + 7) / 8 * 8 * m : items * ((m + 7) / 8 * 8));
+    L.m_tiles = (int)((out + 128 * L.form.kind - 1) / (128 * L.form.kind));
+    return (unsigned)mm_tile_grid(L.form, L.n_rows, L.n_mats, L.by_item, out);
 }
 inline bool mm_at16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 // Rows of `cols` elements to rows of `pitch`, zeros behind them; of the matrices (mat_rows rows each) that have rows.

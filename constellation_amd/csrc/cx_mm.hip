@@ -7,9 +7,7 @@ namespace {
 
 template <class T, class S, bool GATED>
 hipError_t run(MmLaunch& L, hipStream_t s) {
-    const int out = GATED ? S::BM / 2 : S::BM, width = GATED ? L.rows / 2 : L.rows;
-    L.m_tiles = (width + out - 1) / out;
-    cx_launch(k_mm<T, S, GATED>, dim3(mm_grid(L)), dim3(S::kThreads), 0, s, L);
+    cx_launch(k_mm<T, S, GATED>, dim3(mm_grid(L, L.rows)), dim3(S::kThreads), 0, s, L);
     return hipGetLastError();
 }
 
@@ -123,7 +121,7 @@ hipError_t launch_mm_pad(const MmPad& p, hipStream_t s) {
 }
 
 hipError_t launch_mm_sum(const MmLaunch& L, int out, bool gated, hipStream_t s) {
-    const int chunks = ((gated ? out / 2 : out) + 1023) / 1024;
+    const int chunks = mm_sum_chunks(gated ? out / 2 : out);
     cx_launch(L.type == kMmI8 ? k_mm_sum<true> : k_mm_sum<false>, dim3((unsigned)((int64_t)L.n_rows * chunks)), dim3(256), 0, s, L, out, (int)gated, chunks);
     return hipGetLastError();
 }

@@ -146,8 +146,7 @@ __global__ __launch_bounds__(64 * kMmFewWaves, 2) void k_mm_few(MmLaunch L, int 
 
 template <class T, int RW, bool GATED>
 hipError_t mm_few_run(MmLaunch& L, bool vec, hipStream_t s) {
-    const int kCols = GATED ? 8 : 16, width = GATED ? L.rows / 2 : L.rows, splits = L.form.splits, per = kMmFewWaves / splits * RW;
-    const int blocks = ((width + kCols - 1) / kCols + per - 1) / per;
+    const int splits = L.form.splits, blocks = (int)mm_few_blocks(L.form, L.rows);
     const int64_t items = mm_items(L.n_rows, L.n_mats, L.offsets != nullptr, 16);
     cx_launch(vec ? k_mm_few<T, RW, GATED, true> : k_mm_few<T, RW, GATED, false>, dim3((unsigned)(items * blocks)), dim3(64 * kMmFewWaves), 0, s, L,
               splits, blocks);

@@ -6,24 +6,7 @@ namespace {
 
 template <class T, class S>
 hipError_t dx(MmLaunch& L, hipStream_t s) {
-    L.m_tiles = (L.cols + S::BM - 1) / S::BM;
-    cx_launch(k_mm_dx<T, S>, dim3(mm_grid(L)), dim3(S::kThreads), 0, s, L);
-    return hipGetLastError();
-}
-
-template <class T, class S>
-hipError_t dw(MmLaunch& L, hipStream_t s) {
-    L.m_tiles = (L.cols + S::BM - 1) / S::BM;
-    const int64_t tiles = (int64_t)L.n_mats * L.m_tiles * ((L.rows + S::BN - 1) / S::BN);
-    cx_launch(k_mm_dw<T, S>, dim3((unsigned)tiles), dim3(S::kThreads), 0, s, L);
-    return hipGetLastError();
-}
-
-template <class T, class S>
-hipError_t dw_short(MmLaunch& L, hipStream_t s) {
-    L.m_tiles = (L.cols + S::BM - 1) / S::BM;
-    const int64_t tiles = (int64_t)L.n_mats * L.m_tiles * ((L.rows + S::BN - 1) / S::BN);
-    cx_launch(k_mm_dw_short<T, S>, dim3((unsigned)((tiles + 511) / 512 * 512)), dim3(S::kThreads), 0, s, L);
+    cx_launch(k_mm_dx<T, S>, dim3(mm_grid(L, L.cols)), dim3(S::kThreads), 0, s, L);
     return hipGetLastError();
 }
 
@@ -35,10 +18,17 @@ hipError_t dx_pick(MmLaunch& L, hipStream_t s) {
 
 template <class T>
 hipError_t dw_pick(MmLaunch& L, hipStream_t s) {
-    const int64_t tiles = (int64_t)L.n_mats * ((L.cols + 255) / 256) * ((L.rows + 255) / 256);
-    if (tiles < 256) return dw<T, MmSmall>(L, s);
-    // 4096 x 7168: 32 matrices with 512 rows each 1162 us with short steps and 1215 with long ones, one with 2048 109 and 100
-    return L.n_rows < (int64_t)L.n_mats * 1024 ? dw_short<T, MmMid>(L, s) : dw<T, MmBig>(L, s);
+    static_assert(MmSmall::BM == 128 && MmSmall::BN == 128 && MmBig::BM == 256 && MmBig::BN == 256 && MmMid::BM == 256 && MmMid::BN == 128, "mm_dw_grid");
+    const int kind = mm_dw_kind(L.n_rows, L.n_mats, L.rows, L.cols), m = kind == 1 ? MmSmall::BM : MmBig::BM;
+    const dim3 grid((unsigned)mm_dw_grid(kind, L.n_mats, L.rows, L.cols));
+    L.m_tiles = (L.cols + m - 1) / m;
+    if (kind == 1)
+        cx_launch(k_mm_dw<T, MmSmall>, grid, dim3(MmSmall::kThreads), 0, s, L);
+    else if (kind == 2)
+        cx_launch(k_mm_dw<T, MmBig>, grid, dim3(MmBig::kThreads), 0, s, L);
+    else
+        cx_launch(k_mm_dw_short<T, MmMid>, grid, dim3(MmMid::kThreads), 0, s, L);
+    return hipGetLastError();
 }
 
 // h = silu(g) u has dg = dh u sig(g) (1 + g (1 - sig(g))) and du = dh silu(g); each rounded once.  One value

@@ -809,9 +809,9 @@ int check_mm(cx_ctx* ctx, int el, int n_mats, int rows, int cols, int gated, con
     if (gated && rows % 2 != 0) return fail(CX_EINVAL, "a gated matrix has an even number of rows");
     if (n_rows < 0) return fail(CX_EINVAL, "bad n_rows");
     if (!offsets && n_mats != 1) return fail(CX_EINVAL, "a stack of %d matrices needs offsets", n_mats);
-    if (!mm_grid_ok(n_rows, n_mats, rows, cols)) return fail(CX_EINVAL, "too many rows or matrices for one launch");
     return CX_OK;
 }
+int mm_too_large() { return fail(CX_EINVAL, "too many rows or matrices for one launch"); }
 
 int check_scratch(size_t need, const void* scratch, size_t bytes) {
     if (need && (!scratch || bytes < need || reinterpret_cast<uintptr_t>(scratch) % 16))
@@ -859,6 +859,7 @@ int matmul(cx_ctx* ctx, MmLaunch L, void* scratch, size_t scratch_bytes, void* s
     if (!L.x || !L.w || !L.y || (el == 1 && (!L.x_scale || !L.w_scale))) return fail(CX_EINVAL, "NULL buffer");
     if (!mm_at16(L.x) || !mm_at16(L.w)) return fail(CX_EINVAL, "x and weights must start on 16 bytes");
     const MmPlan p = mm_plan(el, L.n_x, L.n_mats, L.rows, L.cols, L.n_rows, L.offsets != nullptr);
+    if (!mm_grid_ok(L.n_rows, L.n_mats, L.rows, L.cols, L.offsets != nullptr, &p.form, nullptr, false)) return mm_too_large();
     if ((rc = check_scratch(p.bytes, scratch, scratch_bytes))) return rc;
     if ((rc = set_device(ctx->device))) return rc;
     L.err_flag = ctx->err_flag;
@@ -1872,6 +1873,7 @@ int cx_matmul_grad(cx_ctx* ctx, const void* dy, const void* x, const void* w, in
     if ((n_rows > 0 && (!dy || (dw && !x))) || (dx && !w)) return fail(CX_EINVAL, "NULL buffer");
     if (!mm_at16(dy) || (dw && !mm_at16(x)) || (dx && !mm_at16(w))) return fail(CX_EINVAL, "dy, x and weights must start on 16 bytes");
     const GradScratch z = n_rows > 0 ? grad_scratch(n_mats, rows, cols, pre != nullptr, n_rows, offsets != nullptr, dx != nullptr, dw != nullptr) : GradScratch{};
+    if (!mm_grid_ok(n_rows, n_mats, rows, cols, offsets != nullptr, nullptr, dx && n_rows > 0 ? &z.dx : nullptr, dw != nullptr)) return mm_too_large();
     if ((rc = check_scratch(z.bytes, scratch, scratch_bytes))) return rc;
     if ((rc = set_device(ctx->device))) return rc;
     hipStream_t s = static_cast<hipStream_t>(stream);
@@ -2028,6 +2030,9 @@ int cx_i8_moe(cx_ctx* ctx, const cx_i8_layer* w, const void* x, int in_dtype, in
     if (!x || !y || (top_k > 0 && (!topk_ids || !topk_w))) return fail(CX_EINVAL, "NULL buffer");
     if (!mm_at16(w->gate_up) || !mm_at16(w->down)) return fail(CX_EINVAL, "weights must start on 16 bytes");
     const I8MoeScratch z = i8_moe_scratch(*w, n_tokens, top_k);
+    if (!mm_grid_ok(pairs, w->n_mats, 2 * w->inter, w->hidden, true, &z.gate_up.form, nullptr, false) ||
+        !mm_grid_ok(pairs, w->n_mats, w->hidden, w->inter, true, &z.down.form, nullptr, false))
+        return mm_too_large();
     if ((rc = check_scratch(z.bytes, scratch, scratch_bytes))) return rc;
     if ((rc = set_device(ctx->device))) return rc;
     hipStream_t s = static_cast<hipStream_t>(stream);

@@ -467,10 +467,42 @@ inline MmForm mm_form(int64_t n_rows, int n_mats, bool stack, int64_t out, int64
     return best;
 }
 
-// Launches stay within 2^32 threads and 2^30 rows, at the smallest tiles and with every matrix's last tile short.
-inline bool mm_grid_ok(int64_t n_rows, int n_mats, int rows, int cols) {
-    const int64_t items = mm_items(n_rows, n_mats, true, 16) + 8, tiles = (std::max(rows, cols) + 63) / 64 + 8;
-    return n_rows <= (1 << 30) && items * tiles < ((int64_t)1 << 24) && n_mats * (((int64_t)rows + 127) / 128) * ((cols + 127) / 128) < ((int64_t)1 << 24);
+// Workgroups of a form's tiles, `out` wide.  Where tile m of every item runs on one XCD (one matrix), tiles are counted in
+// eights, otherwise items are.
+inline int64_t mm_tile_grid(const MmForm& f, int64_t n_rows, int n_mats, bool stack, int64_t out) {
+    const int64_t items = mm_items(n_rows, n_mats, stack, f.item_rows), m = (out + 128 * f.kind - 1) / (128 * f.kind) * f.splits;
+    return stack ? (items + 7) / 8 * 8 * m : items * ((m + 7) / 8 * 8);
+}
+// Kind 0: workgroups of an item.
+inline int64_t mm_few_blocks(const MmForm& f, int64_t out) {
+    const int per = kMmFewWaves / f.splits * f.tiles;
+    return ((out + 15) / 16 + per - 1) / per;
+}
+constexpr int mm_sum_chunks(int64_t width) { return (int)((width + 1023) / 1024); }  // workgroups of a row's partial sums
+
+// The gradient at the weights.  1: tiles of 128 x 128; 2: of 256 x 256; 3: of 256 columns and 128 rows with short steps.
+// 4096 x 7168: 32 matrices with 512 rows each 1162 us with short steps and 1215 with long ones, one with 2048 109 and 100
+inline int mm_dw_kind(int64_t n_rows, int n_mats, int rows, int cols) {
+    if ((int64_t)n_mats * ((cols + 255) / 256) * ((rows + 255) / 256) < 256) return 1;
+    return n_rows < (int64_t)n_mats * 1024 ? 3 : 2;
+}
+inline int64_t mm_dw_grid(int kind, int n_mats, int rows, int cols) {
+    const int m = kind == 1 ? 128 : 256, n = kind == 2 ? 256 : 128;
+    const int64_t tiles = (int64_t)n_mats * ((cols + m - 1) / m) * ((rows + n - 1) / n);
+    return kind == 3 ? (tiles + 511) / 512 * 512 : tiles;
+}
+
+// Whether launches hold a call's workgroups: of the forward product (y its form), of the gradient at x (dx its form) and of
+// that at the weights, each where it is there.
+inline bool mm_grid_ok(int64_t n_rows, int n_mats, int rows, int cols, bool stack = true, const MmForm* y = nullptr, const MmForm* dx = nullptr,
+                       bool dw = true) {
+    auto holds = [&](const MmForm& f, int64_t out) {
+        if (f.kind == 0) return rows_grid_ok(mm_items(n_rows, n_mats, stack, f.item_rows) * mm_few_blocks(f, out), 64 * kMmFewWaves);
+        return rows_grid_ok(mm_tile_grid(f, n_rows, n_mats, stack, out), 256 * f.kind) && (f.splits == 1 || rows_grid_ok(n_rows * mm_sum_chunks(out), 256));
+    };
+    if (n_rows > (1 << 30) || (y && !holds(*y, rows)) || (dx && !holds(*dx, cols))) return false;
+    const int kind = mm_dw_kind(n_rows, n_mats, rows, cols);
+    return !dw || rows_grid_ok(mm_dw_grid(kind, n_mats, rows, cols), kind == 2 ? 512 : 256);
 }
 
 }  // namespace cx

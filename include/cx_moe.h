@@ -422,7 +422,8 @@ CX_API int cx_q4_moe(cx_ctx* ctx, const cx_q4_desc* gate_up, const cx_q4_desc* d
  * once.  x, weights and dy start on 16 bytes, other buffers at any address of their type's
  * alignment; rows that are no whole 16-byte pieces are copied to such rows in the scratch, but for
  * few rows of x.  n_mats is at most 1024, rows and cols 2^22 (8-bit:
- * cols 131071), n_rows 2^30, and a matrix has fewer than 2^32 bytes. */
+ * cols 131071), n_rows 2^30, and a matrix has fewer than 2^32 bytes.  A call whose tiles of outputs (128 or 256 a side; of few
+ * rows 16 rows by up to 256) one launch of 2^32 threads does not hold is refused: of one matrix from about 2^28 rows or 2^38 outputs on. */
 
 /* y = x W^T.  gated: rows is even and the halves are a gate and an up matrix G, U:
  * y = silu(x G^T) * (x U^T); pre (nullable, for the gradient) receives [x G^T, x U^T],
