@@ -123,11 +123,17 @@ hipError_t launch_mm_i8(MmLaunch L, hipStream_t s) { return L.gated ? pick<true>
 
 hipError_t launch_quantize_i8(const void* x, int x_type, int n_rows, int cols, int8_t* q, float* scale, hipStream_t s) {
     // rows of 2048: 3001 in 8.5 us with a wave each and 10.3 with four, one in 4.0 and 2.5; 4096 rows of 512 in 5.2 and 9.6
-    if (cols <= 512 || (cols <= 2048 && n_rows >= 2048))
-        cx_launch(k_quantize_i8<1>, dim3((unsigned)((n_rows + (int64_t)3) / 4)), dim3(kI8Threads), 0, s, x, x_type, n_rows, cols, q, scale);
-    else
-        cx_launch(k_quantize_i8<4>, dim3((unsigned)n_rows), dim3(kI8Threads), 0, s, x, x_type, n_rows, cols, q, scale);
-    return hipGetLastError();
+    const int rows = cols <= 512 || (cols <= 2048 && n_rows >= 2048) ? 4 : 1;  // of a workgroup
+    const int most = rows << 23;                                               // of a launch, whose threads are counted in 32 bits
+    const size_t row = (size_t)cols * (x_type == CX_DTYPE_F32 ? 4 : 2);
+    for (int64_t r = 0; r < n_rows; r += most) {
+        const int n = (int)std::min<int64_t>(most, n_rows - r);
+        cx_launch(rows == 4 ? k_quantize_i8<1> : k_quantize_i8<4>, dim3((unsigned)((n + (int64_t)rows - 1) / rows)), dim3(kI8Threads), 0, s,
+                  static_cast<const char*>(x) + r * row, x_type, n, cols, q + r * cols, scale + r);
+        const hipError_t e = hipGetLastError();
+        if (e != hipSuccess) return e;
+    }
+    return hipSuccess;
 }
 
 }  // namespace cx

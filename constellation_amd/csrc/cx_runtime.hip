@@ -1934,7 +1934,6 @@ int cx_quantize_i8(cx_ctx* ctx, const void* x, int x_dtype, int n_rows, int cols
     if (!act_any(x_dtype)) return fail(CX_EINVAL, "x must be fp16, bf16 or fp32");
     if (n_rows == 0) return CX_OK;
     if (!x || !q || !scale) return fail(CX_EINVAL, "NULL buffer");
-    if (!rows_grid_ok(n_rows, 256)) return fail(CX_EINVAL, "too many rows for one launch");
     hipStream_t s = static_cast<hipStream_t>(stream);
     Span sp(ctx, "quantize", s);
     CX_HIP(launch_quantize_i8(x, x_dtype, n_rows, cols, q, scale, s));
@@ -2062,7 +2061,7 @@ int cx_i8_moe(cx_ctx* ctx, const cx_i8_layer* w, const void* x, int in_dtype, in
     c.out = y;
     c.out_f32 = y_f32;
     c.err_flag = ctx->err_flag;
-    if (!rows_grid_ok(pairs, 256) || !rows_grid_ok(combine_workgroups(c), kRowThreads)) return fail(CX_EINVAL, "too many rows for one launch");
+    if (!rows_grid_ok(combine_workgroups(c), kRowThreads)) return fail(CX_EINVAL, "too many rows for one launch");
     MmLaunch L{};
     L.type = kMmI8;
     L.n_mats = w->n_mats;

@@ -4,7 +4,7 @@ from __future__ import annotations
 import pytest
 import torch
 
-from test_gpu_q4 import BF, HALF, TINY, U, rand
+from test_gpu_q4 import BF, HALF, SF, TINY, U, rand
 
 pytestmark = pytest.mark.gpu
 
@@ -26,4 +26,19 @@ def test_many_rows_of_a_small_matrix(gpu):
     assert torch.equal(dx, dx[:1].expand_as(dx))
     want, tol = dy.double() @ w.double(), (dy.double().abs() @ w.double().abs()) * 24 * U
     assert bool(((dx[0].double() - want).abs() <= tol + (want.abs() + tol) * HALF[BF] + TINY[BF]).all())
+    gpu.sync()
+
+
+@pytest.mark.parametrize("dtype", [BF, SF])
+def test_many_rows_to_8_bits(gpu, dtype):
+    """More rows than one launch holds: 2^25 of a wave each."""
+    block, n = 40_003, 839
+    assert block * n > (1 << 25) + 3
+    print(f"[mm] {block * n} rows to 8 bits {dtype}", flush=True)
+    x = rand(4, block, 9, dtype=dtype)
+    q, s = gpu.quantize_i8(x.cuda())
+    want = (x.float().abs().amax(1) / torch.tensor(127.0)).clamp_min(1e-12)
+    assert torch.equal(s.cpu(), want) and torch.equal(q.cpu(), torch.round(x.float() / want[:, None]).to(torch.int8))
+    many, scales = gpu.quantize_i8(x.cuda().repeat(n, 1))
+    assert torch.equal(many.view(n, block, 9), q.expand(n, block, 9)) and torch.equal(scales.view(n, block), s.expand(n, block))
     gpu.sync()
