@@ -205,7 +205,8 @@ __device__ __forceinline__ uint32_t mm_lds_addr(const unsigned char* p) {
 
 // Fragment reads are written as asm: of plain loads the compiler cannot tell which slot a pending direct load
 // writes, and waits for all of them.  Every output is an operand of mm_wait, so it stays live and unread until the
-// read has landed.
+// read has landed; that the compiler neither copies nor spills one before is checked on the built kernels
+// (tests/test_matmul_fragments.py).
 template <int OFF>
 __device__ __forceinline__ void mm_read16(u32x4& v, uint32_t at) {
     static_assert(OFF >= 0 && OFF < 65536, "offset field");
