@@ -11,6 +11,7 @@ from typing import NamedTuple, Optional, Sequence, Union
 
 import numpy as np
 import torch
+from torch.autograd import forward_ad as _forward_ad
 
 from ._lib import (BF16, E4M3, F32, FP16, CxError, DeviceInfo, ExpertDesc, I8LayerDesc, MoeLayerRequestInfo,
                    Q4Desc, check, lib)
@@ -38,8 +39,9 @@ def _rows_2d(t: torch.Tensor) -> tuple[int, int]:
 
 def _fit32(*counts: int) -> None:
     """The C ABI's counts are ints; a larger one would arrive as another."""
-    if max(counts) > 2 ** 31 - 1:
-        raise ValueError(f"{max(counts)}: rows, columns, matrices and top_k must fit 32 bits")
+    for n in counts:
+        if n > 0x7FFFFFFF:
+            raise ValueError(f"{n}: rows, columns, matrices and top_k must fit 32 bits")
 
 
 def _at16(t: torch.Tensor) -> torch.Tensor:
@@ -67,15 +69,17 @@ def _device(index: int) -> torch.device:
 
 def _outside_autograd(name: str, gradient: Optional[str], *tensors: Optional[torch.Tensor]) -> None:
     """A result without a graph must not pass for one with it.  gradient: the call that a backward makes, if there is one."""
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
-        raise ValueError(f"{name} records no graph: call it under torch.no_grad()" +
-                         (f" or in an autograd.Function whose backward is {gradient}" if gradient else ""))
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                raise ValueError(f"{name} records no graph: call it under torch.no_grad()" +
+                                 (f" or in an autograd.Function whose backward is {gradient}" if gradient else ""))
     # forward mode, which no_grad does not stop: tangents are looked for (a microsecond) where there may be some
-    fwd = torch.autograd.forward_ad
-    if getattr(fwd, "_current_level", 0) >= 0 and torch._C._is_fwd_grad_enabled() and any(
-            t is not None and fwd.unpack_dual(t).tangent is not None for t in tensors):
-        raise ValueError(f"{name} records no graph, and a tensor has a tangent of forward mode: call it on primals or in an "
-                         f"autograd.Function with a jvp")
+    if getattr(_forward_ad, "_current_level", 0) >= 0 and torch._C._is_fwd_grad_enabled():
+        for t in tensors:
+            if t is not None and _forward_ad.unpack_dual(t).tangent is not None:
+                raise ValueError(f"{name} records no graph, and a tensor has a tangent of forward mode: call it on primals or in "
+                                 "an autograd.Function with a jvp")
 
 
 def _stream(device: int) -> int:
@@ -726,11 +730,12 @@ class Context:
         _outside_autograd("quantize_i8", None, x)
         if x.dim() < 1:
             raise ValueError("expected rows")
-        _fit32(x.shape[:-1].numel(), x.shape[-1])
         x = x.contiguous()
         q = torch.empty_like(x, dtype=torch.int8)
         scale = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)
-        check(lib().cx_quantize_i8(self.handle, x.data_ptr(), cx_dtype(x.dtype), scale.numel(), x.shape[-1],
+        rows, cols = scale.numel(), x.shape[-1]
+        _fit32(rows, cols)
+        check(lib().cx_quantize_i8(self.handle, x.data_ptr(), cx_dtype(x.dtype), rows, cols,
                                    q.data_ptr(), scale.data_ptr(), self.stream()))
         return q, scale
 
