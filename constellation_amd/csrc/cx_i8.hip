@@ -54,8 +54,8 @@ __device__ __forceinline__ void i8_piece(const void* x, int type, size_t at, int
 }
 
 // A row's largest size, then codes from correctly rounded quotients.  W waves have a row, 4 / W rows a workgroup, and hold
-// it in registers between the two (up to 2048 W columns), so that it is read once.  1024 rows of 7168 in 9.4 us, launch
-// included, where a copy of the same bytes takes 4.5: a row's load, its maximum and its codes wait for each other.
+// it in registers between the two (up to 2048 W columns), so that it is read once.  1024 rows of 7168 in 9.4 us of a series
+// (12.4 traced after a pause), where a copy of the same bytes takes 4.5: a row's load, its maximum and its codes wait for each other.
 template <int W>
 __global__ __launch_bounds__(kI8Threads) void k_quantize_i8(const void* x, int type, int n_rows, int cols, int8_t* q, float* scale) {
     __shared__ uint32_t part[kI8Threads / 64];
@@ -122,7 +122,8 @@ __global__ __launch_bounds__(kI8Threads) void k_quantize_i8(const void* x, int t
 hipError_t launch_mm_i8(MmLaunch L, hipStream_t s) { return L.gated ? pick<true>(L, s) : pick<false>(L, s); }
 
 hipError_t launch_quantize_i8(const void* x, int x_type, int n_rows, int cols, int8_t* q, float* scale, hipStream_t s) {
-    // rows of 2048: 3001 in 8.5 us with a wave each and 10.3 with four, one in 4.0 and 2.5; 4096 rows of 512 in 5.2 and 9.6
+    // a wave each and four, us: rows of 512: 256 3.4 and 3.5, 1024 3.6 and 4.7, 4096 5.1 and 10.6; of 1024: 512 3.9 and 3.8, 1500 4.4 and
+    // 5.7, 2048 4.5 and 7.0; of 2048: one 4.0 and 2.5, 512 4.9 and 3.8, 1024 5.1 and 5.3, 2048 6.2 and 7.6, 16384 30 and 46
     const int rows = cols <= 512 || (cols <= 2048 && n_rows >= 2048) ? 4 : 1;  // of a workgroup
     const int most = rows << 23;                                               // of a launch, whose threads are counted in 32 bits
     const size_t row = (size_t)cols * (x_type == CX_DTYPE_F32 ? 4 : 2);

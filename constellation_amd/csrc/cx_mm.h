@@ -420,7 +420,9 @@ __device__ __forceinline__ void mm_core(const MmSrc<S::BM, S::kThreads, T::kEl, 
 // The same for the gradient at the weights, whose operands both lie across the contraction: steps of 32 rows, which are whole lines
 // all the same, so that three of them for 256 x 128 results leave room for a second workgroup on the CU.  A matrix's share of
 // rows is short and its results are many: one workgroup stores while the other multiplies (32 matrices of 4096 x 7168, 512 rows
-// each: with one of 256 x 256 results a CU 1215 us, of which 370 were stores that nothing ran beside).
+// each: with one of 256 x 256 results a CU 1226 us, of which 370 were stores that nothing ran beside; so 1120 to 1180, 1284 traced
+// after a pause).  Matrix cores are 43 % busy: the 1.88 GB of results go through the L2 that holds the operands, which are
+// fetched 4.7 times (1.72 GB for 0.37).
 template <class S>
 struct MmShort {
     static constexpr int kSlots = 3, kStepM = S::BM * 64, kStepN = S::BN * 64, kStep = kStepM + kStepN, kLds = kSlots * kStep;
@@ -655,8 +657,9 @@ __device__ __forceinline__ int mm_row_of_x(const MmLaunch& L, int p) {
 }
 
 // Forward: a workgroup reads its weights and rows once each from L2.  32 matrices of 4096 x 7168, gated, 512 rows each on
-// average: 990 us when dealt unevenly (854 evenly), matrix cores 70 % busy; what they miss are tiles that an item's last
-// rows do not fill and the ends of a workgroup's 112 steps, which nothing runs beside.  m: weight rows; a gated tile has TM / 2 results of gate rows and the same rows of the up
+// average: 977 to 1054 us when dealt unevenly (854 evenly, 1.13 PFLOP/s; one matrix of 4096 rows 1.4), matrix cores 70 % busy.
+// Two things bound it: traffic, as each item of up to 256 rows reads its matrix again (4.8 GB fetched where 2.1 are
+// unique, about 5 TB/s, a copy's rate), and tiles that an item's last rows do not fill.  m: weight rows; a gated tile has TM / 2 results of gate rows and the same rows of the up
 // half per wave, so that both factors of an output meet in one lane.
 template <class T, class S, bool GATED>
 __device__ __forceinline__ void mm_forward(const MmLaunch& L, const MmWork& work, unsigned char* lds) {
@@ -751,7 +754,8 @@ __global__ __launch_bounds__(S::kThreads, 2) void k_mm(MmLaunch L) {
 }
 
 // The gradient at x.  m: columns of the weights, read across their rows by transposing reads, so that no transposed copy of
-// them is made; n: rows of dy.  16384 rows by 32 x 4096 x 7168: 960 to 975 us, matrix cores 67 % busy.
+// them is made; n: rows of dy.  16384 rows by 32 x 4096 x 7168: 950 to 975 us, matrix cores 67 % busy
+// and 4.9 GB fetched (5 TB/s): every item reads its matrix again, as in the forward product.
 template <class T, class S>
 __device__ __forceinline__ void mm_dx(const MmLaunch& L, const MmWork& work, unsigned char* lds) {
     const MmItem it = work.it;

@@ -433,11 +433,20 @@ inline MmForm mm_few_form(int64_t busy, int rows, int steps) {
 }
 
 // The cost of a form is estimated, in us: a step of a tile, tiles beside each other on a CU, rounds of workgroups, and the
-// partial sums' way through memory.  Rows by 4096 x 7168 gated, us: 40 rows with tiles of 128 59, in 4 ranges 25 (tiles of
-// 256: 88, 33); 256 rows 71, 32 (145, 52); 512 rows 71, 44 (142, 54); 1024 rows 72, 79 (141, 67); 2048 rows 110, 149
-// (141, 128); 4096 rows 209, 344 (172, 289).  32 matrices of 4096 x 7168, 16384 rows, at x: 1302 (964).
-// Few rows: up to 16 a matrix on average.  8 rows 17 (through LDS in 4 ranges 24), 16 rows 20 (24), 24 rows 32 (24).  The
-// host does not know how rows are dealt: where one matrix of many gets them all, its weights are read once for each 16.
+// partial sums' way through memory.  Measured in bf16, us: the rule's form, in brackets the best other one where it is faster
+// by more than 2 %.
+//   gated rows by 4096 x 7168   17: 25.8, 16 ranges (8 ranges 21.1)   20 to 32: 21   64: 23   128: 26   256: 32   512: 45
+//                               1024: 72, one range of tiles of 128 (two of 256: 70)   1536: 89   2048: 105
+//     in one range of tiles of 128 up to 256 rows take 55 there
+//   rows by 7168 x 2048         17: 12   64: 14   256: 19, items of 64 (of 32: 17)   1024: 32   2048: 53   3001: 82
+//   rows by 2048 x 1040         17: 9.3 (few rows 4.7)   64 and 256: 9.3   1000: 12   3001: 22 (tiles of 256: 21)
+//   at x, 4096 x 7168           300: 36   1000: 61   3001: 152
+//   rows dealt at random over 64 of 7168 x 2048    512: 415, few rows (tiles of 128 360)   1024: 513 (tiles of 256 375)
+//                               1088: 377   1536: 387   2048: 396   4096: 444   8192: 488;   at x 2048: 339 (331)   4096: 415
+// So it errs just above 16 rows, and by 15 to 37 % for 8 to 16 rows a matrix of stacks, where tiles read the weights faster (5.2
+// TB/s, 4.5) and a matrix's 17th row reads it again.
+// Few rows: up to 16 a matrix on average.  8 rows by 4096 x 7168 gated 17 (through LDS 21), 16 rows 20.0 (21.0), 24 rows 32 (21).
+// The host does not know how rows are dealt: where one matrix of many gets them all, its weights are read once for each 16.
 //
 // out: the output's width, in which tiles of 128 or 256 lie (of a gated product the weights' rows); depth: bytes of the
 // contraction; few: the kernel of few rows is there.
@@ -481,7 +490,12 @@ inline int64_t mm_few_blocks(const MmForm& f, int64_t out) {
 constexpr int mm_sum_chunks(int64_t width) { return (int)((width + 1023) / 1024); }  // workgroups of a row's partial sums
 
 // The gradient at the weights.  1: tiles of 128 x 128; 2: of 256 x 256; 3: of 256 columns and 128 rows with short steps.
-// 4096 x 7168: 32 matrices with 512 rows each 1162 us with short steps and 1215 with long ones, one with 2048 109 and 100
+// Measured in bf16, us, of 1, 2, 3.  Fewer than 256 large tiles: 1000 rows by 2048 x 1040 (40 tiles) 19, 31, 34; 4096 rows by
+// 2048 x 4096 (128) 67, 83, 108, but by 4 of 2048 x 1040 (160) 49, 37, 38 and 2048 rows by 4096 x 3840 (240) 71, 59, 62; by
+// 4096 x 4096 (256) 69, 61, 63.  Rows a matrix: 32 of 4096 x 7168 with 512 each 1488, 1226, 1180, with 1024 2268, 1886, 1858, with
+// 2048 3924, 3275, 3210; 16 of 1024 x 1024 with 2048 each 103, 70, 64; one of 4096 x 7168 with 512 45, 44, 44, with 1024 68, 65, 65,
+// with 2048 114, 104, 113, with 4096 209, 188, 207.  So 160 tiles already fill the card better, and in stacks short steps
+// stay ahead past 1024 rows, by 2 to 9 %.
 inline int mm_dw_kind(int64_t n_rows, int n_mats, int rows, int cols) {
     if ((int64_t)n_mats * ((cols + 255) / 256) * ((rows + 255) / 256) < 256) return 1;
     return n_rows < (int64_t)n_mats * 1024 ? 3 : 2;
