@@ -363,7 +363,7 @@ class I8Layer(_OwnLayer):
     `gate_up` [E, 2 * inter, hidden] (a gate and then an up matrix) and `down` [E, hidden, inter].  With `shared` the
     last of the stacks' experts is the layer's shared one.  Context.moe and Context.moe_layer take it in place of a
     Layer, and so does moe_dispatch.LocalNode.  `experts`, `n_experts`: as Q4Layer's, of the routed experts.  The
-    layer keeps the tensors."""
+    layer keeps the tensors: new values may be copied into them, but others take another layer."""
 
     def __init__(self, ctx: "Context", gate_up: torch.Tensor, gate_up_scale: torch.Tensor, down: torch.Tensor,
                  down_scale: torch.Tensor, *, shared: bool = False, experts: Optional[Sequence[int]] = None,
@@ -771,6 +771,10 @@ class Context:
         self._here(x, *others)
         if isinstance(layer, I8Layer):
             self._here(layer.gate_up)
+            d = layer.desc
+            if (layer.gate_up.data_ptr() != d.gate_up or layer.down.data_ptr() != d.down or
+                    layer.gate_up_scale.data_ptr() != d.gate_up_scale or layer.down_scale.data_ptr() != d.down_scale):
+                raise ValueError("a tensor of the layer was replaced: new values are copied into it, or make another layer")
         elif layer.gate_up.device != self.device:
             raise ValueError(f"layer on cuda:{layer.gate_up.device}, context on cuda:{self.device}")
         elif not all(m._live for m in (layer.gate_up, layer.down, *(layer.shared or ()))):

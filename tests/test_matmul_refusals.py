@@ -195,3 +195,24 @@ def test_layer_arguments(ctx):  # noqa: F811
         ctx.moe(layer, z(T, K + 1), torch.zeros(T, 2), torch.ones(T, 2))
     with pytest.raises(TypeError):
         ctx.moe_layer_request(layer, b"")
+
+
+@pytest.mark.parametrize("name", ["gate_up", "gate_up_scale", "down", "down_scale"])
+def test_a_layer_whose_tensors_were_replaced(ctx, name):  # noqa: F811
+    """Its descriptor points to those that it was made of, whose memory may be another's by then."""
+    q = torch.int8
+    layer = I8Layer(ctx, z(E, 2 * N, K, dtype=q), torch.ones(E, 2 * N), z(E, K, N, dtype=q), torch.ones(E, K))
+    call = lambda: ctx.moe(layer, z(T, K), torch.zeros(T, 2), torch.ones(T, 2))  # noqa: E731
+    getattr(layer, name).copy_(torch.ones_like(getattr(layer, name)))  # values in place are the layer's own
+    with pytest.raises(Called, match="cx_i8_moe_scratch"):
+        call()
+    old = getattr(layer, name)
+    setattr(layer, name, old.clone())
+    with pytest.raises(ValueError, match="replaced"):
+        call()
+    setattr(layer, name, old)
+    with pytest.raises(Called, match="cx_i8_moe_scratch"):
+        call()
+    old.data = old.data.clone()
+    with pytest.raises(ValueError, match="replaced"):
+        call()
