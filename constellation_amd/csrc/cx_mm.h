@@ -657,7 +657,7 @@ __device__ __forceinline__ int mm_row_of_x(const MmLaunch& L, int p) {
 }
 
 // Forward: a workgroup reads its weights and rows once each from L2.  32 matrices of 4096 x 7168, gated, 512 rows each on
-// average: 977 to 1054 us when dealt unevenly (854 evenly, 1.13 PFLOP/s; one matrix of 4096 rows 1.4), matrix cores 70 % busy.
+// average: 967 to 1054 us when dealt unevenly (854 evenly, 1.13 PFLOP/s; one matrix of 4096 rows 1.4), matrix cores 70 % busy.
 // Two things bound it: traffic, as each item of up to 256 rows reads its matrix again (4.8 GB fetched where 2.1 are
 // unique, about 5 TB/s, a copy's rate), and tiles that an item's last rows do not fill.  m: weight rows; a gated tile has TM / 2 results of gate rows and the same rows of the up
 // half per wave, so that both factors of an output meet in one lane.

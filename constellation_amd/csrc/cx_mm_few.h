@@ -30,7 +30,7 @@ __device__ __forceinline__ u32x4 mm_piece(const char* q, int have) {
 // Up to 16 rows fit one MFMA's columns, so that the weights are read once and nothing is shared that LDS would serve.  Memory
 // bounds it: 1 row by 4096 x 7168 gated 14.8 us on weights from HBM (4.0 TB/s) and 12.4 after itself, when the last-level cache
 // holds the 59 MB (4.7 TB/s); 69 through LDS; 16 rows 20, where x costs L2 as many bytes as the weights cost HBM; 232 rows over
-// 64 matrices, which no cache holds, 197 to 219 (4.6 to 5.1 TB/s); 8-bit 8.4.  Rows at odd
+// 64 matrices, which no cache holds, 197 to 238 by the deal (about 4.7 TB/s); 8-bit 8.4.  Rows at odd
 // addresses (7161 columns) 24: lanes' pieces straddle lines; with more of them in flight it was 26.
 //
 // A workgroup's 8 waves are `splits` ranges of the columns times 8 / splits groups of RW tiles of 16 weight
