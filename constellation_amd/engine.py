@@ -385,10 +385,13 @@ class I8Layer(_OwnLayer):
         self.gate_up, self.gate_up_scale, self.down, self.down_scale = gate_up, gate_up_scale, down, down_scale
         self.shared = self if shared else None
         E, self.hidden, self.inter = down.shape
-        self.desc = I8LayerDesc(gate_up.data_ptr(), gate_up_scale.data_ptr(), down.data_ptr(), down_scale.data_ptr(), E,
-                                self.hidden, self.inter, int(shared))
+        self._at = self._places()
+        self.desc = I8LayerDesc(*self._at, E, self.hidden, self.inter, int(shared))
         self._hold(E - int(shared), experts, n_experts)
         self._scratch: dict = {}  # sizes by tokens and top_k
+
+    def _places(self) -> tuple[int, ...]:
+        return self.gate_up.data_ptr(), self.gate_up_scale.data_ptr(), self.down.data_ptr(), self.down_scale.data_ptr()
 
     @classmethod
     def quantize(cls, ctx: "Context", gate_up: torch.Tensor, down: torch.Tensor, **kw) -> "I8Layer":
@@ -771,9 +774,7 @@ class Context:
         self._here(x, *others)
         if isinstance(layer, I8Layer):
             self._here(layer.gate_up)
-            d = layer.desc
-            if (layer.gate_up.data_ptr() != d.gate_up or layer.down.data_ptr() != d.down or
-                    layer.gate_up_scale.data_ptr() != d.gate_up_scale or layer.down_scale.data_ptr() != d.down_scale):
+            if layer._places() != layer._at:
                 raise ValueError("a tensor of the layer was replaced: new values are copied into it, or make another layer")
         elif layer.gate_up.device != self.device:
             raise ValueError(f"layer on cuda:{layer.gate_up.device}, context on cuda:{self.device}")
